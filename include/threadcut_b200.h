@@ -15,7 +15,7 @@
  *   tc_splice_copy            threadcut/kv.py:34-41             splice(...) copy path (non-growing caches)
  *   tc_merge_partials         threadcut/flash_decode.py:68-69   softmax(lse) merge of split partials
  *   tc_decode_attention_paged, tc_prefill_attention_paged, tc_paged_rotate_keys, tc_paged_write,
- *   tc_paged_gather
+ *   tc_paged_append_rope, tc_paged_gather
  *                             threadcut/README.md:141-144       the paged KV layout named there as the next
  *                             step (no reference code): decode over pages (flash_decode.py:57-69 semantics),
  *                             splice as page drop + in-place key rotation (kv.py:28-41,83-92 semantics),
@@ -318,6 +318,24 @@ int tc_paged_write(const void* k_src, const void* v_src, void* k_pool, void* v_p
                    int64_t src_stride_h, int64_t src_stride_t, int64_t vsrc_stride_h, int64_t vsrc_stride_t,
                    int64_t page_rows, int64_t num_pages, int64_t pool_stride_page, int64_t pool_stride_h,
                    int64_t pool_stride_row, const int32_t* slots, int dtype, void* stream);
+
+/* A step's rows of one layer rotated and written in one launch, in place of q/k norm + RoPE (transformers'
+ * Qwen3Attention, as tc_qk_norm_rope for one token) and tc_paged_write: k and v [hkv][t][d] go to the
+ * slots (DEVICE int32 [t][2] = (page, row), distinct; a slot outside the pool is skipped), q [hq][t][d]
+ * to q_out (hq == 0 and NULL: keys and values only; q_out may be q). Queries and keys get, in fp32 and
+ * rounded once to dtype: RMSNorm over d with q_norm_weight / k_norm_weight [d] (NULL: none), then over
+ * the first `rot` elements x*cos + rotate_half(x)*sin, cos/sin [t][rot] of table_dtype (dtype or TC_F32)
+ * with row strides cos_stride_t / sin_stride_t; elements from `rot` on pass through. d and rot even,
+ * rot <= d <= 512; all dtypes; last dimensions contiguous. (The torch chain and tc_qk_norm_rope round
+ * after each op, so the two agree to a few roundings, not to the bit.) */
+int tc_paged_append_rope(const void* q, const void* k, const void* v, void* q_out, void* k_pool, void* v_pool, int hq,
+                         int hkv, int d, int64_t t, int64_t q_stride_h, int64_t q_stride_t, int64_t k_stride_h,
+                         int64_t k_stride_t, int64_t v_stride_h, int64_t v_stride_t, int64_t q_out_stride_h,
+                         int64_t q_out_stride_t, const void* q_norm_weight, const void* k_norm_weight, float eps,
+                         const void* cos_t, const void* sin_t, int rot, int64_t cos_stride_t, int64_t sin_stride_t,
+                         int table_dtype, int64_t page_rows, int64_t num_pages, int64_t pool_stride_page,
+                         int64_t pool_stride_h, int64_t pool_stride_row, const int32_t* slots, int dtype,
+                         void* stream);
 
 /* One layer's sequence copied out of the pools in logical order: k_out/v_out [hkv][n][d] (element
  * strides out_stride_h/out_stride_n, last dim contiguous); `tiles` is the DEVICE int32 [n_tiles][4]

@@ -1,0 +1,39 @@
+"""Argument checks of the serving operators without a GPU: the C entries refuse bad arguments (and accept
+empty work) before touching CUDA, and the Python wrappers refuse CPU tensors."""
+import ctypes
+
+import pytest
+import torch
+
+from threadcut_b200 import _lib
+from threadcut_b200.paged import append_rope
+
+P = ctypes.c_void_p(256)  # an aligned address that is never read: every call below ends before a launch
+N = None
+
+
+def append_status(q=P, k=P, v=P, qo=P, kp=P, vp=P, hq=8, hkv=2, d=64, t=4, eps=1e-6, cos=P, sin=P, rot=64, table=2,
+                  rows=64, pages=4, slots=P, dtype=2):
+    return _lib.lib().tc_paged_append_rope(q, k, v, qo, kp, vp, hq, hkv, d, t, *[64] * 8, N, N, eps, cos, sin, rot, 64,
+                                           64, table, rows, pages, 4096, 64, 64, slots, dtype, N)
+
+
+@pytest.mark.parametrize("bad,status", [
+    (dict(dtype=9), 3), (dict(table=1), 3), (dict(dtype=0, table=2), 3), (dict(d=63, rot=32), 1), (dict(d=514), 1),
+    (dict(d=0), 1), (dict(rot=66), 1), (dict(rot=3), 1), (dict(rot=0), 1), (dict(hkv=0), 1), (dict(hq=-1), 1),
+    (dict(t=-1), 1), (dict(rows=0), 1), (dict(pages=0), 1), (dict(eps=-1.0), 1), (dict(eps=float("nan")), 1),
+    (dict(q=N), 1), (dict(qo=N), 1), (dict(k=N), 1), (dict(v=N), 1), (dict(kp=N), 1), (dict(vp=N), 1), (dict(cos=N), 1),
+    (dict(sin=N), 1), (dict(slots=N), 1)])
+def test_append_refuses(bad, status):
+    assert append_status(**bad) == status
+
+
+def test_append_of_no_tokens_does_nothing():
+    assert append_status(t=0) == 0
+    assert append_status(t=0, q=N, qo=N, hq=0) == 0
+
+
+def test_cpu_tensors_are_refused():
+    x = torch.zeros(2, 4, 64)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        append_rope(x, x, x[0], x[0], x[None], x[None], torch.zeros(4, 2, dtype=torch.int32))

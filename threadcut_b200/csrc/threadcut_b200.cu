@@ -12,6 +12,7 @@
 #include "decode_attn.cuh"
 #include "rope_splice.cuh"
 #include "paged.cuh"
+#include "paged_append.cuh"
 #include "split.cuh"
 #include "prefill_attn.cuh"
 #include "layer_ops.cuh"
@@ -959,6 +960,78 @@ int tc_paged_write(const void* k_src, const void* v_src, void* k_pool, void* v_p
   const int blocks = grid_for(tasks, 256, sm_count(current_device()), 8);
   const cudaError_t e =
       TC_ROPE_DISPATCH(launch_paged_write, dtype, vec, p, blocks, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? TC_OK : TC_ERR_CUDA;
+}
+
+}  // extern "C"
+
+namespace {
+template <typename T>
+cudaError_t launch_paged_append(const PagedAppendParams& p, int sms, cudaStream_t st) {
+  const int blocks = grid_for(p.t * (p.hq + 2 * (int64_t)p.hkv), 8, sms, 8);
+  return launch_ex(paged_append_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, st, p);
+}
+}  // namespace
+
+extern "C" {
+
+int tc_paged_append_rope(const void* q, const void* k, const void* v, void* q_out, void* k_pool, void* v_pool, int hq,
+                         int hkv, int d, int64_t t, int64_t q_stride_h, int64_t q_stride_t, int64_t k_stride_h,
+                         int64_t k_stride_t, int64_t v_stride_h, int64_t v_stride_t, int64_t q_out_stride_h,
+                         int64_t q_out_stride_t, const void* q_norm_weight, const void* k_norm_weight, float eps,
+                         const void* cos_t, const void* sin_t, int rot, int64_t cos_stride_t, int64_t sin_stride_t,
+                         int table_dtype, int64_t page_rows, int64_t num_pages, int64_t pool_stride_page,
+                         int64_t pool_stride_h, int64_t pool_stride_row, const int32_t* slots, int dtype,
+                         void* stream) {
+  if (!valid_dtype(dtype) || (table_dtype != dtype && table_dtype != TC_F32)) return TC_ERR_DTYPE;
+  if (hkv < 1 || hkv > 65535 || hq < 0 || hq > 65535 || d < 2 || d > kMaxAppendDim || (d & 1) || rot < 2 || rot > d ||
+      (rot & 1) || t < 0 || page_rows < 1 || num_pages < 1 || !(eps >= 0.f))
+    return TC_ERR_INVALID;
+  if (t == 0) return TC_OK;
+  if (k == nullptr || v == nullptr || k_pool == nullptr || v_pool == nullptr || slots == nullptr || cos_t == nullptr ||
+      sin_t == nullptr || (hq > 0 && (q == nullptr || q_out == nullptr)))
+    return TC_ERR_INVALID;
+  PagedAppendParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.q = q;
+  p.k = k;
+  p.v = v;
+  p.q_out = q_out;
+  p.kp = k_pool;
+  p.vp = v_pool;
+  p.q_w = q_norm_weight;
+  p.k_w = k_norm_weight;
+  p.cos_t = cos_t;
+  p.sin_t = sin_t;
+  p.hq = hq;
+  p.hkv = hkv;
+  p.d = d;
+  p.rot = rot;
+  p.table_f32 = table_dtype == TC_F32;
+  p.t = t;
+  p.q_sh = q_stride_h;
+  p.q_st = q_stride_t;
+  p.k_sh = k_stride_h;
+  p.k_st = k_stride_t;
+  p.v_sh = v_stride_h;
+  p.v_st = v_stride_t;
+  p.qo_sh = q_out_stride_h;
+  p.qo_st = q_out_stride_t;
+  p.cos_st = cos_stride_t;
+  p.sin_st = sin_stride_t;
+  p.page_rows = page_rows;
+  p.num_pages = num_pages;
+  p.s_page = pool_stride_page;
+  p.s_h = pool_stride_h;
+  p.s_row = pool_stride_row;
+  p.slots = slots;
+  p.eps = eps;
+  p.inv_d = 1.f / (float)d;
+  const int sms = sm_count(current_device());
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const cudaError_t e = dtype == TC_F32    ? launch_paged_append<float>(p, sms, st)
+                        : dtype == TC_BF16 ? launch_paged_append<__nv_bfloat16>(p, sms, st)
+                                           : launch_paged_append<__half>(p, sms, st);
   return e == cudaSuccess ? TC_OK : TC_ERR_CUDA;
 }
 

@@ -28,7 +28,7 @@ from . import _lib
 from ._lib import check, dtype_code, lib, require_cuda, stream_ptr, workspaces
 from .match import Split
 
-__all__ = ["PageTable", "PagedKV", "TILE_ROWS"]
+__all__ = ["PageTable", "PagedKV", "TILE_ROWS", "append_rope"]
 
 TILE_ROWS = 32  # rows per tile-table entry (the decode kernel's tile height)
 
@@ -223,6 +223,75 @@ class PageTable:
         return np.stack((runs[idx, 0], runs[idx, 1] + k), axis=1)
 
 
+def append_rope(k, v, cos, sin, k_pool, v_pool, slots, *, q=None, q_norm=None, k_norm=None, eps=1e-6):
+    """Normalises (optional) and rotates a step's queries and keys and writes keys and values to
+    their slots of one layer's pools, in one launch (tc_paged_append_rope).
+
+    k, v: [hkv, t, d] (or [1, hkv, t, d]) raw projections; q: [hq, t, d] or None; cos, sin: [t, rot]
+    (or [1, t, rot]: transformers' position_embeddings) of the data's dtype or fp32, rot <= d (elements
+    from rot on pass through); q_norm / k_norm: RMSNorm weights [d] or None. k_pool, v_pool:
+    [pages, hkv, page_rows, d]; slots: int32 [t, 2] (page, row), distinct (PagedKV.reserve). Any
+    strides with a contiguous last dimension. Returns the rotated queries, in q's shape and stored
+    token by token ([t, hq, d]), or None. fp32 inside, each output rounded once."""
+    what = "append_rope"
+    require_cuda(k, v, cos, sin, k_pool, v_pool, slots, *(x for x in (q, q_norm, k_norm) if x is not None), what=what)
+    batched = k.dim() == 4
+    if batched:
+        if k.shape[0] != 1 or v.dim() != 4 or v.shape[0] != 1 or (q is not None and (q.dim() != 4 or q.shape[0] != 1)):
+            raise ValueError(f"{what}: one sequence per call (batch 1)")
+        k, v, q = k[0], v[0], q[0] if q is not None else None
+    if cos.dim() == 3 and cos.shape[0] == 1:
+        cos = cos[0]
+    if sin.dim() == 3 and sin.shape[0] == 1:
+        sin = sin[0]
+    if k.dim() != 3 or v.shape != k.shape or (q is not None and q.dim() != 3):
+        raise ValueError(f"{what}: expected k, v [hkv, t, d] and q [hq, t, d]; got {tuple(k.shape)}, {tuple(v.shape)}"
+                         + (f", {tuple(q.shape)}" if q is not None else ""))
+    hkv, t, d = k.shape
+    hq = q.shape[0] if q is not None else 0
+    if q is not None and tuple(q.shape) != (hq, t, d):
+        raise ValueError(f"{what}: q {tuple(q.shape)} does not match k {tuple(k.shape)}")
+    rot = cos.shape[-1]
+    if cos.dim() != 2 or cos.shape[0] != t or sin.shape != cos.shape or sin.dtype != cos.dtype:
+        raise ValueError(f"{what}: cos/sin must be [{t}, rot] of one dtype, got {tuple(cos.shape)}, {tuple(sin.shape)}")
+    if d % 2 or d > 512 or rot % 2 or not 2 <= rot <= d:
+        raise ValueError(f"{what}: needs an even head size <= 512 and an even rot in [2, d], got d = {d}, rot = {rot}")
+    if k_pool.dim() != 4 or k_pool.shape[1] != hkv or k_pool.shape[3] != d or v_pool.shape != k_pool.shape:
+        raise ValueError(f"{what}: pools must be [pages, {hkv}, page_rows, {d}], got {tuple(k_pool.shape)}")
+    if k_pool.stride(-1) != 1 or v_pool.stride() != k_pool.stride():
+        raise ValueError(f"{what}: the pools must have equal strides and a contiguous last dimension (they are written)")
+    if tuple(slots.shape) != (t, 2) or slots.dtype != torch.int32 or not slots.is_contiguous():
+        raise ValueError(f"{what}: slots must be a contiguous int32 [{t}, 2] tensor")
+    for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
+        if w is not None and (tuple(w.shape) != (d,) or w.dtype != k.dtype):
+            raise ValueError(f"{what}: {name} must be [{d}] of {k.dtype}")
+    code = dtype_code(k, what)
+    for x in (v, k_pool, v_pool) if q is None else (v, k_pool, v_pool, q):
+        if x.dtype != k.dtype:
+            raise TypeError(f"threadcut_b200.{what}: dtype mismatch {k.dtype} vs {x.dtype}")
+    if cos.dtype != k.dtype and cos.dtype != torch.float32:
+        raise TypeError(f"threadcut_b200.{what}: cos/sin must be {k.dtype} or fp32, got {cos.dtype}")
+    k, v, cos, sin = (x if x.stride(-1) == 1 else x.contiguous() for x in (k, v, cos, sin))
+    q_norm, k_norm = (w if w is None or w.stride(0) == 1 else w.contiguous() for w in (q_norm, k_norm))
+    out = None
+    if q is not None:
+        q = q if q.stride(-1) == 1 else q.contiguous()
+        out = torch.empty((t, hq, d), dtype=q.dtype, device=q.device).transpose(0, 1)
+    dev = k.device
+    ks, vs, ps = k.stride(), v.stride(), k_pool.stride()
+    qs, os = (q.stride(), out.stride()) if q is not None else ((0, 0), (0, 0))
+    with torch.cuda.device(dev):
+        st = lib().tc_paged_append_rope(
+            q.data_ptr() if q is not None else None, k.data_ptr(), v.data_ptr(),
+            out.data_ptr() if q is not None else None, k_pool.data_ptr(), v_pool.data_ptr(), hq, hkv, d, t, qs[0],
+            qs[1], ks[0], ks[1], vs[0], vs[1], os[0], os[1], q_norm.data_ptr() if q_norm is not None else None,
+            k_norm.data_ptr() if k_norm is not None else None, float(eps), cos.data_ptr(), sin.data_ptr(), rot,
+            cos.stride(0), sin.stride(0), _lib.DTYPE_CODE[cos.dtype], k_pool.shape[2], k_pool.shape[0], ps[0], ps[1],
+            ps[2], slots.data_ptr(), code, stream_ptr(dev))
+    check("tc_paged_append_rope", st)
+    return out[None] if batched and out is not None else out
+
+
 class PagedKV:
     """Paged K/V of `layers` attention layers of one sequence on one GPU.
 
@@ -306,6 +375,15 @@ class PagedKV:
                 k.data_ptr(), v.data_ptr(), self.k[layer].data_ptr(), self.v[layer].data_ptr(), self.hkv, self.d, t,
                 k.stride(0), k.stride(1), v.stride(0), v.stride(1), self.page_rows, self.table.num_pages,
                 sp, sh, sr, self._slots.data_ptr(), dtype_code(k, "PagedKV.write"), stream_ptr(self.device)))
+
+    def append(self, layer, k, v, cos, sin, *, q=None, q_norm=None, k_norm=None, eps=1e-6):
+        """Rotates the reserved step's raw keys (and queries) of one layer and writes keys and values
+        to its slots in one launch: append_rope into this layer's pools. Returns the rotated queries."""
+        t = k.shape[-2]
+        if self._slots is None or self._slots.shape[0] != t:
+            raise ValueError("PagedKV.append: reserve(t) the step's slots first (same t)")
+        return append_rope(k, v, cos, sin, self.k[layer], self.v[layer], self._slots, q=q, q_norm=q_norm,
+                           k_norm=k_norm, eps=eps)
 
     def decode(self, layer, q, scale, *, k_new=None, v_new=None, splits=None, stable_tiles=0):
         """Decode attention of q [hkv, g, d] over the whole sequence (threadcut/flash_decode.py:57-69
