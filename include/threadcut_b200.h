@@ -228,6 +228,23 @@ int tc_decode_attention_batched(const void* q, const void* k, const void* v, voi
                                 float scale, int splits, int dtype,
                                 void* workspace, size_t workspace_bytes, void* stream);
 
+/* tc_decode_attention_batched with a sliding window and a few first tokens that stay visible (sinks):
+ * of its n_b = lengths[b] rows (NULL: n; a length outside [0, n] is clamped) sequence b's query, its
+ * newest token, sees rows j < sinks and j >= n_b - window (window >= 1 counts the newest row itself,
+ * as transformers' sliding_window does; sinks >= 0). Only those rows are read. n_b == 0 gives zeros.
+ * Workspace as for the other decode calls, of at least
+ * tc_decode_attention_window_workspace_size(...) bytes. No counterpart in the reference, whose decode
+ * attends to the whole cache (threadcut/flash_decode.py:57-69). */
+size_t tc_decode_attention_window_workspace_size(int batch, int hkv, int g, int d, int64_t n, int64_t window,
+                                                 int64_t sinks, int splits, int dtype);
+int tc_decode_attention_window(const void* q, const void* k, const void* v, void* out, int batch, int hkv, int g,
+                               int d, int64_t n, const int32_t* lengths, int64_t window, int64_t sinks,
+                               int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_g, int64_t k_stride_b,
+                               int64_t k_stride_h, int64_t k_stride_n, int64_t v_stride_b, int64_t v_stride_h,
+                               int64_t v_stride_n, int64_t out_stride_b, int64_t out_stride_h, int64_t out_stride_g,
+                               float scale, int splits, int dtype, void* workspace, size_t workspace_bytes,
+                               void* stream);
+
 /* Ragged decode: sequence b has its own K/V allocation k_ptrs[b]/v_ptrs[b] of shape
  * [hkv, cap_b >= lengths[b], d] with head stride head_strides[b] (elements) and token stride
  * kv_stride_n, shared by K and V. k_ptrs, v_ptrs, head_strides and lengths are DEVICE arrays.

@@ -104,3 +104,22 @@ def test_pool_exhaustion_raises():
     tab.reserve(64)
     with pytest.raises(MemoryError):
         tab.reserve(1)
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_window_tiles_list_the_sinks_and_the_window(seed):
+    rng = random.Random(seed)
+    tab = PageTable(60, 40)
+    for _ in range(12):
+        tab.reserve(rng.choice([1, 5, 40, 90]))
+        if tab.n > 60 and rng.random() < 0.4:
+            a = rng.randint(0, tab.n // 2)
+            c0 = rng.randint(a, tab.n)
+            tab.splice(Split(a, c0, rng.randint(0, tab.n - c0)))
+        pos = [tuple(x) for x in tab.positions().tolist()]
+        for window in (1, 7, 32, 33, 200, 10 ** 9):
+            for sinks in (0, 1, 31, 64):
+                tiles = tab.window_tiles(window, sinks)
+                assert ((tiles[:, 2] >= 1) & (tiles[:, 2] <= TILE_ROWS)).all()
+                rows = [(p, r) for p, r0, c in tiles.tolist() for r in range(r0, r0 + c)]
+                assert rows == [x for j, x in enumerate(pos) if j < sinks or j >= tab.n - window]

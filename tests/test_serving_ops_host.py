@@ -37,3 +37,24 @@ def test_cpu_tensors_are_refused():
     x = torch.zeros(2, 4, 64)
     with pytest.raises(RuntimeError, match="CUDA"):
         append_rope(x, x, x[0], x[0], x[None], x[None], torch.zeros(4, 2, dtype=torch.int32))
+
+
+def window_status(q=P, k=P, v=P, out=P, b=2, hkv=2, g=4, d=128, n=100, window=10, sinks=2, scale=0.1, dtype=2, ws=P,
+                  nb=1 << 30):
+    return _lib.lib().tc_decode_attention_window(q, k, v, out, b, hkv, g, d, n, N, window, sinks, *[128] * 12, scale, 0,
+                                                 dtype, ws, nb, N)
+
+
+@pytest.mark.parametrize("bad,status", [
+    (dict(dtype=5), 3), (dict(window=0), 1), (dict(window=-4), 1), (dict(sinks=-1), 1), (dict(g=17), 1), (dict(g=0), 1),
+    (dict(b=0), 1), (dict(hkv=0), 1), (dict(n=-1), 1), (dict(n=1 << 31), 1), (dict(q=N), 1), (dict(out=N), 1),
+    (dict(k=N), 1), (dict(v=N), 1), (dict(scale=float("nan")), 1), (dict(scale=float("inf")), 1), (dict(d=48), 1),
+    (dict(dtype=0, d=256), 2)])
+def test_window_decode_refuses(bad, status):
+    assert window_status(**bad) == status
+
+
+def test_window_workspace_follows_the_window_not_the_cache():
+    size = _lib.lib().tc_decode_attention_window_workspace_size
+    assert size(64, 8, 4, 128, 1 << 20, 2048, 16, 0, 2) == size(64, 8, 4, 128, 1 << 24, 2048, 16, 0, 2)
+    assert size(64, 8, 4, 128, 1 << 20, 0, 16, 0, 2) == 0 and size(64, 8, 4, 128, 100, 5, -1, 0, 2) == 0

@@ -44,6 +44,9 @@ SIGNATURES = {
                                 + [_f, _i, _i, _vp, _sz, _vp]),
     "tc_decode_attention_batched": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i64, _vp] + [_i64] * 12
                                     + [_f, _i, _i, _vp, _sz, _vp]),
+    "tc_decode_attention_window_workspace_size": (_sz, [_i, _i, _i, _i, _i64, _i64, _i64, _i, _i]),
+    "tc_decode_attention_window": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i64, _vp, _i64, _i64] + [_i64] * 12
+                                   + [_f, _i, _i, _vp, _sz, _vp]),
     "tc_decode_attention_ragged": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i64, _i64, _i64]
                                    + [_i64] * 6 + [_f, _i, _i, _vp, _sz, _vp]),
     "tc_ragged_tensormaps_size": (_sz, [_i]),
@@ -237,6 +240,16 @@ class _Workspaces:
 
 
 workspaces = _Workspaces()
+
+
+def decode_workspace(rows, device, nbytes):
+    """A decode workspace for a call that may be under stream capture: the cached buffer of this
+    stream, or, while a CUDA graph is captured, a buffer of that graph's own (zeroed in the graph).
+    A cached buffer must not enter a graph: it is replaced when a later call needs a larger one, and
+    its zeros would be written by a replay only."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.zeros(nbytes, dtype=torch.uint8, device=device)
+    return workspaces.get(("decode", rows), device, nbytes)
 
 
 def device_errors(clear=True):

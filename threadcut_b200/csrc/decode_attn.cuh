@@ -113,7 +113,41 @@ struct DecodeParams {
   int64_t n_tiles;
   int64_t stable_tiles;  // paged: tiles [0, stable_tiles) and their rows are written by no kernel
                          // that can still be running when this one starts (0: none)
+  // window mode (contiguous rows, no append): of a sequence's n rows only the first `sinks` and the
+  // last `window` are read (see WindowRows); window == 0: all rows.
+  int64_t window, sinks;
 };
+
+// The rows a windowed decode reads: [0, sinks) and [w0, n) with w0 = n - window, or, where the two
+// meet, all of [0, n). Tile t of kTile rows starts at row(t) and holds at most kTile rows; the sinks'
+// tiles come first and the window's begin at w0 itself, so no tile mixes the two and a masked row
+// is always behind its tile's valid ones.
+struct WindowRows {
+  int64_t n, w0, sinks;
+  int64_t sink_tiles;
+  __device__ WindowRows(int64_t n_, int64_t window, int64_t sinks_) : n(n_), w0(n_ - window), sinks(sinks_) {
+    if (w0 <= sinks) {
+      w0 = 0;
+      sinks = 0;
+    }
+    sink_tiles = (sinks + kTile - 1) / kTile;
+  }
+  __device__ int64_t tiles() const { return sink_tiles + (n - w0 + kTile - 1) / kTile; }
+  __device__ int64_t row(int64_t t) const { return t < sink_tiles ? t * kTile : w0 + (t - sink_tiles) * kTile; }
+  __device__ int valid(int64_t t) const {
+    const int64_t left = (t < sink_tiles ? sinks : n) - row(t);
+    return left < kTile ? (int)left : kTile;
+  }
+};
+
+// Valid length of sequence b; in window mode clamped into [0, p.n] (the tiles are read by number, so a
+// length outside the tensor must not reach them).
+template <bool kWindow>
+__device__ __forceinline__ int64_t seq_length(const DecodeParams& p, int b) {
+  int64_t n = p.lengths ? (int64_t)p.lengths[b] : p.n;
+  if constexpr (kWindow) n = n < 0 ? 0 : (n > p.n ? p.n : n);
+  return n;
+}
 
 // Stores one output element at element offset `off` of p.out, in T or (partial mode) fp32.
 template <typename T>
@@ -540,9 +574,9 @@ __device__ __forceinline__ uint32_t swz(int row, int col) {
 // ------------------------------------------------------------------------------------------------
 // Tensor-core path: T in {bf16, f16}, D in {64, 128, 256}, NG = number of 8-head column tiles
 // (g <= 8*NG). K/V tiles arrive by tensor-map TMA: one cp.async.bulk.tensor per 64-column box.
-// kPaged: K/V rows come through the tile table (p.tiles); a separate instantiation, so the
-// contiguous kernel carries none of it.
-template <typename T, int D, int NG, bool kPaged>
+// kPaged: K/V rows come through the tile table (p.tiles); kWindow: the tiles are those of WindowRows.
+// Separate instantiations, so the contiguous kernel carries none of either.
+template <typename T, int D, int NG, bool kPaged, bool kWindow>
 __global__ void __launch_bounds__(32 * (kCWarps + 1), 1)
     decode_mma_kernel(const __grid_constant__ DecodeParams p) {
   using G = MmaGeom<D>;
@@ -574,7 +608,7 @@ __global__ void __launch_bounds__(32 * (kCWarps + 1), 1)
   }
   __syncthreads();  // barriers initialised before the producer may arm them below
   int staged = 0;   // producer lane: leading tiles already issued before pdl_wait()
-  if (!kPaged && warp == kCWarps && lane == 0) {
+  if (!kPaged && !kWindow && warp == kCWarps && lane == 0) {
     // Before waiting for the previous kernel (it may still be running):
     //  * tiles whose rows the caller declared stable (p.stable_rows, uniform lengths, where n and
     //    the partition come from kernel parameters) are loaded into the pipeline right away;
@@ -637,8 +671,9 @@ __global__ void __launch_bounds__(32 * (kCWarps + 1), 1)
   }
   pdl_launch();
   pdl_wait();  // everything below may read what the previous kernel in the stream wrote
-  const int64_t n = p.lengths ? (int64_t)p.lengths[b] : p.n;
-  const int64_t seq_tiles = kPaged ? p.n_tiles : (n + kTile - 1) / kTile;
+  const int64_t n = seq_length<kWindow>(p, b);
+  const WindowRows win(n, kWindow ? p.window : n, kWindow ? p.sinks : 0);
+  const int64_t seq_tiles = kPaged ? p.n_tiles : (kWindow ? win.tiles() : (n + kTile - 1) / kTile);
   const int nsplit = (kPaged ? seq_tiles > 0 : n > 0) ? (int)((seq_tiles + p.tiles_per_split - 1) / p.tiles_per_split) : 1;
   if (split >= nsplit) return;  // whole CTA leaves together; the barriers are never used
   int64_t tt0, tt1;
@@ -703,6 +738,7 @@ __global__ void __launch_bounds__(32 * (kCWarps + 1), 1)
           cbj = te.x;
           tok = te.y;
         }
+        if constexpr (kWindow) tok = (int)win.row(tt0 + j);
 #pragma unroll
         for (int bx = 0; bx < NBOX; ++bx) {
           tma_load_4d(st + bx * G::kBoxBytes, mk, bx * 64, tok, h, cbj, &full[s], pol);
@@ -758,6 +794,8 @@ __global__ void __launch_bounds__(32 * (kCWarps + 1), 1)
       if constexpr (kPaged) {
         const int vt = tab_entry(j).z;  // device table: clamp into [0, kTile]
         valid = vt < 0 ? 0 : (vt > kTile ? kTile : vt);
+      } else if constexpr (kWindow) {
+        valid = win.valid(tt0 + j);
       } else {
         const int64_t rem = t1 - (t0 + (int64_t)j * kTile);
         valid = rem < kTile ? (int)rem : kTile;
@@ -800,7 +838,8 @@ __global__ void __launch_bounds__(32 * (kCWarps + 1), 1)
       }
       if (valid < kTile) {
         // rows past this slice may hold another sequence's or uninitialised data (ragged caches
-        // are mapped to their capacity): zero those V rows so a masked p = 0 never meets a NaN
+        // are mapped to their capacity; behind a window's sinks lie rows nobody sees): zero those V
+        // rows so a masked p = 0 never meets a NaN
         const uint4 z = make_uint4(0u, 0u, 0u, 0u);
         for (int idx = lane; idx < (kTile - valid) * (D / 8); idx += 32) {
           const int row = valid + idx / (D / 8), cc = idx % (D / 8);
@@ -957,7 +996,8 @@ struct GenGeom {
                                    : merge_scratch_bytes(32 * kGenWarps);
 };
 
-template <typename T, int D>
+// kWindow: row t of the partition is row t of the sinks, then of the window (WindowRows).
+template <typename T, int D, bool kWindow>
 __global__ void __launch_bounds__(32 * kGenWarps) decode_generic_kernel(const __grid_constant__ DecodeParams p) {
   using G = GenGeom<D>;
   constexpr int HP = G::HP;
@@ -971,6 +1011,14 @@ __global__ void __launch_bounds__(32 * kGenWarps) decode_generic_kernel(const __
   const T* vh;
   int64_t n;
   resolve_seq<T>(p, b, h, kh, vh, n);
+  int64_t skip = 0, sinks = 0;  // rows between the sinks and the window
+  if constexpr (kWindow) {
+    n = seq_length<true>(p, b);
+    const WindowRows win(n, p.window, p.sinks);
+    sinks = win.sinks;
+    skip = win.w0 - sinks;
+    n -= skip;
+  }
   const int64_t seq_tiles = (n + kTile - 1) / kTile;
   const int nsplit = n > 0 ? (int)((seq_tiles + p.tiles_per_split - 1) / p.tiles_per_split) : 1;
   if (split >= nsplit) return;
@@ -996,7 +1044,8 @@ __global__ void __launch_bounds__(32 * kGenWarps) decode_generic_kernel(const __
       acc[i][j] = 0.f;
     }
   }
-  for (int64_t t = t0 + warp; t < t1; t += kGenWarps) {
+  for (int64_t r = t0 + warp; r < t1; r += kGenWarps) {
+    const int64_t t = kWindow && r >= sinks ? r + skip : r;
     float kv[DPL], vv[DPL];
 #pragma unroll
     for (int j = 0; j < DPL; ++j) {

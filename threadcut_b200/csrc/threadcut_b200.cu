@@ -157,6 +157,14 @@ DecodePlan plan_decode(int batch, int hkv, int64_t max_n, int64_t total_tokens, 
   return pl;
 }
 
+// Rows to plan a windowed decode for: the most tiles (in rows) that any sequence of at most n rows
+// reads. A sequence no longer than window + sinks reads all its rows; a longer one the sinks' tiles
+// and the window's, which start at the window's own first row.
+int64_t window_plan_rows(int64_t n, int64_t window, int64_t sinks) {
+  if (window >= n || sinks >= n - window) return n;
+  return kTile * (cdiv(sinks, kTile) + cdiv(window, kTile));
+}
+
 struct WsLayout {
   size_t counters = 0, ml = 0, o = 0, total = 0;
 };
@@ -233,7 +241,9 @@ cudaError_t launch_pdl(void (*fn)(KArgs...), dim3 grid, dim3 block, size_t smem,
 
 template <typename T, int D, int NG>
 cudaError_t launch_mma(const DecodeParams& p, dim3 grid, cudaStream_t st, int dev) {
-  auto fn = p.tiles != nullptr ? decode_mma_kernel<T, D, NG, true> : decode_mma_kernel<T, D, NG, false>;
+  auto fn = p.tiles != nullptr ? decode_mma_kernel<T, D, NG, true, false>
+            : p.window > 0     ? decode_mma_kernel<T, D, NG, false, true>
+                               : decode_mma_kernel<T, D, NG, false, false>;
   const int smem = MmaGeom<D>::kSmem;
   const int threads = 32 * (kCWarps + 1);
   cudaError_t e = set_smem(reinterpret_cast<const void*>(fn), smem, dev);
@@ -243,7 +253,7 @@ cudaError_t launch_mma(const DecodeParams& p, dim3 grid, cudaStream_t st, int de
 
 template <typename T, int D>
 cudaError_t launch_gen(const DecodeParams& p, dim3 grid, cudaStream_t st, int dev) {
-  auto fn = decode_generic_kernel<T, D>;
+  auto fn = p.window > 0 ? decode_generic_kernel<T, D, true> : decode_generic_kernel<T, D, false>;
   const int smem = GenGeom<D>::kSmem;
   cudaError_t e = set_smem(reinterpret_cast<const void*>(fn), smem, dev);
   if (e != cudaSuccess) return e;
@@ -306,7 +316,8 @@ int run_decode(DecodeParams p, int dtype, int d, bool ragged, int64_t max_n, int
     p.k_app = p.v_app = nullptr;
   }
   const int dev = current_device();
-  const DecodePlan pl = plan_decode(p.batch, p.hkv, max_n, total_tokens, ragged, splits_req,
+  const int64_t plan_n = p.window > 0 ? window_plan_rows(max_n, p.window, p.sinks) : max_n;
+  const DecodePlan pl = plan_decode(p.batch, p.hkv, plan_n, total_tokens, ragged, splits_req,
                                     use_mma ? kMmaCtasPerSm : kGenCtasPerSm, sm_count(dev));
   const WsLayout w = decode_ws_layout(p.batch, p.hkv, p.g, d, pl.max_splits);
   if (ws == nullptr || ws_bytes < w.total) return TC_ERR_WORKSPACE;
@@ -699,6 +710,51 @@ int tc_decode_attention_batched(const void* q, const void* k, const void* v, voi
   p.v = v;
   p.lengths = lengths;
   p.n = n;
+  p.sq_b = q_stride_b;
+  p.sq_h = q_stride_h;
+  p.sq_g = q_stride_g;
+  p.so_b = out_stride_b;
+  p.so_h = out_stride_h;
+  p.so_g = out_stride_g;
+  p.sk_b = k_stride_b;
+  p.sk_h = k_stride_h;
+  p.sk_n = k_stride_n;
+  p.sv_b = v_stride_b;
+  p.sv_h = v_stride_h;
+  p.sv_n = v_stride_n;
+  p.hkv = hkv;
+  p.g = g;
+  p.batch = batch;
+  const bool al = aligned16(k) && aligned16(v) && stride16(k_stride_b, dtype) && stride16(k_stride_h, dtype) &&
+                  stride16(k_stride_n, dtype) && stride16(v_stride_b, dtype) && stride16(v_stride_h, dtype) &&
+                  stride16(v_stride_n, dtype);
+  return run_decode(p, dtype, d, lengths != nullptr, n, 0, splits, al, scale, workspace, workspace_bytes,
+                    static_cast<cudaStream_t>(stream));
+}
+
+size_t tc_decode_attention_window_workspace_size(int batch, int hkv, int g, int d, int64_t n, int64_t window,
+                                                 int64_t sinks, int splits, int dtype) {
+  if (n < 0 || window < 1 || sinks < 0) return 0;
+  return tc_decode_attention_workspace_size(batch, hkv, g, d, window_plan_rows(n, window, sinks), 0, splits, dtype);
+}
+
+int tc_decode_attention_window(const void* q, const void* k, const void* v, void* out, int batch, int hkv, int g,
+                               int d, int64_t n, const int32_t* lengths, int64_t window, int64_t sinks,
+                               int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_g, int64_t k_stride_b,
+                               int64_t k_stride_h, int64_t k_stride_n, int64_t v_stride_b, int64_t v_stride_h,
+                               int64_t v_stride_n, int64_t out_stride_b, int64_t out_stride_h, int64_t out_stride_g,
+                               float scale, int splits, int dtype, void* workspace, size_t workspace_bytes,
+                               void* stream) {
+  if (window < 1 || sinks < 0 || n > INT32_MAX || (n > 0 && (k == nullptr || v == nullptr))) return TC_ERR_INVALID;
+  DecodeParams p = base_params();
+  p.q = q;
+  p.out = out;
+  p.k = k;
+  p.v = v;
+  p.lengths = lengths;
+  p.n = n;
+  p.window = window < n ? window : (n > 0 ? n : 1);
+  p.sinks = sinks < n ? sinks : n;
   p.sq_b = q_stride_b;
   p.sq_h = q_stride_h;
   p.sq_g = q_stride_g;

@@ -10,6 +10,7 @@ called through tc_decode_attention; there is no CPU or Triton path.
 Extra entry points beside it (same math): `decode_attention_lse` (also returns the natural-log
 LSE, the partial form for sequence-sharded decode), `decode_attention_batched` (b > 1 sequences
 in one strided tensor, the b > 1 decode branch of threadcut/attention.py:41-42),
+`decode_attention_window` (that with a sliding window and sinks),
 `decode_attention_ragged` (per-sequence caches and lengths) and `merge_partials` (LSE merge).
 """
 import ctypes
@@ -20,7 +21,7 @@ from . import _lib
 from ._lib import check, dtype_code, lib, require_cuda, stream_ptr, workspaces
 
 __all__ = ["decode_attention", "decode_attention_append", "decode_attention_lse", "decode_attention_partial", "decode_attention_batched",
-           "decode_attention_ragged", "merge_partials", "RaggedKV"]
+           "decode_attention_ragged", "decode_attention_window", "merge_partials", "RaggedKV"]
 
 
 def _last_contig(t):
@@ -252,6 +253,56 @@ def decode_attention_batched(q, k, v, scale, lengths=None, *, splits=None):
             float(scale), s, code, ws.data_ptr(), ws.numel(), stream_ptr(dev))
     check("tc_decode_attention_batched", st)
     return out
+
+
+def decode_attention_window(q, k, v, scale, window, sinks=0, lengths=None, *, splits=None):
+    """decode_attention_batched with a sliding window and first tokens that stay visible (sinks): each
+    sequence's query is its newest token and sees, of its n_b rows, those with j < sinks or
+    j >= n_b - window (window >= 1 counts the newest row; only visible rows are read).
+
+    q: [b, hkv, g, d]; k, v: [b, hkv, n, d]; lengths: optional int32 CUDA tensor [b] of valid lengths
+    (clamped into [0, n]; 0 gives zeros). One sequence may come without the batch dimension (q
+    [hkv, g, d], k/v [hkv, n, d]). Returns q's shape."""
+    what = "decode_attention_window"
+    require_cuda(q, k, v, what=what)
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        _check_same_dtype(what, q, k, v)
+    single = q.dim() == 3
+    if single:
+        q, k, v = q[None], k[None], v[None]
+    if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape:
+        raise ValueError(f"{what}: expected q [b, hkv, g, d], k/v [b, hkv, n, d]; got {tuple(q.shape)}, "
+                         f"{tuple(k.shape)}, {tuple(v.shape)}")
+    b, hkv, g, d = q.shape
+    n = k.shape[2]
+    if tuple(k.shape) != (b, hkv, n, d):
+        raise ValueError(f"{what}: k/v shape {tuple(k.shape)} does not match q {tuple(q.shape)}")
+    window, sinks = int(window), int(sinks)
+    if window < 1 or sinks < 0:
+        raise ValueError(f"{what}: needs window >= 1 and sinks >= 0, got {window} and {sinks}")
+    window, sinks = min(window, max(n, 1)), min(sinks, n)
+    q, k, v = _last_contig(q), _last_contig(k), _last_contig(v)
+    dev = q.device
+    lens_ptr = None
+    if lengths is not None:
+        if lengths.dtype != torch.int32 or lengths.device != dev or not lengths.is_contiguous():
+            lengths = lengths.to(device=dev, dtype=torch.int32).contiguous()
+        if lengths.shape != (b,):
+            raise ValueError(f"{what}: lengths must be [{b}]")
+        lens_ptr = lengths.data_ptr()
+    code = dtype_code(q, what)
+    out = torch.empty((b, hkv, g, d), dtype=q.dtype, device=dev)
+    L = lib()
+    s = int(splits or 0)
+    with torch.cuda.device(dev):
+        nb = L.tc_decode_attention_window_workspace_size(b, hkv, g, d, n, window, sinks, s, code)
+        ws = _lib.decode_workspace(b * hkv, dev, nb)
+        st = L.tc_decode_attention_window(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), b, hkv, g, d, n, lens_ptr, window, sinks,
+            *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3], float(scale), s, code,
+            ws.data_ptr(), ws.numel(), stream_ptr(dev))
+    check("tc_decode_attention_window", st)
+    return out[0] if single else out
 
 
 class RaggedKV:

@@ -212,6 +212,16 @@ class PageTable:
         out[:, 2] = np.minimum(TILE_ROWS, sel[:, 2] - off)
         return out
 
+    def window_tiles(self, window, sinks):
+        """Tile table of the rows a windowed decode reads: tokens [0, sinks) and [n - window, n), or every
+        token where the two meet."""
+        lo = self.n - window
+        if lo <= sinks:
+            return self.tiles()
+        end, start, tile0 = self._index()
+        return np.concatenate((self._span(0, sinks, end, start, tile0)[1],
+                               self._span(lo, self.n, end, start, tile0)[1]))
+
     def positions(self):
         """(page, row) of every logical token, int64 [n, 2] (for gathers and checks)."""
         runs = self._runs
@@ -317,6 +327,8 @@ class PagedKV:
         self._slots = None       # device int32 [t, 2] of the step reserved last
         self._tiles_dev = None   # device int32 [capacity, 3]: the tile table, rows [0, n) valid
         self._tiles_ver = -1     # table version the device copy reflects
+        self._win = None         # (version, window, sinks) of the windowed table below
+        self._win_dev = None     # device int32 [T, 3]: the tiles a windowed decode reads
         self._ktab = None        # device int32 [T, 4]: tiles + logical start, for prefill
         self._ktab_starts = None
         self._ktab_ver = -1
@@ -385,13 +397,27 @@ class PagedKV:
         return append_rope(k, v, cos, sin, self.k[layer], self.v[layer], self._slots, q=q, q_norm=q_norm,
                            k_norm=k_norm, eps=eps)
 
-    def decode(self, layer, q, scale, *, k_new=None, v_new=None, splits=None, stable_tiles=0):
+    def _window_tiles(self, window, sinks):
+        """Device tile table of a windowed decode, its length and the tokens it lists; rebuilt when the
+        sequence or the window changed (once a step for all layers)."""
+        key = (self.table.version, window, sinks)
+        if self._win != key:
+            tab = np.ascontiguousarray(self.table.window_tiles(window, sinks))
+            # a fresh tensor: an earlier step's launches may still be reading the old one
+            self._win_dev = torch.from_numpy(tab).to(self.device)
+            self._win = key
+        nt = self._win_dev.shape[0]
+        return (self._win_dev if nt else None), nt, min(self.table.n, window + sinks)
+
+    def decode(self, layer, q, scale, *, k_new=None, v_new=None, splits=None, stable_tiles=0, window=None, sinks=0):
         """Decode attention of q [hkv, g, d] over the whole sequence (threadcut/flash_decode.py:57-69
         semantics). With k_new/v_new [hkv, d] the last reserved row (a one-token step) is written by
         the same launch (fused append). stable_tiles: the leading tiles of the table (see
         `n_tiles`) whose rows no kernel still running writes, which the launch may load before the
         previous one ends (0: none; n_tiles - 1 in a layer-by-layer decode step with fused append,
-        where each launch writes only the last row of its own layer)."""
+        where each launch writes only the last row of its own layer). window / sinks: the query sees
+        only the first `sinks` and the last `window` tokens (the newest one counted), as
+        flash_decode.decode_attention_window; stable_tiles is ignored then."""
         require_cuda(q, what="PagedKV.decode")
         hkv, g, d = q.shape
         if hkv != self.hkv or d != self.d or q.dtype != self.dtype:
@@ -409,7 +435,15 @@ class PagedKV:
                 k_new, v_new = k_new.contiguous(), v_new.contiguous()
         if q.stride(-1) != 1:
             q = q.contiguous()
-        tiles, nt = self._tiles()
+        if window is None:
+            (tiles, nt), n = self._tiles(), self.table.n
+            if sinks:
+                raise ValueError("PagedKV.decode: sinks go with a window")
+        else:
+            if window < 1 or sinks < 0:
+                raise ValueError(f"PagedKV.decode: needs window >= 1 and sinks >= 0, got {window} and {sinks}")
+            tiles, nt, n = self._window_tiles(int(window), int(sinks))
+            stable_tiles = 0
         out = torch.empty((hkv, g, d), dtype=q.dtype, device=q.device)
         code = dtype_code(q, "PagedKV.decode")
         ws = workspaces.get(("decode", hkv), q.device, _lib.decode_workspace_bound(1, hkv, g, d, code))
@@ -418,7 +452,7 @@ class PagedKV:
             check("tc_decode_attention_paged", lib().tc_decode_attention_paged(
                 q.data_ptr(), self.k[layer].data_ptr(), self.v[layer].data_ptr(), out.data_ptr(), hkv, g, d,
                 self.page_rows, self.table.num_pages, sp, sh, sr, tiles.data_ptr() if tiles is not None else None,
-                nt, self.table.n, k_new.data_ptr() if k_new is not None else None,
+                nt, n, k_new.data_ptr() if k_new is not None else None,
                 v_new.data_ptr() if v_new is not None else None, k_new.stride(0) if k_new is not None else 0,
                 v_new.stride(0) if v_new is not None else 0, q.stride(0), q.stride(1), out.stride(0), out.stride(1),
                 float(scale), int(splits or 0), code, int(stable_tiles), ws.data_ptr(), ws.numel(),
