@@ -191,6 +191,47 @@ int tc_prefill_attention(const void* q, const void* k, const void* v, void* out,
                          float scale, int splits, int dtype,
                          void* workspace, size_t workspace_bytes, void* stream);
 
+/* tc_prefill_attention with a sliding window and first tokens that stay visible (sinks), for `batch`
+ * sequences of equal lengths: query p of the newest lq of lk tokens sees the keys j <= lk - lq + p with
+ * j < sinks or j > lk - lq + p - window (window >= 1 counts the query's own token, as transformers'
+ * sliding_window does). q [batch, hq, lq, d], k/v [batch, hkv, lk, d] with hq a multiple of hkv, out
+ * [batch, lq, hq, d], any strides with a contiguous last dimension; d <= 256, every dtype. 16-bit,
+ * d in {64, 128}, hq <= 128 hkv, scale > 0 and 16-byte aligned bases and strides run on the tcgen05 tensor
+ * cores and visit only the key tiles that some query of the block sees; the rest runs a plain kernel.
+ * In the tcgen05 kernel a key row inside such a tile that is hidden from one of the block's queries meets
+ * it with a zero weight, so V must be finite there, as in any masked product. splits = 0 picks the number
+ * of KV splits; workspace of tc_prefill_window_workspace_size() bytes (0: none; no initial contents).
+ * No counterpart in the reference, whose prefill sees the whole cache (threadcut/attention.py:43-46). */
+size_t tc_prefill_window_workspace_size(int batch, int hq, int hkv, int lq, int lk, int d, int64_t window,
+                                        int64_t sinks, int splits);
+int tc_prefill_attention_window(const void* q, const void* k, const void* v, void* out, int batch, int hq, int hkv,
+                                int lq, int lk, int d, int64_t window, int64_t sinks, int64_t q_stride_b,
+                                int64_t q_stride_h, int64_t q_stride_p, int64_t k_stride_b, int64_t k_stride_h,
+                                int64_t k_stride_n, int64_t v_stride_b, int64_t v_stride_h, int64_t v_stride_n,
+                                int64_t out_stride_b, int64_t out_stride_p, int64_t out_stride_h, float scale,
+                                int splits, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Decode attention of `batch` sequences that share ONE cached prefix, each with its own suffix (several
+ * continuations of one context): q [batch, hkv, g, d], k_prefix/v_prefix [hkv, n, d], k/v
+ * [batch, hkv, m, d] of which the first lengths[b] rows count (DEVICE int32, NULL: m; clamped into
+ * [0, m]), out [batch, hkv, g, d] = softmax(scale q [prefix ; suffix_b]^T) [prefix ; suffix_b]; n == 0,
+ * m == 0 and empty suffixes are fine, nothing at all gives zeros. The prefix is read once for the whole
+ * batch: its rows meet all batch*g queries of a KV head in one matrix product. g <= 128, d <= 256, every
+ * dtype, any strides with a contiguous last dimension; 16-bit, d in {64, 128, 256}, scale > 0 and 16-byte
+ * aligned bases and strides run on the tcgen05 tensor cores, the rest a plain kernel. Workspace of
+ * tc_decode_attention_shared_workspace_size() bytes, 16-byte aligned, with no initial contents (nothing is
+ * kept in it between calls). The reference decodes one sequence over its own cache
+ * (threadcut/flash_decode.py:57-69); this is the merge of :68-69 over the prefix and the suffix. */
+size_t tc_decode_attention_shared_workspace_size(int batch, int hkv, int g, int d, int64_t n, int64_t m, int dtype);
+int tc_decode_attention_shared(const void* q, const void* k_prefix, const void* v_prefix, const void* k, const void* v,
+                               void* out, int batch, int hkv, int g, int d, int64_t n, int64_t m,
+                               const int32_t* lengths, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_g,
+                               int64_t kp_stride_h, int64_t kp_stride_n, int64_t vp_stride_h, int64_t vp_stride_n,
+                               int64_t k_stride_b, int64_t k_stride_h, int64_t k_stride_n, int64_t v_stride_b,
+                               int64_t v_stride_h, int64_t v_stride_n, int64_t out_stride_b, int64_t out_stride_h,
+                               int64_t out_stride_g, float scale, int dtype, void* workspace, size_t workspace_bytes,
+                               void* stream);
+
 /* Decode attention that allocates nothing, for callers that cannot hand us device memory: for
  * example a plugin running inside another runtime that owns every device allocation and forbids
  * allocating in its execute hook, a loop where the implicit synchronisation of cudaMalloc is not

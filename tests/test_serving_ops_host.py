@@ -58,3 +58,32 @@ def test_window_workspace_follows_the_window_not_the_cache():
     size = _lib.lib().tc_decode_attention_window_workspace_size
     assert size(64, 8, 4, 128, 1 << 20, 2048, 16, 0, 2) == size(64, 8, 4, 128, 1 << 24, 2048, 16, 0, 2)
     assert size(64, 8, 4, 128, 1 << 20, 0, 16, 0, 2) == 0 and size(64, 8, 4, 128, 100, 5, -1, 0, 2) == 0
+
+
+def prefill_status(q=P, k=P, v=P, out=P, b=1, hq=8, hkv=2, lq=4, lk=100, d=128, window=10, sinks=2, scale=0.1, splits=0,
+                   dtype=2, ws=N, nb=0):
+    return _lib.lib().tc_prefill_attention_window(q, k, v, out, b, hq, hkv, lq, lk, d, window, sinks, *[128] * 12, scale,
+                                                  splits, dtype, ws, nb, N)
+
+
+@pytest.mark.parametrize("bad,status", [
+    (dict(dtype=5), 3), (dict(window=0), 1), (dict(sinks=-1), 1), (dict(hq=7), 1), (dict(hq=1), 1), (dict(hkv=0), 1),
+    (dict(b=0), 1), (dict(b=65536), 1), (dict(lq=0), 1), (dict(lk=3), 1), (dict(d=0), 1), (dict(d=257), 1),
+    (dict(splits=-1), 1), (dict(q=N), 1), (dict(k=N), 1), (dict(v=N), 1), (dict(out=N), 1),
+    (dict(scale=float("nan")), 1), (dict(scale=float("inf")), 1)])
+def test_window_prefill_refuses(bad, status):
+    assert prefill_status(**bad) == status
+
+
+def shared_status(q=P, kp=P, vp=P, k=P, v=P, out=P, b=2, hkv=2, g=4, d=128, n=100, m=10, scale=0.1, dtype=2, ws=N, nb=0):
+    return _lib.lib().tc_decode_attention_shared(q, kp, vp, k, v, out, b, hkv, g, d, n, m, N, *[128] * 16, scale, dtype,
+                                                 ws, nb, N)
+
+
+@pytest.mark.parametrize("bad,status", [
+    (dict(dtype=5), 3), (dict(b=0), 1), (dict(b=65536), 1), (dict(hkv=0), 1), (dict(g=0), 1), (dict(g=129), 1),
+    (dict(d=0), 1), (dict(d=257), 1), (dict(n=-1), 1), (dict(m=-1), 1), (dict(n=1 << 31), 1), (dict(m=1 << 31), 1),
+    (dict(q=N), 1), (dict(out=N), 1), (dict(kp=N), 1), (dict(vp=N), 1), (dict(k=N), 1), (dict(v=N), 1),
+    (dict(scale=float("nan")), 1), (dict(scale=float("-inf")), 1)])
+def test_shared_decode_refuses(bad, status):
+    assert shared_status(**bad) == status

@@ -15,6 +15,7 @@
 #include "paged_append.cuh"
 #include "split.cuh"
 #include "prefill_attn.cuh"
+#include "rows_attn.cuh"
 #include "layer_ops.cuh"
 #include "peer.cuh"
 #include "gemv_stream.cuh"
@@ -1928,6 +1929,130 @@ int tc_peer_gather_merge(const float* o_local, const float* lse_local, void* out
     e = launch_pdl(gather_merge_kernel<float>, grid, dim3(kGmThreads), 0, st, o_local, lse_local,
                    static_cast<float*>(out), lse_out, rows, d, out_stride_row, gp);
   return e == cudaSuccess ? TC_OK : TC_ERR_CUDA;
+}
+
+}  // extern "C"
+
+// ------------------------------------------------------------------------------- window prefill, shared prefix
+namespace {
+int launch_rows(const RowsParams& p, int dtype, cudaStream_t st) {
+  const int64_t rows = (int64_t)p.batch * p.hkv * p.g * p.lq;
+  if (rows > INT32_MAX) return TC_ERR_INVALID;
+  const dim3 grid((unsigned)rows), block(32 * kRowsWarps);
+  const cudaError_t e = dtype == TC_F32    ? launch_ex(rows_attn_kernel<float>, grid, block, 0, st, p)
+                        : dtype == TC_BF16 ? launch_ex(rows_attn_kernel<__nv_bfloat16>, grid, block, 0, st, p)
+                                           : launch_ex(rows_attn_kernel<__half>, grid, block, 0, st, p);
+  return e == cudaSuccess ? TC_OK : TC_ERR_CUDA;
+}
+
+bool finite_scale(float s) { return s == s && s != INFINITY && s != -INFINITY; }
+}  // namespace
+
+extern "C" {
+
+size_t tc_prefill_window_workspace_size(int batch, int hq, int hkv, int lq, int lk, int d, int64_t window,
+                                        int64_t sinks, int splits) {
+  (void)batch, (void)hq, (void)hkv, (void)lq, (void)lk, (void)d, (void)window, (void)sinks, (void)splits;
+  return 0;
+}
+
+int tc_prefill_attention_window(const void* q, const void* k, const void* v, void* out, int batch, int hq, int hkv,
+                                int lq, int lk, int d, int64_t window, int64_t sinks, int64_t q_stride_b,
+                                int64_t q_stride_h, int64_t q_stride_p, int64_t k_stride_b, int64_t k_stride_h,
+                                int64_t k_stride_n, int64_t v_stride_b, int64_t v_stride_h, int64_t v_stride_n,
+                                int64_t out_stride_b, int64_t out_stride_p, int64_t out_stride_h, float scale,
+                                int splits, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!valid_dtype(dtype)) return TC_ERR_DTYPE;
+  if (batch < 1 || batch > 65535 || hkv < 1 || hkv > 65535 || hq < hkv || hq % hkv != 0 || hq > 65535 || lq < 1 ||
+      lk < lq || d < 1 || d > kRowsMaxDim || window < 1 || sinks < 0 || splits < 0 || q == nullptr || k == nullptr ||
+      v == nullptr || out == nullptr || !finite_scale(scale))
+    return TC_ERR_INVALID;
+  (void)workspace, (void)workspace_bytes;
+  RowsParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.q = q;
+  p.out = out;
+  p.sq_b = q_stride_b;
+  p.sq_h = q_stride_h * (hq / hkv);
+  p.sq_g = q_stride_h;
+  p.sq_p = q_stride_p;
+  p.so_b = out_stride_b;
+  p.so_h = out_stride_h * (hq / hkv);
+  p.so_g = out_stride_h;
+  p.so_p = out_stride_p;
+  p.k0 = p.k1 = k;
+  p.v0 = p.v1 = v;
+  p.sk0_b = p.sk1_b = k_stride_b;
+  p.sk0_h = p.sk1_h = k_stride_h;
+  p.sk0_n = p.sk1_n = k_stride_n;
+  p.sv0_b = p.sv1_b = v_stride_b;
+  p.sv0_h = p.sv1_h = v_stride_h;
+  p.sv0_n = p.sv1_n = v_stride_n;
+  p.batch = batch;
+  p.hkv = hkv;
+  p.g = hq / hkv;
+  p.d = d;
+  p.lq = lq;
+  p.window = window < lk ? window : lk;
+  p.sinks = sinks < lk ? sinks : lk;
+  p.lk = lk;
+  p.c = scale * kLog2e;
+  return launch_rows(p, dtype, static_cast<cudaStream_t>(stream));
+}
+
+size_t tc_decode_attention_shared_workspace_size(int batch, int hkv, int g, int d, int64_t n, int64_t m, int dtype) {
+  (void)batch, (void)hkv, (void)g, (void)d, (void)n, (void)m, (void)dtype;
+  return 0;
+}
+
+int tc_decode_attention_shared(const void* q, const void* k_prefix, const void* v_prefix, const void* k, const void* v,
+                               void* out, int batch, int hkv, int g, int d, int64_t n, int64_t m,
+                               const int32_t* lengths, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_g,
+                               int64_t kp_stride_h, int64_t kp_stride_n, int64_t vp_stride_h, int64_t vp_stride_n,
+                               int64_t k_stride_b, int64_t k_stride_h, int64_t k_stride_n, int64_t v_stride_b,
+                               int64_t v_stride_h, int64_t v_stride_n, int64_t out_stride_b, int64_t out_stride_h,
+                               int64_t out_stride_g, float scale, int dtype, void* workspace, size_t workspace_bytes,
+                               void* stream) {
+  if (!valid_dtype(dtype)) return TC_ERR_DTYPE;
+  if (batch < 1 || batch > 65535 || hkv < 1 || hkv > 65535 || g < 1 || g > 128 || d < 1 || d > kRowsMaxDim || n < 0 ||
+      n > INT32_MAX || m < 0 || m > INT32_MAX || q == nullptr || out == nullptr || !finite_scale(scale) ||
+      (n > 0 && (k_prefix == nullptr || v_prefix == nullptr)) || (m > 0 && (k == nullptr || v == nullptr)))
+    return TC_ERR_INVALID;
+  (void)workspace, (void)workspace_bytes;
+  RowsParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.q = q;
+  p.out = out;
+  p.sq_b = q_stride_b;
+  p.sq_h = q_stride_h;
+  p.sq_g = q_stride_g;
+  p.so_b = out_stride_b;
+  p.so_h = out_stride_h;
+  p.so_g = out_stride_g;
+  p.k0 = k_prefix;
+  p.v0 = v_prefix;
+  p.sk0_h = kp_stride_h;
+  p.sk0_n = kp_stride_n;
+  p.sv0_h = vp_stride_h;
+  p.sv0_n = vp_stride_n;
+  p.k1 = k;
+  p.v1 = v;
+  p.sk1_b = k_stride_b;
+  p.sk1_h = k_stride_h;
+  p.sk1_n = k_stride_n;
+  p.sv1_b = v_stride_b;
+  p.sv1_h = v_stride_h;
+  p.sv1_n = v_stride_n;
+  p.batch = batch;
+  p.hkv = hkv;
+  p.g = g;
+  p.d = d;
+  p.lq = 1;
+  p.n0 = n;
+  p.n1 = m;
+  p.lengths = lengths;
+  p.c = scale * kLog2e;
+  return launch_rows(p, dtype, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

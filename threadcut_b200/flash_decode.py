@@ -10,7 +10,8 @@ called through tc_decode_attention; there is no CPU or Triton path.
 Extra entry points beside it (same math): `decode_attention_lse` (also returns the natural-log
 LSE, the partial form for sequence-sharded decode), `decode_attention_batched` (b > 1 sequences
 in one strided tensor, the b > 1 decode branch of threadcut/attention.py:41-42),
-`decode_attention_window` (that with a sliding window and sinks),
+`decode_attention_window` (that with a sliding window and sinks), `decode_attention_shared` (sequences
+that continue one shared prefix),
 `decode_attention_ragged` (per-sequence caches and lengths) and `merge_partials` (LSE merge).
 """
 import ctypes
@@ -21,7 +22,7 @@ from . import _lib
 from ._lib import check, dtype_code, lib, require_cuda, stream_ptr, workspaces
 
 __all__ = ["decode_attention", "decode_attention_append", "decode_attention_lse", "decode_attention_partial", "decode_attention_batched",
-           "decode_attention_ragged", "decode_attention_window", "merge_partials", "RaggedKV"]
+           "decode_attention_ragged", "decode_attention_shared", "decode_attention_window", "merge_partials", "RaggedKV"]
 
 
 def _last_contig(t):
@@ -303,6 +304,50 @@ def decode_attention_window(q, k, v, scale, window, sinks=0, lengths=None, *, sp
             ws.data_ptr(), ws.numel(), stream_ptr(dev))
     check("tc_decode_attention_window", st)
     return out[0] if single else out
+
+
+def decode_attention_shared(q, k_prefix, v_prefix, k, v, scale, lengths=None):
+    """Decode attention of b sequences that share one cached prefix, each with its own suffix (samples or
+    sub-agents that continue one context): q [b, hkv, g, d], k_prefix/v_prefix [hkv, n, d] (a GrowingLayer
+    view without its batch dimension), k/v [b, hkv, m, d] of which sequence i's first lengths[i] rows count
+    (int32 CUDA [b], clamped into [0, m]; None: all m). Returns [b, hkv, g, d], attention over the prefix
+    and then the suffix. The prefix is read once for the whole batch. An empty prefix or suffix is fine;
+    with neither the result is zeros."""
+    what = "decode_attention_shared"
+    require_cuda(q, k_prefix, v_prefix, k, v, what=what)
+    for x in (k_prefix, v_prefix, k, v):
+        if x.dtype != q.dtype:
+            _check_same_dtype(what, q, x)
+    if q.dim() != 4 or k_prefix.dim() != 3 or k.dim() != 4 or v_prefix.shape != k_prefix.shape or v.shape != k.shape:
+        raise ValueError(f"{what}: expected q [b, hkv, g, d], k_prefix/v_prefix [hkv, n, d], k/v [b, hkv, m, d]; got "
+                         f"{tuple(q.shape)}, {tuple(k_prefix.shape)}, {tuple(v_prefix.shape)}, {tuple(k.shape)}, "
+                         f"{tuple(v.shape)}")
+    b, hkv, g, d = q.shape
+    n, m = k_prefix.shape[1], k.shape[2]
+    if k_prefix.shape != (hkv, n, d) or k.shape != (b, hkv, m, d):
+        raise ValueError(f"{what}: k_prefix {tuple(k_prefix.shape)} / k {tuple(k.shape)} do not match q {tuple(q.shape)}")
+    q, k_prefix, v_prefix, k, v = (_last_contig(x) for x in (q, k_prefix, v_prefix, k, v))
+    dev = q.device
+    lens_ptr = None
+    if lengths is not None:
+        if lengths.dtype != torch.int32 or lengths.device != dev or not lengths.is_contiguous():
+            lengths = lengths.to(device=dev, dtype=torch.int32).contiguous()
+        if lengths.shape != (b,):
+            raise ValueError(f"{what}: lengths must be [{b}]")
+        lens_ptr = lengths.data_ptr()
+    code = dtype_code(q, what)
+    out = torch.empty((b, hkv, g, d), dtype=q.dtype, device=dev)
+    L = lib()
+    with torch.cuda.device(dev):
+        nb = L.tc_decode_attention_shared_workspace_size(b, hkv, g, d, n, m, code)
+        ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
+        st = L.tc_decode_attention_shared(
+            q.data_ptr(), k_prefix.data_ptr(), v_prefix.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), b, hkv,
+            g, d, n, m, lens_ptr, *q.stride()[:3], *k_prefix.stride()[:2], *v_prefix.stride()[:2], *k.stride()[:3],
+            *v.stride()[:3], *out.stride()[:3], float(scale), code, ws.data_ptr() if ws is not None else None, nb,
+            stream_ptr(dev))
+    check("tc_decode_attention_shared", st)
+    return out
 
 
 class RaggedKV:

@@ -10,9 +10,9 @@ whether the kernel takes the inputs; the plugin keeps torch SDPA for everything 
 import torch
 
 from . import _lib
-from ._lib import check, lib, require_cuda, stream_ptr, workspaces
+from ._lib import check, dtype_code, lib, require_cuda, stream_ptr, workspaces
 
-__all__ = ["prefill_attention", "supported", "causal_offset_mask"]
+__all__ = ["prefill_attention", "prefill_attention_window", "supported", "causal_offset_mask"]
 
 
 def supported(query, key, value):
@@ -56,4 +56,42 @@ def prefill_attention(query, key, value, scale, *, splits=None):
             k.stride(0), k.stride(1), v.stride(0), v.stride(1), out.stride(1), out.stride(2), float(scale), s,
             _lib.DTYPE_CODE[query.dtype], ws.data_ptr() if ws is not None else None, nb, stream_ptr(query.device))
     check(what, st)
+    return out
+
+
+def prefill_attention_window(query, key, value, scale, window, sinks=0, *, splits=None):
+    """Causal attention of a chunk over the cache that ends with it, with a sliding window and sinks: query
+    [b, hq, lq, d], key/value [b, hkv, lk, d] (hq a multiple of hkv, d <= 256, any dtype of the package).
+    Query position p sees the keys j <= lk - lq + p with j < sinks or j > lk - lq + p - window (window >= 1
+    counts the query's own token). Returns [b, lq, hq, d] contiguous."""
+    what = "prefill_attention_window"
+    require_cuda(query, key, value, what=what)
+    if query.dim() != 4 or key.dim() != 4 or value.shape != key.shape:
+        raise ValueError(f"{what}: expected query [b, hq, lq, d], key/value [b, hkv, lk, d]; got {tuple(query.shape)}, "
+                         f"{tuple(key.shape)}, {tuple(value.shape)}")
+    b, hq, lq, d = query.shape
+    hkv, lk = key.shape[1], key.shape[2]
+    if key.shape[0] != b or key.shape[3] != d or hkv < 1 or hq % hkv or not 1 <= lq <= lk:
+        raise ValueError(f"{what}: key {tuple(key.shape)} does not fit query {tuple(query.shape)} (1 <= lq <= lk, hq a "
+                         "multiple of hkv)")
+    if key.dtype != query.dtype or value.dtype != query.dtype:
+        raise TypeError(f"threadcut_b200.{what}: dtype mismatch {query.dtype} vs {key.dtype}/{value.dtype}")
+    window, sinks = int(window), int(sinks)
+    if window < 1 or sinks < 0:
+        raise ValueError(f"{what}: needs window >= 1 and sinks >= 0, got {window} and {sinks}")
+    window, sinks = min(window, lk), min(sinks, lk)
+    code = dtype_code(query, what)
+    q, k, v = (x if x.stride(-1) == 1 else x.contiguous() for x in (query, key, value))
+    dev = query.device
+    out = torch.empty((b, lq, hq, d), dtype=query.dtype, device=dev)
+    L = lib()
+    s = int(splits or 0)
+    with torch.cuda.device(dev):
+        nb = L.tc_prefill_window_workspace_size(b, hq, hkv, lq, lk, d, window, sinks, s)
+        ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
+        st = L.tc_prefill_attention_window(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), b, hq, hkv, lq, lk, d, window, sinks,
+            *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3], float(scale), s, code,
+            ws.data_ptr() if ws is not None else None, nb, stream_ptr(dev))
+    check("tc_prefill_attention_window", st)
     return out
