@@ -26,6 +26,11 @@
 //                      exceeds it by 2^8, so O_x is rescaled in TMEM (tcgen05.ld/st) only on jumps.
 //                      The epilogue divides by l and stores (or, with KV splits, writes fp32
 //                      partials and the natural-log LSE for a merge).
+// kWindow (a sliding window with sinks) is the same pipeline over another list of key tiles: those holding
+// sinks, then those from the first key that the block's first query sees. Its geometry is the caller's:
+// any g <= 128 query heads per KV head (a Q tile is g heads x floor(128 / g) positions; rows past them are
+// dead), d of 64 or 128, a batch. A tile in which some row hides some key is masked key by key; a tile
+// fully visible to the Q tile costs the compare of its two ends.
 // TMEM: 512 columns — S_0 | S_1 | O_0 | O_1. mbarriers order the roles (q_full, kv_full/kv_empty per
 // stage, s_full/p_full/o_full per Q tile); every wait is bounded, a failed wait makes all roles
 // skip to the end, and the MMA lane's final commit is waited for before TMEM is freed.
@@ -46,15 +51,15 @@ constexpr int kPfThreads = 384;   // warps 0-3 / 4-7 softmax of Q tile 0 / 1, 8 
 constexpr int kPfRegsSoftmax = 232;
 constexpr int kPfRegsOther = 40;
 constexpr int kPfGroup = 4;       // query heads per KV head handled by the kernel
-constexpr int kPfSmem = 1024 + kPfTiles * 32768 + 2 * 65536;  // alignment slack, Q tiles, 2 K/V stages
+constexpr int pf_smem(int d) { return 1024 + (kPfTiles + 4) * 256 * d; }  // alignment slack, Q tiles, 2 K/V stages
 constexpr uint32_t kPfSpin = 1u << 20;  // mbarrier polls before a wait gives up (about a second)
 // A row keeps its running max until a tile's max exceeds it by more than this (log2 units): P stays
 // below 2^8 (exact enough in 16 bits) and O is rescaled in TMEM only on such jumps.
 constexpr float kPfLazyMax = 8.f;
 
 struct PrefillParams {
-  CUtensorMap tmq;  // (d, lq, hq, 1), box (64, 32, 4, 1)
-  CUtensorMap tmk;  // (d, lk, hkv, 1), box (64, 128, 1, 1)
+  CUtensorMap tmq;  // (d, lq, hq, batch), box (64, 32, 4, 1), with a window (64, 128 / g, g, 1)
+  CUtensorMap tmk;  // (d, lk, hkv, batch), box (64, 128, 1, 1)
   CUtensorMap tmv;
   void* out;        // element (p, head, dim) at p*so_p + head*so_h + dim
   int64_t so_p, so_h;
@@ -72,18 +77,26 @@ struct PrefillParams {
   int n_sub;
   int oob_page;
   const int32_t* qb_tiles;
+  // window: query p sees key j iff j <= off + p and (j < sinks or j > off + p - window). pq = 128 / g
+  // positions per Q tile. Paged: qb_tiles[2 qb] is the tile of the block's first window key and
+  // qb_tiles[2 qb + 1] the end; sink_tiles tiles hold the sinks.
+  int window, sinks, sink_tiles;
+  int g, pq;
+  int64_t so_b;     // out and the split partials of sequence b: rows from b*lq*hq on
 };
 
 // TMEM columns (fp32 words) of Q tile x: S (and P over its first 64 columns), then O.
 __device__ __forceinline__ uint32_t pf_col_s(int x) { return (uint32_t)(x * 128); }
 __device__ __forceinline__ uint32_t pf_col_o(int x) { return (uint32_t)(256 + x * 128); }
 
-template <typename T, bool kPaged>
+template <typename T, int D, bool kPaged, bool kWindow>
 __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const __grid_constant__ PrefillParams p) {
+  constexpr int kTileB = 256 * D;            // one Q, K or V tile: D/64 boxes x 128 rows x 128 B
+  constexpr int kBoxes = D / 64;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
-  uint8_t* sQ = smem;                        // Q tile x at +32768*x: 2 boxes x 128 rows x 128 B
-  uint8_t* sKV = smem + kPfTiles * 32768;    // stage s: K at +65536*s, V at +65536*s + 32768
+  uint8_t* sQ = smem;                        // Q tile x at +kTileB*x
+  uint8_t* sKV = smem + kPfTiles * kTileB;   // stage s: K at +2*kTileB*s, V at +2*kTileB*s + kTileB
   __shared__ __align__(8) uint64_t q_full, kv_full[2], kv_empty[2], s_full[kPfTiles], p_full[kPfTiles],
       o_full[kPfTiles], fin;
   __shared__ uint32_t s_tmem;
@@ -92,12 +105,24 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const __grid_con
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // heaviest causal Q blocks first (blocks are dispatched in blockIdx.x order): longest-first
   // scheduling shortens the tail when the grid is more than one wave
-  const int qb = gridDim.x - 1 - blockIdx.x, h = blockIdx.y, split = blockIdx.z;
-  const int p0 = qb * kPfQ * kPfTiles;  // first position of Q tile 0; tile x starts at p0 + 32x
+  const int qb = gridDim.x - 1 - blockIdx.x, split = blockIdx.z;
+  const int b = kWindow ? blockIdx.y / p.hkv : 0, h = kWindow ? blockIdx.y % p.hkv : blockIdx.y;
+  const int group = kWindow ? p.g : kPfGroup;  // query heads per KV head
+  const int pq = kWindow ? p.pq : kPfQ;        // positions per Q tile
+  const int p0 = qb * pq * kPfTiles;    // first position of Q tile 0; tile x starts at p0 + pq*x
   const int off = p.lk - p.lq;          // key j is visible to position pos iff j <= off + pos
-  const int kend = p.lk < off + p0 + kPfQ * kPfTiles ? p.lk : off + p0 + kPfQ * kPfTiles;
-  // >= 1: key 0 is visible to every position
-  const int ntot = kPaged ? p.qb_tiles[qb] : (kend + kPfKeys - 1) / kPfKeys;
+  const int kend = p.lk < off + p0 + pq * kPfTiles ? p.lk : off + p0 + pq * kPfTiles;
+  // window: tile t of the list is key tile t for the first sink_tiles, then key tile t + skip
+  int sink_tiles = 0, skip = 0;
+  if constexpr (kWindow) {
+    const int first = off + p0 + 1 - p.window;  // the block's first window key
+    const int wt = kPaged ? p.qb_tiles[2 * qb] : (first > 0 ? first / kPfKeys : 0);
+    sink_tiles = p.sink_tiles < wt ? p.sink_tiles : wt;
+    skip = wt - sink_tiles;
+  }
+  // >= 1: key 0 is visible to every position (window: the block's first query sees its own token)
+  const int ntot = (kPaged ? p.qb_tiles[kWindow ? 2 * qb + 1 : qb] : (kend + kPfKeys - 1) / kPfKeys) - skip;
+  auto key_tile = [&](int t) { return kWindow && t >= sink_tiles ? t + skip : t; };
   const int t_lo = (int)((int64_t)ntot * split / p.nsplit);
   const int ntile = (int)((int64_t)ntot * (split + 1) / p.nsplit) - t_lo;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
@@ -133,16 +158,16 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const __grid_con
       prefetch_tensormap(&p.tmq);
       prefetch_tensormap(&p.tmk);
       prefetch_tensormap(&p.tmv);
-      mbar_arrive_expect_tx(&q_full, (uint32_t)(kPfTiles * 32768));
+      mbar_arrive_expect_tx(&q_full, (uint32_t)(kPfTiles * kBoxes * 128 * (kWindow ? group * pq : 128)));
       for (int x = 0; x < kPfTiles; ++x)
-        for (int bx = 0; bx < 2; ++bx)
-          tma_load_4d(sQ + x * 32768 + bx * 16384, &p.tmq, bx * 64, p0 + kPfQ * x, h * kPfGroup, 0, &q_full, pol);
+        for (int bx = 0; bx < kBoxes; ++bx)
+          tma_load_4d(sQ + x * kTileB + bx * 16384, &p.tmq, bx * 64, p0 + pq * x, h * group, b, &q_full, pol);
       int armed = 0;  // K/V tiles whose copies were issued
       int4 nxt[4];      // paged: the next tile's sub-tile entries, read one tile ahead
       auto fetch = [&](int j) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          const int si = 4 * (t_lo + j) + c;
+          const int si = 4 * key_tile(t_lo + j) + c;
           nxt[c] = si < p.n_sub ? p.ktab[si] : make_int4(p.oob_page, 0, 0, 0);
         }
       };
@@ -160,22 +185,23 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const __grid_con
           s_abort = 1;
           break;
         }
-        mbar_arrive_expect_tx(&kv_full[s], 65536u);
-        uint8_t* st = sKV + s * 65536;
+        mbar_arrive_expect_tx(&kv_full[s], (uint32_t)(2 * kTileB));
+        uint8_t* st = sKV + s * 2 * kTileB;
         if constexpr (kPaged) {
           // four 32-row boxes per 64 columns, at row offsets 0/32/64/96 of the 128-row swizzled tile
           // (the 128-byte swizzle repeats every 8 rows, so the tile image is the contiguous one)
 #pragma unroll
           for (int c = 0; c < 4; ++c)
-            for (int bx = 0; bx < 2; ++bx) {
+            for (int bx = 0; bx < kBoxes; ++bx) {
               tma_load_4d(st + bx * 16384 + c * 4096, &p.tmk, bx * 64, cur[c].y, h, cur[c].x, &kv_full[s], pol);
-              tma_load_4d(st + 32768 + bx * 16384 + c * 4096, &p.tmv, bx * 64, cur[c].y, h, cur[c].x, &kv_full[s],
+              tma_load_4d(st + kTileB + bx * 16384 + c * 4096, &p.tmv, bx * 64, cur[c].y, h, cur[c].x, &kv_full[s],
                           pol);
             }
         } else {
-          for (int bx = 0; bx < 2; ++bx) {
-            tma_load_4d(st + bx * 16384, &p.tmk, bx * 64, (t_lo + j) * kPfKeys, h, 0, &kv_full[s], pol);
-            tma_load_4d(st + 32768 + bx * 16384, &p.tmv, bx * 64, (t_lo + j) * kPfKeys, h, 0, &kv_full[s], pol);
+          const int key = key_tile(t_lo + j) * kPfKeys;
+          for (int bx = 0; bx < kBoxes; ++bx) {
+            tma_load_4d(st + bx * 16384, &p.tmk, bx * 64, key, h, b, &kv_full[s], pol);
+            tma_load_4d(st + kTileB + bx * 16384, &p.tmv, bx * 64, key, h, b, &kv_full[s], pol);
           }
         }
         armed = j + 1;
@@ -190,17 +216,17 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const __grid_con
     // ---------------- tcgen05.mma issue: per K/V tile S_0, S_1, P V_0, P V_1
     if (lane == 0) {
       const uint32_t idS = umma_idesc_f16(kBf16, false, 128, 128);
-      const uint32_t idO = umma_idesc_f16(kBf16, true, 128, 128);
-      auto issue_s = [&](int x, int j) {  // S_x = Q_x K_j^T over d in 8 steps of 16
-        const uint32_t q0 = smem_u32(sQ + x * 32768), k0 = smem_u32(sKV + (j & 1) * 65536);
-        for (int kd = 0; kd < 8; ++kd) {
+      const uint32_t idO = umma_idesc_f16(kBf16, true, 128, D);
+      auto issue_s = [&](int x, int j) {  // S_x = Q_x K_j^T over d in steps of 16
+        const uint32_t q0 = smem_u32(sQ + x * kTileB), k0 = smem_u32(sKV + (j & 1) * 2 * kTileB);
+        for (int kd = 0; kd < D / 16; ++kd) {
           const uint32_t o = (uint32_t)((kd >> 2) * 16384 + (kd & 3) * 32);
           umma_f16(tmem + pf_col_s(x), umma_desc_sw128(q0 + o, 16, 1024), umma_desc_sw128(k0 + o, 16, 1024), idS,
                    kd > 0);
         }
       };
       auto issue_pv = [&](int x, int j) {  // O_x (+)= P_x V_j, P_x from TMEM (8 columns per 16 keys)
-        const uint32_t v0 = smem_u32(sKV + (j & 1) * 65536 + 32768);
+        const uint32_t v0 = smem_u32(sKV + (j & 1) * 2 * kTileB + kTileB);
         for (int kk = 0; kk < 8; ++kk)
           umma_f16_tmem_a(tmem + pf_col_o(x), tmem + pf_col_s(x) + (uint32_t)(kk * 8),
                           umma_desc_sw128(v0 + kk * 2048, 16384, 1024), idO, j > 0 || kk > 0);
@@ -237,12 +263,16 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const __grid_con
     }
   } else if (warp < 8) {
     // ---------------- softmax: Q tile x = warp / 4; thread = TMEM lane (warp % 4)*32 + lane = row
-    // (query head h*4 + warp % 4, position p0 + 32x + lane)
+    // (query head h*4 + warp % 4, position p0 + 32x + lane; window: head row / pq, position row % pq)
     reg_alloc<kPfRegsSoftmax>();
     const int x = warp >> 2, wq = warp & 3;
-    const int pos = p0 + kPfQ * x + lane;
-    const int limit = off + pos;                 // last visible key of this row
-    const int limit_min = off + p0 + kPfQ * x;   // smallest limit in this Q tile
+    const int head_i = kWindow ? (wq * 32 + lane) / pq : wq;  // >= group: a dead row
+    const int pos = p0 + pq * x + (kWindow ? (wq * 32 + lane) - head_i * pq : lane);
+    const bool live = pos < p.lq && (!kWindow || head_i < group);
+    const int limit = off + pos;               // last visible key of this row
+    const int limit_min = off + p0 + pq * x;   // smallest limit in this Q tile
+    const int lo = kWindow ? limit - p.window + 1 : 0;                  // first window key of this row
+    const int lo_max = kWindow ? limit_min + pq - p.window : 0;         // largest lo in this Q tile
     const uint32_t lb = (uint32_t)(wq * 32) << 16;
     const uint32_t tS = tmem + pf_col_s(x), tO = tmem + pf_col_o(x);
     float m = -INFINITY, l = 0.f;
@@ -252,7 +282,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const __grid_con
       if constexpr (kPaged) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          const int si = 4 * (t_lo + j) + c;
+          const int si = 4 * key_tile(t_lo + j) + c;
           te[c] = si < p.n_sub ? p.ktab[si] : make_int4(0, 0, 0, 0);
         }
       }
@@ -265,29 +295,35 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const __grid_con
       for (int cch = 0; cch < 4; ++cch) tmem_ld32(tS + lb + cch * 32, v[cch]);
       tmem_wait_ld();
       // raw scores, masked (-inf) past this row's last visible key; row max over 8 partial chains
-      const int ja = t_lo + j;
+      const int key0 = key_tile(t_lo + j) * kPfKeys;
       float mx[8];
 #pragma unroll
       for (int r = 0; r < 8; ++r) mx[r] = -INFINITY;
       if constexpr (kPaged) {
         // chunk c of the row is sub-tile c: slot e holds logical key te[c].w + e if e < te[c].z
         const bool full = te[0].z == 32 && te[1].z == 32 && te[2].z == 32 && te[3].z == 32 &&
-                          te[3].w + 31 <= limit_min;
+                          te[3].w + 31 <= limit_min &&
+                          (!kWindow || te[0].w >= lo_max || te[3].w + 31 < p.sinks);
         if (!full) {
 #pragma unroll
           for (int cch = 0; cch < 4; ++cch)
 #pragma unroll
             for (int e = 0; e < 32; ++e)
-              if (e >= te[cch].z || te[cch].w + e > limit) v[cch][e] = __float_as_uint(-INFINITY);
+              if (e >= te[cch].z || te[cch].w + e > limit ||
+                  (kWindow && te[cch].w + e < lo && te[cch].w + e >= p.sinks))
+                v[cch][e] = __float_as_uint(-INFINITY);
         }
       } else {
-        const bool masked_tile = (ja + 1) * kPfKeys - 1 > limit_min;
+        const bool masked_tile = key0 + kPfKeys - 1 > limit_min ||
+                                 (kWindow && key0 < lo_max && key0 + kPfKeys - 1 >= p.sinks);
         if (masked_tile) {
 #pragma unroll
           for (int cch = 0; cch < 4; ++cch)
 #pragma unroll
             for (int e = 0; e < 32; ++e)
-              if (ja * kPfKeys + cch * 32 + e > limit) v[cch][e] = __float_as_uint(-INFINITY);
+              if (key0 + cch * 32 + e > limit ||
+                  (kWindow && key0 + cch * 32 + e < lo && key0 + cch * 32 + e >= p.sinks))
+                v[cch][e] = __float_as_uint(-INFINITY);
         }
       }
 #pragma unroll
@@ -329,7 +365,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const __grid_con
       // s_full's commit covers P V of tile j-1 (issued before S of tile j), so O is current here
       if (j >= 1 && __any_sync(0xffffffffu, alpha != 1.f)) {
 #pragma unroll
-        for (int cch = 0; cch < 4; ++cch) {
+        for (int cch = 0; cch < D / 32; ++cch) {
           uint32_t o[32];
           tmem_ld32(tO + lb + cch * 32, o);
           tmem_wait_ld();
@@ -350,14 +386,14 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const __grid_con
     } else {
       if (ntile > 0) tmem_fence_after();
       const float inv = l > 0.f ? 1.f / l : 0.f;
-      const int head = h * kPfGroup + wq;
+      const int head = h * group + head_i;
       if (p.nsplit > 1) {
         // normalised fp32 partial + natural-log LSE (an empty split: zeros and -inf)
-        const int64_t row = (int64_t)pos * p.hq + head;
-        const int64_t rows = (int64_t)p.lq * p.hq;
-        float* orow = p.o_part + ((int64_t)split * rows + row) * 128;
+        const int64_t row = ((int64_t)b * p.lq + pos) * p.hq + head;
+        const int64_t rows = (int64_t)p.lq * p.hq * (kWindow ? gridDim.y / p.hkv : 1);
+        float* orow = p.o_part + ((int64_t)split * rows + row) * D;
 #pragma unroll
-        for (int cch = 0; cch < 4; ++cch) {
+        for (int cch = 0; cch < D / 32; ++cch) {
           uint32_t o[32];
           if (ntile > 0) {
             tmem_ld32(tO + lb + cch * 32, o);
@@ -366,7 +402,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const __grid_con
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] = 0u;
           }
-          if (pos < p.lq) {
+          if (live) {
 #pragma unroll
             for (int q4 = 0; q4 < 8; ++q4)
               *reinterpret_cast<float4*>(orow + cch * 32 + q4 * 4) =
@@ -374,16 +410,16 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const __grid_con
                               __uint_as_float(o[4 * q4 + 2]) * inv, __uint_as_float(o[4 * q4 + 3]) * inv);
           }
         }
-        if (pos < p.lq)
+        if (live)
           p.lse_part[(int64_t)split * rows + row] = l > 0.f ? (m + __log2f(l)) * 0.6931471805599453f : -INFINITY;
       } else {
-        T* orow = static_cast<T*>(p.out) + (int64_t)pos * p.so_p + (int64_t)head * p.so_h;
+        T* orow = static_cast<T*>(p.out) + b * p.so_b + (int64_t)pos * p.so_p + (int64_t)head * p.so_h;
 #pragma unroll
-        for (int cch = 0; cch < 4; ++cch) {
+        for (int cch = 0; cch < D / 32; ++cch) {
           uint32_t o[32];
           tmem_ld32(tO + lb + cch * 32, o);
           tmem_wait_ld();
-          if (pos < p.lq) {
+          if (live) {
 #pragma unroll
             for (int q4 = 0; q4 < 4; ++q4) {
               uint4 w;

@@ -120,6 +120,19 @@ bool encode_map4(CUtensorMap* m, const void* base, int dtype, const int64_t (&di
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// encode_map4 of a tensor as a caller gave it: the stride of an extent of 1 carries nothing and gets a
+// harmless value.
+bool encode_view4(CUtensorMap* m, const void* base, int dtype, const int64_t (&dims)[4], int64_t s1, int64_t s2,
+                  int64_t s3, const uint32_t (&box)[4]) {
+  int64_t st[3] = {s1, s2, s3};
+  int64_t next = (dims[0] + 7) / 8 * 8;
+  for (int i = 0; i < 3; ++i) {
+    if (dims[i + 1] == 1) st[i] = next;
+    next = st[i] * dims[i + 1];
+  }
+  return encode_map4(m, base, dtype, dims, st, box);
+}
+
 // ------------------------------------------------------------------------------- decode planning
 struct DecodePlan {
   int64_t tps = 1;         // tiles per split
@@ -1328,11 +1341,12 @@ size_t tc_prefill_workspace_size(int hq, int hkv, int lq, int lk, int splits) {
 }  // extern "C"
 
 namespace {
-template <typename T, bool kPaged>
+template <typename T, bool kPaged, int D = 128, bool kWindow = false>
 cudaError_t launch_prefill_t(const PrefillParams& p, dim3 grid, int dev, cudaStream_t s) {
-  const cudaError_t e = set_smem(reinterpret_cast<const void*>(prefill_kernel<T, kPaged>), kPfSmem, dev);
+  const auto fn = prefill_kernel<T, D, kPaged, kWindow>;
+  const cudaError_t e = set_smem(reinterpret_cast<const void*>(fn), pf_smem(D), dev);
   if (e != cudaSuccess) return e;
-  prefill_kernel<T, kPaged><<<grid, kPfThreads, kPfSmem, s>>>(p);
+  fn<<<grid, kPfThreads, pf_smem(D), s>>>(p);
   return cudaGetLastError();
 }
 
@@ -1948,12 +1962,89 @@ int launch_rows(const RowsParams& p, int dtype, cudaStream_t st) {
 bool finite_scale(float s) { return s == s && s != INFINITY && s != -INFINITY; }
 }  // namespace
 
+namespace {
+// The tcgen05 windowed prefill: its geometry and its plan.
+struct WindowPrefill {
+  bool use = false;
+  int pq = 0;      // positions per Q tile
+  int blocks = 0;  // query blocks of kPfTiles tiles
+  int splits = 1;
+};
+
+// `tiles`: key tiles that the busiest query block visits.
+int window_splits(int64_t ctas, int64_t tiles, int sms) {
+  if (ctas >= 2 * (int64_t)sms) return 1;
+  int best = 1;
+  double best_eff = 0.0;
+  for (int s = 1; s <= 16 && (s == 1 || tiles / s >= 4); ++s) {
+    const int64_t waves = cdiv(ctas * s, sms);
+    const double eff = (double)(ctas * s) / (double)(waves * sms);
+    if (eff >= 0.95) return s;
+    if (eff > best_eff + 0.02) {
+      best_eff = eff;
+      best = s;
+    }
+  }
+  return best;
+}
+
+WindowPrefill plan_window_prefill(int batch, int hq, int hkv, int lq, int lk, int d, int64_t window, int64_t sinks,
+                                  int splits_req) {
+  WindowPrefill w;
+  const int g = hq / hkv;
+  w.use = (d == 64 || d == 128) && g <= 128 && (int64_t)batch * hkv <= 65535;
+  if (!w.use) return w;
+  w.pq = 128 / g;
+  w.blocks = (int)cdiv(lq, kPfTiles * w.pq);
+  const int64_t span = window + kPfTiles * w.pq < lk ? window + kPfTiles * w.pq : lk;
+  int64_t tiles = cdiv(span, kPfKeys) + 1 + cdiv(sinks, kPfKeys);
+  if (tiles > cdiv(lk, kPfKeys)) tiles = cdiv(lk, kPfKeys);
+  w.splits = splits_req > 0 ? (splits_req > 16 ? 16 : splits_req)
+                            : window_splits((int64_t)w.blocks * hkv * batch, tiles, sm_count(current_device()));
+  return w;
+}
+
+template <typename T>
+cudaError_t launch_window_prefill_t(const PrefillParams& p, int d, bool paged, dim3 grid, int dev, cudaStream_t s) {
+  if (d == 64)
+    return paged ? launch_prefill_t<T, true, 64, true>(p, grid, dev, s) : launch_prefill_t<T, false, 64, true>(p, grid, dev, s);
+  return paged ? launch_prefill_t<T, true, 128, true>(p, grid, dev, s) : launch_prefill_t<T, false, 128, true>(p, grid, dev, s);
+}
+
+// Partials of `splits` KV splits: fp32 rows of d, then their log-sum-exps.
+size_t window_ws_bytes(int64_t rows, int d, int splits) {
+  return splits <= 1 ? 0 : sizeof(float) * (size_t)splits * (size_t)rows * (size_t)(d + 1);
+}
+
+// p: maps, tables and strides set; runs the kernel and, with splits, the merge.
+int run_window_prefill(PrefillParams& p, const WindowPrefill& w, int batch, int d, bool paged, int dtype,
+                       void* workspace, cudaStream_t st) {
+  const int64_t rows = (int64_t)batch * p.lq * p.hq;
+  p.pq = w.pq;
+  p.g = p.hq / p.hkv;
+  p.nsplit = w.splits;
+  if (w.splits > 1) {
+    p.o_part = static_cast<float*>(workspace);
+    p.lse_part = p.o_part + (size_t)w.splits * rows * d;
+  }
+  const int dev = current_device();
+  const dim3 grid((unsigned)w.blocks, (unsigned)(batch * p.hkv), (unsigned)w.splits);
+  const cudaError_t e = dtype == TC_BF16 ? launch_window_prefill_t<__nv_bfloat16>(p, d, paged, grid, dev, st)
+                                         : launch_window_prefill_t<__half>(p, d, paged, grid, dev, st);
+  if (e != cudaSuccess) return TC_ERR_CUDA;
+  if (w.splits > 1) return tc_merge_partials(p.o_part, p.lse_part, p.out, nullptr, w.splits, rows, d, d, dtype, st);
+  return TC_OK;
+}
+}  // namespace
+
 extern "C" {
 
 size_t tc_prefill_window_workspace_size(int batch, int hq, int hkv, int lq, int lk, int d, int64_t window,
                                         int64_t sinks, int splits) {
-  (void)batch, (void)hq, (void)hkv, (void)lq, (void)lk, (void)d, (void)window, (void)sinks, (void)splits;
-  return 0;
+  if (batch < 1 || hkv < 1 || hq < hkv || hq % hkv != 0 || lq < 1 || lk < lq || d < 1 || window < 1 || sinks < 0)
+    return 0;
+  const WindowPrefill w = plan_window_prefill(batch, hq, hkv, lq, lk, d, window, sinks, splits);
+  return window_ws_bytes((int64_t)batch * lq * hq, d, w.splits);
 }
 
 int tc_prefill_attention_window(const void* q, const void* k, const void* v, void* out, int batch, int hq, int hkv,
@@ -1967,7 +2058,44 @@ int tc_prefill_attention_window(const void* q, const void* k, const void* v, voi
       lk < lq || d < 1 || d > kRowsMaxDim || window < 1 || sinks < 0 || splits < 0 || q == nullptr || k == nullptr ||
       v == nullptr || out == nullptr || !finite_scale(scale))
     return TC_ERR_INVALID;
-  (void)workspace, (void)workspace_bytes;
+  window = window < lk ? window : lk;
+  sinks = sinks < lk ? sinks : lk;
+  WindowPrefill w = plan_window_prefill(batch, hq, hkv, lq, lk, d, window, sinks, splits);
+  const int64_t strides[12] = {q_stride_b, q_stride_h, q_stride_p, k_stride_b, k_stride_h, k_stride_n,
+                               v_stride_b, v_stride_h, v_stride_n, out_stride_b, out_stride_p, out_stride_h};
+  // the kernel takes its row maximum before the scale, so the scale must keep the order
+  bool tc5 = w.use && lk <= (1 << 30) && dtype != TC_F32 && scale > 0.f && aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out);
+  for (int64_t x : strides) tc5 = tc5 && stride16(x, dtype);
+  if (tc5) {
+    PrefillParams p;
+    std::memset(&p, 0, sizeof(p));
+    const int g = hq / hkv;
+    const int64_t qd[4] = {d, lq, hq, batch}, kd[4] = {d, lk, hkv, batch};
+    const uint32_t qbox[4] = {64, (uint32_t)w.pq, (uint32_t)g, 1}, kbox[4] = {64, (uint32_t)kPfKeys, 1, 1};
+    if (encode_view4(&p.tmq, q, dtype, qd, q_stride_p, q_stride_h, q_stride_b, qbox) &&
+        encode_view4(&p.tmk, k, dtype, kd, k_stride_n, k_stride_h, k_stride_b, kbox) &&
+        encode_view4(&p.tmv, v, dtype, kd, v_stride_n, v_stride_h, v_stride_b, kbox)) {
+      // split partials are merged into rows of d contiguous elements: needs the [batch, lq, hq, d] layout
+      if (out_stride_h != d || out_stride_p != (int64_t)hq * d || (batch > 1 && out_stride_b != (int64_t)lq * hq * d))
+        w.splits = 1;
+      if (w.splits > 1 && (workspace == nullptr || !aligned16(workspace) ||
+                           workspace_bytes < window_ws_bytes((int64_t)batch * lq * hq, d, w.splits)))
+        return TC_ERR_WORKSPACE;
+      p.out = out;
+      p.so_b = out_stride_b;
+      p.so_p = out_stride_p;
+      p.so_h = out_stride_h;
+      p.lq = lq;
+      p.lk = lk;
+      p.hq = hq;
+      p.hkv = hkv;
+      p.c = scale * kLog2e;
+      p.window = (int)window;
+      p.sinks = (int)sinks;
+      p.sink_tiles = (int)cdiv(sinks, kPfKeys);
+      return run_window_prefill(p, w, batch, d, false, dtype, workspace, static_cast<cudaStream_t>(stream));
+    }
+  }
   RowsParams p;
   std::memset(&p, 0, sizeof(p));
   p.q = q;
@@ -1993,8 +2121,8 @@ int tc_prefill_attention_window(const void* q, const void* k, const void* v, voi
   p.g = hq / hkv;
   p.d = d;
   p.lq = lq;
-  p.window = window < lk ? window : lk;
-  p.sinks = sinks < lk ? sinks : lk;
+  p.window = window;
+  p.sinks = sinks;
   p.lk = lk;
   p.c = scale * kLog2e;
   return launch_rows(p, dtype, static_cast<cudaStream_t>(stream));
