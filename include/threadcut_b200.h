@@ -232,6 +232,21 @@ int tc_decode_attention_shared(const void* q, const void* k_prefix, const void* 
                                int64_t out_stride_g, float scale, int dtype, void* workspace, size_t workspace_bytes,
                                void* stream);
 
+/* tc_decode_attention_shared with the prefix in a paged cache: the rows that the tile table lists, in any
+ * order (pools, strides and tables as for tc_decode_attention_paged; an entry outside the pool counts as
+ * empty; rows of a listed page behind an entry may hold anything). 16-bit, d in {64, 128, 256},
+ * page_rows >= 32, scale > 0, 16-byte aligned bases and strides. Workspace of
+ * tc_decode_attention_shared_workspace_size(batch, hkv, g, d, 32 * n_tiles, m, dtype) bytes. */
+int tc_decode_attention_shared_paged(const void* q, const void* k_pool, const void* v_pool, const void* k, const void* v,
+                                     void* out, int batch, int hkv, int g, int d, int64_t page_rows, int64_t num_pages,
+                                     int64_t pool_stride_page, int64_t pool_stride_h, int64_t pool_stride_row,
+                                     const int32_t* tiles, int64_t n_tiles, int64_t m, const int32_t* lengths,
+                                     int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_g, int64_t k_stride_b,
+                                     int64_t k_stride_h, int64_t k_stride_n, int64_t v_stride_b, int64_t v_stride_h,
+                                     int64_t v_stride_n, int64_t out_stride_b, int64_t out_stride_h,
+                                     int64_t out_stride_g, float scale, int dtype, void* workspace,
+                                     size_t workspace_bytes, void* stream);
+
 /* Decode attention that allocates nothing, for callers that cannot hand us device memory: for
  * example a plugin running inside another runtime that owns every device allocation and forbids
  * allocating in its execute hook, a loop where the implicit synchronisation of cudaMalloc is not

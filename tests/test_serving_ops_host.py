@@ -87,3 +87,18 @@ def shared_status(q=P, kp=P, vp=P, k=P, v=P, out=P, b=2, hkv=2, g=4, d=128, n=10
     (dict(scale=float("nan")), 1), (dict(scale=float("-inf")), 1)])
 def test_shared_decode_refuses(bad, status):
     assert shared_status(**bad) == status
+
+
+def shared_paged_status(q=P, kp=P, vp=P, k=P, v=P, out=P, b=2, hkv=2, g=4, d=128, rows=64, pages=4, page_stride=64, tiles=P,
+                        nt=3, m=10, scale=0.1, dtype=2, ws=N, nb=0, qs=128):
+    return _lib.lib().tc_decode_attention_shared_paged(q, kp, vp, k, v, out, b, hkv, g, d, rows, pages, page_stride, 64, 64,
+                                                       tiles, nt, m, N, qs, *[128] * 11, scale, dtype, ws, nb, N)
+
+
+@pytest.mark.parametrize("bad,status", [
+    (dict(dtype=0), 3), (dict(b=0), 1), (dict(hkv=0), 1), (dict(g=0), 1), (dict(g=129), 1), (dict(d=96), 1),
+    (dict(rows=31), 1), (dict(pages=0), 1), (dict(tiles=N), 1), (dict(nt=-1), 1), (dict(m=-1), 1), (dict(q=N), 1),
+    (dict(out=N), 1), (dict(kp=N), 1), (dict(vp=N), 1), (dict(k=N), 1), (dict(v=N), 1), (dict(scale=0.0), 1),
+    (dict(scale=float("nan")), 1), (dict(page_stride=65), 2), (dict(qs=127), 2), (dict(q=ctypes.c_void_p(8)), 2)])
+def test_shared_paged_decode_refuses(bad, status):
+    assert shared_paged_status(**bad) == status

@@ -6,6 +6,8 @@ import torch
 from attn_bounds import assert_within, attend64
 from threadcut_b200 import _lib
 from threadcut_b200.flash_decode import decode_attention_batched, decode_attention_shared
+from threadcut_b200.match import Split
+from threadcut_b200.paged import PagedKV
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -197,7 +199,77 @@ def test_new_lengths_reach_a_replayed_graph():
         assert_within(out, *reference(q, kp, vp, k, v, 0.1, torch.tensor([a, c])))
 
 
+def paged_prefix(hkv, d, dtype, page_rows, gen, pieces, splice=None):
+    kv = PagedKV(2, hkv, d, max_tokens=sum(pieces) + 500, page_rows=page_rows, dtype=dtype, device=DEV)
+    for t in pieces:
+        kv.reserve(t)
+        for layer in range(2):
+            kv.write(layer, *(torch.randn(hkv, t, d, generator=gen, device=DEV).to(dtype) for _ in range(2)))
+    if splice:
+        kv.splice(Split(*splice), 1e4 ** (-torch.arange(0, d, 2).float() / d))
+    return kv
+
+
+@pytest.mark.parametrize("dtype,d", [(BF16, 128), (F16, 64), (BF16, 256)])
+@pytest.mark.parametrize("page_rows,pieces,splice", [
+    (64, (1,), None), (64, (500,), None), (32, (33, 1, 90), None), (100, (700, 5, 1), None),
+    (64, (900, 3), (101, 250, 555)), (40, (600, 40, 7), (33, 34, 500)), (64, (2000,), (70, 1500, 500))])
+@pytest.mark.parametrize("b", [1, 5, 40])
+def test_a_paged_prefix(dtype, d, page_rows, pieces, splice, b):
+    hkv, g, m = 2, 4, 90
+    gen = torch.Generator(device=DEV).manual_seed(b)
+    kv = paged_prefix(hkv, d, dtype, page_rows, gen, pieces, splice)
+    q, _, _, k, v = make(b, hkv, g, d, 1, m, dtype)
+    lens = torch.tensor([(29 * i) % (m + 1) for i in range(b)], device=DEV, dtype=torch.int32)
+    for layer in range(2):
+        kp, vp = kv.gather(layer)
+        out = kv.decode_shared(layer, q, k, v, 0.1, lens)
+        assert_within(out, *reference(q, kp, vp, k, v, 0.1, lens.cpu()))
+    # rows of the pages that no run lists may hold anything
+    live = torch.zeros(kv.table.num_pages, page_rows, dtype=torch.bool, device=DEV)
+    pos = torch.from_numpy(kv.table.positions()).to(DEV)
+    live[pos[:, 0], pos[:, 1]] = True
+    for pool in (kv.k[1], kv.v[1]):
+        pool.transpose(1, 2)[~live] = float("nan")
+    assert torch.equal(kv.decode_shared(1, q, k, v, 0.1, lens), out)
+
+
+def test_an_empty_paged_prefix_and_unaligned_suffixes():
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    kv = PagedKV(1, 2, 128, max_tokens=64, device=DEV)
+    q, kp, vp, k, v = make(3, 2, 4, 128, 0, 20, BF16)
+    assert_within(kv.decode_shared(0, q, k, v, 0.1), *reference(q, kp, vp, k, v, 0.1, torch.full((3,), 20)))
+    kv = paged_prefix(2, 128, BF16, 64, gen, (77,))
+    kp, vp = kv.gather(0)
+    odd = torch.randn(3, 2, 21, 130, generator=gen, device=DEV).to(BF16)[:, :, 1:, 1:129]
+    assert_within(kv.decode_shared(0, q, odd, odd, 0.1), *reference(q, kp, vp, odd, odd, 0.1, torch.full((3,), 20)))
+    empty = k[:, :, :0]
+    assert_within(kv.decode_shared(0, q, empty, empty, 0.1), *reference(q, kp, vp, empty, empty, 0.1, torch.zeros(3)))
+
+
+def test_table_entries_outside_the_pool_count_as_empty():
+    gen = torch.Generator(device=DEV).manual_seed(2)
+    kv = paged_prefix(2, 128, BF16, 64, gen, (300,))
+    q, _, _, k, v = make(2, 2, 4, 128, 1, 20, BF16)
+    kp, vp = kv.gather(0)
+    keep = torch.ones(300, dtype=torch.bool, device=DEV)
+    tiles, _ = kv._tiles()  # the device copy: entries 1, 4 and 6 are made bad
+    for i, bad in ((1, (-1, 0, 32)), (4, (kv.table.num_pages, 0, 32)), (6, (0, 40, 32))):
+        keep[32 * i:32 * i + 32] = False
+        tiles[i] = torch.tensor(bad, dtype=torch.int32)
+    out = kv.decode_shared(0, q, k, v, 0.1)
+    assert_within(out, *reference(q, kp[:, keep], vp[:, keep], k, v, 0.1, torch.full((2,), 20)))
+
+
 def test_refusals():
+    kv = PagedKV(1, 2, 128, max_tokens=64, device=DEV)
+    q, kp, vp, k, v = make(2, 2, 4, 128, 20, 10, BF16)
+    for bad in ((q, k[:1], v[:1], 0.1), (q, k, v[:, :, :3], 0.1), (q[..., :64], k, v, 0.1), (q, k, v, 0.0), (q, k, v, -1.0),
+                (q, k, v, 0.1, torch.zeros(3, device=DEV, dtype=torch.int32))):
+        with pytest.raises(ValueError):
+            kv.decode_shared(0, *bad)
+    with pytest.raises(TypeError):
+        kv.decode_shared(0, q.half(), k.half(), v.half(), 0.1)
     q, kp, vp, k, v = make(2, 2, 4, 128, 20, 10, BF16)
     with pytest.raises(ValueError):
         decode_attention_shared(q, kp[:1], vp[:1], k, v, 0.1)

@@ -59,6 +59,8 @@ SIGNATURES = {
     "tc_decode_attention_shared_workspace_size": (_sz, [_i, _i, _i, _i, _i64, _i64, _i]),
     "tc_decode_attention_shared": (_i, [_vp] * 6 + [_i] * 4 + [_i64, _i64, _vp] + [_i64] * 16
                                    + [_f, _i, _vp, _sz, _vp]),
+    "tc_decode_attention_shared_paged": (_i, [_vp] * 6 + [_i] * 4 + [_i64] * 5 + [_vp, _i64, _i64, _vp] + [_i64] * 12
+                                         + [_f, _i, _vp, _sz, _vp]),
     "tc_split_workspace_size": (_sz, [_i64]),
     "tc_split": (_i, [_vp, _i64, _vp, _i64, _i, _i, _vp, _vp, _sz, _vp]),
     "tc_ragged_encode_tensormaps": (_i, [_vp, ctypes.POINTER(_vp), ctypes.POINTER(_vp), ctypes.POINTER(_i64),

@@ -1,0 +1,467 @@
+// Decode attention of a batch over ONE shared prefix and each sequence's own suffix, on the tcgen05 tensor
+// cores (sm_100a). The prefix of a KV head meets all batch*g query rows that share it in one product, so
+// its K and V are read once for the batch; a suffix meets its sequence's g rows.
+//
+//   out = sum_parts 2^(m_p - M) o_p / sum_parts 2^(m_p - M) l_p,   M = max m_p
+//
+// over parts (slices of the prefix, slices of the suffix), each part's o_p = sum_j 2^(s_j - m_p) v_j and
+// l_p = sum_j 2^(s_j - m_p) with s_j = scale log2(e) q.k_j and m_p a running maximum: the log-sum-exp merge of
+// threadcut/flash_decode.py:68-69 over both kinds of slices.
+//
+// shared_attn_kernel: one CTA per part (prefix: KV head, tile of up to 128 query rows, slice; suffix: sequence,
+// KV head, slice), two resident per SM at d <= 128 (one waits for memory or softmax while the other
+// multiplies), each:
+//   warp 4 (one lane): TMA, the query rows once, then K and V tiles of 64 keys through a ring of slots in the
+//                      order the products take them (K0 K1 V0 K2 V1 ...).
+//   warp 5 (one lane): tcgen05.mma: S = Q K^T (128 x 64 keys x d, fp32 in TMEM, two S buffers so the next
+//                      tile's S is there when a softmax ends), O += P V with P from TMEM.
+//   warps 0-3:         softmax, a thread per query row; warps without live rows leave at once (a suffix has g
+//                      rows). The maximum is kept until a tile passes it by 2^8, so O is rescaled rarely.
+// Rows behind a slice's end inside its last tile: the scores are masked and the staged V rows zeroed, so
+// whatever memory holds there is not met. shared_merge_kernel joins the parts, a warp per query row.
+#pragma once
+
+#include <type_traits>
+
+#include "tc_common.cuh"
+
+namespace tc {
+
+constexpr int kShKeys = 64;       // keys per K/V tile
+constexpr int kShThreads = 192;   // 4 softmax warps, TMA, MMA
+constexpr uint32_t kShSpin = 1u << 20;  // mbarrier polls before a wait gives up (about a second)
+constexpr float kShLazyMax = 8.f;
+
+template <int D>
+struct SharedGeom {
+  static constexpr int kBoxes = D / 64;
+  static constexpr int kQBytes = 128 * D * 2;
+  static constexpr int kSlotBytes = kShKeys * D * 2;
+  static constexpr int kBoxBytes = kShKeys * 128;
+  // two CTAs per SM at D <= 128 (2 x 113 KB of shared memory, 2 x 256 TMEM columns), one at D = 256
+  static constexpr int kSlots = D == 64 ? 10 : 5;
+  static constexpr int kCtasPerSm = D == 256 ? 1 : 2;
+  static constexpr int kTmemCols = D == 256 ? 512 : 256;
+  static constexpr int kSmem = 1024 + kQBytes + kSlots * kSlotBytes;
+};
+
+struct SharedParams {
+  CUtensorMap tmq;   // (d, g, batch, hkv), box (64, g, 128 / g, 1): the rows of a prefix part
+  CUtensorMap tmq1;  // the same, box (64, g, 1, 1): the rows of a suffix part
+  CUtensorMap tmkp, tmvp;  // prefix: (d, n, hkv, 1), box (64, 64, 1, 1); paged (d, page rows, hkv, pages), box (64, 32, 1, 1)
+  CUtensorMap tmk, tmv;    // suffixes: (d, m, hkv, batch), box (64, 64, 1, 1)
+  const int32_t* lengths;  // [batch] or null (= m)
+  const int32_t* tiles;    // paged prefix: [n_tiles][3] = page, first row, rows <= 32; key tile j is entries 2j, 2j + 1
+  int n_tiles;
+  int num_pages, page_rows;
+  int batch, hkv, g;
+  int bt;           // sequences per prefix row tile (128 / g)
+  int row_tiles;    // cdiv(batch, bt)
+  int n, m;
+  int np;           // prefix parts per (KV head, row tile); the first hkv*row_tiles*np CTAs
+  int ns;           // suffix parts per (sequence, KV head)
+  float c;          // scale * log2(e)
+  float* o;         // [np + ns][batch*hkv*g][d] unnormalised
+  float2* ml;       // [np + ns][batch*hkv*g] (maximum in log2, sum)
+};
+
+// mbarriers and flags of a CTA.
+template <int kSlots>
+struct SharedCtl {
+  uint64_t q_full, full[kSlots], empty[kSlots], s_full[2], p_full[2], pv_done[2], fin;
+  uint32_t tmem;
+  int abort;
+};
+
+__device__ __forceinline__ int shared_suffix(const SharedParams& p, int b) {
+  const int len = p.lengths != nullptr ? p.lengths[b] : p.m;
+  return len < 0 ? 0 : (len > p.m ? p.m : len);
+}
+
+// Key tiles [t0, t1) of part s of np over `tiles` tiles.
+__device__ __forceinline__ void shared_range(int tiles, int s, int np, int& t0, int& t1) {
+  t0 = (int)((int64_t)tiles * s / np);
+  t1 = (int)((int64_t)tiles * (s + 1) / np);
+}
+
+template <typename T, int D, bool kPaged>
+__global__ void __launch_bounds__(kShThreads, SharedGeom<D>::kCtasPerSm)
+    shared_attn_kernel(const __grid_constant__ SharedParams p) {
+  using G = SharedGeom<D>;
+  constexpr int kSlots = G::kSlots;
+  constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+  // All shared memory is dynamic, so that two CTAs fit an SM: the tiles from the first 1 KB boundary on,
+  // and the control block in whichever part of the 1 KB of slack is not spent on reaching it.
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t gap = (1024 - (smem_u32(smem_raw) & 1023)) & 1023;
+  uint8_t* smem = smem_raw + gap;
+  uint8_t* sQ = smem;                // D/64 boxes of 128 rows x 128 B
+  uint8_t* sKV = smem + G::kQBytes;  // slot s: D/64 boxes of 64 rows x 128 B
+  static_assert(sizeof(SharedCtl<kSlots>) <= 512, "the control block must fit either side of the tiles");
+  SharedCtl<kSlots>& ctl =
+      *reinterpret_cast<SharedCtl<kSlots>*>(gap >= 512 ? smem_raw : sKV + kSlots * G::kSlotBytes);
+  uint64_t &q_full = ctl.q_full, &fin = ctl.fin;
+  uint64_t *full = ctl.full, *empty = ctl.empty, *s_full = ctl.s_full, *p_full = ctl.p_full, *pv_done = ctl.pv_done;
+  volatile int& s_abort = ctl.abort;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  pdl_launch();
+  pdl_wait();  // queries, lengths, tables and the cache may be the previous kernel's
+  // ---- this CTA's part
+  const int prefix_parts = p.hkv * p.row_tiles * p.np;
+  const bool prefix = (int)blockIdx.x < prefix_parts;
+  int part, h, b0, live, t0, t1, end;  // b0: first sequence of the rows; live: query rows; end: keys of the source
+  if (prefix) {
+    // row tiles of one slice are neighbours in the launch order: the second finds K and V in L2
+    int i = blockIdx.x;
+    b0 = (i % p.row_tiles) * p.bt;
+    i /= p.row_tiles;
+    h = i % p.hkv;
+    part = i / p.hkv;
+    live = (p.batch - b0 < p.bt ? p.batch - b0 : p.bt) * p.g;
+    end = p.n;
+    shared_range(kPaged ? (p.n_tiles + 1) / 2 : (p.n + kShKeys - 1) / kShKeys, part, p.np, t0, t1);
+  } else {
+    int i = blockIdx.x - prefix_parts;
+    const int s = i % p.ns;
+    i /= p.ns;
+    h = i % p.hkv;
+    b0 = i / p.hkv;
+    live = p.g;
+    end = shared_suffix(p, b0);
+    shared_range((end + kShKeys - 1) / kShKeys, s, p.ns, t0, t1);
+    part = p.np + s;
+  }
+  const int nt = t1 - t0;
+  if (nt == 0) return;  // nothing in this slice; the merge knows and skips it
+  const bool paged = kPaged && prefix;
+  const int nlive = (live + 31) >> 5;  // softmax warps with rows
+
+  if (threadIdx.x == 0) {
+    mbar_init(&q_full, 1);
+    for (int s = 0; s < kSlots; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&s_full[s], 1);
+      mbar_init(&p_full[s], nlive);
+      mbar_init(&pv_done[s], 1);
+    }
+    mbar_init(&fin, 1);
+    fence_mbar_init();
+    s_abort = 0;
+  }
+  if (warp == 0) tmem_alloc(&ctl.tmem, G::kTmemCols);
+  tmem_fence_before();
+  __syncthreads();
+  tmem_fence_after();
+  const uint32_t tmem = ctl.tmem;         // S buffer x (and P over it) at +64x, O at +128
+  const uint32_t tO = tmem + 128;
+  // Place of K_j and V_j in the ring's order K0 K1 V0 K2 V1 ... (the order the products take them).
+  auto k_at = [](int j) { return j < 2 ? j : 2 * j - 1; };
+  auto v_at = [nt](int j) { return j < nt - 1 ? 2 * j + 2 : 2 * nt - 1; };
+  // (page, first row, rows) of sub-tile c of key tile t; a table entry outside the pool counts as empty
+  auto sub = [&](int t, int c) -> int3 {
+    const int i = 2 * t + c;
+    if (i >= p.n_tiles) return make_int3(p.num_pages, 0, 0);
+    const int32_t* e = p.tiles + 3 * (int64_t)i;
+    const int page = e[0], row = e[1], rows = e[2];
+    if (page < 0 || page >= p.num_pages || row < 0 || rows < 0 || rows > 32 || row + rows > p.page_rows)
+      return make_int3(p.num_pages, 0, 0);
+    return make_int3(page, row, rows);
+  };
+
+  if (warp == 4) {
+    // ---------------- TMA
+    if (lane == 0) {
+      const uint64_t pol = policy_evict_first(), keep = policy_evict_last();
+      const CUtensorMap* mq = prefix ? &p.tmq : &p.tmq1;
+      const CUtensorMap* mk = prefix ? &p.tmkp : &p.tmk;
+      const CUtensorMap* mv = prefix ? &p.tmvp : &p.tmv;
+      const uint64_t kvpol = prefix && p.row_tiles > 1 ? keep : pol;  // read again by the next row tile
+      mbar_arrive_expect_tx(&q_full, (uint32_t)(G::kBoxes * 128 * p.g * (prefix ? p.bt : 1)));
+      for (int bx = 0; bx < G::kBoxes; ++bx) tma_load_4d(sQ + bx * 16384, mq, bx * 64, 0, b0, h, &q_full, pol);
+      int armed = 0;
+      auto load = [&](const CUtensorMap* map, int t) -> bool {
+        const int s = armed % kSlots, r = armed / kSlots;
+        if (s_abort || (r > 0 && !mbar_wait(&empty[s], (r - 1) & 1, TC_DEVERR_PIPE_TIMEOUT, kShSpin))) return false;
+        mbar_arrive_expect_tx(&full[s], (uint32_t)G::kSlotBytes);
+        uint8_t* st = sKV + s * G::kSlotBytes;
+        if (paged) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const int3 e = sub(t, c);
+            for (int bx = 0; bx < G::kBoxes; ++bx)
+              tma_load_4d(st + bx * G::kBoxBytes + c * 4096, map, bx * 64, e.y, h, e.x, &full[s], kvpol);
+          }
+        } else {
+          for (int bx = 0; bx < G::kBoxes; ++bx)
+            tma_load_4d(st + bx * G::kBoxBytes, map, bx * 64, t * kShKeys, h, prefix ? 0 : b0, &full[s], kvpol);
+        }
+        ++armed;
+        return true;
+      };
+      bool ok = load(mk, t0) && (nt < 2 || load(mk, t0 + 1));
+      for (int j = 0; ok && j < nt; ++j) ok = load(mv, t0 + j) && (j + 2 >= nt || load(mk, t0 + j + 2));
+      if (!ok) s_abort = 1;
+      // copies still in flight after an abort must land before the CTA leaves (normally these phases
+      // completed long ago and the waits return at once)
+      for (int i = armed - kSlots > 0 ? armed - kSlots : 0; i < armed; ++i)
+        mbar_wait(&full[i % kSlots], (i / kSlots) & 1, TC_DEVERR_PIPE_TIMEOUT, kShSpin);
+      mbar_wait(&q_full, 0, TC_DEVERR_PIPE_TIMEOUT, kShSpin);
+    }
+  } else if (warp == 5) {
+    // ---------------- tcgen05.mma: S(0) S(1), then per tile P V(j), S(j + 2). Products of one thread run
+    // in issue order, so S(j + 2) overwrites P(j) only after P V(j) read it.
+    if (lane == 0) {
+      const uint32_t idS = umma_idesc_f16(kBf16, false, 128, kShKeys);
+      const uint32_t idO = umma_idesc_f16(kBf16, true, 128, D);
+      const uint32_t q0 = smem_u32(sQ), kv0 = smem_u32(sKV);
+      auto wait_slot = [&](int i) {
+        return !s_abort && mbar_wait(&full[i % kSlots], (i / kSlots) & 1, TC_DEVERR_PIPE_TIMEOUT, kShSpin);
+      };
+      auto issue_s = [&](int j) -> bool {
+        const int i = k_at(j);
+        if (!wait_slot(i)) return false;
+        tmem_fence_after();
+        const uint32_t k0 = kv0 + (i % kSlots) * G::kSlotBytes;
+        for (int kd = 0; kd < D / 16; ++kd)
+          umma_f16(tmem + 64 * (j & 1), umma_desc_sw128(q0 + (kd >> 2) * 16384 + (kd & 3) * 32, 16, 1024),
+                   umma_desc_sw128(k0 + (kd >> 2) * G::kBoxBytes + (kd & 3) * 32, 16, 1024), idS, kd > 0);
+        umma_commit(&empty[i % kSlots]);
+        umma_commit(&s_full[j & 1]);
+        return true;
+      };
+      bool ok = mbar_wait(&q_full, 0, TC_DEVERR_PIPE_TIMEOUT, kShSpin) && issue_s(0) && (nt < 2 || issue_s(1));
+      for (int j = 0; ok && j < nt; ++j) {
+        const int i = v_at(j);
+        ok = wait_slot(i) && mbar_wait(&p_full[j & 1], (j >> 1) & 1, TC_DEVERR_PIPE_TIMEOUT, kShSpin);
+        if (!ok) break;
+        tmem_fence_after();
+        const uint32_t v0 = kv0 + (i % kSlots) * G::kSlotBytes;
+        for (int kk = 0; kk < kShKeys / 16; ++kk)
+          umma_f16_tmem_a(tO, tmem + 64 * (j & 1) + kk * 8, umma_desc_sw128(v0 + kk * 2048, G::kBoxBytes, 1024), idO,
+                          j > 0 || kk > 0);
+        umma_commit(&empty[i % kSlots]);
+        umma_commit(&pv_done[j & 1]);
+        if (j + 2 < nt) ok = issue_s(j + 2);
+      }
+      if (!ok) s_abort = 1;
+      umma_commit(&fin);  // completes once every product issued above has
+    }
+  } else if (warp < nlive) {
+    // ---------------- softmax: thread = TMEM lane = query row (sequence b0 + row / g, head row % g)
+    const int row = warp * 32 + lane;
+    const uint32_t lb = (uint32_t)(warp * 32) << 16;
+    float m = -INFINITY, l = 0.f;
+    bool ok = true;
+    for (int j = 0; j < nt; ++j) {
+      const uint32_t tS = tmem + lb + 64 * (j & 1);
+      // valid keys of the tile's halves of 32
+      int v0, v1;
+      if (paged) {
+        v0 = sub(t0 + j, 0).z;
+        v1 = sub(t0 + j, 1).z;
+      } else {
+        const int left = end - (t0 + j) * kShKeys;
+        v0 = left < 32 ? left : 32;
+        v1 = left < 64 ? (left > 32 ? left - 32 : 0) : 32;
+      }
+      // warp-uniform: tcgen05.ld/st and the votes below are warp-collective
+      ok = __all_sync(0xffffffffu, !s_abort && mbar_wait(&s_full[j & 1], (j >> 1) & 1, TC_DEVERR_PIPE_TIMEOUT, kShSpin));
+      if (!ok) break;
+      tmem_fence_after();
+      uint32_t v[2][32];
+      tmem_ld32(tS, v[0]);
+      tmem_ld32(tS + 32, v[1]);
+      tmem_wait_ld();
+      if (v0 + v1 < kShKeys) {
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          if (e >= v0) v[0][e] = __float_as_uint(-INFINITY);
+          if (e >= v1) v[1][e] = __float_as_uint(-INFINITY);
+        }
+        // the staged V rows behind the end: zeros, so that a zero weight never meets a NaN
+        const int i = v_at(j);
+        ok = __all_sync(0xffffffffu, mbar_wait(&full[i % kSlots], (i / kSlots) & 1, TC_DEVERR_PIPE_TIMEOUT, kShSpin));
+        if (!ok) break;
+        uint8_t* st = sKV + (i % kSlots) * G::kSlotBytes;
+        for (int x = row; x < kShKeys * (D / 8); x += nlive * 32) {
+          const int r = x / (D / 8), cc = x % (D / 8);
+          if ((r & 31) >= (r < 32 ? v0 : v1))
+            *reinterpret_cast<uint4*>(st + (cc >> 3) * G::kBoxBytes + r * 128 + (cc & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+        }
+        fence_proxy_async_smem();
+      }
+      float mx[8];
+#pragma unroll
+      for (int r = 0; r < 8; ++r) mx[r] = -INFINITY;
+#pragma unroll
+      for (int cch = 0; cch < 2; ++cch)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          mx[e & 7] = fmax3(mx[e & 7], __uint_as_float(v[cch][2 * e]), __uint_as_float(v[cch][2 * e + 1]));
+      const float mt = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])),
+                             fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7]))) * p.c;  // exp2 domain (c > 0)
+      const bool bump = mt > m + kShLazyMax;
+      const float mn = bump ? mt : m;
+      const float alpha = !bump ? 1.f : (m == -INFINITY ? 0.f : fast_exp2(m - mn));
+      const float mref = mn == -INFINITY ? 0.f : mn;
+      float2 rs[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+      uint32_t w[32];  // 16-bit pairs: keys 2e, 2e + 1
+#pragma unroll
+      for (int e = 0; e < 32; ++e) {
+        const float2 xy = ffma2(make_float2(__uint_as_float(v[e >> 4][2 * (e & 15)]), __uint_as_float(v[e >> 4][2 * (e & 15) + 1])),
+                                make_float2(p.c, p.c), make_float2(-mref, -mref));
+        const float2 pp = make_float2(fast_exp2(xy.x), fast_exp2(xy.y));
+        rs[e & 1] = fadd2(rs[e & 1], pp);
+        w[e] = Mma<T>::pack(pp.x, pp.y);
+      }
+      tmem_st32(tS, w);
+      l = l * alpha + ((rs[0].x + rs[1].x) + (rs[0].y + rs[1].y));
+      m = mn;
+      if (j >= 1 && __any_sync(0xffffffffu, alpha != 1.f)) {
+        // O holds P V of the tiles before j once P V(j - 1) is done (P V(j) waits for this warp)
+        ok = __all_sync(0xffffffffu, !s_abort && mbar_wait(&pv_done[(j - 1) & 1], ((j - 1) >> 1) & 1, TC_DEVERR_PIPE_TIMEOUT, kShSpin));
+        if (!ok) break;
+        tmem_fence_after();
+#pragma unroll
+        for (int cch = 0; cch < D / 32; ++cch) {
+          uint32_t o[32];
+          tmem_ld32(tO + lb + cch * 32, o);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+          tmem_st32(tO + lb + cch * 32, o);
+        }
+      }
+      tmem_wait_st();
+      tmem_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full[j & 1]);
+    }
+    if (ok)
+      ok = __all_sync(0xffffffffu, !s_abort && mbar_wait(&fin, 0, TC_DEVERR_PIPE_TIMEOUT, kShSpin));
+    if (!ok) {
+      s_abort = 1;
+    } else {
+      tmem_fence_after();
+      const int64_t rows = (int64_t)p.batch * p.hkv * p.g;
+      const int bi = row / p.g;
+      const int64_t r = ((int64_t)(b0 + bi) * p.hkv + h) * p.g + (row - bi * p.g);
+      float* orow = p.o + ((int64_t)part * rows + r) * D;
+#pragma unroll
+      for (int cch = 0; cch < D / 32; ++cch) {
+        uint32_t o[32];
+        tmem_ld32(tO + lb + cch * 32, o);
+        tmem_wait_ld();
+        if (row < live) {
+#pragma unroll
+          for (int q4 = 0; q4 < 8; ++q4)
+            *reinterpret_cast<uint4*>(orow + cch * 32 + q4 * 4) =
+                make_uint4(o[4 * q4], o[4 * q4 + 1], o[4 * q4 + 2], o[4 * q4 + 3]);
+        }
+      }
+      if (row < live) p.ml[(int64_t)part * rows + r] = make_float2(m, l);
+    }
+  }
+  // every product has completed before the TMEM columns are freed (bounded: a lost commit only errs)
+  tmem_fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    mbar_wait(&fin, 0, TC_DEVERR_PIPE_TIMEOUT, kShSpin);
+    tmem_fence_after();
+    tmem_dealloc(tmem, G::kTmemCols);
+  }
+}
+
+struct SharedMergeParams {
+  const float* o;
+  const float2* ml;
+  const int32_t* lengths;
+  void* out;
+  int64_t so_b, so_h, so_g;
+  int batch, hkv, g, m, np, ns;
+};
+
+// One warp per query row: lane l folds the float4 columns l, l + 32, ...; parts in a fixed order.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) shared_merge_kernel(const __grid_constant__ SharedMergeParams p) {
+  constexpr int kCols = D / 4, kPer = (kCols + 31) / 32;  // float4 columns, per lane
+  constexpr int kLoads = 8;
+  pdl_launch();
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const int64_t rows = (int64_t)p.batch * p.hkv * p.g;
+  const int64_t r = blockIdx.x * (int64_t)(blockDim.x >> 5) + (threadIdx.x >> 5);
+  if (r >= rows) return;
+  const int i = (int)(r % p.g), h = (int)(r / p.g % p.hkv), b = (int)(r / p.g / p.hkv);
+  int len = p.lengths != nullptr ? p.lengths[b] : p.m;
+  len = len < 0 ? 0 : (len > p.m ? p.m : len);
+  const int tiles = (len + kShKeys - 1) / kShKeys;
+  float M = -INFINITY, L = 0.f;
+  float4 A[kPer];
+#pragma unroll
+  for (int x = 0; x < kPer; ++x) A[x] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s0 = 0; s0 < p.np + p.ns; s0 += kLoads) {
+    float2 ml[kLoads];
+    float4 o[kLoads][kPer];
+#pragma unroll
+    for (int k = 0; k < kLoads; ++k) {
+      const int s = s0 + k;
+      bool use = s < p.np + p.ns;
+      if (use && s >= p.np) {
+        int t0, t1;
+        shared_range(tiles, s - p.np, p.ns, t0, t1);
+        use = t1 > t0;
+      }
+      ml[k] = use ? __ldcg(p.ml + s * rows + r) : make_float2(-INFINITY, 0.f);
+#pragma unroll
+      for (int x = 0; x < kPer; ++x) {
+        const int col = lane + 32 * x;
+        o[k][x] = use && col < kCols ? __ldcg(reinterpret_cast<const float4*>(p.o + (s * rows + r) * D) + col)
+                                     : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+    }
+    float mc = M;
+#pragma unroll
+    for (int k = 0; k < kLoads; ++k) mc = fmaxf(mc, ml[k].x);
+    const float a = M == -INFINITY ? 0.f : fast_exp2(M - mc);
+    L *= a;
+#pragma unroll
+    for (int x = 0; x < kPer; ++x) {
+      A[x].x *= a;
+      A[x].y *= a;
+      A[x].z *= a;
+      A[x].w *= a;
+    }
+#pragma unroll
+    for (int k = 0; k < kLoads; ++k) {
+      const float w = ml[k].x == -INFINITY ? 0.f : fast_exp2(ml[k].x - mc);
+      L += w * ml[k].y;
+#pragma unroll
+      for (int x = 0; x < kPer; ++x) {
+        A[x].x += w * o[k][x].x;
+        A[x].y += w * o[k][x].y;
+        A[x].z += w * o[k][x].z;
+        A[x].w += w * o[k][x].w;
+      }
+    }
+    M = mc;
+  }
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  T* out = static_cast<T*>(p.out) + b * p.so_b + h * p.so_h + i * p.so_g;
+#pragma unroll
+  for (int x = 0; x < kPer; ++x) {
+    const int col = lane + 32 * x;
+    if (col < kCols) {
+      uint2 w;
+      w.x = Mma<T>::pack(A[x].x * inv, A[x].y * inv);
+      w.y = Mma<T>::pack(A[x].z * inv, A[x].w * inv);
+      *reinterpret_cast<uint2*>(out + 4 * col) = w;
+    }
+  }
+}
+
+}  // namespace tc

@@ -16,6 +16,7 @@
 #include "split.cuh"
 #include "prefill_attn.cuh"
 #include "rows_attn.cuh"
+#include "shared_attn.cuh"
 #include "layer_ops.cuh"
 #include "peer.cuh"
 #include "gemv_stream.cuh"
@@ -2037,6 +2038,153 @@ int run_window_prefill(PrefillParams& p, const WindowPrefill& w, int batch, int 
 }
 }  // namespace
 
+namespace {
+// Parts of the tcgen05 shared-prefix decode and its workspace.
+struct SharedPlan {
+  int bt = 1, row_tiles = 1;  // sequences per prefix row tile, row tiles
+  int np = 0, ns = 0;         // parts of the prefix, of each suffix
+  int64_t ctas = 0;
+  size_t ml = 0, bytes = 0;   // offset of the (maximum, sum) array; total
+};
+
+constexpr int kShMaxParts = 64;
+
+SharedPlan plan_shared(int batch, int hkv, int g, int d, int64_t n, int64_t m) {
+  SharedPlan w;
+  w.bt = 128 / g;
+  w.row_tiles = (int)cdiv(batch, w.bt);
+  const int64_t slots = (int64_t)sm_count(current_device()) * (d == 256 ? 1 : 2);
+  const int64_t tp = cdiv(n, kShKeys), ts = cdiv(m, kShKeys);
+  // parts of about equal length, as many as are resident at once
+  int64_t x = cdiv(hkv * (w.row_tiles * tp + batch * ts), slots);
+  if (x < 2) x = 2;
+  w.np = (int)(cdiv(tp, x) < kShMaxParts ? cdiv(tp, x) : kShMaxParts);
+  w.ns = (int)(cdiv(ts, x) < kShMaxParts ? cdiv(ts, x) : kShMaxParts);
+  w.ctas = (int64_t)hkv * ((int64_t)w.row_tiles * w.np + (int64_t)batch * w.ns);
+  const size_t rows = (size_t)batch * hkv * g, parts = (size_t)(w.np + w.ns);
+  w.ml = round256(sizeof(float) * parts * rows * d);
+  w.bytes = w.ml + round256(sizeof(float2) * parts * rows);
+  return w;
+}
+
+template <typename T, int D>
+cudaError_t launch_shared_t(const SharedParams& p, const SharedMergeParams& mp, int64_t ctas, int dev, cudaStream_t st) {
+  const auto fn = p.tiles != nullptr ? shared_attn_kernel<T, D, true> : shared_attn_kernel<T, D, false>;
+  cudaError_t e = set_smem(reinterpret_cast<const void*>(fn), SharedGeom<D>::kSmem, dev);
+  if (e == cudaSuccess && ctas > 0)
+    e = launch_ex(fn, dim3((unsigned)ctas), dim3(kShThreads), SharedGeom<D>::kSmem, st, p);
+  if (e != cudaSuccess) return e;
+  const int64_t rows = (int64_t)p.batch * p.hkv * p.g;
+  return launch_ex(shared_merge_kernel<T, D>, dim3((unsigned)cdiv(rows, 8)), dim3(256), 0, st, mp);
+}
+
+template <typename T>
+cudaError_t dispatch_shared(const SharedParams& p, const SharedMergeParams& mp, int d, int64_t ctas, int dev,
+                            cudaStream_t st) {
+  switch (d) {
+    case 64: return launch_shared_t<T, 64>(p, mp, ctas, dev, st);
+    case 128: return launch_shared_t<T, 128>(p, mp, ctas, dev, st);
+    case 256: return launch_shared_t<T, 256>(p, mp, ctas, dev, st);
+  }
+  return cudaErrorInvalidValue;
+}
+
+// The tensors of a shared-prefix decode call.
+struct SharedCall {
+  const void *q, *kp, *vp, *k, *v;
+  void* out;
+  int batch, hkv, g, d;
+  int64_t n, m;
+  const int32_t* lengths;
+  int64_t sq[3], skp[2], svp[2], sk[3], sv[3], so[3];  // (b, h, g), (h, n), (h, n), (b, h, n) twice, (b, h, g)
+  float scale;
+  int dtype;
+  // paged prefix (tiles non-null): kp / vp are pools, skp = (head, row) and page their strides
+  const int32_t* tiles;
+  int64_t n_tiles, page, page_rows, num_pages;
+};
+
+// Whether the tcgen05 kernel takes the call: 16-byte rows everywhere, and a scale that keeps the order of
+// the scores (the kernel takes the row maximum before it).
+bool shared_tc5(const SharedCall& c) {
+  bool ok = c.dtype != TC_F32 && mma_dim(c.d) && c.scale > 0.f && c.n <= (1 << 30) && c.m <= (1 << 30) &&
+            aligned16(c.q) && aligned16(c.out) && aligned16(c.kp) && aligned16(c.vp) && aligned16(c.k) && aligned16(c.v) &&
+            stride16(c.page, c.dtype);
+  for (int64_t x : c.sq) ok = ok && stride16(x, c.dtype);
+  for (int64_t x : c.so) ok = ok && stride16(x, c.dtype);
+  for (int64_t x : c.skp) ok = ok && stride16(x, c.dtype);
+  for (int64_t x : c.svp) ok = ok && stride16(x, c.dtype);
+  for (int64_t x : c.sk) ok = ok && stride16(x, c.dtype);
+  for (int64_t x : c.sv) ok = ok && stride16(x, c.dtype);
+  return ok;
+}
+
+// Runs the tcgen05 kernel and the merge; -1 where a tensor map cannot describe the call's strides.
+int run_shared_tc5(const SharedCall& c, void* workspace, size_t workspace_bytes, cudaStream_t st) {
+  const SharedPlan w = plan_shared(c.batch, c.hkv, c.g, c.d, c.n, c.m);
+  if (w.ctas > INT32_MAX) return TC_ERR_INVALID;
+  SharedParams p;
+  std::memset(&p, 0, sizeof(p));
+  const int64_t qd[4] = {c.d, c.g, c.batch, c.hkv};
+  const int64_t sd[4] = {c.d, c.m, c.hkv, c.batch};
+  const uint32_t qbox[4] = {64, (uint32_t)c.g, (uint32_t)w.bt, 1}, qbox1[4] = {64, (uint32_t)c.g, 1, 1};
+  const uint32_t box[4] = {64, (uint32_t)kShKeys, 1, 1};
+  if (!encode_view4(&p.tmq, c.q, c.dtype, qd, c.sq[2], c.sq[0], c.sq[1], qbox) ||
+      !encode_view4(&p.tmq1, c.q, c.dtype, qd, c.sq[2], c.sq[0], c.sq[1], qbox1))
+    return -1;
+  if (c.tiles != nullptr) {
+    if (!encode_kv_map(&p.tmkp, c.kp, c.dtype, c.d, c.page_rows, c.hkv, c.num_pages, c.skp[1], c.skp[0], c.page) ||
+        !encode_kv_map(&p.tmvp, c.vp, c.dtype, c.d, c.page_rows, c.hkv, c.num_pages, c.svp[1], c.svp[0], c.page))
+      return -1;
+  } else if (c.n > 0) {
+    const int64_t pd[4] = {c.d, c.n, c.hkv, 1};
+    if (!encode_view4(&p.tmkp, c.kp, c.dtype, pd, c.skp[1], c.skp[0], 0, box) ||
+        !encode_view4(&p.tmvp, c.vp, c.dtype, pd, c.svp[1], c.svp[0], 0, box))
+      return -1;
+  }
+  if (c.m > 0 && (!encode_view4(&p.tmk, c.k, c.dtype, sd, c.sk[2], c.sk[1], c.sk[0], box) ||
+                  !encode_view4(&p.tmv, c.v, c.dtype, sd, c.sv[2], c.sv[1], c.sv[0], box)))
+    return -1;
+  if (w.bytes > 0 && (workspace == nullptr || !aligned16(workspace) || workspace_bytes < w.bytes)) return TC_ERR_WORKSPACE;
+  p.lengths = c.lengths;
+  p.tiles = c.tiles;
+  p.n_tiles = (int)c.n_tiles;
+  p.num_pages = (int)c.num_pages;
+  p.page_rows = (int)c.page_rows;
+  p.batch = c.batch;
+  p.hkv = c.hkv;
+  p.g = c.g;
+  p.bt = w.bt;
+  p.row_tiles = w.row_tiles;
+  p.n = (int)c.n;
+  p.m = (int)c.m;
+  p.np = w.np;
+  p.ns = w.ns;
+  p.c = c.scale * kLog2e;
+  p.o = static_cast<float*>(workspace);
+  p.ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + w.ml);
+  SharedMergeParams mp;
+  std::memset(&mp, 0, sizeof(mp));
+  mp.o = p.o;
+  mp.ml = p.ml;
+  mp.lengths = c.lengths;
+  mp.out = c.out;
+  mp.so_b = c.so[0];
+  mp.so_h = c.so[1];
+  mp.so_g = c.so[2];
+  mp.batch = c.batch;
+  mp.hkv = c.hkv;
+  mp.g = c.g;
+  mp.m = (int)c.m;
+  mp.np = w.np;
+  mp.ns = w.ns;
+  const int dev = current_device();
+  const cudaError_t e = c.dtype == TC_BF16 ? dispatch_shared<__nv_bfloat16>(p, mp, c.d, w.ctas, dev, st)
+                                           : dispatch_shared<__half>(p, mp, c.d, w.ctas, dev, st);
+  return e == cudaSuccess ? TC_OK : TC_ERR_CUDA;
+}
+}  // namespace
+
 extern "C" {
 
 size_t tc_prefill_window_workspace_size(int batch, int hq, int hkv, int lq, int lk, int d, int64_t window,
@@ -2129,8 +2277,8 @@ int tc_prefill_attention_window(const void* q, const void* k, const void* v, voi
 }
 
 size_t tc_decode_attention_shared_workspace_size(int batch, int hkv, int g, int d, int64_t n, int64_t m, int dtype) {
-  (void)batch, (void)hkv, (void)g, (void)d, (void)n, (void)m, (void)dtype;
-  return 0;
+  if (batch < 1 || hkv < 1 || g < 1 || g > 128 || n < 0 || m < 0 || dtype == TC_F32 || !mma_dim(d)) return 0;
+  return plan_shared(batch, hkv, g, d, n, m).bytes;
 }
 
 int tc_decode_attention_shared(const void* q, const void* k_prefix, const void* v_prefix, const void* k, const void* v,
@@ -2146,7 +2294,14 @@ int tc_decode_attention_shared(const void* q, const void* k_prefix, const void* 
       n > INT32_MAX || m < 0 || m > INT32_MAX || q == nullptr || out == nullptr || !finite_scale(scale) ||
       (n > 0 && (k_prefix == nullptr || v_prefix == nullptr)) || (m > 0 && (k == nullptr || v == nullptr)))
     return TC_ERR_INVALID;
-  (void)workspace, (void)workspace_bytes;
+  const SharedCall call = {q, k_prefix, v_prefix, k, v, out, batch, hkv, g, d, n, m, lengths,
+                           {q_stride_b, q_stride_h, q_stride_g}, {kp_stride_h, kp_stride_n}, {vp_stride_h, vp_stride_n},
+                           {k_stride_b, k_stride_h, k_stride_n}, {v_stride_b, v_stride_h, v_stride_n},
+                           {out_stride_b, out_stride_h, out_stride_g}, scale, dtype, nullptr, 0, 0, 0, 0};
+  if (shared_tc5(call)) {
+    const int s = run_shared_tc5(call, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+    if (s >= 0) return s;
+  }
   RowsParams p;
   std::memset(&p, 0, sizeof(p));
   p.q = q;
@@ -2181,6 +2336,33 @@ int tc_decode_attention_shared(const void* q, const void* k_prefix, const void* 
   p.lengths = lengths;
   p.c = scale * kLog2e;
   return launch_rows(p, dtype, static_cast<cudaStream_t>(stream));
+}
+
+int tc_decode_attention_shared_paged(const void* q, const void* k_pool, const void* v_pool, const void* k, const void* v,
+                                     void* out, int batch, int hkv, int g, int d, int64_t page_rows, int64_t num_pages,
+                                     int64_t pool_stride_page, int64_t pool_stride_h, int64_t pool_stride_row,
+                                     const int32_t* tiles, int64_t n_tiles, int64_t m, const int32_t* lengths,
+                                     int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_g, int64_t k_stride_b,
+                                     int64_t k_stride_h, int64_t k_stride_n, int64_t v_stride_b, int64_t v_stride_h,
+                                     int64_t v_stride_n, int64_t out_stride_b, int64_t out_stride_h,
+                                     int64_t out_stride_g, float scale, int dtype, void* workspace,
+                                     size_t workspace_bytes, void* stream) {
+  if (dtype != TC_BF16 && dtype != TC_F16) return TC_ERR_DTYPE;
+  if (batch < 1 || batch > 65535 || hkv < 1 || hkv > 65535 || g < 1 || g > 128 || !mma_dim(d) || page_rows < kTile ||
+      page_rows > (1 << 30) || num_pages < 1 || num_pages >= (1 << 30) || n_tiles < 0 || n_tiles > (1 << 25) || m < 0 ||
+      m > (1 << 30) || q == nullptr || out == nullptr || k_pool == nullptr || v_pool == nullptr ||
+      (n_tiles > 0 && tiles == nullptr) || (m > 0 && (k == nullptr || v == nullptr)) || !finite_scale(scale) ||
+      !(scale > 0.f))
+    return TC_ERR_INVALID;
+  // a key tile is two table entries, so the plan is that of 32 rows an entry
+  const SharedCall call = {q, k_pool, v_pool, k, v, out, batch, hkv, g, d, n_tiles * kTile, m, lengths,
+                           {q_stride_b, q_stride_h, q_stride_g}, {pool_stride_h, pool_stride_row},
+                           {pool_stride_h, pool_stride_row}, {k_stride_b, k_stride_h, k_stride_n},
+                           {v_stride_b, v_stride_h, v_stride_n}, {out_stride_b, out_stride_h, out_stride_g}, scale,
+                           dtype, n_tiles > 0 ? tiles : nullptr, n_tiles, pool_stride_page, page_rows, num_pages};
+  if (!shared_tc5(call)) return TC_ERR_ALIGN;
+  const int s = run_shared_tc5(call, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+  return s >= 0 ? s : TC_ERR_INVALID;
 }
 
 }  // extern "C"

@@ -302,6 +302,14 @@ def append_rope(k, v, cos, sin, k_pool, v_pool, slots, *, q=None, q_norm=None, k
     return out[None] if batched and out is not None else out
 
 
+def _rows16(x):
+    """x itself if its rows start on 16-byte boundaries (the tensor-map rule), else a contiguous copy."""
+    es = x.element_size()
+    if x.stride(-1) == 1 and x.data_ptr() % 16 == 0 and all(s * es % 16 == 0 for s in x.stride()[:-1]):
+        return x
+    return x.contiguous()
+
+
 class PagedKV:
     """Paged K/V of `layers` attention layers of one sequence on one GPU.
 
@@ -457,6 +465,50 @@ class PagedKV:
                 v_new.stride(0) if v_new is not None else 0, q.stride(0), q.stride(1), out.stride(0), out.stride(1),
                 float(scale), int(splits or 0), code, int(stable_tiles), ws.data_ptr(), ws.numel(),
                 stream_ptr(q.device)))
+        return out
+
+    def decode_shared(self, layer, q, k, v, scale, lengths=None):
+        """flash_decode.decode_attention_shared with this sequence as the prefix, straight over its pages:
+        q [b, hkv, g, d], the continuations' suffixes k/v [b, hkv, m, d] of which the first lengths[i] rows
+        count (int32 CUDA [b], clamped into [0, m]; None: all m). 16-bit, d in {64, 128, 256}, g <= 128,
+        scale > 0. Returns [b, hkv, g, d]."""
+        what = "PagedKV.decode_shared"
+        require_cuda(q, k, v, what=what)
+        if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape:
+            raise ValueError(f"{what}: expected q [b, hkv, g, d], k/v [b, hkv, m, d]; got {tuple(q.shape)}, "
+                             f"{tuple(k.shape)}, {tuple(v.shape)}")
+        b, hkv, g, d = q.shape
+        m = k.shape[2]
+        if hkv != self.hkv or d != self.d or k.shape != (b, hkv, m, d):
+            raise ValueError(f"{what}: q {tuple(q.shape)} / k {tuple(k.shape)} do not match the cache")
+        if q.dtype != self.dtype or k.dtype != self.dtype or v.dtype != self.dtype or self.dtype == torch.float32:
+            raise TypeError(f"threadcut_b200.{what}: needs the cache's 16-bit dtype {self.dtype}, got {q.dtype}, "
+                            f"{k.dtype}, {v.dtype}")
+        if not scale > 0:
+            raise ValueError(f"{what}: needs scale > 0, got {scale}")
+        q, k, v = (_rows16(x) for x in (q, k, v))
+        lens_ptr = None
+        if lengths is not None:
+            if lengths.dtype != torch.int32 or lengths.device != q.device or not lengths.is_contiguous():
+                lengths = lengths.to(device=q.device, dtype=torch.int32).contiguous()
+            if lengths.shape != (b,):
+                raise ValueError(f"{what}: lengths must be [{b}]")
+            lens_ptr = lengths.data_ptr()
+        tiles, nt = self._tiles()
+        out = torch.empty((b, hkv, g, d), dtype=q.dtype, device=q.device)
+        L = lib()
+        code = dtype_code(q, what)
+        sp, sh, sr = self._strides()
+        with torch.cuda.device(q.device):
+            nb = L.tc_decode_attention_shared_workspace_size(b, hkv, g, d, TILE_ROWS * nt, m, code)
+            ws = torch.empty(nb, dtype=torch.uint8, device=q.device) if nb else None
+            st = L.tc_decode_attention_shared_paged(
+                q.data_ptr(), self.k[layer].data_ptr(), self.v[layer].data_ptr(), k.data_ptr(), v.data_ptr(),
+                out.data_ptr(), b, hkv, g, d, self.page_rows, self.table.num_pages, sp, sh, sr,
+                tiles.data_ptr() if tiles is not None else None, nt, m, lens_ptr, *q.stride()[:3], *k.stride()[:3],
+                *v.stride()[:3], *out.stride()[:3], float(scale), code, ws.data_ptr() if ws is not None else None, nb,
+                stream_ptr(q.device))
+        check("tc_decode_attention_shared_paged", st)
         return out
 
     def _prefill_table(self):
