@@ -1037,8 +1037,39 @@ int tc_paged_write(const void* k_src, const void* v_src, void* k_pool, void* v_p
 }  // extern "C"
 
 namespace {
+// Whether rows, tables and weights are whole 16-byte chunks on 16-byte boundaries and a row is a power of
+// two of chunk pairs: what paged_append_vec_kernel takes.
+bool paged_append_vec(PagedAppendParams& p, int dtype) {
+  const int vec = dtype == TC_F32 ? 4 : 8, tab = p.table_f32 ? TC_F32 : dtype;
+  if (p.d % (2 * vec) != 0 || p.rot % (2 * vec) != 0) return false;
+  p.pairs = p.d / (2 * vec);
+  if (p.pairs > 32 || (p.pairs & (p.pairs - 1)) != 0) return false;
+  for (const void* x : {p.q, p.k, p.v, (const void*)p.q_out, (const void*)p.kp, (const void*)p.vp, p.q_w, p.k_w, p.cos_t,
+                        p.sin_t})
+    if (!aligned16(x)) return false;
+  for (int64_t x : {p.k_sh, p.k_st, p.v_sh, p.v_st, p.s_page, p.s_h, p.s_row})
+    if (!stride16(x, dtype)) return false;
+  if (p.hq > 0)
+    for (int64_t x : {p.q_sh, p.q_st, p.qo_sh, p.qo_st})
+      if (!stride16(x, dtype)) return false;
+  return stride16(p.cos_st, tab) && stride16(p.sin_st, tab);
+}
+
+template <typename T, typename TT>
+cudaError_t launch_paged_append_vec(const PagedAppendParams& p, int sms, cudaStream_t st) {
+  const int heads = p.hq + 2 * p.hkv, rows = 32 / p.pairs;
+  const int64_t wide = p.t * cdiv(heads, 4 * rows);
+  // Four rows a thread once the warps fill the GPU (64 a SM); one while latency counts.
+  if (wide >= 64 * (int64_t)sms)
+    return launch_ex(paged_append_vec_kernel<T, TT, 4>, dim3((unsigned)cdiv(wide, 8)), dim3(256), 0, st, p);
+  return launch_ex(paged_append_vec_kernel<T, TT, 1>, dim3((unsigned)cdiv(p.t * cdiv(heads, rows), 8)), dim3(256), 0, st,
+                   p);
+}
+
 template <typename T>
-cudaError_t launch_paged_append(const PagedAppendParams& p, int sms, cudaStream_t st) {
+cudaError_t launch_paged_append(PagedAppendParams& p, int dtype, int sms, cudaStream_t st) {
+  if (paged_append_vec(p, dtype) && p.t * (p.hq + 2 * (int64_t)p.hkv) <= INT32_MAX)
+    return p.table_f32 ? launch_paged_append_vec<T, float>(p, sms, st) : launch_paged_append_vec<T, T>(p, sms, st);
   const int blocks = grid_for(p.t * (p.hq + 2 * (int64_t)p.hkv), 8, sms, 8);
   return launch_ex(paged_append_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, st, p);
 }
@@ -1100,9 +1131,9 @@ int tc_paged_append_rope(const void* q, const void* k, const void* v, void* q_ou
   p.inv_d = 1.f / (float)d;
   const int sms = sm_count(current_device());
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = dtype == TC_F32    ? launch_paged_append<float>(p, sms, st)
-                        : dtype == TC_BF16 ? launch_paged_append<__nv_bfloat16>(p, sms, st)
-                                           : launch_paged_append<__half>(p, sms, st);
+  const cudaError_t e = dtype == TC_F32    ? launch_paged_append<float>(p, dtype, sms, st)
+                        : dtype == TC_BF16 ? launch_paged_append<__nv_bfloat16>(p, dtype, sms, st)
+                                           : launch_paged_append<__half>(p, dtype, sms, st);
   return e == cudaSuccess ? TC_OK : TC_ERR_CUDA;
 }
 
