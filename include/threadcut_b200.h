@@ -288,8 +288,8 @@ int tc_decode_attention_batched(const void* q, const void* k, const void* v, voi
  * of its n_b = lengths[b] rows (NULL: n; a length outside [0, n] is clamped) sequence b's query, its
  * newest token, sees rows j < sinks and j >= n_b - window (window >= 1 counts the newest row itself,
  * as transformers' sliding_window does; sinks >= 0). Only those rows are read. n_b == 0 gives zeros.
- * Workspace as for the other decode calls, of at least
- * tc_decode_attention_window_workspace_size(...) bytes. No counterpart in the reference, whose decode
+ * Workspace as for the other decode calls (zero prefix), of at least
+ * tc_decode_attention_window_workspace_size(...) bytes; 0 means none is needed (NULL will do). No counterpart in the reference, whose decode
  * attends to the whole cache (threadcut/flash_decode.py:57-69). */
 size_t tc_decode_attention_window_workspace_size(int batch, int hkv, int g, int d, int64_t n, int64_t window,
                                                  int64_t sinks, int splits, int dtype);

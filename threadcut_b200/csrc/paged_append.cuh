@@ -17,6 +17,9 @@ namespace tc {
 
 constexpr int kMaxAppendDim = 512;  // head size of the paged append (a warp holds a row in 2 KB of shared memory)
 
+constexpr int kAppendThreads = 128;
+constexpr int kAppendRows = 2;  // rows a thread of paged_append_vec_kernel takes
+
 struct PagedAppendParams {
   const void* q;  // [hq][t][d] with element strides (q_sh, q_st), or null
   const void* k;  // [hkv][t][d]
@@ -97,118 +100,176 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const __grid_constant
   }
 }
 
-// Rows of 16-byte chunks (p.pairs, a power of two <= 32, thread pairs of chunks a row): a thread holds a
-// chunk and its rotation partner, so a row is p.pairs threads and a warp 32 / p.pairs heads of ONE token,
-// whose cos and sin it keeps in registers for kRows rows each. Bytes are the bound; kRows rows are loaded
-// before the first is used to keep enough of them in flight.
-template <typename T, typename TT, int kRows>
-__global__ void __launch_bounds__(256) paged_append_vec_kernel(const __grid_constant__ PagedAppendParams p) {
-  constexpr int VEC = 16 / sizeof(T);
+// A 16-byte chunk as fp32 pairs and back.
+template <typename T, int VEC>
+__device__ __forceinline__ void widen(const Chunk<T, VEC>& c, float2 (&x)[VEC / 2]) {
+#pragma unroll
+  for (int e = 0; e < VEC / 2; ++e) x[e] = make_float2(to_f32(c.v[2 * e]), to_f32(c.v[2 * e + 1]));
+}
+template <typename T, int VEC>
+__device__ __forceinline__ Chunk<T, VEC> narrow(const float2 (&x)[VEC / 2]) {
+  Chunk<T, VEC> c;
+#pragma unroll
+  for (int e = 0; e < VEC / 2; ++e) {
+    if constexpr (sizeof(T) == 2) {
+      const uint32_t w = Mma<T>::pack(x[e].x, x[e].y);
+      memcpy(&c.v[2 * e], &w, 4);
+    } else {
+      c.v[2 * e] = x[e].x;
+      c.v[2 * e + 1] = x[e].y;
+    }
+  }
+  return c;
+}
+
+// Rows of 16-byte chunks: a thread holds a chunk and its rotation partner, so a row is p.pairs threads (a
+// power of two <= 32) and a warp takes 32 / p.pairs heads of ONE token at a time, kRows times: kRows query
+// rows a thread, or kRows / 2 keys and the values of the same heads. With the weight w folded into the
+// token's cos and sin once,
+//   out_a = (r x_a) (w_a cos_a) - (r x_b) (w_b sin_a),   out_b = (r x_b) (w_b cos_b) + (r x_a) (w_a sin_b),
+// a row costs three packed operations an output pair beside its conversions.
+// Bound by bytes for long chunks, by latency for short ones: resident warps count in both. 16,384 tokens of
+// 48 bf16 heads of 128 (411 MB): 2 rows a thread and 7 CTAs an SM (72 registers) 78.6 us, 5.2 TB/s; 6 CTAs 81.8,
+// 8 CTAs (spills) 83.7; 4 rows 86.9, 8 rows 102; with the formula's own order of operations, unpacked, 106.
+template <typename T, typename TT>
+__global__ void __launch_bounds__(kAppendThreads, 7)
+    paged_append_vec_kernel(const __grid_constant__ PagedAppendParams p) {
+  constexpr int kRows = kAppendRows;
+  static_assert(kRows % 2 == 0, "half of a key/value warp's rows are keys");
+  constexpr int VEC = 16 / sizeof(T), P2 = VEC / 2;
   constexpr int kTabVec = 16 / sizeof(TT);
   pdl_launch();
   pdl_wait();
   const int lane = threadIdx.x & 31;
-  const int heads = p.hq + 2 * p.hkv;
-  const int per_warp = 32 / p.pairs * kRows;  // heads a warp takes
-  const int groups = (heads + per_warp - 1) / per_warp;
-  const int64_t task = blockIdx.x * (int64_t)(blockDim.x >> 5) + (threadIdx.x >> 5);
-  const int64_t tok = task / groups;
+  const int step = 32 / p.pairs;  // heads side by side in the warp
+  const int q_groups = (p.hq + step * kRows - 1) / (step * kRows);
+  const int kv_groups = (p.hkv + step * kRows / 2 - 1) / (step * kRows / 2);
+  const int groups = q_groups + kv_groups;
+  const uint32_t task = blockIdx.x * (kAppendThreads / 32) + (threadIdx.x >> 5);
+  const uint32_t tok = task / groups;
   if (tok >= p.t) return;
-  const int head0 = (int)(task - tok * groups) * per_warp + lane / p.pairs;
+  const int grp = (int)(task - tok * groups);
+  const bool isq = grp < q_groups;
   const int c = lane & (p.pairs - 1);
   const int turned = p.rot / (2 * VEC);  // pairs that rotate; the others pass through side by side
   const bool turns = c < turned;
   const int ia = (turns ? c : 2 * c) * VEC, ib = turns ? ia + p.rot / 2 : ia + VEC;
 
-  const int64_t page = p.slots[2 * tok], row = p.slots[2 * tok + 1];
-  const bool slot = page >= 0 && page < p.num_pages && row >= 0 && row < p.page_rows;
+  // ---- the rows: this thread's row u is head h0 + u * step (keys: u < kRows / 2, then their values)
   Chunk<T, VEC> a[kRows], b[kRows];
   T* dst[kRows];
+  if (isq) {
+    const int h0 = grp * step * kRows + lane / p.pairs;
+    const T* src = static_cast<const T*>(p.q) + tok * p.q_st + h0 * p.q_sh;
+    T* out = static_cast<T*>(p.q_out) + tok * p.qo_st + h0 * p.qo_sh;
 #pragma unroll
-  for (int u = 0; u < kRows; ++u) {
-    const int hh = head0 + u * (32 / p.pairs);
-    const T* src = nullptr;
-    dst[u] = nullptr;
-    if (hh < p.hq) {
-      src = static_cast<const T*>(p.q) + hh * p.q_sh + tok * p.q_st;
-      dst[u] = static_cast<T*>(p.q_out) + hh * p.qo_sh + tok * p.qo_st;
-    } else if (hh < heads && slot) {
-      const bool isv = hh >= p.hq + p.hkv;
-      const int h = hh - p.hq - (isv ? p.hkv : 0);
-      src = isv ? static_cast<const T*>(p.v) + h * p.v_sh + tok * p.v_st
-                : static_cast<const T*>(p.k) + h * p.k_sh + tok * p.k_st;
-      dst[u] = static_cast<T*>(isv ? p.vp : p.kp) + page * p.s_page + h * p.s_h + row * p.s_row;
+    for (int u = 0; u < kRows; ++u) {
+      const bool use = h0 + u * step < p.hq;
+      dst[u] = use ? out + u * step * p.qo_sh : nullptr;
+      if (use) {
+        a[u] = ld_chunk<T, VEC>(src + u * step * p.q_sh + ia);
+        b[u] = ld_chunk<T, VEC>(src + u * step * p.q_sh + ib);
+      } else {
+        a[u] = b[u] = Chunk<T, VEC>{};
+      }
     }
-    if (src != nullptr) {
-      a[u] = ld_chunk<T, VEC>(src + ia);
-      b[u] = ld_chunk<T, VEC>(src + ib);
-    } else {
-      a[u] = b[u] = Chunk<T, VEC>{};
+  } else {
+    const int h0 = (grp - q_groups) * step * (kRows / 2) + lane / p.pairs;
+    const int2 slot = *reinterpret_cast<const int2*>(p.slots + 2 * (int64_t)tok);
+    const bool in = slot.x >= 0 && slot.x < p.num_pages && slot.y >= 0 && slot.y < p.page_rows;
+    const int64_t at = in ? slot.x * p.s_page + slot.y * p.s_row : 0;
+#pragma unroll
+    for (int u = 0; u < kRows; ++u) {
+      const bool isv = u >= kRows / 2;
+      const int h = h0 + (isv ? u - kRows / 2 : u) * step;
+      const bool use = in && h < p.hkv;
+      dst[u] = use ? static_cast<T*>(isv ? p.vp : p.kp) + at + h * p.s_h : nullptr;
+      if (use) {
+        const T* src = isv ? static_cast<const T*>(p.v) + tok * p.v_st + h * p.v_sh
+                           : static_cast<const T*>(p.k) + tok * p.k_st + h * p.k_sh;
+        a[u] = ld_chunk<T, VEC>(src + ia);
+        b[u] = ld_chunk<T, VEC>(src + ib);
+      } else {
+        a[u] = b[u] = Chunk<T, VEC>{};
+      }
     }
   }
-  float ca[VEC], cb[VEC], sa[VEC], sb[VEC];
-  if (turns && head0 < p.hq + p.hkv) {
+
+  // ---- the token's factors
+  float2 fac[P2], fas[P2], fbc[P2], fbs[P2];  // of z_a and z_b in out_a, of z_b and z_a in out_b
+  const T* w = static_cast<const T*>(isq ? p.q_w : p.k_w);
+  if (turns) {
     const TT* ct = static_cast<const TT*>(p.cos_t) + tok * p.cos_st;
     const TT* st = static_cast<const TT*>(p.sin_t) + tok * p.sin_st;
 #pragma unroll
     for (int x = 0; x < VEC; x += kTabVec) {
-      const Chunk<TT, kTabVec> t0 = ld_chunk<TT, kTabVec>(ct + ia + x), t1 = ld_chunk<TT, kTabVec>(ct + ib + x);
-      const Chunk<TT, kTabVec> t2 = ld_chunk<TT, kTabVec>(st + ia + x), t3 = ld_chunk<TT, kTabVec>(st + ib + x);
+      float2 t0[kTabVec / 2], t1[kTabVec / 2], t2[kTabVec / 2], t3[kTabVec / 2];
+      widen<TT, kTabVec>(ld_chunk<TT, kTabVec>(ct + ia + x), t0);
+      widen<TT, kTabVec>(ld_chunk<TT, kTabVec>(st + ia + x), t1);
+      widen<TT, kTabVec>(ld_chunk<TT, kTabVec>(ct + ib + x), t2);
+      widen<TT, kTabVec>(ld_chunk<TT, kTabVec>(st + ib + x), t3);
 #pragma unroll
-      for (int e = 0; e < kTabVec && x + e < VEC; ++e) {
-        ca[x + e] = to_f32(t0.v[e]);
-        cb[x + e] = to_f32(t1.v[e]);
-        sa[x + e] = to_f32(t2.v[e]);
-        sb[x + e] = to_f32(t3.v[e]);
+      for (int e = 0; e < kTabVec / 2; ++e) {
+        fac[x / 2 + e] = t0[e];
+        fas[x / 2 + e] = make_float2(-t1[e].x, -t1[e].y);
+        fbc[x / 2 + e] = t2[e];
+        fbs[x / 2 + e] = t3[e];
       }
     }
   } else {
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      ca[e] = cb[e] = 1.f;
-      sa[e] = sb[e] = 0.f;
+    for (int e = 0; e < P2; ++e) {
+      fac[e] = fbc[e] = make_float2(1.f, 1.f);
+      fas[e] = fbs[e] = make_float2(0.f, 0.f);
+    }
+  }
+  if (w != nullptr) {
+    float2 wa[P2], wb[P2];
+    widen<T, VEC>(ld_chunk<T, VEC>(w + ia), wa);
+    widen<T, VEC>(ld_chunk<T, VEC>(w + ib), wb);
+#pragma unroll
+    for (int e = 0; e < P2; ++e) {
+      fac[e] = fmul2(fac[e], wa[e]);
+      fas[e] = fmul2(fas[e], wb[e]);
+      fbc[e] = fmul2(fbc[e], wb[e]);
+      fbs[e] = fmul2(fbs[e], wa[e]);
     }
   }
 #pragma unroll
   for (int u = 0; u < kRows; ++u) {
-    const int hh = head0 + u * (32 / p.pairs);
-    const bool isq = hh < p.hq, isv = hh >= p.hq + p.hkv;
-    const T* w = static_cast<const T*>(isq ? p.q_w : p.k_w);
-    float xa[VEC], xb[VEC], ss = 0.f;
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      xa[e] = to_f32(a[u].v[e]);
-      xb[e] = to_f32(b[u].v[e]);
-      ss += xa[e] * xa[e] + xb[e] * xb[e];
-    }
-    for (int o = p.pairs >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    if (dst[u] == nullptr) continue;
-    if (!isv) {
+    if (isq || u < kRows / 2) {
+      float2 xa[P2], xb[P2];
+      widen<T, VEC>(a[u], xa);
+      widen<T, VEC>(b[u], xb);
       if (w != nullptr) {
+        float2 s2 = fmul2(xa[0], xa[0]);
+#pragma unroll
+        for (int e = 1; e < P2; ++e) s2 = ffma2(xa[e], xa[e], s2);
+#pragma unroll
+        for (int e = 0; e < P2; ++e) s2 = ffma2(xb[e], xb[e], s2);
+        float ss = s2.x + s2.y;
+        for (int o = p.pairs >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
         const float r = rsqrtf(ss * p.inv_d + p.eps);
-        const Chunk<T, VEC> wa = ld_chunk<T, VEC>(w + ia), wb = ld_chunk<T, VEC>(w + ib);
+        const float2 r2 = make_float2(r, r);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          xa[e] = xa[e] * r * to_f32(wa.v[e]);
-          xb[e] = xb[e] * r * to_f32(wb.v[e]);
-        }
-      }
-      if (turns) {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const float oa = xa[e] * ca[e] - xb[e] * sa[e];
-          xb[e] = xb[e] * cb[e] + xa[e] * sb[e];
-          xa[e] = oa;
+        for (int e = 0; e < P2; ++e) {
+          xa[e] = fmul2(xa[e], r2);
+          xb[e] = fmul2(xb[e], r2);
         }
       }
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        a[u].v[e] = from_f32<T>(xa[e]);
-        b[u].v[e] = from_f32<T>(xb[e]);
+      for (int e = 0; e < P2; ++e) {
+        const float2 oa = ffma2(xa[e], fac[e], fmul2(xb[e], fas[e]));
+        xb[e] = ffma2(xb[e], fbc[e], fmul2(xa[e], fbs[e]));
+        xa[e] = oa;
       }
+      a[u] = narrow<T, VEC>(xa);
+      b[u] = narrow<T, VEC>(xb);
     }
-    st_chunk<T, VEC>(dst[u] + ia, a[u]);
-    st_chunk<T, VEC>(dst[u] + ib, b[u]);
+    if (dst[u] != nullptr) {
+      st_chunk<T, VEC>(dst[u] + ia, a[u]);
+      st_chunk<T, VEC>(dst[u] + ib, b[u]);
+    }
   }
 }
 

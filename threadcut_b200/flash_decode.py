@@ -297,11 +297,11 @@ def decode_attention_window(q, k, v, scale, window, sinks=0, lengths=None, *, sp
     s = int(splits or 0)
     with torch.cuda.device(dev):
         nb = L.tc_decode_attention_window_workspace_size(b, hkv, g, d, n, window, sinks, s, code)
-        ws = _lib.decode_workspace(b * hkv, dev, nb)
+        ws = _lib.decode_workspace(b * hkv, dev, nb) if nb else None
         st = L.tc_decode_attention_window(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), b, hkv, g, d, n, lens_ptr, window, sinks,
             *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3], float(scale), s, code,
-            ws.data_ptr(), ws.numel(), stream_ptr(dev))
+            ws.data_ptr() if ws is not None else None, nb, stream_ptr(dev))
     check("tc_decode_attention_window", st)
     return out[0] if single else out
 
