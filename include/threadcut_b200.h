@@ -219,7 +219,7 @@ int tc_prefill_attention_window(const void* q, const void* k, const void* v, voi
  * batch: its rows meet all batch*g queries of a KV head in one matrix product. g <= 128, d <= 256, every
  * dtype, any strides with a contiguous last dimension; 16-bit, d in {64, 128, 256}, scale > 0 and 16-byte
  * aligned bases and strides run on the tcgen05 tensor cores, the rest a plain kernel. Workspace of
- * tc_decode_attention_shared_workspace_size() bytes, 16-byte aligned, with no initial contents (nothing is
+ * tc_decode_attention_shared_workspace_size() bytes, 32-byte aligned, with no initial contents (nothing is
  * kept in it between calls). The reference decodes one sequence over its own cache
  * (threadcut/flash_decode.py:57-69); this is the merge of :68-69 over the prefix and the suffix. */
 size_t tc_decode_attention_shared_workspace_size(int batch, int hkv, int g, int d, int64_t n, int64_t m, int dtype);

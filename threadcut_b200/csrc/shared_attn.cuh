@@ -8,17 +8,19 @@
 // l_p = sum_j 2^(s_j - m_p) with s_j = scale log2(e) q.k_j and m_p a running maximum: the log-sum-exp merge of
 // threadcut/flash_decode.py:68-69 over both kinds of slices.
 //
-// shared_attn_kernel: one CTA per part (prefix: KV head, tile of up to 128 query rows, slice; suffix: sequence,
-// KV head, slice), two resident per SM at d <= 128 (one waits for memory or softmax while the other
-// multiplies), each:
-//   warp 4 (one lane): TMA, the query rows once, then K and V tiles of 64 keys through a ring of slots in the
-//                      order the products take them (K0 K1 V0 K2 V1 ...).
-//   warp 5 (one lane): tcgen05.mma: S = Q K^T (128 x 64 keys x d, fp32 in TMEM, two S buffers so the next
-//                      tile's S is there when a softmax ends), O += P V with P from TMEM.
-//   warps 0-3:         softmax, a thread per query row; warps without live rows leave at once (a suffix has g
-//                      rows). The maximum is kept until a tile passes it by 2^8, so O is rescaled rarely.
+// shared_attn_kernel: a CTA per part, with
+//   one TMA lane:  the query rows once, then K and V tiles of 64 keys through a ring of slots in the order the
+//                  products take them (K0 K1 V0 K2 V1 ...);
+//   one MMA lane:  tcgen05.mma: S = Q K^T (128 x 64 keys x d, fp32 in TMEM, two S buffers so the next tile's S is
+//                  there when a softmax ends), O += P V with P from TMEM;
+//   softmax warps: a thread per query row; warps without live rows leave at once (a suffix has g rows). The
+//                  maximum is kept until a tile passes it by 2^8, so O is rescaled rarely.
+// Up to 128 rows (kLanes = 1): prefix and suffix parts in one launch, two CTAs per SM at d <= 128, one waiting for
+// memory or softmax while the other multiplies. More rows (kLanes = 2, d <= 128): each K/V tile of the prefix
+// meets two row tiles in one CTA per SM, so that it crosses from L2 once; the suffix parts are a second launch
+// that starts as the first one's CTAs leave.
 // Rows behind a slice's end inside its last tile: the scores are masked and the staged V rows zeroed, so
-// whatever memory holds there is not met. shared_merge_kernel joins the parts, a warp per query row.
+// whatever memory holds there is not met. shared_merge_kernel joins the parts.
 #pragma once
 
 #include <type_traits>
@@ -28,21 +30,22 @@
 namespace tc {
 
 constexpr int kShKeys = 64;       // keys per K/V tile
-constexpr int kShThreads = 192;   // 4 softmax warps, TMA, MMA
+constexpr int sh_threads(int lanes) { return 128 * lanes + 64; }  // softmax warps, TMA, MMA
 constexpr uint32_t kShSpin = 1u << 20;  // mbarrier polls before a wait gives up (about a second)
 constexpr float kShLazyMax = 8.f;
 
-template <int D>
+template <int D, int kLanes>
 struct SharedGeom {
+  static_assert(kLanes == 1 || D <= 128, "two lanes of D = 256 do not fit TMEM");
   static constexpr int kBoxes = D / 64;
-  static constexpr int kQBytes = 128 * D * 2;
+  static constexpr int kQBytes = 128 * D * 2;  // a lane's query rows
   static constexpr int kSlotBytes = kShKeys * D * 2;
   static constexpr int kBoxBytes = kShKeys * 128;
-  // two CTAs per SM at D <= 128 (2 x 113 KB of shared memory, 2 x 256 TMEM columns), one at D = 256
-  static constexpr int kSlots = D == 64 ? 10 : 5;
-  static constexpr int kCtasPerSm = D == 256 ? 1 : 2;
-  static constexpr int kTmemCols = D == 256 ? 512 : 256;
-  static constexpr int kSmem = 1024 + kQBytes + kSlots * kSlotBytes;
+  // 113 KB of shared memory and 256 TMEM columns, twice an SM; or 225 KB and 512 columns once
+  static constexpr int kSlots = (D == 64 ? 10 : 5) * kLanes;
+  static constexpr int kCtasPerSm = D == 256 || kLanes == 2 ? 1 : 2;
+  static constexpr int kTmemCols = D == 256 || kLanes == 2 ? 512 : 256;
+  static constexpr int kSmem = 1024 + kLanes * kQBytes + kSlots * kSlotBytes;
 };
 
 struct SharedParams {
@@ -58,23 +61,31 @@ struct SharedParams {
   int bt;           // sequences per prefix row tile (128 / g)
   int row_tiles;    // cdiv(batch, bt)
   int n, m;
-  int np;           // prefix parts per (KV head, row tile); the first hkv*row_tiles*np CTAs
+  int np;           // prefix parts per (KV head, row tile or pair of them): the CTAs below prefix_ctas
   int ns;           // suffix parts per (sequence, KV head)
+  int prefix_ctas;  // of this launch
+  int wait_last;    // this launch runs beside the one before it, which waited for everything it reads
   float c;          // scale * log2(e)
   float* o;         // [np + ns][batch*hkv*g][d] unnormalised
   float2* ml;       // [np + ns][batch*hkv*g] (maximum in log2, sum)
 };
 
+// 32 bytes to a 32-byte aligned address: a whole sector a thread.
+__device__ __forceinline__ void st_v8(float* p, const uint32_t* v) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+
 // mbarriers and flags of a CTA.
-template <int kSlots>
+template <int kSlots, int kLanes>
 struct SharedCtl {
-  uint64_t q_full, full[kSlots], empty[kSlots], s_full[2], p_full[2], pv_done[2], fin;
+  uint64_t q_full, full[kSlots], empty[kSlots], s_full[kLanes][2], p_full[kLanes][2], pv_done[kLanes][2], fin;
   uint32_t tmem;
-  int abort;
 };
 
 __device__ __forceinline__ int shared_suffix(const SharedParams& p, int b) {
-  const int len = p.lengths != nullptr ? p.lengths[b] : p.m;
+  const int len = p.lengths != nullptr ? __ldcg(p.lengths + b) : p.m;
   return len < 0 ? 0 : (len > p.m ? p.m : len);
 }
 
@@ -84,80 +95,98 @@ __device__ __forceinline__ void shared_range(int tiles, int s, int np, int& t0, 
   t1 = (int)((int64_t)tiles * (s + 1) / np);
 }
 
-template <typename T, int D, bool kPaged>
-__global__ void __launch_bounds__(kShThreads, SharedGeom<D>::kCtasPerSm)
+template <typename T, int D, bool kPaged, int kLanes>
+__global__ void __launch_bounds__(sh_threads(kLanes), SharedGeom<D, kLanes>::kCtasPerSm)
     shared_attn_kernel(const __grid_constant__ SharedParams p) {
-  using G = SharedGeom<D>;
+  using G = SharedGeom<D, kLanes>;
+  using Ctl = SharedCtl<G::kSlots, kLanes>;
   constexpr int kSlots = G::kSlots;
+  constexpr int kTmaWarp = 4 * kLanes, kMmaWarp = kTmaWarp + 1;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   // All shared memory is dynamic, so that two CTAs fit an SM: the tiles from the first 1 KB boundary on,
   // and the control block in whichever part of the 1 KB of slack is not spent on reaching it.
   extern __shared__ uint8_t smem_raw[];
   const uint32_t gap = (1024 - (smem_u32(smem_raw) & 1023)) & 1023;
-  uint8_t* smem = smem_raw + gap;
-  uint8_t* sQ = smem;                // D/64 boxes of 128 rows x 128 B
-  uint8_t* sKV = smem + G::kQBytes;  // slot s: D/64 boxes of 64 rows x 128 B
-  static_assert(sizeof(SharedCtl<kSlots>) <= 512, "the control block must fit either side of the tiles");
-  SharedCtl<kSlots>& ctl =
-      *reinterpret_cast<SharedCtl<kSlots>*>(gap >= 512 ? smem_raw : sKV + kSlots * G::kSlotBytes);
-  uint64_t &q_full = ctl.q_full, &fin = ctl.fin;
-  uint64_t *full = ctl.full, *empty = ctl.empty, *s_full = ctl.s_full, *p_full = ctl.p_full, *pv_done = ctl.pv_done;
-  volatile int& s_abort = ctl.abort;
+  uint8_t* sQ = smem_raw + gap;              // lane x at +kQBytes*x: D/64 boxes of 128 rows x 128 B
+  uint8_t* sKV = sQ + kLanes * G::kQBytes;   // slot s: D/64 boxes of 64 rows x 128 B
+  static_assert(sizeof(Ctl) <= 512, "the control block must fit either side of the tiles");
+  Ctl& ctl = *reinterpret_cast<Ctl*>(gap >= 512 ? smem_raw : sKV + kSlots * G::kSlotBytes);
+  uint64_t *full = ctl.full, *empty = ctl.empty;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  pdl_launch();
-  pdl_wait();  // queries, lengths, tables and the cache may be the previous kernel's
   // ---- this CTA's part
-  const int prefix_parts = p.hkv * p.row_tiles * p.np;
-  const bool prefix = (int)blockIdx.x < prefix_parts;
-  int part, h, b0, live, t0, t1, end;  // b0: first sequence of the rows; live: query rows; end: keys of the source
+  const bool prefix = (int)blockIdx.x < p.prefix_ctas;
+  int part, h, b0, s0 = 0, lanes = 1;  // b0: first sequence of lane 0's rows; lanes: row tiles present
+  int live[kLanes];                    // query rows of each lane
   if (prefix) {
-    // row tiles of one slice are neighbours in the launch order: the second finds K and V in L2
+    // row tiles of one slice are neighbours in the launch order
+    const int groups = (p.row_tiles + kLanes - 1) / kLanes;
     int i = blockIdx.x;
-    b0 = (i % p.row_tiles) * p.bt;
-    i /= p.row_tiles;
+    const int rt = (i % groups) * kLanes;
+    i /= groups;
     h = i % p.hkv;
     part = i / p.hkv;
-    live = (p.batch - b0 < p.bt ? p.batch - b0 : p.bt) * p.g;
-    end = p.n;
-    shared_range(kPaged ? (p.n_tiles + 1) / 2 : (p.n + kShKeys - 1) / kShKeys, part, p.np, t0, t1);
+    b0 = rt * p.bt;
+    if (kLanes == 2 && rt + 1 < p.row_tiles) lanes = 2;
+#pragma unroll
+    for (int x = 0; x < kLanes; ++x) {
+      const int left = p.batch - b0 - x * p.bt;
+      live[x] = left <= 0 ? 0 : (left < p.bt ? left : p.bt) * p.g;
+    }
   } else {
-    int i = blockIdx.x - prefix_parts;
-    const int s = i % p.ns;
+    int i = blockIdx.x - p.prefix_ctas;
+    s0 = i % p.ns;
     i /= p.ns;
     h = i % p.hkv;
     b0 = i / p.hkv;
-    live = p.g;
-    end = shared_suffix(p, b0);
-    shared_range((end + kShKeys - 1) / kShKeys, s, p.ns, t0, t1);
-    part = p.np + s;
+    live[0] = p.g;
+    if (kLanes == 2) live[kLanes - 1] = 0;
+    part = p.np + s0;
   }
-  const int nt = t1 - t0;
-  if (nt == 0) return;  // nothing in this slice; the merge knows and skips it
-  const bool paged = kPaged && prefix;
-  const int nlive = (live + 31) >> 5;  // softmax warps with rows
-
+  const CUtensorMap* mq = prefix ? &p.tmq : &p.tmq1;
+  const CUtensorMap* mk = prefix ? &p.tmkp : &p.tmk;
+  const CUtensorMap* mv = prefix ? &p.tmvp : &p.tmv;
   if (threadIdx.x == 0) {
-    mbar_init(&q_full, 1);
+    mbar_init(&ctl.q_full, 1);
     for (int s = 0; s < kSlots; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
-    for (int s = 0; s < 2; ++s) {
-      mbar_init(&s_full[s], 1);
-      mbar_init(&p_full[s], nlive);
-      mbar_init(&pv_done[s], 1);
-    }
-    mbar_init(&fin, 1);
+#pragma unroll
+    for (int x = 0; x < kLanes; ++x)
+      for (int s = 0; s < 2; ++s) {
+        mbar_init(&ctl.s_full[x][s], 1);
+        mbar_init(&ctl.p_full[x][s], live[x] > 0 ? (live[x] + 31) >> 5 : 1);  // softmax warps with rows
+        mbar_init(&ctl.pv_done[x][s], 1);
+      }
+    mbar_init(&ctl.fin, 1);
     fence_mbar_init();
-    s_abort = 0;
   }
   if (warp == 0) tmem_alloc(&ctl.tmem, G::kTmemCols);
+  if (warp == kTmaWarp && lane == 0) {
+    prefetch_tensormap(mq);
+    prefetch_tensormap(mk);
+    prefetch_tensormap(mv);
+  }
   tmem_fence_before();
   __syncthreads();
   tmem_fence_after();
-  const uint32_t tmem = ctl.tmem;         // S buffer x (and P over it) at +64x, O at +128
-  const uint32_t tO = tmem + 128;
+  const uint32_t tmem = ctl.tmem;  // lane x from +256x: S buffer i (and P over it) at +64i, O at +128
+  // Queries, lengths, tables and the cache may be the previous kernel's. A launch beside its predecessor
+  // (wait_last) starts when every CTA of that one is past its own wait, so only its end has to be ordered:
+  // the merge behind it needs the parts of both.
+  if (!p.wait_last) pdl_wait();
+  pdl_launch();
+  int t0, t1, end;  // this part's key tiles, and the keys of its source
+  if (prefix) {
+    end = p.n;
+    shared_range(kPaged ? (p.n_tiles + 1) / 2 : (p.n + kShKeys - 1) / kShKeys, part, p.np, t0, t1);
+  } else {
+    end = shared_suffix(p, b0);
+    shared_range((end + kShKeys - 1) / kShKeys, s0, p.ns, t0, t1);
+  }
+  const int nt = t1 - t0;  // 0: nothing in this slice, every role falls through; the merge knows and skips it
+  const bool paged = kPaged && prefix;
   // Place of K_j and V_j in the ring's order K0 K1 V0 K2 V1 ... (the order the products take them).
   auto k_at = [](int j) { return j < 2 ? j : 2 * j - 1; };
   auto v_at = [nt](int j) { return j < nt - 1 ? 2 * j + 2 : 2 * nt - 1; };
@@ -172,20 +201,18 @@ __global__ void __launch_bounds__(kShThreads, SharedGeom<D>::kCtasPerSm)
     return make_int3(page, row, rows);
   };
 
-  if (warp == 4) {
+  if (nt > 0 && warp == kTmaWarp) {
     // ---------------- TMA
     if (lane == 0) {
-      const uint64_t pol = policy_evict_first(), keep = policy_evict_last();
-      const CUtensorMap* mq = prefix ? &p.tmq : &p.tmq1;
-      const CUtensorMap* mk = prefix ? &p.tmkp : &p.tmk;
-      const CUtensorMap* mv = prefix ? &p.tmvp : &p.tmv;
-      const uint64_t kvpol = prefix && p.row_tiles > 1 ? keep : pol;  // read again by the next row tile
-      mbar_arrive_expect_tx(&q_full, (uint32_t)(G::kBoxes * 128 * p.g * (prefix ? p.bt : 1)));
-      for (int bx = 0; bx < G::kBoxes; ++bx) tma_load_4d(sQ + bx * 16384, mq, bx * 64, 0, b0, h, &q_full, pol);
+      const uint64_t pol = policy_evict_first();
+      mbar_arrive_expect_tx(&ctl.q_full, (uint32_t)(lanes * G::kBoxes * 128 * p.g * (prefix ? p.bt : 1)));
+      for (int x = 0; x < lanes; ++x)
+        for (int bx = 0; bx < G::kBoxes; ++bx)
+          tma_load_4d(sQ + x * G::kQBytes + bx * 16384, mq, bx * 64, 0, b0 + x * p.bt, h, &ctl.q_full, pol);
       int armed = 0;
       auto load = [&](const CUtensorMap* map, int t) -> bool {
         const int s = armed % kSlots, r = armed / kSlots;
-        if (s_abort || (r > 0 && !mbar_wait(&empty[s], (r - 1) & 1, TC_DEVERR_PIPE_TIMEOUT, kShSpin))) return false;
+        if (r > 0 && !mbar_wait(&empty[s], (r - 1) & 1, TC_DEVERR_PIPE_TIMEOUT, kShSpin)) return false;
         mbar_arrive_expect_tx(&full[s], (uint32_t)G::kSlotBytes);
         uint8_t* st = sKV + s * G::kSlotBytes;
         if (paged) {
@@ -193,67 +220,78 @@ __global__ void __launch_bounds__(kShThreads, SharedGeom<D>::kCtasPerSm)
           for (int c = 0; c < 2; ++c) {
             const int3 e = sub(t, c);
             for (int bx = 0; bx < G::kBoxes; ++bx)
-              tma_load_4d(st + bx * G::kBoxBytes + c * 4096, map, bx * 64, e.y, h, e.x, &full[s], kvpol);
+              tma_load_4d(st + bx * G::kBoxBytes + c * 4096, map, bx * 64, e.y, h, e.x, &full[s], pol);
           }
         } else {
           for (int bx = 0; bx < G::kBoxes; ++bx)
-            tma_load_4d(st + bx * G::kBoxBytes, map, bx * 64, t * kShKeys, h, prefix ? 0 : b0, &full[s], kvpol);
+            tma_load_4d(st + bx * G::kBoxBytes, map, bx * 64, t * kShKeys, h, prefix ? 0 : b0, &full[s], pol);
         }
         ++armed;
         return true;
       };
       bool ok = load(mk, t0) && (nt < 2 || load(mk, t0 + 1));
       for (int j = 0; ok && j < nt; ++j) ok = load(mv, t0 + j) && (j + 2 >= nt || load(mk, t0 + j + 2));
-      if (!ok) s_abort = 1;
-      // copies still in flight after an abort must land before the CTA leaves (normally these phases
+      // copies still in flight after a wait gave up must land before the CTA leaves (normally these phases
       // completed long ago and the waits return at once)
       for (int i = armed - kSlots > 0 ? armed - kSlots : 0; i < armed; ++i)
         mbar_wait(&full[i % kSlots], (i / kSlots) & 1, TC_DEVERR_PIPE_TIMEOUT, kShSpin);
-      mbar_wait(&q_full, 0, TC_DEVERR_PIPE_TIMEOUT, kShSpin);
+      mbar_wait(&ctl.q_full, 0, TC_DEVERR_PIPE_TIMEOUT, kShSpin);
     }
-  } else if (warp == 5) {
-    // ---------------- tcgen05.mma: S(0) S(1), then per tile P V(j), S(j + 2). Products of one thread run
-    // in issue order, so S(j + 2) overwrites P(j) only after P V(j) read it.
-    if (lane == 0) {
+  } else if (nt > 0 && warp == kMmaWarp) {
+    if (elect_one()) {
+      // ---------------- tcgen05.mma: S(0) S(1), then per tile and lane P V(j), S(j + 2). Products of one thread
+      // run in issue order, so S(j + 2) overwrites P(j) only after P V(j) read it. This thread's waits and issues
+      // set the pace of a CTA with two lanes: elect_one() keeps its descriptors uniform.
       const uint32_t idS = umma_idesc_f16(kBf16, false, 128, kShKeys);
       const uint32_t idO = umma_idesc_f16(kBf16, true, 128, D);
-      const uint32_t q0 = smem_u32(sQ), kv0 = smem_u32(sKV);
-      auto wait_slot = [&](int i) {
-        return !s_abort && mbar_wait(&full[i % kSlots], (i / kSlots) & 1, TC_DEVERR_PIPE_TIMEOUT, kShSpin);
-      };
-      auto issue_s = [&](int j) -> bool {
-        const int i = k_at(j);
-        if (!wait_slot(i)) return false;
+      // descriptors of the first K step; a byte offset of 16n adds n (the address field does not overflow)
+      const uint64_t dq = umma_desc_sw128(smem_u32(sQ), 16, 1024);
+      const uint64_t dk = umma_desc_sw128(smem_u32(sKV), 16, 1024);
+      const uint64_t dv = umma_desc_sw128(smem_u32(sKV), G::kBoxBytes, 1024);
+      auto wait = [&](uint64_t* bar, int phase) { return mbar_wait(bar, phase & 1, TC_DEVERR_PIPE_TIMEOUT, kShSpin); };
+      auto wait_slot = [&](int i) { return wait(&full[i % kSlots], i / kSlots); };
+      auto issue_s = [&](int x, int j) -> bool {
+        const int i = k_at(j), s = i % kSlots;
+        if (x == 0 && !wait_slot(i)) return false;
         tmem_fence_after();
-        const uint32_t k0 = kv0 + (i % kSlots) * G::kSlotBytes;
+        const uint64_t q = dq + x * (G::kQBytes >> 4), k = dk + s * (G::kSlotBytes >> 4);
+#pragma unroll
         for (int kd = 0; kd < D / 16; ++kd)
-          umma_f16(tmem + 64 * (j & 1), umma_desc_sw128(q0 + (kd >> 2) * 16384 + (kd & 3) * 32, 16, 1024),
-                   umma_desc_sw128(k0 + (kd >> 2) * G::kBoxBytes + (kd & 3) * 32, 16, 1024), idS, kd > 0);
-        umma_commit(&empty[i % kSlots]);
-        umma_commit(&s_full[j & 1]);
+          umma_f16(tmem + 256 * x + 64 * (j & 1), q + (((kd >> 2) * 16384 + (kd & 3) * 32) >> 4),
+                   k + (((kd >> 2) * G::kBoxBytes + (kd & 3) * 32) >> 4), idS, kd > 0);
+        if (x == lanes - 1) umma_commit(&empty[s]);
+        umma_commit(&ctl.s_full[x][j & 1]);
         return true;
       };
-      bool ok = mbar_wait(&q_full, 0, TC_DEVERR_PIPE_TIMEOUT, kShSpin) && issue_s(0) && (nt < 2 || issue_s(1));
+      bool ok = wait(&ctl.q_full, 0);
+      for (int j = 0; j < 2 && j < nt; ++j)
+        for (int x = 0; ok && x < lanes; ++x) ok = issue_s(x, j);
       for (int j = 0; ok && j < nt; ++j) {
-        const int i = v_at(j);
-        ok = wait_slot(i) && mbar_wait(&p_full[j & 1], (j >> 1) & 1, TC_DEVERR_PIPE_TIMEOUT, kShSpin);
-        if (!ok) break;
-        tmem_fence_after();
-        const uint32_t v0 = kv0 + (i % kSlots) * G::kSlotBytes;
-        for (int kk = 0; kk < kShKeys / 16; ++kk)
-          umma_f16_tmem_a(tO, tmem + 64 * (j & 1) + kk * 8, umma_desc_sw128(v0 + kk * 2048, G::kBoxBytes, 1024), idO,
-                          j > 0 || kk > 0);
-        umma_commit(&empty[i % kSlots]);
-        umma_commit(&pv_done[j & 1]);
-        if (j + 2 < nt) ok = issue_s(j + 2);
+        const int i = v_at(j), s = i % kSlots;
+        for (int x = 0; ok && x < lanes; ++x) {
+          ok = (x > 0 || wait_slot(i)) && wait(&ctl.p_full[x][j & 1], j >> 1);
+          if (!ok) break;
+          tmem_fence_after();
+          const uint64_t v = dv + s * (G::kSlotBytes >> 4);
+#pragma unroll
+          for (int kk = 0; kk < kShKeys / 16; ++kk)
+            umma_f16_tmem_a(tmem + 256 * x + 128, tmem + 256 * x + 64 * (j & 1) + kk * 8, v + ((kk * 2048) >> 4), idO,
+                            j > 0 || kk > 0);
+          if (x == lanes - 1) umma_commit(&empty[s]);
+          umma_commit(&ctl.pv_done[x][j & 1]);
+          if (j + 2 < nt) ok = issue_s(x, j + 2);
+        }
       }
-      if (!ok) s_abort = 1;
-      umma_commit(&fin);  // completes once every product issued above has
+      umma_commit(&ctl.fin);  // completes once every product issued above has
     }
-  } else if (warp < nlive) {
-    // ---------------- softmax: thread = TMEM lane = query row (sequence b0 + row / g, head row % g)
-    const int row = warp * 32 + lane;
-    const uint32_t lb = (uint32_t)(warp * 32) << 16;
+  } else if (nt > 0 && warp < 4 * kLanes && (warp & 3) * 32 < live[kLanes == 2 ? warp >> 2 : 0]) {
+    // ---------------- softmax: thread = TMEM lane = query row of lane x (sequence bx0 + row / g, head row % g)
+    const int x = kLanes == 2 ? warp >> 2 : 0, row = (warp & 3) * 32 + lane;
+    const int rows_live = live[x], bx0 = b0 + x * p.bt;
+    const int zero_threads = ((rows_live + 31) >> 5) * 32;  // threads of this lane's softmax
+    const uint32_t lb = ((uint32_t)((warp & 3) * 32) << 16) + 256 * x;
+    const uint32_t tO = tmem + 128;
+    uint64_t *s_full = ctl.s_full[x], *p_full = ctl.p_full[x], *pv_done = ctl.pv_done[x];
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     for (int j = 0; j < nt; ++j) {
@@ -269,7 +307,7 @@ __global__ void __launch_bounds__(kShThreads, SharedGeom<D>::kCtasPerSm)
         v1 = left < 64 ? (left > 32 ? left - 32 : 0) : 32;
       }
       // warp-uniform: tcgen05.ld/st and the votes below are warp-collective
-      ok = __all_sync(0xffffffffu, !s_abort && mbar_wait(&s_full[j & 1], (j >> 1) & 1, TC_DEVERR_PIPE_TIMEOUT, kShSpin));
+      ok = __all_sync(0xffffffffu, mbar_wait(&s_full[j & 1], (j >> 1) & 1, TC_DEVERR_PIPE_TIMEOUT, kShSpin));
       if (!ok) break;
       tmem_fence_after();
       uint32_t v[2][32];
@@ -287,8 +325,8 @@ __global__ void __launch_bounds__(kShThreads, SharedGeom<D>::kCtasPerSm)
         ok = __all_sync(0xffffffffu, mbar_wait(&full[i % kSlots], (i / kSlots) & 1, TC_DEVERR_PIPE_TIMEOUT, kShSpin));
         if (!ok) break;
         uint8_t* st = sKV + (i % kSlots) * G::kSlotBytes;
-        for (int x = row; x < kShKeys * (D / 8); x += nlive * 32) {
-          const int r = x / (D / 8), cc = x % (D / 8);
+        for (int y = row; y < kShKeys * (D / 8); y += zero_threads) {
+          const int r = y / (D / 8), cc = y % (D / 8);
           if ((r & 31) >= (r < 32 ? v0 : v1))
             *reinterpret_cast<uint4*>(st + (cc >> 3) * G::kBoxBytes + r * 128 + (cc & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
         }
@@ -323,7 +361,7 @@ __global__ void __launch_bounds__(kShThreads, SharedGeom<D>::kCtasPerSm)
       m = mn;
       if (j >= 1 && __any_sync(0xffffffffu, alpha != 1.f)) {
         // O holds P V of the tiles before j once P V(j - 1) is done (P V(j) waits for this warp)
-        ok = __all_sync(0xffffffffu, !s_abort && mbar_wait(&pv_done[(j - 1) & 1], ((j - 1) >> 1) & 1, TC_DEVERR_PIPE_TIMEOUT, kShSpin));
+        ok = __all_sync(0xffffffffu, mbar_wait(&pv_done[(j - 1) & 1], ((j - 1) >> 1) & 1, TC_DEVERR_PIPE_TIMEOUT, kShSpin));
         if (!ok) break;
         tmem_fence_after();
 #pragma unroll
@@ -342,38 +380,35 @@ __global__ void __launch_bounds__(kShThreads, SharedGeom<D>::kCtasPerSm)
       if (lane == 0) mbar_arrive(&p_full[j & 1]);
     }
     if (ok)
-      ok = __all_sync(0xffffffffu, !s_abort && mbar_wait(&fin, 0, TC_DEVERR_PIPE_TIMEOUT, kShSpin));
-    if (!ok) {
-      s_abort = 1;
-    } else {
+      ok = __all_sync(0xffffffffu, mbar_wait(&ctl.fin, 0, TC_DEVERR_PIPE_TIMEOUT, kShSpin));
+    if (ok) {
       tmem_fence_after();
       const int64_t rows = (int64_t)p.batch * p.hkv * p.g;
       const int bi = row / p.g;
-      const int64_t r = ((int64_t)(b0 + bi) * p.hkv + h) * p.g + (row - bi * p.g);
+      const int64_t r = ((int64_t)(bx0 + bi) * p.hkv + h) * p.g + (row - bi * p.g);
       float* orow = p.o + ((int64_t)part * rows + r) * D;
 #pragma unroll
       for (int cch = 0; cch < D / 32; ++cch) {
         uint32_t o[32];
         tmem_ld32(tO + lb + cch * 32, o);
         tmem_wait_ld();
-        if (row < live) {
+        if (row < rows_live) {
 #pragma unroll
-          for (int q4 = 0; q4 < 8; ++q4)
-            *reinterpret_cast<uint4*>(orow + cch * 32 + q4 * 4) =
-                make_uint4(o[4 * q4], o[4 * q4 + 1], o[4 * q4 + 2], o[4 * q4 + 3]);
+          for (int q8 = 0; q8 < 4; ++q8) st_v8(orow + cch * 32 + q8 * 8, o + 8 * q8);
         }
       }
-      if (row < live) p.ml[(int64_t)part * rows + r] = make_float2(m, l);
+      if (row < rows_live) p.ml[(int64_t)part * rows + r] = make_float2(m, l);
     }
   }
   // every product has completed before the TMEM columns are freed (bounded: a lost commit only errs)
   tmem_fence_before();
   __syncthreads();
   if (warp == 0) {
-    mbar_wait(&fin, 0, TC_DEVERR_PIPE_TIMEOUT, kShSpin);
+    if (nt > 0) mbar_wait(&ctl.fin, 0, TC_DEVERR_PIPE_TIMEOUT, kShSpin);
     tmem_fence_after();
     tmem_dealloc(tmem, G::kTmemCols);
   }
+  if (p.wait_last) pdl_wait();
 }
 
 struct SharedMergeParams {
@@ -383,34 +418,39 @@ struct SharedMergeParams {
   void* out;
   int64_t so_b, so_h, so_g;
   int batch, hkv, g, m, np, ns;
+  int wpr;  // warps per query row
 };
 
-// One warp per query row: lane l folds the float4 columns l, l + 32, ...; parts in a fixed order.
+// p.wpr warps per query row (a power of two <= 8, eight warps a CTA): warp w of a row folds parts w, w + wpr, ...,
+// lane l the float4 columns l, l + 32, ...; the warps' states are joined in shared memory in their order.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) shared_merge_kernel(const __grid_constant__ SharedMergeParams p) {
   constexpr int kCols = D / 4, kPer = (kCols + 31) / 32;  // float4 columns, per lane
-  constexpr int kLoads = 8;
+  constexpr int kLoads = 4;
+  __shared__ float s_m[8], s_l[8];
+  __shared__ float4 s_a[8][kCols];
   pdl_launch();
   pdl_wait();
-  const int lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t rows = (int64_t)p.batch * p.hkv * p.g;
-  const int64_t r = blockIdx.x * (int64_t)(blockDim.x >> 5) + (threadIdx.x >> 5);
-  if (r >= rows) return;
-  const int i = (int)(r % p.g), h = (int)(r / p.g % p.hkv), b = (int)(r / p.g / p.hkv);
+  const int64_t r = blockIdx.x * (int64_t)(8 / p.wpr) + warp / p.wpr;
+  const bool row = r < rows;
+  const int i = (int)(r % p.g), h = (int)(r / p.g % p.hkv), b = row ? (int)(r / p.g / p.hkv) : 0;
   int len = p.lengths != nullptr ? p.lengths[b] : p.m;
   len = len < 0 ? 0 : (len > p.m ? p.m : len);
   const int tiles = (len + kShKeys - 1) / kShKeys;
+  const int parts = row ? p.np + p.ns : 0;
   float M = -INFINITY, L = 0.f;
   float4 A[kPer];
 #pragma unroll
   for (int x = 0; x < kPer; ++x) A[x] = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int s0 = 0; s0 < p.np + p.ns; s0 += kLoads) {
+  for (int p0 = warp & (p.wpr - 1); p0 < parts; p0 += kLoads * p.wpr) {
     float2 ml[kLoads];
     float4 o[kLoads][kPer];
 #pragma unroll
     for (int k = 0; k < kLoads; ++k) {
-      const int s = s0 + k;
-      bool use = s < p.np + p.ns;
+      const int s = p0 + k * p.wpr;
+      bool use = s < parts;
       if (use && s >= p.np) {
         int t0, t1;
         shared_range(tiles, s - p.np, p.ns, t0, t1);
@@ -450,6 +490,37 @@ __global__ void __launch_bounds__(256) shared_merge_kernel(const __grid_constant
     }
     M = mc;
   }
+  if (p.wpr > 1) {
+    if (lane == 0) {
+      s_m[warp] = M;
+      s_l[warp] = L;
+    }
+#pragma unroll
+    for (int x = 0; x < kPer; ++x)
+      if (lane + 32 * x < kCols) s_a[warp][lane + 32 * x] = A[x];
+    __syncthreads();
+    if ((warp & (p.wpr - 1)) != 0) return;
+    float Mt = M;
+    for (int w = 1; w < p.wpr; ++w) Mt = fmaxf(Mt, s_m[warp + w]);
+    L = 0.f;
+#pragma unroll
+    for (int x = 0; x < kPer; ++x) A[x] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int w = 0; w < p.wpr; ++w) {
+      const float f = s_m[warp + w] == -INFINITY ? 0.f : fast_exp2(s_m[warp + w] - Mt);
+      L += f * s_l[warp + w];
+#pragma unroll
+      for (int x = 0; x < kPer; ++x) {
+        if (lane + 32 * x < kCols) {
+          const float4 v = s_a[warp + w][lane + 32 * x];
+          A[x].x += f * v.x;
+          A[x].y += f * v.y;
+          A[x].z += f * v.z;
+          A[x].w += f * v.w;
+        }
+      }
+    }
+  }
+  if (!row) return;
   const float inv = L == 0.f ? 0.f : 1.f / L;
   T* out = static_cast<T*>(p.out) + b * p.so_b + h * p.so_h + i * p.so_g;
 #pragma unroll

@@ -156,6 +156,13 @@ __device__ __forceinline__ uint32_t umma_idesc_f16(bool bf16, bool b_mn_major, i
   return (1u << 4) | (fmt << 7) | (fmt << 10) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) |
          ((uint32_t)(M >> 4) << 24);
 }
+// True in one lane of a converged warp, in a form the compiler knows to be one thread: code under it keeps
+// warp-uniform operands (descriptors, addresses) in uniform registers.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t pred;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(pred));
+  return pred != 0;
+}
 // D[tmem] (+)= A . B for one K=16 step; issued by a single thread.
 __device__ __forceinline__ void umma_f16(uint32_t tmem_d, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
                                          bool accumulate) {
