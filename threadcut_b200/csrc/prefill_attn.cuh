@@ -214,22 +214,27 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const __grid_con
     }
   } else if (warp == 9) {
     // ---------------- tcgen05.mma issue: per K/V tile S_0, S_1, P V_0, P V_1
-    if (lane == 0) {
+    if (elect_one()) {
       const uint32_t idS = umma_idesc_f16(kBf16, false, 128, 128);
       const uint32_t idO = umma_idesc_f16(kBf16, true, 128, D);
+      // descriptors of the first K step of stage 0; a byte offset of 16n adds n (the address field holds it)
+      const uint64_t dq = umma_desc_sw128(smem_u32(sQ), 16, 1024);
+      const uint64_t dk = umma_desc_sw128(smem_u32(sKV), 16, 1024);
+      const uint64_t dv = umma_desc_sw128(smem_u32(sKV) + kTileB, 16384, 1024);
       auto issue_s = [&](int x, int j) {  // S_x = Q_x K_j^T over d in steps of 16
-        const uint32_t q0 = smem_u32(sQ + x * kTileB), k0 = smem_u32(sKV + (j & 1) * 2 * kTileB);
+        const uint64_t q = dq + x * (kTileB >> 4), k = dk + (j & 1) * (2 * kTileB >> 4);
+#pragma unroll
         for (int kd = 0; kd < D / 16; ++kd) {
-          const uint32_t o = (uint32_t)((kd >> 2) * 16384 + (kd & 3) * 32);
-          umma_f16(tmem + pf_col_s(x), umma_desc_sw128(q0 + o, 16, 1024), umma_desc_sw128(k0 + o, 16, 1024), idS,
-                   kd > 0);
+          const int o = ((kd >> 2) * 16384 + (kd & 3) * 32) >> 4;
+          umma_f16(tmem + pf_col_s(x), q + o, k + o, idS, kd > 0);
         }
       };
       auto issue_pv = [&](int x, int j) {  // O_x (+)= P_x V_j, P_x from TMEM (8 columns per 16 keys)
-        const uint32_t v0 = smem_u32(sKV + (j & 1) * 2 * kTileB + kTileB);
+        const uint64_t v = dv + (j & 1) * (2 * kTileB >> 4);
+#pragma unroll
         for (int kk = 0; kk < 8; ++kk)
-          umma_f16_tmem_a(tmem + pf_col_o(x), tmem + pf_col_s(x) + (uint32_t)(kk * 8),
-                          umma_desc_sw128(v0 + kk * 2048, 16384, 1024), idO, j > 0 || kk > 0);
+          umma_f16_tmem_a(tmem + pf_col_o(x), tmem + pf_col_s(x) + (uint32_t)(kk * 8), v + (kk * 2048 >> 4), idO,
+                          j > 0 || kk > 0);
       };
       // tcgen05.mma ops of one thread run in issue order, so S_x(j+1) may be issued straight after
       // the P V_x(j) that reads P_x(j) from the same columns.

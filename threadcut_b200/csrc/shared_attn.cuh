@@ -8,17 +8,18 @@
 // l_p = sum_j 2^(s_j - m_p) with s_j = scale log2(e) q.k_j and m_p a running maximum: the log-sum-exp merge of
 // threadcut/flash_decode.py:68-69 over both kinds of slices.
 //
-// shared_attn_kernel: a CTA per part, with
-//   one TMA lane:  the query rows once, then K and V tiles of 64 keys through a ring of slots in the order the
-//                  products take them (K0 K1 V0 K2 V1 ...);
-//   one MMA lane:  tcgen05.mma: S = Q K^T (128 x 64 keys x d, fp32 in TMEM, two S buffers so the next tile's S is
-//                  there when a softmax ends), O += P V with P from TMEM;
-//   softmax warps: a thread per query row; warps without live rows leave at once (a suffix has g rows). The
-//                  maximum is kept until a tile passes it by 2^8, so O is rescaled rarely.
-// Up to 128 rows (kLanes = 1): prefix and suffix parts in one launch, two CTAs per SM at d <= 128, one waiting for
-// memory or softmax while the other multiplies. More rows (kLanes = 2, d <= 128): each K/V tile of the prefix
-// meets two row tiles in one CTA per SM, so that it crosses from L2 once; the suffix parts are a second launch
-// that starts as the first one's CTAs leave.
+// shared_attn_kernel: a CTA per part (prefix: KV head, tile of up to 128 query rows, slice; suffix: sequence, KV
+// head, slice), two resident per SM at d <= 128, one waiting for memory or softmax while the other multiplies:
+//   warp 4 (one lane): TMA, the query rows once, then K and V tiles of 64 keys through a ring of slots in the
+//                      order the products take them (K0 K1 V0 K2 V1 ...).
+//   warp 5 (one lane): tcgen05.mma: S = Q K^T (128 x 64 keys x d, fp32 in TMEM, two S buffers so the next tile's S
+//                      is there when a softmax ends), O += P V with P from TMEM.
+//   warps 0-3:         softmax, a thread per query row; warps without live rows leave at once (a suffix has g
+//                      rows). The maximum is kept until a tile passes it by 2^8, so O is rescaled rarely.
+// Up to 128 rows the loop runs at the DRAM's pace (b = 1 over 98,304 rows: 66 us, 6.1 TB/s); with more, each row tile
+// fetches the tiles from L2 again and 256 rows take 118 us for 98,304 keys. One CTA an SM that multiplied each tile
+// with two row tiles moved half the bytes from L2 and took 125 us: its two chains of softmax and products, not
+// the fetches, set the pace, and two smaller CTAs overlap start and end better (16,384 keys: 39 us against 50).
 // Rows behind a slice's end inside its last tile: the scores are masked and the staged V rows zeroed, so
 // whatever memory holds there is not met. shared_merge_kernel joins the parts.
 #pragma once
@@ -30,22 +31,21 @@
 namespace tc {
 
 constexpr int kShKeys = 64;       // keys per K/V tile
-constexpr int sh_threads(int lanes) { return 128 * lanes + 64; }  // softmax warps, TMA, MMA
+constexpr int kShThreads = 192;   // 4 softmax warps, TMA, MMA
 constexpr uint32_t kShSpin = 1u << 20;  // mbarrier polls before a wait gives up (about a second)
 constexpr float kShLazyMax = 8.f;
 
-template <int D, int kLanes>
+template <int D>
 struct SharedGeom {
-  static_assert(kLanes == 1 || D <= 128, "two lanes of D = 256 do not fit TMEM");
   static constexpr int kBoxes = D / 64;
-  static constexpr int kQBytes = 128 * D * 2;  // a lane's query rows
+  static constexpr int kQBytes = 128 * D * 2;
   static constexpr int kSlotBytes = kShKeys * D * 2;
   static constexpr int kBoxBytes = kShKeys * 128;
-  // 113 KB of shared memory and 256 TMEM columns, twice an SM; or 225 KB and 512 columns once
-  static constexpr int kSlots = (D == 64 ? 10 : 5) * kLanes;
-  static constexpr int kCtasPerSm = D == 256 || kLanes == 2 ? 1 : 2;
-  static constexpr int kTmemCols = D == 256 || kLanes == 2 ? 512 : 256;
-  static constexpr int kSmem = 1024 + kLanes * kQBytes + kSlots * kSlotBytes;
+  // two CTAs per SM at D <= 128 (2 x 113 KB of shared memory, 2 x 256 TMEM columns), one at D = 256
+  static constexpr int kSlots = D == 64 ? 10 : 5;
+  static constexpr int kCtasPerSm = D == 256 ? 1 : 2;
+  static constexpr int kTmemCols = D == 256 ? 512 : 256;
+  static constexpr int kSmem = 1024 + kQBytes + kSlots * kSlotBytes;
 };
 
 struct SharedParams {
@@ -61,10 +61,8 @@ struct SharedParams {
   int bt;           // sequences per prefix row tile (128 / g)
   int row_tiles;    // cdiv(batch, bt)
   int n, m;
-  int np;           // prefix parts per (KV head, row tile or pair of them): the CTAs below prefix_ctas
+  int np;           // prefix parts per (KV head, row tile): the first hkv*row_tiles*np CTAs
   int ns;           // suffix parts per (sequence, KV head)
-  int prefix_ctas;  // of this launch
-  int wait_last;    // this launch runs beside the one before it, which waited for everything it reads
   float c;          // scale * log2(e)
   float* o;         // [np + ns][batch*hkv*g][d] unnormalised
   float2* ml;       // [np + ns][batch*hkv*g] (maximum in log2, sum)
@@ -78,9 +76,9 @@ __device__ __forceinline__ void st_v8(float* p, const uint32_t* v) {
 }
 
 // mbarriers and flags of a CTA.
-template <int kSlots, int kLanes>
+template <int kSlots>
 struct SharedCtl {
-  uint64_t q_full, full[kSlots], empty[kSlots], s_full[kLanes][2], p_full[kLanes][2], pv_done[kLanes][2], fin;
+  uint64_t q_full, full[kSlots], empty[kSlots], s_full[2], p_full[2], pv_done[2], fin;
   uint32_t tmem;
 };
 
@@ -95,54 +93,47 @@ __device__ __forceinline__ void shared_range(int tiles, int s, int np, int& t0, 
   t1 = (int)((int64_t)tiles * (s + 1) / np);
 }
 
-template <typename T, int D, bool kPaged, int kLanes>
-__global__ void __launch_bounds__(sh_threads(kLanes), SharedGeom<D, kLanes>::kCtasPerSm)
+template <typename T, int D, bool kPaged>
+__global__ void __launch_bounds__(kShThreads, SharedGeom<D>::kCtasPerSm)
     shared_attn_kernel(const __grid_constant__ SharedParams p) {
-  using G = SharedGeom<D, kLanes>;
-  using Ctl = SharedCtl<G::kSlots, kLanes>;
+  using G = SharedGeom<D>;
+  using Ctl = SharedCtl<G::kSlots>;
   constexpr int kSlots = G::kSlots;
-  constexpr int kTmaWarp = 4 * kLanes, kMmaWarp = kTmaWarp + 1;
+  constexpr int kTmaWarp = 4, kMmaWarp = 5;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   // All shared memory is dynamic, so that two CTAs fit an SM: the tiles from the first 1 KB boundary on,
   // and the control block in whichever part of the 1 KB of slack is not spent on reaching it.
   extern __shared__ uint8_t smem_raw[];
   const uint32_t gap = (1024 - (smem_u32(smem_raw) & 1023)) & 1023;
-  uint8_t* sQ = smem_raw + gap;              // lane x at +kQBytes*x: D/64 boxes of 128 rows x 128 B
-  uint8_t* sKV = sQ + kLanes * G::kQBytes;   // slot s: D/64 boxes of 64 rows x 128 B
+  uint8_t* sQ = smem_raw + gap;      // D/64 boxes of 128 rows x 128 B
+  uint8_t* sKV = sQ + G::kQBytes;    // slot s: D/64 boxes of 64 rows x 128 B
   static_assert(sizeof(Ctl) <= 512, "the control block must fit either side of the tiles");
   Ctl& ctl = *reinterpret_cast<Ctl*>(gap >= 512 ? smem_raw : sKV + kSlots * G::kSlotBytes);
-  uint64_t *full = ctl.full, *empty = ctl.empty;
+  uint64_t *full = ctl.full, *empty = ctl.empty, *s_full = ctl.s_full, *p_full = ctl.p_full, *pv_done = ctl.pv_done;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   // ---- this CTA's part
-  const bool prefix = (int)blockIdx.x < p.prefix_ctas;
-  int part, h, b0, s0 = 0, lanes = 1;  // b0: first sequence of lane 0's rows; lanes: row tiles present
-  int live[kLanes];                    // query rows of each lane
+  const int prefix_ctas = p.hkv * p.row_tiles * p.np;
+  const bool prefix = (int)blockIdx.x < prefix_ctas;
+  int part, h, b0, s0 = 0, live;  // b0: first sequence of the rows; live: query rows
   if (prefix) {
-    // row tiles of one slice are neighbours in the launch order
-    const int groups = (p.row_tiles + kLanes - 1) / kLanes;
+    // row tiles of one slice are neighbours in the launch order: the later finds K and V in L2
     int i = blockIdx.x;
-    const int rt = (i % groups) * kLanes;
-    i /= groups;
+    b0 = (i % p.row_tiles) * p.bt;
+    i /= p.row_tiles;
     h = i % p.hkv;
     part = i / p.hkv;
-    b0 = rt * p.bt;
-    if (kLanes == 2 && rt + 1 < p.row_tiles) lanes = 2;
-#pragma unroll
-    for (int x = 0; x < kLanes; ++x) {
-      const int left = p.batch - b0 - x * p.bt;
-      live[x] = left <= 0 ? 0 : (left < p.bt ? left : p.bt) * p.g;
-    }
+    live = (p.batch - b0 < p.bt ? p.batch - b0 : p.bt) * p.g;
   } else {
-    int i = blockIdx.x - p.prefix_ctas;
+    int i = blockIdx.x - prefix_ctas;
     s0 = i % p.ns;
     i /= p.ns;
     h = i % p.hkv;
     b0 = i / p.hkv;
-    live[0] = p.g;
-    if (kLanes == 2) live[kLanes - 1] = 0;
+    live = p.g;
     part = p.np + s0;
   }
+  const int nlive = (live + 31) >> 5;  // softmax warps with rows
   const CUtensorMap* mq = prefix ? &p.tmq : &p.tmq1;
   const CUtensorMap* mk = prefix ? &p.tmkp : &p.tmk;
   const CUtensorMap* mv = prefix ? &p.tmvp : &p.tmv;
@@ -152,13 +143,11 @@ __global__ void __launch_bounds__(sh_threads(kLanes), SharedGeom<D, kLanes>::kCt
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
-#pragma unroll
-    for (int x = 0; x < kLanes; ++x)
-      for (int s = 0; s < 2; ++s) {
-        mbar_init(&ctl.s_full[x][s], 1);
-        mbar_init(&ctl.p_full[x][s], live[x] > 0 ? (live[x] + 31) >> 5 : 1);  // softmax warps with rows
-        mbar_init(&ctl.pv_done[x][s], 1);
-      }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&s_full[s], 1);
+      mbar_init(&p_full[s], nlive);
+      mbar_init(&pv_done[s], 1);
+    }
     mbar_init(&ctl.fin, 1);
     fence_mbar_init();
   }
@@ -171,12 +160,10 @@ __global__ void __launch_bounds__(sh_threads(kLanes), SharedGeom<D, kLanes>::kCt
   tmem_fence_before();
   __syncthreads();
   tmem_fence_after();
-  const uint32_t tmem = ctl.tmem;  // lane x from +256x: S buffer i (and P over it) at +64i, O at +128
-  // Queries, lengths, tables and the cache may be the previous kernel's. A launch beside its predecessor
-  // (wait_last) starts when every CTA of that one is past its own wait, so only its end has to be ordered:
-  // the merge behind it needs the parts of both.
-  if (!p.wait_last) pdl_wait();
+  const uint32_t tmem = ctl.tmem;  // S buffer i (and P over it) at +64i, O at +128
+  const uint32_t tO = tmem + 128;
   pdl_launch();
+  pdl_wait();  // queries, lengths, tables and the cache may be the previous kernel's
   int t0, t1, end;  // this part's key tiles, and the keys of its source
   if (prefix) {
     end = p.n;
@@ -205,10 +192,8 @@ __global__ void __launch_bounds__(sh_threads(kLanes), SharedGeom<D, kLanes>::kCt
     // ---------------- TMA
     if (lane == 0) {
       const uint64_t pol = policy_evict_first();
-      mbar_arrive_expect_tx(&ctl.q_full, (uint32_t)(lanes * G::kBoxes * 128 * p.g * (prefix ? p.bt : 1)));
-      for (int x = 0; x < lanes; ++x)
-        for (int bx = 0; bx < G::kBoxes; ++bx)
-          tma_load_4d(sQ + x * G::kQBytes + bx * 16384, mq, bx * 64, 0, b0 + x * p.bt, h, &ctl.q_full, pol);
+      mbar_arrive_expect_tx(&ctl.q_full, (uint32_t)(G::kBoxes * 128 * p.g * (prefix ? p.bt : 1)));
+      for (int bx = 0; bx < G::kBoxes; ++bx) tma_load_4d(sQ + bx * 16384, mq, bx * 64, 0, b0, h, &ctl.q_full, pol);
       int armed = 0;
       auto load = [&](const CUtensorMap* map, int t) -> bool {
         const int s = armed % kSlots, r = armed / kSlots;
@@ -238,10 +223,10 @@ __global__ void __launch_bounds__(sh_threads(kLanes), SharedGeom<D, kLanes>::kCt
       mbar_wait(&ctl.q_full, 0, TC_DEVERR_PIPE_TIMEOUT, kShSpin);
     }
   } else if (nt > 0 && warp == kMmaWarp) {
+    // ---------------- tcgen05.mma: S(0) S(1), then per tile P V(j), S(j + 2). Products of one thread run in issue
+    // order, so S(j + 2) overwrites P(j) only after P V(j) read it. K and V are waited for before P, while the
+    // softmax works: each wait costs this thread some 200 cycles even when the phase is long over.
     if (elect_one()) {
-      // ---------------- tcgen05.mma: S(0) S(1), then per tile and lane P V(j), S(j + 2). Products of one thread
-      // run in issue order, so S(j + 2) overwrites P(j) only after P V(j) read it. This thread's waits and issues
-      // set the pace of a CTA with two lanes: elect_one() keeps its descriptors uniform.
       const uint32_t idS = umma_idesc_f16(kBf16, false, 128, kShKeys);
       const uint32_t idO = umma_idesc_f16(kBf16, true, 128, D);
       // descriptors of the first K step; a byte offset of 16n adds n (the address field does not overflow)
@@ -250,48 +235,40 @@ __global__ void __launch_bounds__(sh_threads(kLanes), SharedGeom<D, kLanes>::kCt
       const uint64_t dv = umma_desc_sw128(smem_u32(sKV), G::kBoxBytes, 1024);
       auto wait = [&](uint64_t* bar, int phase) { return mbar_wait(bar, phase & 1, TC_DEVERR_PIPE_TIMEOUT, kShSpin); };
       auto wait_slot = [&](int i) { return wait(&full[i % kSlots], i / kSlots); };
-      auto issue_s = [&](int x, int j) -> bool {
-        const int i = k_at(j), s = i % kSlots;
-        if (x == 0 && !wait_slot(i)) return false;
-        tmem_fence_after();
-        const uint64_t q = dq + x * (G::kQBytes >> 4), k = dk + s * (G::kSlotBytes >> 4);
+      auto issue_s = [&](int j) {
+        const int s = k_at(j) % kSlots;
+        const uint64_t k = dk + s * (G::kSlotBytes >> 4);
 #pragma unroll
         for (int kd = 0; kd < D / 16; ++kd)
-          umma_f16(tmem + 256 * x + 64 * (j & 1), q + (((kd >> 2) * 16384 + (kd & 3) * 32) >> 4),
+          umma_f16(tmem + 64 * (j & 1), dq + (((kd >> 2) * 16384 + (kd & 3) * 32) >> 4),
                    k + (((kd >> 2) * G::kBoxBytes + (kd & 3) * 32) >> 4), idS, kd > 0);
-        if (x == lanes - 1) umma_commit(&empty[s]);
-        umma_commit(&ctl.s_full[x][j & 1]);
-        return true;
+        umma_commit(&empty[s]);
+        umma_commit(&s_full[j & 1]);
       };
       bool ok = wait(&ctl.q_full, 0);
-      for (int j = 0; j < 2 && j < nt; ++j)
-        for (int x = 0; ok && x < lanes; ++x) ok = issue_s(x, j);
+      for (int j = 0; ok && j < 2 && j < nt; ++j) {
+        ok = wait_slot(k_at(j));
+        if (ok) issue_s(j);
+      }
       for (int j = 0; ok && j < nt; ++j) {
-        const int i = v_at(j), s = i % kSlots;
-        for (int x = 0; ok && x < lanes; ++x) {
-          ok = (x > 0 || wait_slot(i)) && wait(&ctl.p_full[x][j & 1], j >> 1);
-          if (!ok) break;
-          tmem_fence_after();
-          const uint64_t v = dv + s * (G::kSlotBytes >> 4);
+        const int s = v_at(j) % kSlots;
+        ok = wait_slot(v_at(j)) && (j + 2 >= nt || wait_slot(k_at(j + 2))) && wait(&p_full[j & 1], j >> 1);
+        if (!ok) break;
+        tmem_fence_after();
+        const uint64_t v = dv + s * (G::kSlotBytes >> 4);
 #pragma unroll
-          for (int kk = 0; kk < kShKeys / 16; ++kk)
-            umma_f16_tmem_a(tmem + 256 * x + 128, tmem + 256 * x + 64 * (j & 1) + kk * 8, v + ((kk * 2048) >> 4), idO,
-                            j > 0 || kk > 0);
-          if (x == lanes - 1) umma_commit(&empty[s]);
-          umma_commit(&ctl.pv_done[x][j & 1]);
-          if (j + 2 < nt) ok = issue_s(x, j + 2);
-        }
+        for (int kk = 0; kk < kShKeys / 16; ++kk)
+          umma_f16_tmem_a(tO, tmem + 64 * (j & 1) + kk * 8, v + ((kk * 2048) >> 4), idO, j > 0 || kk > 0);
+        umma_commit(&empty[s]);
+        umma_commit(&pv_done[j & 1]);
+        if (j + 2 < nt) issue_s(j + 2);
       }
       umma_commit(&ctl.fin);  // completes once every product issued above has
     }
-  } else if (nt > 0 && warp < 4 * kLanes && (warp & 3) * 32 < live[kLanes == 2 ? warp >> 2 : 0]) {
-    // ---------------- softmax: thread = TMEM lane = query row of lane x (sequence bx0 + row / g, head row % g)
-    const int x = kLanes == 2 ? warp >> 2 : 0, row = (warp & 3) * 32 + lane;
-    const int rows_live = live[x], bx0 = b0 + x * p.bt;
-    const int zero_threads = ((rows_live + 31) >> 5) * 32;  // threads of this lane's softmax
-    const uint32_t lb = ((uint32_t)((warp & 3) * 32) << 16) + 256 * x;
-    const uint32_t tO = tmem + 128;
-    uint64_t *s_full = ctl.s_full[x], *p_full = ctl.p_full[x], *pv_done = ctl.pv_done[x];
+  } else if (nt > 0 && warp < nlive) {
+    // ---------------- softmax: thread = TMEM lane = query row (sequence b0 + row / g, head row % g)
+    const int row = threadIdx.x;
+    const uint32_t lb = (uint32_t)(warp * 32) << 16;
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     for (int j = 0; j < nt; ++j) {
@@ -325,7 +302,7 @@ __global__ void __launch_bounds__(sh_threads(kLanes), SharedGeom<D, kLanes>::kCt
         ok = __all_sync(0xffffffffu, mbar_wait(&full[i % kSlots], (i / kSlots) & 1, TC_DEVERR_PIPE_TIMEOUT, kShSpin));
         if (!ok) break;
         uint8_t* st = sKV + (i % kSlots) * G::kSlotBytes;
-        for (int y = row; y < kShKeys * (D / 8); y += zero_threads) {
+        for (int y = row; y < kShKeys * (D / 8); y += nlive * 32) {
           const int r = y / (D / 8), cc = y % (D / 8);
           if ((r & 31) >= (r < 32 ? v0 : v1))
             *reinterpret_cast<uint4*>(st + (cc >> 3) * G::kBoxBytes + r * 128 + (cc & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
@@ -385,19 +362,19 @@ __global__ void __launch_bounds__(sh_threads(kLanes), SharedGeom<D, kLanes>::kCt
       tmem_fence_after();
       const int64_t rows = (int64_t)p.batch * p.hkv * p.g;
       const int bi = row / p.g;
-      const int64_t r = ((int64_t)(bx0 + bi) * p.hkv + h) * p.g + (row - bi * p.g);
+      const int64_t r = ((int64_t)(b0 + bi) * p.hkv + h) * p.g + (row - bi * p.g);
       float* orow = p.o + ((int64_t)part * rows + r) * D;
 #pragma unroll
       for (int cch = 0; cch < D / 32; ++cch) {
         uint32_t o[32];
         tmem_ld32(tO + lb + cch * 32, o);
         tmem_wait_ld();
-        if (row < rows_live) {
+        if (row < live) {
 #pragma unroll
           for (int q8 = 0; q8 < 4; ++q8) st_v8(orow + cch * 32 + q8 * 8, o + 8 * q8);
         }
       }
-      if (row < rows_live) p.ml[(int64_t)part * rows + r] = make_float2(m, l);
+      if (row < live) p.ml[(int64_t)part * rows + r] = make_float2(m, l);
     }
   }
   // every product has completed before the TMEM columns are freed (bounded: a lost commit only errs)
@@ -408,7 +385,6 @@ __global__ void __launch_bounds__(sh_threads(kLanes), SharedGeom<D, kLanes>::kCt
     tmem_fence_after();
     tmem_dealloc(tmem, G::kTmemCols);
   }
-  if (p.wait_last) pdl_wait();
 }
 
 struct SharedMergeParams {

@@ -2100,9 +2100,8 @@ namespace {
 // Parts of the tcgen05 shared-prefix decode and its workspace.
 struct SharedPlan {
   int bt = 1, row_tiles = 1;  // sequences per prefix row tile, row tiles
-  int lanes = 1;              // row tiles per prefix CTA
   int np = 0, ns = 0;         // parts of the prefix, of each suffix
-  int64_t prefix_ctas = 0, suffix_ctas = 0;
+  int64_t ctas = 0;
   size_t ml = 0, bytes = 0;   // offset of the (maximum, sum) array; total
 };
 
@@ -2113,63 +2112,64 @@ int parts_of(int64_t tiles, int64_t per_part) {
   return (int)(n < kShMaxParts ? n : kShMaxParts);
 }
 
+// The number of parts with the least estimated time, in key tiles of a slot. A CTA costs its tiles and about
+// kShCtaTiles more (start and end); the prefix parts are dispatched first and the suffixes, of 0.6 of the longest
+// on average (the host does not know the lengths), fill the slots beside and behind them; the parts' fp32 rows
+// are written and read, at half the pace of tiles. `groups` (KV head, row tile) pairs of tp tiles, `tails` suffixes
+// of up to ts. Chosen for, and measured with 8 KV heads of 128, bf16: 8 sequences, 16,384 + 700 tokens, 22 to 24 prefix
+// parts (one wave) 20.8 us, 26 parts (a few CTAs too many) 25.0; 32 sequences, 8,192 + 16: 13 parts 20.5 us, 26 parts 22.6,
+// 64 parts 32.3; 64 sequences, 16,384 + 1,024: 6 parts 53 us, 4 parts 71, 18 parts 63.
+constexpr double kShCtaTiles = 6.0;
+constexpr double kShTileBytes = 32768.0;
+
+void plan_shared_parts(SharedPlan& w, int64_t groups, int64_t tails, int64_t tp, int64_t ts, int64_t row_floats,
+                       int64_t slots) {
+  double best = 0.0;
+  bool first = true;
+  for (int parts = 1; parts <= kShMaxParts; ++parts) {
+    // tiles a part: the prefix's share, or, without a prefix, the suffix's
+    const int64_t x = cdiv(tp > 0 ? tp : (ts > 0 ? ts : 1), parts);
+    if (x < 2 && !first) break;
+    const int np = parts_of(tp, x), ns = parts_of(ts, x);
+    const double a = (double)x + kShCtaTiles, s = (ns > 0 ? 0.6 * (double)ts / ns : 0.0) + kShCtaTiles;
+    const int64_t prefix = groups * np, rest = prefix % slots;
+    double t = (double)(prefix / slots) * a;  // full waves of prefix parts
+    double left = (double)(tails * ns);
+    if (rest > 0) {  // the last one, with suffixes beside it
+      t += a;
+      left -= (double)(slots - rest) * (double)(int64_t)(a / s);
+    }
+    if (left > 0) t += left * s / (double)slots + s / 2;
+    t += 2.0 * (np + ns) * (double)row_floats * 2.0 * sizeof(float) / (kShTileBytes * (double)slots);
+    if (first || t < best) {
+      best = t;
+      w.np = np;
+      w.ns = ns;
+      first = false;
+    }
+  }
+}
+
 SharedPlan plan_shared(int batch, int hkv, int g, int d, int64_t n, int64_t m) {
   SharedPlan w;
   w.bt = 128 / g;
   w.row_tiles = (int)cdiv(batch, w.bt);
-  const int64_t sms = sm_count(current_device()), slots = sms * (d == 256 ? 1 : 2);
+  const int64_t slots = (int64_t)sm_count(current_device()) * (d == 256 ? 1 : 2);
   const int64_t tp = cdiv(n, kShKeys), ts = cdiv(m, kShKeys);
-  if (w.row_tiles > 1 && d <= 128 && n > 0) {
-    // the prefix by itself, in whole waves of one CTA an SM, then the suffixes
-    w.lanes = 2;
-    const int64_t groups = hkv * cdiv(w.row_tiles, 2);
-    int64_t parts = sms / groups;
-    if (parts < 1) parts = 1;
-    w.np = parts_of(tp, cdiv(tp, parts) < 4 ? 4 : cdiv(tp, parts));
-    w.ns = parts_of(ts, cdiv((int64_t)batch * hkv * ts, slots) < 4 ? 4 : cdiv((int64_t)batch * hkv * ts, slots));
-    w.prefix_ctas = groups * w.np;
-  } else {
-    // parts of about equal length, as many as are resident at once
-    int64_t x = cdiv(hkv * (w.row_tiles * tp + batch * ts), slots);
-    if (x < 2) x = 2;
-    w.np = parts_of(tp, x);
-    w.ns = parts_of(ts, x);
-    w.prefix_ctas = (int64_t)hkv * w.row_tiles * w.np;
-  }
-  w.suffix_ctas = (int64_t)batch * hkv * w.ns;
+  plan_shared_parts(w, (int64_t)hkv * w.row_tiles, (int64_t)batch * hkv, tp, ts, (int64_t)batch * hkv * g * d, slots);
+  w.ctas = (int64_t)hkv * ((int64_t)w.row_tiles * w.np + (int64_t)batch * w.ns);
   const size_t rows = (size_t)batch * hkv * g, parts = (size_t)(w.np + w.ns);
   w.ml = round256(sizeof(float) * parts * rows * d);
   w.bytes = w.ml + round256(sizeof(float2) * parts * rows);
   return w;
 }
 
-template <typename T, int D, int kLanes>
-cudaError_t launch_shared_part(SharedParams& p, int64_t prefix_ctas, int64_t ctas, bool wait_last, int dev,
-                               cudaStream_t st) {
-  const auto fn = p.tiles != nullptr && prefix_ctas > 0 ? shared_attn_kernel<T, D, true, kLanes>
-                                                        : shared_attn_kernel<T, D, false, kLanes>;
-  const int smem = SharedGeom<D, kLanes>::kSmem;
-  const cudaError_t e = set_smem(reinterpret_cast<const void*>(fn), smem, dev);
-  if (e != cudaSuccess || ctas == 0) return e;
-  p.prefix_ctas = (int)prefix_ctas;
-  p.wait_last = wait_last;
-  return launch_ex(fn, dim3((unsigned)ctas), dim3(sh_threads(kLanes)), smem, st, p);
-}
-
 template <typename T, int D>
-cudaError_t launch_shared_t(SharedParams& p, SharedMergeParams& mp, const SharedPlan& w, int dev, cudaStream_t st) {
-  cudaError_t e;
-  if constexpr (D <= 128) {
-    if (w.lanes == 2) {
-      e = launch_shared_part<T, D, 2>(p, w.prefix_ctas, w.prefix_ctas, false, dev, st);
-      // beside it, not behind it; without programmatic launches the stream orders the two
-      if (e == cudaSuccess) e = launch_shared_part<T, D, 1>(p, 0, w.suffix_ctas, pdl_enabled(), dev, st);
-    } else {
-      e = launch_shared_part<T, D, 1>(p, w.prefix_ctas, w.prefix_ctas + w.suffix_ctas, false, dev, st);
-    }
-  } else {
-    e = launch_shared_part<T, D, 1>(p, w.prefix_ctas, w.prefix_ctas + w.suffix_ctas, false, dev, st);
-  }
+cudaError_t launch_shared_t(const SharedParams& p, SharedMergeParams& mp, int64_t ctas, int dev, cudaStream_t st) {
+  const auto fn = p.tiles != nullptr ? shared_attn_kernel<T, D, true> : shared_attn_kernel<T, D, false>;
+  const int smem = SharedGeom<D>::kSmem;
+  cudaError_t e = set_smem(reinterpret_cast<const void*>(fn), smem, dev);
+  if (e == cudaSuccess && ctas > 0) e = launch_ex(fn, dim3((unsigned)ctas), dim3(kShThreads), smem, st, p);
   if (e != cudaSuccess) return e;
   const int64_t rows = (int64_t)p.batch * p.hkv * p.g;
   mp.wpr = 1;  // each warp takes about four parts, one round of loads
@@ -2178,12 +2178,12 @@ cudaError_t launch_shared_t(SharedParams& p, SharedMergeParams& mp, const Shared
 }
 
 template <typename T>
-cudaError_t dispatch_shared(SharedParams& p, SharedMergeParams& mp, const SharedPlan& w, int d, int dev,
+cudaError_t dispatch_shared(const SharedParams& p, SharedMergeParams& mp, int64_t ctas, int d, int dev,
                             cudaStream_t st) {
   switch (d) {
-    case 64: return launch_shared_t<T, 64>(p, mp, w, dev, st);
-    case 128: return launch_shared_t<T, 128>(p, mp, w, dev, st);
-    case 256: return launch_shared_t<T, 256>(p, mp, w, dev, st);
+    case 64: return launch_shared_t<T, 64>(p, mp, ctas, dev, st);
+    case 128: return launch_shared_t<T, 128>(p, mp, ctas, dev, st);
+    case 256: return launch_shared_t<T, 256>(p, mp, ctas, dev, st);
   }
   return cudaErrorInvalidValue;
 }
@@ -2221,7 +2221,7 @@ bool shared_tc5(const SharedCall& c) {
 // Runs the tcgen05 kernel and the merge; -1 where a tensor map cannot describe the call's strides.
 int run_shared_tc5(const SharedCall& c, void* workspace, size_t workspace_bytes, cudaStream_t st) {
   const SharedPlan w = plan_shared(c.batch, c.hkv, c.g, c.d, c.n, c.m);
-  if (w.prefix_ctas + w.suffix_ctas > INT32_MAX) return TC_ERR_INVALID;
+  if (w.ctas > INT32_MAX) return TC_ERR_INVALID;
   SharedParams p;
   std::memset(&p, 0, sizeof(p));
   const int64_t qd[4] = {c.d, c.g, c.batch, c.hkv};
@@ -2280,8 +2280,8 @@ int run_shared_tc5(const SharedCall& c, void* workspace, size_t workspace_bytes,
   mp.np = w.np;
   mp.ns = w.ns;
   const int dev = current_device();
-  const cudaError_t e = c.dtype == TC_BF16 ? dispatch_shared<__nv_bfloat16>(p, mp, w, c.d, dev, st)
-                                           : dispatch_shared<__half>(p, mp, w, c.d, dev, st);
+  const cudaError_t e = c.dtype == TC_BF16 ? dispatch_shared<__nv_bfloat16>(p, mp, w.ctas, c.d, dev, st)
+                                           : dispatch_shared<__half>(p, mp, w.ctas, c.d, dev, st);
   return e == cudaSuccess ? TC_OK : TC_ERR_CUDA;
 }
 }  // namespace
