@@ -48,8 +48,8 @@ constexpr int kPfKeys = 128;      // keys per K/V tile
 constexpr int kPfThreads = 384;   // warps 0-3 / 4-7 softmax of Q tile 0 / 1, 8 TMA, 9 MMA, 10-11 idle
 // Registers per thread after the warpgroup split (setmaxnreg): the launch gives 384 x 168 = 64512,
 // softmax warpgroups 2 x 128 x 232 + the TMA/MMA warpgroup 128 x 40 = 64512.
-constexpr int kPfRegsSoftmax = 232;
-constexpr int kPfRegsOther = 40;
+constexpr int kPfRegsSoftmax = 224;
+constexpr int kPfRegsOther = 56;
 constexpr int kPfGroup = 4;       // query heads per KV head handled by the kernel
 constexpr int pf_smem(int d) { return 1024 + (kPfTiles + 4) * 256 * d; }  // alignment slack, Q tiles, 2 K/V stages
 constexpr uint32_t kPfSpin = 1u << 20;  // mbarrier polls before a wait gives up (about a second)
@@ -147,6 +147,10 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const __grid_con
   __syncthreads();
   tmem_fence_after();
   const uint32_t tmem = s_tmem;
+  if constexpr (kWindow) {  // launched with programmatic dependent launch
+    pdl_launch();
+    pdl_wait();
+  }
 
   if (warp >= 8) {
     reg_dealloc<kPfRegsOther>();
@@ -447,6 +451,47 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const __grid_con
     tmem_fence_after();
     tmem_dealloc(tmem, 512);
   }
+}
+
+struct WindowMergeParams {
+  const float* o;    // [parts][rows][d] normalised partials
+  const float* lse;  // [parts][rows] natural log; -inf: nothing
+  void* out;         // [rows][d] contiguous
+  int parts;
+  int64_t rows;
+};
+
+// Log-sum-exp merge of a windowed prefill's KV splits, a warp per row. (One CTA per row, as the merge of few
+// decode rows has it, took about 30 us for the 16,384 rows of a 512-token chunk of 32 heads; this takes ???.)
+template <typename T, int D>
+__global__ void __launch_bounds__(256) window_merge_kernel(const __grid_constant__ WindowMergeParams p) {
+  constexpr int kPer = D / 64;  // float2 columns per lane
+  pdl_launch();
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const int64_t row = blockIdx.x * (int64_t)8 + (threadIdx.x >> 5);
+  if (row >= p.rows) return;
+  const float mine = lane < p.parts ? p.lse[lane * p.rows + row] : -INFINITY;  // at most 16 parts
+  const float M = warp_max(mine);
+  const float w = mine == -INFINITY ? 0.f : __expf(mine - M);
+  const float total = warp_sum(w);
+  const float inv = total > 0.f ? 1.f / total : 0.f;
+  float2 a[kPer];
+#pragma unroll
+  for (int x = 0; x < kPer; ++x) a[x] = make_float2(0.f, 0.f);
+  for (int s = 0; s < p.parts; ++s) {
+    const float ws = __shfl_sync(0xffffffffu, w, s) * inv;
+    const float2* o = reinterpret_cast<const float2*>(p.o + (s * p.rows + row) * D);
+#pragma unroll
+    for (int x = 0; x < kPer; ++x) {
+      const float2 v = __ldcg(o + lane + 32 * x);
+      a[x].x += ws * v.x;
+      a[x].y += ws * v.y;
+    }
+  }
+  uint32_t* out = reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + row * D);
+#pragma unroll
+  for (int x = 0; x < kPer; ++x) out[lane + 32 * x] = Mma<T>::pack(a[x].x, a[x].y);
 }
 
 }  // namespace tc

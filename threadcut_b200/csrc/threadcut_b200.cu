@@ -1405,6 +1405,7 @@ cudaError_t launch_prefill_t(const PrefillParams& p, dim3 grid, int dev, cudaStr
   const auto fn = prefill_kernel<T, D, kPaged, kWindow>;
   const cudaError_t e = set_smem(reinterpret_cast<const void*>(fn), pf_smem(D), dev);
   if (e != cudaSuccess) return e;
+  if constexpr (kWindow) return launch_ex(fn, grid, dim3(kPfThreads), pf_smem(D), s, p);
   fn<<<grid, kPfThreads, pf_smem(D), s>>>(p);
   return cudaGetLastError();
 }
@@ -2030,18 +2031,16 @@ struct WindowPrefill {
   int splits = 1;
 };
 
-// `tiles`: key tiles that the busiest query block visits.
+// KV splits with the least estimated time, in key tiles: waves of one CTA an SM, each CTA its share of the
+// `tiles` that the busiest query block visits and about three more for its start and end, and the merge.
 int window_splits(int64_t ctas, int64_t tiles, int sms) {
-  if (ctas >= 2 * (int64_t)sms) return 1;
   int best = 1;
-  double best_eff = 0.0;
-  for (int s = 1; s <= 16 && (s == 1 || tiles / s >= 4); ++s) {
-    const int64_t waves = cdiv(ctas * s, sms);
-    const double eff = (double)(ctas * s) / (double)(waves * sms);
-    if (eff >= 0.95) return s;
-    if (eff > best_eff + 0.02) {
-      best_eff = eff;
+  double best_t = 0.0;
+  for (int s = 1; s <= 16 && s <= tiles; ++s) {
+    const double t = (double)cdiv(ctas * s, sms) * ((double)tiles / s + 3.0) + (s > 1 ? 2.0 : 0.0);
+    if (s == 1 || t < best_t) {
       best = s;
+      best_t = t;
     }
   }
   return best;
@@ -2091,8 +2090,16 @@ int run_window_prefill(PrefillParams& p, const WindowPrefill& w, int batch, int 
   const cudaError_t e = dtype == TC_BF16 ? launch_window_prefill_t<__nv_bfloat16>(p, d, paged, grid, dev, st)
                                          : launch_window_prefill_t<__half>(p, d, paged, grid, dev, st);
   if (e != cudaSuccess) return TC_ERR_CUDA;
-  if (w.splits > 1) return tc_merge_partials(p.o_part, p.lse_part, p.out, nullptr, w.splits, rows, d, d, dtype, st);
-  return TC_OK;
+  if (w.splits == 1) return TC_OK;
+  const WindowMergeParams mp = {p.o_part, p.lse_part, p.out, w.splits, rows};
+  const dim3 mgrid((unsigned)cdiv(rows, 8)), mblock(256);
+  const bool bf16 = dtype == TC_BF16;
+  const cudaError_t me =
+      d == 64 ? (bf16 ? launch_ex(window_merge_kernel<__nv_bfloat16, 64>, mgrid, mblock, 0, st, mp)
+                      : launch_ex(window_merge_kernel<__half, 64>, mgrid, mblock, 0, st, mp))
+              : (bf16 ? launch_ex(window_merge_kernel<__nv_bfloat16, 128>, mgrid, mblock, 0, st, mp)
+                      : launch_ex(window_merge_kernel<__half, 128>, mgrid, mblock, 0, st, mp));
+  return me == cudaSuccess ? TC_OK : TC_ERR_CUDA;
 }
 }  // namespace
 
