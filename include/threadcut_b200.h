@@ -211,6 +211,22 @@ int tc_prefill_attention_window(const void* q, const void* k, const void* v, voi
                                 int64_t out_stride_b, int64_t out_stride_p, int64_t out_stride_h, float scale,
                                 int splits, int dtype, void* workspace, size_t workspace_bytes, void* stream);
 
+/* tc_prefill_attention_window over a paged cache (one sequence; pools and the sub-tile table as for
+ * tc_prefill_attention_paged, whose rule on unlisted pool rows holds too). Key tile j being sub-tiles
+ * [4j, 4j + 4), qb_tiles (DEVICE int32 [blocks][2], a block being 2 * floor(128 / (hq / hkv)) queries) holds,
+ * for block i from query p0 on, the last key tile with a logical start at or below
+ * max(0, lk - lq + p0 + 1 - window) and the number of key tiles with a logical start below
+ * min(lk, lk - lq + p0 + block); sink_tiles = the key tiles with a logical start below `sinks`. 16-bit, d in
+ * {64, 128}, hq <= 128 hkv, scale > 0. Workspace as tc_prefill_window_workspace_size(1, hq, hkv, lq,
+ * max(lq, 128 * ceil(n_sub / 4)), d, window, sinks, splits). */
+int tc_prefill_attention_window_paged(const void* q, const void* k_pool, const void* v_pool, void* out, int hq, int hkv,
+                                      int lq, int lk, int d, int64_t page_rows, int64_t num_pages,
+                                      int64_t pool_stride_page, int64_t pool_stride_h, int64_t pool_stride_row,
+                                      const int32_t* ktab, int64_t n_sub, const int32_t* qb_tiles, int sink_tiles,
+                                      int64_t window, int64_t sinks, int64_t q_stride_h, int64_t q_stride_p,
+                                      int64_t out_stride_p, int64_t out_stride_h, float scale, int splits, int dtype,
+                                      void* workspace, size_t workspace_bytes, void* stream);
+
 /* Decode attention of `batch` sequences that share ONE cached prefix, each with its own suffix (several
  * continuations of one context): q [batch, hkv, g, d], k_prefix/v_prefix [hkv, n, d], k/v
  * [batch, hkv, m, d] of which the first lengths[b] rows count (DEVICE int32, NULL: m; clamped into

@@ -103,3 +103,20 @@ def shared_paged_status(q=P, kp=P, vp=P, k=P, v=P, out=P, b=2, hkv=2, g=4, d=128
     (dict(scale=float("nan")), 1), (dict(page_stride=65), 2), (dict(qs=127), 2), (dict(q=ctypes.c_void_p(8)), 2)])
 def test_shared_paged_decode_refuses(bad, status):
     assert shared_paged_status(**bad) == status
+
+
+def prefill_paged_status(q=P, kp=P, vp=P, out=P, hq=8, hkv=2, lq=4, lk=100, d=128, rows=64, pages=4, page_stride=64,
+                         ktab=P, n_sub=4, qb=P, sink_tiles=1, window=10, sinks=2, qs=128, scale=0.1, splits=0, dtype=2):
+    return _lib.lib().tc_prefill_attention_window_paged(q, kp, vp, out, hq, hkv, lq, lk, d, rows, pages, page_stride, 64,
+                                                        64, ktab, n_sub, qb, sink_tiles, window, sinks, qs, 128, 128, 128,
+                                                        scale, splits, dtype, N, 0, N)
+
+
+@pytest.mark.parametrize("bad,status", [
+    (dict(dtype=0), 3), (dict(hq=7), 1), (dict(hkv=0), 1), (dict(hq=258), 1), (dict(lq=0), 1), (dict(lk=3), 1),
+    (dict(d=256), 1), (dict(rows=31), 1), (dict(pages=0), 1), (dict(n_sub=0), 1), (dict(sink_tiles=-1), 1),
+    (dict(window=0), 1), (dict(sinks=-1), 1), (dict(scale=0.0), 1), (dict(scale=float("nan")), 1), (dict(splits=-1), 1),
+    (dict(q=N), 1), (dict(kp=N), 1), (dict(vp=N), 1), (dict(out=N), 1), (dict(ktab=N), 1), (dict(qb=N), 1),
+    (dict(page_stride=65), 2), (dict(qs=127), 2), (dict(ktab=ctypes.c_void_p(8)), 2)])
+def test_window_paged_prefill_refuses(bad, status):
+    assert prefill_paged_status(**bad) == status

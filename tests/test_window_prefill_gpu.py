@@ -5,6 +5,8 @@ import torch
 
 from attn_bounds import assert_within, attend64
 from threadcut_b200 import _lib
+from threadcut_b200.match import Split
+from threadcut_b200.paged import PagedKV
 from threadcut_b200.prefill import prefill_attention, prefill_attention_window
 
 pytestmark = pytest.mark.gpu
@@ -138,6 +140,43 @@ def test_another_stream_and_two_replayed_graphs():
         torch.cuda.synchronize()
         for want, x, (_, y) in zip(wants, got, graphs):
             assert torch.equal(want, x) and torch.equal(want, y)
+
+
+@pytest.mark.parametrize("dtype,d,g", [(BF16, 128, 4), (F16, 64, 2), (BF16, 128, 7), (F16, 64, 1)])
+@pytest.mark.parametrize("page_rows,splice", [(64, None), (32, (101, 250, 555)), (100, (33, 34, 500))])
+@pytest.mark.parametrize("window,sinks", [(1, 0), (60, 4), (129, 200), (10 ** 12, 0)])
+def test_a_paged_cache(dtype, d, g, page_rows, splice, window, sinks):
+    hkv = 2
+    gen = torch.Generator(device=DEV).manual_seed(5)
+    kv = PagedKV(1, hkv, d, max_tokens=2500, page_rows=page_rows, dtype=dtype, device=DEV)
+    for t in (700, 5, 200):
+        kv.reserve(t)
+        kv.write(0, *(torch.randn(hkv, t, d, generator=gen, device=DEV).to(dtype) for _ in range(2)))
+    if splice:
+        kv.splice(Split(*splice), 1e4 ** (-torch.arange(0, d, 2).float() / d))
+    for lq in (1, 77, 300):
+        kv.reserve(lq)
+        kv.write(0, *(torch.randn(hkv, lq, d, generator=gen, device=DEV).to(dtype) for _ in range(2)))
+        q = torch.randn(1, lq, hkv * g, d, generator=gen, device=DEV).to(dtype).transpose(1, 2)
+        k, v = kv.gather(0)
+        want = reference(q, k[None], v[None], 0.1, window, sinks)
+        for splits in (None, 3):
+            assert_within(kv.prefill(0, q, 0.1, window=window, sinks=sinks, splits=splits), *want)
+
+
+def test_a_window_and_sinks_over_a_paged_cache_need_a_fitting_call():
+    kv = PagedKV(1, 2, 128, max_tokens=64, device=DEV)
+    kv.reserve(20)
+    q = torch.zeros(1, 8, 5, 128, device=DEV, dtype=BF16)
+    for bad in (dict(window=0), dict(window=3, sinks=-1), dict(sinks=2)):
+        with pytest.raises(ValueError):
+            kv.prefill(0, q, 0.1, **bad)
+    with pytest.raises(ValueError):
+        kv.prefill(0, q, -0.1, window=3)
+    with pytest.raises(ValueError):
+        kv.prefill(0, q[:, :7], 0.1, window=3)
+    with pytest.raises(ValueError):
+        kv.prefill(0, torch.zeros(1, 8, 21, 128, device=DEV, dtype=BF16), 0.1, window=3)
 
 
 def test_refusals():

@@ -56,6 +56,8 @@ SIGNATURES = {
                              + [_f, _i, _i, _vp, _sz, _vp]),
     "tc_prefill_window_workspace_size": (_sz, [_i] * 6 + [_i64, _i64, _i]),
     "tc_prefill_attention_window": (_i, [_vp, _vp, _vp, _vp] + [_i] * 6 + [_i64] * 14 + [_f, _i, _i, _vp, _sz, _vp]),
+    "tc_prefill_attention_window_paged": (_i, [_vp] * 4 + [_i] * 5 + [_i64] * 5 + [_vp, _i64, _vp, _i] + [_i64] * 6
+                                          + [_f, _i, _i, _vp, _sz, _vp]),
     "tc_decode_attention_shared_workspace_size": (_sz, [_i, _i, _i, _i, _i64, _i64, _i]),
     "tc_decode_attention_shared": (_i, [_vp] * 6 + [_i] * 4 + [_i64, _i64, _vp] + [_i64] * 16
                                    + [_f, _i, _vp, _sz, _vp]),

@@ -2384,6 +2384,62 @@ int tc_prefill_attention_window(const void* q, const void* k, const void* v, voi
   return launch_rows(p, dtype, static_cast<cudaStream_t>(stream));
 }
 
+int tc_prefill_attention_window_paged(const void* q, const void* k_pool, const void* v_pool, void* out, int hq, int hkv,
+                                      int lq, int lk, int d, int64_t page_rows, int64_t num_pages,
+                                      int64_t pool_stride_page, int64_t pool_stride_h, int64_t pool_stride_row,
+                                      const int32_t* ktab, int64_t n_sub, const int32_t* qb_tiles, int sink_tiles,
+                                      int64_t window, int64_t sinks, int64_t q_stride_h, int64_t q_stride_p,
+                                      int64_t out_stride_p, int64_t out_stride_h, float scale, int splits, int dtype,
+                                      void* workspace, size_t workspace_bytes, void* stream) {
+  if (dtype != TC_BF16 && dtype != TC_F16) return TC_ERR_DTYPE;
+  if (hkv < 1 || hkv > 65535 || hq < hkv || hq % hkv != 0 || hq / hkv > 128 || lq < 1 || lk < lq || lk > (1 << 30) ||
+      (d != 64 && d != 128) || q == nullptr || k_pool == nullptr || v_pool == nullptr || out == nullptr ||
+      ktab == nullptr || qb_tiles == nullptr || splits < 0 || n_sub < 1 || n_sub > (1 << 25) || page_rows < kTile ||
+      page_rows > (1 << 30) || num_pages < 1 || num_pages >= (1 << 30) || window < 1 || sinks < 0 || sink_tiles < 0 ||
+      !finite_scale(scale) || !(scale > 0.f))
+    return TC_ERR_INVALID;
+  const int64_t st[7] = {q_stride_h, q_stride_p, out_stride_p, out_stride_h, pool_stride_page, pool_stride_h,
+                         pool_stride_row};
+  for (int64_t x : st)
+    if (!stride16(x, dtype)) return TC_ERR_ALIGN;
+  if (!aligned16(q) || !aligned16(k_pool) || !aligned16(v_pool) || !aligned16(out) || !aligned16(ktab))
+    return TC_ERR_ALIGN;
+  const int slots = (int)cdiv(n_sub, 4) * kPfKeys;  // key slots the tiles hold (planning only)
+  const int64_t w_in = window < lk ? window : lk, s_in = sinks < lk ? sinks : lk;
+  WindowPrefill w = plan_window_prefill(1, hq, hkv, lq, slots > lq ? slots : lq, d, w_in, s_in, splits);
+  // split partials are merged into rows of d contiguous elements: needs the [lq, hq, d] layout
+  if (out_stride_h != d || out_stride_p != (int64_t)hq * d) w.splits = 1;
+  if (w.splits > 1 && (workspace == nullptr || !aligned16(workspace) ||
+                       workspace_bytes < window_ws_bytes((int64_t)lq * hq, d, w.splits)))
+    return TC_ERR_WORKSPACE;
+  PrefillParams p;
+  std::memset(&p, 0, sizeof(p));
+  const int64_t qd[4] = {d, lq, hq, 1};
+  const uint32_t qbox[4] = {64, (uint32_t)w.pq, (uint32_t)(hq / hkv), 1};
+  if (!encode_view4(&p.tmq, q, dtype, qd, q_stride_p, q_stride_h, 0, qbox) ||
+      !encode_kv_map(&p.tmk, k_pool, dtype, d, page_rows, hkv, num_pages, pool_stride_row, pool_stride_h,
+                     pool_stride_page) ||
+      !encode_kv_map(&p.tmv, v_pool, dtype, d, page_rows, hkv, num_pages, pool_stride_row, pool_stride_h,
+                     pool_stride_page))
+    return TC_ERR_INVALID;
+  p.ktab = reinterpret_cast<const int4*>(ktab);
+  p.n_sub = (int)n_sub;
+  p.oob_page = (int)num_pages;
+  p.qb_tiles = qb_tiles;
+  p.out = out;
+  p.so_p = out_stride_p;
+  p.so_h = out_stride_h;
+  p.lq = lq;
+  p.lk = lk;
+  p.hq = hq;
+  p.hkv = hkv;
+  p.c = scale * kLog2e;
+  p.window = (int)w_in;
+  p.sinks = (int)s_in;
+  p.sink_tiles = sink_tiles;
+  return run_window_prefill(p, w, 1, d, true, dtype, workspace, static_cast<cudaStream_t>(stream));
+}
+
 size_t tc_decode_attention_shared_workspace_size(int batch, int hkv, int g, int d, int64_t n, int64_t m, int dtype) {
   if (batch < 1 || hkv < 1 || g < 1 || g > 128 || n < 0 || m < 0 || dtype == TC_F32 || !mma_dim(d)) return 0;
   return plan_shared(batch, hkv, g, d, n, m).bytes;

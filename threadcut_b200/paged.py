@@ -523,11 +523,54 @@ class PagedKV:
             self._ktab_ver = self.table.version
         return self._ktab, self._ktab_starts
 
-    def prefill(self, layer, query, scale, *, splits=None):
+    def _prefill_window(self, layer, query, scale, window, sinks, splits):
+        """prefill with a sliding window and sinks (tc_prefill_attention_window_paged)."""
+        what = "PagedKV.prefill"
+        _, hq, lq, d = query.shape
+        n = self.table.n
+        if (query.shape[0] != 1 or d != self.d or d not in (64, 128) or hq % self.hkv or hq // self.hkv > 128
+                or query.dtype != self.dtype or query.dtype not in (torch.bfloat16, torch.float16) or not 1 <= lq <= n):
+            raise ValueError(f"{what}: query {tuple(query.shape)} {query.dtype} does not fit the cache")
+        if window < 1 or sinks < 0 or not scale > 0:
+            raise ValueError(f"{what}: needs window >= 1, sinks >= 0 and scale > 0, got {window}, {sinks} and {scale}")
+        ktab, starts = self._prefill_table()
+        tile_starts = starts[::4]
+        block = 2 * (128 // (hq // self.hkv))
+        p0 = (n - lq) + block * np.arange(-(-lq // block), dtype=np.int64)
+        qb = np.empty((p0.shape[0], 2), np.int32)
+        qb[:, 0] = np.searchsorted(tile_starts, np.maximum(p0 + 1 - window, 0), side="right") - 1
+        qb[:, 1] = np.searchsorted(tile_starts, np.minimum(p0 + block, n), side="left")
+        qb_tiles = torch.from_numpy(qb).to(self.device)
+        q = _rows16(query[0])
+        out = torch.empty((1, lq, hq, d), dtype=query.dtype, device=query.device)
+        L = lib()
+        n_sub = ktab.shape[0]
+        sp, sh, sr = self._strides()
+        with torch.cuda.device(query.device):
+            nb = L.tc_prefill_window_workspace_size(1, hq, self.hkv, lq, max(lq, 128 * (-(-n_sub // 4))), d,
+                                                    min(window, n), min(sinks, n), splits)
+            ws = torch.empty(nb, dtype=torch.uint8, device=query.device) if nb else None
+            st = L.tc_prefill_attention_window_paged(
+                q.data_ptr(), self.k[layer].data_ptr(), self.v[layer].data_ptr(), out.data_ptr(), hq, self.hkv, lq, n, d,
+                self.page_rows, self.table.num_pages, sp, sh, sr, ktab.data_ptr(), n_sub, qb_tiles.data_ptr(),
+                int(np.searchsorted(tile_starts, min(sinks, n), side="left")), min(window, n), min(sinks, n),
+                q.stride(0), q.stride(1), out.stride(1), out.stride(2), float(scale), splits,
+                _lib.DTYPE_CODE[query.dtype], ws.data_ptr() if ws is not None else None, nb, stream_ptr(query.device))
+        check("tc_prefill_attention_window_paged", st)
+        return out
+
+    def prefill(self, layer, query, scale, *, splits=None, window=None, sinks=0):
         """Causal attention of a chunk's queries over the whole paged sequence, whose last lq tokens
         are the chunk (already written): query [1, 4*hkv, lq, 128] (bf16/fp16) -> [1, lq, hq, 128],
-        as threadcut_b200.prefill.prefill_attention on the contiguous cache, with no copy of it."""
+        as threadcut_b200.prefill.prefill_attention on the contiguous cache, with no copy of it.
+        window / sinks: each query sees only the first `sinks` and the last `window` keys up to its own, as
+        prefill.prefill_attention_window; then any number of query heads (up to 128 per KV head) and d of 64
+        or 128."""
         require_cuda(query, what="PagedKV.prefill")
+        if window is not None:
+            return self._prefill_window(layer, query, scale, int(window), int(sinks), int(splits or 0))
+        if sinks:
+            raise ValueError("PagedKV.prefill: sinks go with a window")
         _, hq, lq, d = query.shape
         n = self.table.n
         if (query.shape[0] != 1 or d != 128 or d != self.d or hq != 4 * self.hkv or query.dtype != self.dtype
