@@ -133,8 +133,8 @@ _host = None
 
 
 def host():
-    """The compiled host binding (csrc/host_binding.cpp) with its pointer to this package's loaded
-    tc_decode_attention_stable, or None when it has not been built (the ctypes path is used then).
+    """The compiled host binding (csrc/host_binding.cpp) with its pointers to this package's loaded
+    library, or None when it has not been built (the ctypes path is used then).
     It only moves the argument marshalling out of the interpreter; the kernels are the same."""
     global _host
     if _host is None:
@@ -150,6 +150,10 @@ def host():
                     mod.init(ctypes.cast(handle.tc_decode_attention_stable, ctypes.c_void_p).value)
                     if hasattr(mod, "init_partial"):
                         mod.init_partial(ctypes.cast(handle.tc_decode_attention_partial_stable, ctypes.c_void_p).value)
+                    mod.init_ops(*(ctypes.cast(getattr(handle, name), ctypes.c_void_p).value for name in (
+                        "tc_paged_append_rope", "tc_decode_attention_window", "tc_decode_attention_window_workspace_size",
+                        "tc_prefill_attention_window", "tc_prefill_window_workspace_size", "tc_decode_attention_shared",
+                        "tc_decode_attention_shared_workspace_size")))
                 _host = mod
     return _host or None
 

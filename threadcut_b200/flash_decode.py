@@ -265,6 +265,11 @@ def decode_attention_window(q, k, v, scale, window, sinks=0, lengths=None, *, sp
     (clamped into [0, n]; 0 gives zeros). One sequence may come without the batch dimension (q
     [hkv, g, d], k/v [hkv, n, d]). Returns q's shape."""
     what = "decode_attention_window"
+    hb = _lib.host()
+    if hb is not None:
+        out = hb.window_decode(q, k, v, scale, int(window), int(sinks), lengths, int(splits or 0))
+        if out is not None:
+            return out
     require_cuda(q, k, v, what=what)
     if k.dtype != q.dtype or v.dtype != q.dtype:
         _check_same_dtype(what, q, k, v)
@@ -314,6 +319,11 @@ def decode_attention_shared(q, k_prefix, v_prefix, k, v, scale, lengths=None):
     and then the suffix. The prefix is read once for the whole batch. An empty prefix or suffix is fine;
     with neither the result is zeros."""
     what = "decode_attention_shared"
+    hb = _lib.host()
+    if hb is not None:
+        out = hb.shared_decode(q, k_prefix, v_prefix, k, v, scale, lengths)
+        if out is not None:
+            return out
     require_cuda(q, k_prefix, v_prefix, k, v, what=what)
     for x in (k_prefix, v_prefix, k, v):
         if x.dtype != q.dtype:

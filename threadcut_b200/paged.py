@@ -244,6 +244,10 @@ def append_rope(k, v, cos, sin, k_pool, v_pool, slots, *, q=None, q_norm=None, k
     strides with a contiguous last dimension. Returns the rotated queries, in q's shape and stored
     token by token ([t, hq, d]), or None. fp32 inside, each output rounded once."""
     what = "append_rope"
+    if q is not None and (hb := _lib.host()) is not None:
+        out = hb.append_rope(k, v, cos, sin, k_pool, v_pool, slots, q, q_norm, k_norm, eps)
+        if out is not None:
+            return out
     require_cuda(k, v, cos, sin, k_pool, v_pool, slots, *(x for x in (q, q_norm, k_norm) if x is not None), what=what)
     batched = k.dim() == 4
     if batched:

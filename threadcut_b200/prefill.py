@@ -65,6 +65,11 @@ def prefill_attention_window(query, key, value, scale, window, sinks=0, *, split
     Query position p sees the keys j <= lk - lq + p with j < sinks or j > lk - lq + p - window (window >= 1
     counts the query's own token). Returns [b, lq, hq, d] contiguous."""
     what = "prefill_attention_window"
+    hb = _lib.host()
+    if hb is not None:
+        out = hb.window_prefill(query, key, value, scale, int(window), int(sinks), int(splits or 0))
+        if out is not None:
+            return out
     require_cuda(query, key, value, what=what)
     if query.dim() != 4 or key.dim() != 4 or value.shape != key.shape:
         raise ValueError(f"{what}: expected query [b, hq, lq, d], key/value [b, hkv, lk, d]; got {tuple(query.shape)}, "
