@@ -14,6 +14,10 @@ launch (decode_attention_append) instead of a separate copy before attention (kv
 With a paged cache (kv.new_cache(..., paged=True)) the key is a stand-in: the one-token step decodes
 over the pages (PagedKV.decode, fused append), a causal prefill chunk runs the tcgen05 kernel over
 the pages (PagedKV.prefill), and other branches get a contiguous copy.
+A sliding-window layer (transformers passes its `sliding_window`, and a mask that hides older keys) runs
+the windowed kernels when the mask is that window and nothing else: decode_attention_window for one token,
+prefill_attention_window for a chunk, or their forms over the pages. The comparison reads the mask back
+once per mask tensor, so a step under stream capture keeps the SDPA branch.
 Decode on a non-CUDA tensor raises: there is no CPU path.
 Prefill (q > 1 or a mask): a causal prefill over the cache (query p sees keys up to lk - lq + p;
 b == 1, 4 query heads per KV head, head_dim 128, 16-bit) runs the tcgen05 kernel of
@@ -27,7 +31,8 @@ import torch.nn.functional as F
 from transformers import AttentionInterface
 from transformers.masking_utils import AttentionMaskInterface, causal_mask_function, sdpa_mask
 
-from .flash_decode import decode_attention, decode_attention_append, decode_attention_batched
+from .flash_decode import (decode_attention, decode_attention_append, decode_attention_batched,
+                           decode_attention_window)
 from .kv import FUSED_ATTENTION, paged_pending, pending_append
 from . import prefill as _prefill
 
@@ -64,6 +69,31 @@ def _is_causal_offset(mask, lq, lk):
     return ok
 
 
+_window_seen = {}  # the last mask tensor compared with a window's: (weak reference, version, window, result)
+
+
+def _window_of(query, mask, lq, lk, scaling, kwargs):
+    """The window W of a sliding-window layer whose mask means exactly "query p sees the last W keys up to
+    its own", if the windowed kernels take the call; else None."""
+    w = kwargs.get("sliding_window")
+    d = query.shape[-1]
+    if (not isinstance(w, int) or w < 1 or mask is None or mask.dtype != torch.bool or tuple(mask.shape) != (1, 1, lq, lk)
+            or lq > lk or query.shape[0] != 1 or not query.is_cuda or not scaling > 0
+            or query.dtype not in (torch.bfloat16, torch.float16) or d not in (64, 128)
+            or kwargs.get("softcap") is not None or kwargs.get("s_aux") is not None
+            or torch.cuda.is_current_stream_capturing()):
+        return None
+    hit = _window_seen.get("last")
+    if hit is None or hit[0]() is not mask or hit[1:3] != (mask._version, w):
+        seen = _prefill.causal_offset_mask(lq, lk, mask.device)
+        if w < lk:
+            seen = seen & (torch.arange(lk, device=mask.device)[None, :]
+                           > (lk - lq - w) + torch.arange(lq, device=mask.device)[:, None])
+        hit = (weakref.ref(mask), mask._version, w, bool(torch.equal(mask[0, 0], seen)))
+        _window_seen["last"] = hit
+    return w if hit[3] else None
+
+
 def attention(module, query, key, value, attention_mask, dropout=0.0, scaling=None, **kwargs):
     b, hq, q, d = query.shape
     hkv = key.shape[1]
@@ -71,6 +101,12 @@ def attention(module, query, key, value, attention_mask, dropout=0.0, scaling=No
     scaling = scaling if scaling is not None else d ** -0.5
     paged = paged_pending(key)
     if paged is not None:
+        w = _window_of(query, attention_mask, q, paged.get_seq_length(), scaling, kwargs)
+        if w is not None and q == 1 and g <= 16 and paged._pending is not None:
+            out = paged.decode(query.reshape(hkv, g, d), scaling, window=w).reshape(1, hq, 1, d)
+            return out.transpose(1, 2).contiguous(), None
+        if w is not None and paged._pending is None and g <= 128 and query.dtype == paged.state.kv.dtype:
+            return paged.prefill(query, scaling, window=w), None
         if q == 1 and attention_mask is None and b == 1 and paged._pending is not None:
             # paged cache, one-token step: attend over the pages, the step's row written by the launch
             out = paged.decode(query.reshape(hkv, g, d), scaling).reshape(1, hq, 1, d)
@@ -89,6 +125,12 @@ def attention(module, query, key, value, attention_mask, dropout=0.0, scaling=No
         return out.transpose(1, 2).contiguous(), None
     if layer is not None:
         layer._flush()
+    w = _window_of(query, attention_mask, q, key.shape[2], scaling, kwargs)
+    if w is not None and q == 1 and g <= 16:
+        out = decode_attention_window(query.reshape(hkv, g, d), key[0], value[0], scaling, w).reshape(1, hq, 1, d)
+        return out.transpose(1, 2).contiguous(), None
+    if w is not None and q > 1 and g <= 128:
+        return _prefill.prefill_attention_window(query, key, value, scaling, w), None
     if q == 1 and attention_mask is None:
         if b == 1:
             out = decode_attention(query.reshape(hkv, g, d), key[0], value[0], scaling).reshape(1, hq, 1, d)

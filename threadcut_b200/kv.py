@@ -353,24 +353,25 @@ class PagedLayer(DynamicLayer):
         k, v = kv.gather(self.index)
         return k[None], v[None]
 
-    def decode(self, q, scale):
-        """The step's attention for the threadcut plugin: q [hkv, g, d] over the pages with the
-        pending row written by the same launch."""
+    def decode(self, q, scale, window=None):
+        """The step's attention for the threadcut plugin: q [hkv, g, d] over the pages (their last
+        `window` tokens) with the pending row written by the same launch."""
         k, v = self._pending
         self._pending = None
         self._release()
         kv = self.state.kv
-        return kv.decode(self.index, q, scale, k_new=k, v_new=v, stable_tiles=kv.n_tiles - 1)
+        return kv.decode(self.index, q, scale, k_new=k, v_new=v, stable_tiles=kv.n_tiles - 1, window=window)
 
     def can_prefill(self, query):
         return (self._pending is None and query.shape[0] == 1 and query.shape[-1] == 128
                 and query.shape[1] == 4 * self.state.kv.hkv and query.dtype == self.state.kv.dtype
                 and query.dtype in (torch.bfloat16, torch.float16))
 
-    def prefill(self, query, scale):
-        """The chunk's causal attention for the threadcut plugin, straight over the pages."""
+    def prefill(self, query, scale, window=None):
+        """The chunk's causal attention (over each query's last `window` tokens) for the threadcut
+        plugin, straight over the pages."""
         self._release()
-        return self.state.kv.prefill(self.index, query, scale)
+        return self.state.kv.prefill(self.index, query, scale, window=window)
 
     def materialize(self):
         """Writes the pending row and returns contiguous (K, V) [1, hkv, n, d] (other readers)."""
