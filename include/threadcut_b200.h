@@ -198,8 +198,8 @@ int tc_prefill_attention(const void* q, const void* k, const void* v, void* out,
  * [batch, lq, hq, d], any strides with a contiguous last dimension; d <= 256, every dtype. 16-bit,
  * d in {64, 128}, hq <= 128 hkv, scale > 0 and 16-byte aligned bases and strides run on the tcgen05 tensor
  * cores and visit only the key tiles that some query of the block sees; the rest runs a plain kernel.
- * In the tcgen05 kernel a key row inside such a tile that is hidden from one of the block's queries meets
- * it with a zero weight, so V must be finite there, as in any masked product. splits = 0 picks the number
+ * Keys that no query of the call sees may hold anything; a V row that some query sees meets the others of
+ * its block with a zero weight, so it must be finite, as in any masked product. splits = 0 picks the number
  * of KV splits; workspace of tc_prefill_window_workspace_size() bytes (0: none; no initial contents).
  * No counterpart in the reference, whose prefill sees the whole cache (threadcut/attention.py:43-46). */
 size_t tc_prefill_window_workspace_size(int batch, int hq, int hkv, int lq, int lk, int d, int64_t window,
@@ -212,7 +212,7 @@ int tc_prefill_attention_window(const void* q, const void* k, const void* v, voi
                                 int splits, int dtype, void* workspace, size_t workspace_bytes, void* stream);
 
 /* tc_prefill_attention_window over a paged cache (one sequence; pools and the sub-tile table as for
- * tc_prefill_attention_paged, whose rule on unlisted pool rows holds too). Key tile j being sub-tiles
+ * tc_prefill_attention_paged, but pool rows that no sub-tile lists may hold anything). Key tile j being sub-tiles
  * [4j, 4j + 4), qb_tiles (DEVICE int32 [blocks][2], a block being 2 * floor(128 / (hq / hkv)) queries) holds,
  * for block i from query p0 on, the last key tile with a logical start at or below
  * max(0, lk - lq + p0 + 1 - window) and the number of key tiles with a logical start below

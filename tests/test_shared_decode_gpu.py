@@ -147,6 +147,15 @@ def test_strided_views_and_unaligned_rows(pad):
     assert_within(decode_attention_shared(q, kp, vp, k, v, 0.1), *reference(q, kp, vp, k, v, 0.1, torch.full((3,), 40)))
 
 
+def test_broadcast_tensors():
+    """A prefix expanded over heads, suffixes expanded over sequences, one query for every sequence (stride 0)."""
+    q, kp, vp, k, v = make(3, 4, 2, 128, 150, 40, BF16)
+    for args in ((q, kp[:1].expand(4, -1, -1), vp[:1].expand(4, -1, -1), k, v),
+                 (q, kp, vp, k[:1].expand(3, -1, -1, -1), v[:1].expand(3, -1, -1, -1)),
+                 (q[:1].expand(3, -1, -1, -1), kp, vp, k, v)):
+        assert_within(decode_attention_shared(*args, 0.1), *reference(*args, 0.1, torch.full((3,), 40)))
+
+
 def test_prefix_rows_past_32_bit_element_offsets():
     hkv, n, d = 9, 1 << 21, 128  # 9 * 2^21 * 128 = 2.4e9 elements
     kp = torch.zeros(hkv, n, d, device=DEV, dtype=BF16)

@@ -181,6 +181,26 @@ def test_paged_windows_after_a_splice(page_rows, window, sinks):
             assert torch.equal(out, kv.decode(0, q, 0.1, window=window, sinks=sinks))
 
 
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_an_empty_cache_gives_zeros(d, dtype):
+    q = torch.ones(2, 2, 4, d, device=DEV, dtype=dtype)
+    k = torch.empty(2, 2, 0, d, device=DEV, dtype=dtype)
+    assert not decode_attention_window(q, k, k, 0.1, 5, 1).any()
+    assert not decode_attention_window(q, k, k, 0.1, 5, 1, torch.tensor([0, 3], device=DEV, dtype=torch.int32)).any()
+
+
+def test_broadcast_keys():
+    """Keys and values expanded over sequences or heads (stride 0)."""
+    gen = torch.Generator(device=DEV).manual_seed(2)
+    q, k, v = (torch.randn(3, 4, x, 128, generator=gen, device=DEV).to(BF16) for x in (4, 200, 200))
+    seen = visible(torch.full((3,), 200, device=DEV), 200, 60, 3)
+    for kk, vv in ((k[:1].expand(3, -1, -1, -1), v[:1].expand(3, -1, -1, -1)),
+                   (k[:, :1].expand(-1, 4, -1, -1), v[:, :1].expand(-1, 4, -1, -1))):
+        ref, tol = attend64(q, kk, vv, 0.1, seen, P_SPLIT[BF16])
+        assert_within(decode_attention_window(q, kk, vv, 0.1, 60, 3), ref, tol)
+
+
 def test_refusals():
     x = torch.zeros(2, 2, 8, 128, device=DEV, dtype=BF16)
     for bad in (dict(window=0), dict(window=-1), dict(window=4, sinks=-1)):

@@ -96,17 +96,27 @@ def test_a_window_over_everything_is_the_causal_prefill():
     assert float((a.float() - b.float()).abs().max()) <= 2.0 ** -7  # two roundings of values below 2
 
 
-@pytest.mark.parametrize("dtype,d", [(BF16, 128), (F32, 64)])
-def test_keys_that_no_query_of_the_call_sees_may_hold_anything(dtype, d):
-    """Keys between the sinks' last tile and the first query's first window tile (tiles of 128 keys)."""
-    q, k, v = make(1, 2, 4, 100, 2000, d, dtype)
-    want = prefill_attention_window(q, k, v, 0.1, 256, 5)
-    lo, hi = 128, (2000 - 100 - 255) // 128 * 128
-    for x in (k, v):
-        x[:, :, lo:hi] = float("nan")
-    assert torch.equal(prefill_attention_window(q, k, v, 0.1, 256, 5), want)
-    k[:, :, 5:2000 - 100 - 255] = float("nan")  # a hidden key may hold anything in every tile
-    assert torch.equal(prefill_attention_window(q, k, v, 0.1, 256, 5), want)
+@pytest.mark.parametrize("dtype,d", [(BF16, 128), (F16, 64), (F32, 64)])
+@pytest.mark.parametrize("lq,lk,window,sinks", [(100, 2000, 256, 5), (300, 2000, 33, 130), (1, 700, 1, 0), (40, 500, 60, 0)])
+def test_keys_that_no_query_of_the_call_sees_may_hold_anything(dtype, d, lq, lk, window, sinks):
+    """Also where they share a key tile with keys that are seen."""
+    q, k, v = make(1, 2, 4, lq, lk, d, dtype)
+    want = prefill_attention_window(q, k, v, 0.1, window, sinks)
+    first = lk - lq + 1 - window
+    assert first > sinks
+    for bad in (float("nan"), float("inf"), float("-inf")):
+        for x in (k, v):
+            x[:, :, sinks:first] = bad
+            x._base[:, :, lk:] = bad
+        assert torch.equal(prefill_attention_window(q, k, v, 0.1, window, sinks), want)
+
+
+def test_broadcast_keys():
+    """Keys and values expanded over sequences or heads (stride 0)."""
+    q, k, v = make(2, 4, 2, 50, 300, 128, BF16)
+    for kk, vv in ((k[:1].expand(2, -1, -1, -1), v[:1].expand(2, -1, -1, -1)),
+                   (k[:, :1].expand(-1, 4, -1, -1), v[:, :1].expand(-1, 4, -1, -1))):
+        assert_within(prefill_attention_window(q, kk, vv, 0.1, 60, 3), *reference(q, kk, vv, 0.1, 60, 3))
 
 
 @pytest.mark.parametrize("d,pad", [(128, 8), (128, 1), (64, 3)])
@@ -162,6 +172,15 @@ def test_a_paged_cache(dtype, d, g, page_rows, splice, window, sinks):
         want = reference(q, k[None], v[None], 0.1, window, sinks)
         for splits in (None, 3):
             assert_within(kv.prefill(0, q, 0.1, window=window, sinks=sinks, splits=splits), *want)
+    # rows that no run lists, or that no query sees, may hold anything
+    out = kv.prefill(0, q, 0.1, window=window, sinks=sinks)
+    live = torch.zeros(kv.table.num_pages, page_rows, dtype=torch.bool, device=DEV)
+    pos = torch.from_numpy(kv.table.positions()).to(DEV)
+    seen = visible(lq, kv.n, window, sinks).any(0)
+    live[pos[seen, 0], pos[seen, 1]] = True
+    for pool in (kv.k[0], kv.v[0]):
+        pool.transpose(1, 2)[~live] = float("nan")
+    assert torch.equal(kv.prefill(0, q, 0.1, window=window, sinks=sinks), out)
 
 
 def test_a_window_and_sinks_over_a_paged_cache_need_a_fitting_call():

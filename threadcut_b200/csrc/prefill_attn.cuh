@@ -30,7 +30,8 @@
 // sinks, then those from the first key that the block's first query sees. Its geometry is the caller's:
 // any g <= 128 query heads per KV head (a Q tile is g heads x floor(128 / g) positions; rows past them are
 // dead), d of 64 or 128, a batch. A tile in which some row hides some key is masked key by key; a tile
-// fully visible to the Q tile costs the compare of its two ends.
+// fully visible to the Q tile costs the compare of its two ends. V rows that no query of the block sees are
+// zeroed in the staged tile, so that a zero weight never meets what memory holds there.
 // TMEM: 512 columns — S_0 | S_1 | O_0 | O_1. mbarriers order the roles (q_full, kv_full/kv_empty per
 // stage, s_full/p_full/o_full per Q tile); every wait is bounded, a failed wait makes all roles
 // skip to the end, and the MMA lane's final commit is waited for before TMEM is freed.
@@ -113,9 +114,9 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const __grid_con
   const int off = p.lk - p.lq;          // key j is visible to position pos iff j <= off + pos
   const int kend = p.lk < off + p0 + pq * kPfTiles ? p.lk : off + p0 + pq * kPfTiles;
   // window: tile t of the list is key tile t for the first sink_tiles, then key tile t + skip
-  int sink_tiles = 0, skip = 0;
+  int sink_tiles = 0, skip = 0, first = 0;
   if constexpr (kWindow) {
-    const int first = off + p0 + 1 - p.window;  // the block's first window key
+    first = off + p0 + 1 - p.window;  // the block's first window key
     const int wt = kPaged ? p.qb_tiles[2 * qb] : (first > 0 ? first / kPfKeys : 0);
     sink_tiles = p.sink_tiles < wt ? p.sink_tiles : wt;
     skip = wt - sink_tiles;
@@ -335,6 +336,29 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const __grid_con
                 v[cch][e] = __float_as_uint(-INFINITY);
         }
       }
+      if constexpr (kWindow) {
+        // Rows of the staged V tile that no query of the block sees (between the sinks and the first window
+        // key; paged: behind a sub-tile's rows) become zeros, a row a thread. The products of Q tile 1 come
+        // after those of Q tile 0, so Q tile 0's warps do it for both.
+        const int r = wq * 32 + lane;
+        bool dead;
+        if constexpr (kPaged) {
+          const int4 t = wq < 2 ? (wq == 0 ? te[0] : te[1]) : (wq == 2 ? te[2] : te[3]);  // this warp's sub-tile
+          dead = lane >= t.z || (t.w + lane >= p.sinks && t.w + lane < first);
+        } else {
+          dead = key0 + r >= p.sinks && key0 + r < first;
+        }
+        if (x == 0 && __any_sync(0xffffffffu, dead)) {
+          ok = __all_sync(0xffffffffu, mbar_wait(&kv_full[j & 1], (j >> 1) & 1, TC_DEVERR_PIPE_TIMEOUT, kPfSpin));
+          if (!ok) break;
+          uint8_t* st = sKV + (j & 1) * 2 * kTileB + kTileB + r * 128;
+          if (dead)
+#pragma unroll
+            for (int cc = 0; cc < D / 8; ++cc)
+              *reinterpret_cast<uint4*>(st + (cc >> 3) * 16384 + (cc & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+          fence_proxy_async_smem();
+        }
+      }
 #pragma unroll
       for (int cch = 0; cch < 4; ++cch)
 #pragma unroll
@@ -462,7 +486,7 @@ struct WindowMergeParams {
 };
 
 // Log-sum-exp merge of a windowed prefill's KV splits, a warp per row. (One CTA per row, as the merge of few
-// decode rows has it, took about 30 us for the 16,384 rows of a 512-token chunk of 32 heads; this takes ???.)
+// decode rows has it, took about 30 us for the 16,384 rows of a 512-token chunk of 32 heads; this about 4 us.)
 template <typename T, int D>
 __global__ void __launch_bounds__(256) window_merge_kernel(const __grid_constant__ WindowMergeParams p) {
   constexpr int kPer = D / 64;  // float2 columns per lane

@@ -86,12 +86,13 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
 
 // 4-D map (d, rows, heads, batch) of a 16-bit K or V tensor, box 64 x kTile x 1 x 1, 128-byte
 // swizzle, rows past `rows` read as zeros. Strides in elements; extents of 1 get a harmless
-// stride. Returns false if the driver rejects the description (the caller then uses the generic
-// kernel).
+// stride. Returns false for a broadcast tensor (a stride of 0 over several rows, heads or sequences) and if
+// the driver rejects the description (the caller then uses the generic kernel).
 bool encode_kv_map(CUtensorMap* m, const void* base, int dtype, int d, int64_t rows, int64_t heads, int64_t batch,
                    int64_t s_row, int64_t s_head, int64_t s_batch) {
   const PFN_cuTensorMapEncodeTiled_v12000 fn = encode_fn();
   if (fn == nullptr || base == nullptr) return false;
+  if ((rows > 1 && s_row <= 0) || (heads > 1 && s_head <= 0) || (batch > 1 && s_batch <= 0)) return false;
   if (rows < 1) rows = 1;
   if (heads == 1 || s_head <= 0) s_head = s_row * rows;
   if (batch == 1 || s_batch <= 0) s_batch = s_head * heads;
@@ -122,13 +123,14 @@ bool encode_map4(CUtensorMap* m, const void* base, int dtype, const int64_t (&di
 }
 
 // encode_map4 of a tensor as a caller gave it: the stride of an extent of 1 carries nothing and gets a
-// harmless value.
+// harmless value; a broadcast one (stride 0) is left to the plain kernels.
 bool encode_view4(CUtensorMap* m, const void* base, int dtype, const int64_t (&dims)[4], int64_t s1, int64_t s2,
                   int64_t s3, const uint32_t (&box)[4]) {
   int64_t st[3] = {s1, s2, s3};
   int64_t next = (dims[0] + 7) / 8 * 8;
   for (int i = 0; i < 3; ++i) {
     if (dims[i + 1] == 1) st[i] = next;
+    if (st[i] <= 0) return false;
     next = st[i] * dims[i + 1];
   }
   return encode_map4(m, base, dtype, dims, st, box);
@@ -791,6 +793,10 @@ int tc_decode_attention_window(const void* q, const void* k, const void* v, void
                                float scale, int splits, int dtype, void* workspace, size_t workspace_bytes,
                                void* stream) {
   if (window < 1 || sinks < 0 || n > INT32_MAX || (n > 0 && (k == nullptr || v == nullptr))) return TC_ERR_INVALID;
+  if (n == 0)  // nothing to map or to read: zeros, for every head size
+    return tc_decode_attention_shared(q, nullptr, nullptr, nullptr, nullptr, out, batch, hkv, g, d, 0, 0, nullptr,
+                                      q_stride_b, q_stride_h, q_stride_g, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, out_stride_b,
+                                      out_stride_h, out_stride_g, scale, dtype, nullptr, 0, stream);
   DecodeParams p = base_params();
   p.q = q;
   p.out = out;

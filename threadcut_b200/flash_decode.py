@@ -267,7 +267,7 @@ def decode_attention_window(q, k, v, scale, window, sinks=0, lengths=None, *, sp
     what = "decode_attention_window"
     hb = _lib.host()
     if hb is not None:
-        out = hb.window_decode(q, k, v, scale, int(window), int(sinks), lengths, int(splits or 0))
+        out = hb.window_decode(q, k, v, float(scale), int(window), int(sinks), lengths, int(splits or 0))
         if out is not None:
             return out
     require_cuda(q, k, v, what=what)
@@ -321,7 +321,7 @@ def decode_attention_shared(q, k_prefix, v_prefix, k, v, scale, lengths=None):
     what = "decode_attention_shared"
     hb = _lib.host()
     if hb is not None:
-        out = hb.shared_decode(q, k_prefix, v_prefix, k, v, scale, lengths)
+        out = hb.shared_decode(q, k_prefix, v_prefix, k, v, float(scale), lengths)
         if out is not None:
             return out
     require_cuda(q, k_prefix, v_prefix, k, v, what=what)

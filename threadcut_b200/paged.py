@@ -242,10 +242,11 @@ def append_rope(k, v, cos, sin, k_pool, v_pool, slots, *, q=None, q_norm=None, k
     from rot on pass through); q_norm / k_norm: RMSNorm weights [d] or None. k_pool, v_pool:
     [pages, hkv, page_rows, d]; slots: int32 [t, 2] (page, row), distinct (PagedKV.reserve). Any
     strides with a contiguous last dimension. Returns the rotated queries, in q's shape and stored
-    token by token ([t, hq, d]), or None. fp32 inside, each output rounded once."""
+    token by token ([t, hq, d]), or None. fp32 inside, each output rounded once. The rows it writes are not
+    stable (stable_tiles of a decode) for the launch that follows it."""
     what = "append_rope"
     if q is not None and (hb := _lib.host()) is not None:
-        out = hb.append_rope(k, v, cos, sin, k_pool, v_pool, slots, q, q_norm, k_norm, eps)
+        out = hb.append_rope(k, v, cos, sin, k_pool, v_pool, slots, q, q_norm, k_norm, float(eps))
         if out is not None:
             return out
     require_cuda(k, v, cos, sin, k_pool, v_pool, slots, *(x for x in (q, q_norm, k_norm) if x is not None), what=what)

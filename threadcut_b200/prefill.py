@@ -67,7 +67,7 @@ def prefill_attention_window(query, key, value, scale, window, sinks=0, *, split
     what = "prefill_attention_window"
     hb = _lib.host()
     if hb is not None:
-        out = hb.window_prefill(query, key, value, scale, int(window), int(sinks), int(splits or 0))
+        out = hb.window_prefill(query, key, value, float(scale), int(window), int(sinks), int(splits or 0))
         if out is not None:
             return out
     require_cuda(query, key, value, what=what)
