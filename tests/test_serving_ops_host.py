@@ -120,3 +120,14 @@ def prefill_paged_status(q=P, kp=P, vp=P, out=P, hq=8, hkv=2, lq=4, lk=100, d=12
     (dict(page_stride=65), 2), (dict(qs=127), 2), (dict(ktab=ctypes.c_void_p(8)), 2)])
 def test_window_paged_prefill_refuses(bad, status):
     assert prefill_paged_status(**bad) == status
+
+
+def test_window_sizes_take_any_window():
+    most = (1 << 63) - 1
+    prefill = _lib.lib().tc_prefill_window_workspace_size
+    for args in ((1, 32, 8, 512, 98304, 128), (2, 8, 4, 777, 5001, 64), (1, 8, 2, 1, 1, 128)):
+        assert prefill(*args, most, 0, 3) == prefill(*args, args[4], 0, 3)
+        assert prefill(*args, 100, most, 3) == prefill(*args, 100, args[4], 3)
+    assert prefill(1, 32, 8, 512, 98304, 128, 0, 0, 0) == 0 and prefill(1, 7, 2, 5, 9, 128, 4, 0, 0) == 0
+    decode = _lib.lib().tc_decode_attention_window_workspace_size
+    assert decode(1, 8, 4, 128, 4000, most, most, 0, 2) == decode(1, 8, 4, 128, 4000, 4000, 0, 0, 2)

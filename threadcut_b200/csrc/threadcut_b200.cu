@@ -2305,7 +2305,8 @@ size_t tc_prefill_window_workspace_size(int batch, int hq, int hkv, int lq, int 
                                         int64_t sinks, int splits) {
   if (batch < 1 || hkv < 1 || hq < hkv || hq % hkv != 0 || lq < 1 || lk < lq || d < 1 || window < 1 || sinks < 0)
     return 0;
-  const WindowPrefill w = plan_window_prefill(batch, hq, hkv, lq, lk, d, window, sinks, splits);
+  const WindowPrefill w = plan_window_prefill(batch, hq, hkv, lq, lk, d, window < lk ? window : lk,
+                                              sinks < lk ? sinks : lk, splits);
   return window_ws_bytes((int64_t)batch * lq * hq, d, w.splits);
 }
 
