@@ -179,6 +179,10 @@ def test_paged_windows_after_a_splice(page_rows, window, sinks):
             ref, tol = attend64(q, k, v, 0.1, seen, P_SPLIT[BF16])
             assert_within(out, ref, tol)
             assert torch.equal(out, kv.decode(0, q, 0.1, window=window, sinks=sinks))
+            other = visible(torch.tensor([kv.n], device=DEV), kv.n, window + 7, sinks + 1)[0]  # layers may differ
+            assert_within(kv.decode(0, q, 0.1, window=window + 7, sinks=sinks + 1),
+                          *attend64(q, k, v, 0.1, other, P_SPLIT[BF16]))
+            assert torch.equal(out, kv.decode(0, q, 0.1, window=window, sinks=sinks))
 
 
 @pytest.mark.parametrize("d", [64, 128, 256])

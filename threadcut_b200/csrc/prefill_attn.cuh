@@ -148,7 +148,9 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const __grid_con
   __syncthreads();
   tmem_fence_after();
   const uint32_t tmem = s_tmem;
-  if constexpr (kWindow) {  // launched with programmatic dependent launch
+  if constexpr (kWindow) {
+    // launched with programmatic dependent launch; the next kernel is let in after the allocation above, since its
+    // CTAs may hold TMEM while they wait for this one
     pdl_launch();
     pdl_wait();
   }

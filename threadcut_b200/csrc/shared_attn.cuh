@@ -162,6 +162,7 @@ __global__ void __launch_bounds__(kShThreads, SharedGeom<D>::kCtasPerSm)
   tmem_fence_after();
   const uint32_t tmem = ctl.tmem;  // S buffer i (and P over it) at +64i, O at +128
   const uint32_t tO = tmem + 128;
+  // The next kernel is let in after the allocation above: its CTAs may hold TMEM while they wait for this one.
   pdl_launch();
   pdl_wait();  // queries, lengths, tables and the cache may be the previous kernel's
   int t0, t1, end;  // this part's key tiles, and the keys of its source

@@ -340,8 +340,8 @@ class PagedKV:
         self._slots = None       # device int32 [t, 2] of the step reserved last
         self._tiles_dev = None   # device int32 [capacity, 3]: the tile table, rows [0, n) valid
         self._tiles_ver = -1     # table version the device copy reflects
-        self._win = None         # (version, window, sinks) of the windowed table below
-        self._win_dev = None     # device int32 [T, 3]: the tiles a windowed decode reads
+        self._win = {}           # (window, sinks) -> device int32 [T, 3]: the tiles a windowed decode reads
+        self._win_ver = -1       # table version those tables reflect
         self._ktab = None        # device int32 [T, 4]: tiles + logical start, for prefill
         self._ktab_starts = None
         self._ktab_ver = -1
@@ -411,16 +411,17 @@ class PagedKV:
                            k_norm=k_norm, eps=eps)
 
     def _window_tiles(self, window, sinks):
-        """Device tile table of a windowed decode, its length and the tokens it lists; rebuilt when the
-        sequence or the window changed (once a step for all layers)."""
-        key = (self.table.version, window, sinks)
-        if self._win != key:
-            tab = np.ascontiguousarray(self.table.window_tiles(window, sinks))
+        """Device tile table of a windowed decode, its length and the tokens it lists; built once per
+        window and state of the sequence (once a step for all layers that share a window)."""
+        if self._win_ver != self.table.version:
+            self._win, self._win_ver = {}, self.table.version
+        tab = self._win.get((window, sinks))
+        if tab is None:
             # a fresh tensor: an earlier step's launches may still be reading the old one
-            self._win_dev = torch.from_numpy(tab).to(self.device)
-            self._win = key
-        nt = self._win_dev.shape[0]
-        return (self._win_dev if nt else None), nt, min(self.table.n, window + sinks)
+            tab = torch.from_numpy(np.ascontiguousarray(self.table.window_tiles(window, sinks))).to(self.device)
+            self._win[(window, sinks)] = tab
+        nt = tab.shape[0]
+        return (tab if nt else None), nt, min(self.table.n, window + sinks)
 
     def decode(self, layer, q, scale, *, k_new=None, v_new=None, splits=None, stable_tiles=0, window=None, sinks=0):
         """Decode attention of q [hkv, g, d] over the whole sequence (threadcut/flash_decode.py:57-69
