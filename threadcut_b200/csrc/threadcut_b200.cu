@@ -2279,6 +2279,7 @@ int run_shared_tc5(const SharedCall& c, void* workspace, size_t workspace_bytes,
   p.m = (int)c.m;
   p.np = w.np;
   p.ns = w.ns;
+  p.warm = w.ctas <= (int64_t)sm_count(current_device()) * (c.d == 256 ? 1 : 2);
   p.c = c.scale * kLog2e;
   p.o = static_cast<float*>(workspace);
   p.ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + w.ml);
