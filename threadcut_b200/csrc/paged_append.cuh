@@ -6,7 +6,8 @@
 //   z = x * rsqrt(mean(x^2) + eps) * w                      (with a norm weight; else z = x)
 //   out[i] = z[i] cos[i] - z[i + rot/2] sin[i]              i < rot/2
 //   out[i] = z[i] cos[i] + z[i - rot/2] sin[i]              rot/2 <= i < rot
-//   out[i] = z[i]                                           i >= rot (partial rotation)
+//   out[i] = z[i]                                           i >= rot (partial rotation; x[i] itself, to the bit,
+//                                                           without a weight)
 // in fp32 from the loaded values on, rounded once to T at the store. (The torch chain, and with it
 // tc_qk_norm_rope, rounds to T after each op; one rounding is nearer to the formula.)
 #pragma once
@@ -94,7 +95,7 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const __grid_constant
                                     : to_f32(static_cast<const T*>(p.sin_t)[tok * p.sin_st + i]);
         o = z[i] * c + (i < half ? -z[i + half] : z[i - half]) * s;
       }
-      dst[i] = from_f32<T>(o);
+      dst[i] = i >= p.rot && w == nullptr ? src[i] : from_f32<T>(o);
     }
     __syncwarp();
   }
@@ -129,9 +130,11 @@ __device__ __forceinline__ Chunk<T, VEC> narrow(const float2 (&x)[VEC / 2]) {
 //   out_a = (r x_a) (w_a cos_a) - (r x_b) (w_b sin_a),   out_b = (r x_b) (w_b cos_b) + (r x_a) (w_a sin_b),
 // a row costs three packed operations an output pair beside its conversions.
 // Bound by bytes for long chunks, by latency for short ones: resident warps count in both. 16,384 tokens of
-// 48 bf16 heads of 128 (411 MB): 2 rows a thread and 7 CTAs an SM (72 registers) 78.6 us, 5.2 TB/s; 6 CTAs 81.8,
+// 48 bf16 heads of 128 (411 MB): 2 rows a thread and 7 CTAs an SM (72 registers) 76.7 us, 5.4 TB/s; before the split below 78.6, 6 CTAs 81.8,
 // 8 CTAs (spills) 83.7; 4 rows 86.9, 8 rows 102; with the formula's own order of operations, unpacked, 106.
-template <typename T, typename TT>
+// kPartial: rot < d, some threads hold chunks that pass through. Full rotations have a kernel without their branch
+// (32 bytes of spills a thread instead of 56): the prompt above takes 76.7 us, with one kernel for both 80.4.
+template <typename T, typename TT, bool kPartial>
 __global__ void __launch_bounds__(kAppendThreads, 7)
     paged_append_vec_kernel(const __grid_constant__ PagedAppendParams p) {
   constexpr int kRows = kAppendRows;
@@ -152,7 +155,7 @@ __global__ void __launch_bounds__(kAppendThreads, 7)
   const bool isq = grp < q_groups;
   const int c = lane & (p.pairs - 1);
   const int turned = p.rot / (2 * VEC);  // pairs that rotate; the others pass through side by side
-  const bool turns = c < turned;
+  const bool turns = !kPartial || c < turned;
   const int ia = (turns ? c : 2 * c) * VEC, ib = turns ? ia + p.rot / 2 : ia + VEC;
 
   // ---- the rows: this thread's row u is head h0 + u * step (keys: u < kRows / 2, then their values)
@@ -237,7 +240,9 @@ __global__ void __launch_bounds__(kAppendThreads, 7)
   }
 #pragma unroll
   for (int u = 0; u < kRows; ++u) {
-    if (isq || u < kRows / 2) {
+    // Elements that pass through are not multiplied with their chunk's neighbour (0 * inf is NaN); without a
+    // weight they stay as they were loaded.
+    if ((isq || u < kRows / 2) && (turns || w != nullptr)) {
       float2 xa[P2], xb[P2];
       widen<T, VEC>(a[u], xa);
       widen<T, VEC>(b[u], xb);
@@ -257,11 +262,19 @@ __global__ void __launch_bounds__(kAppendThreads, 7)
           xb[e] = fmul2(xb[e], r2);
         }
       }
+      if (turns) {
 #pragma unroll
-      for (int e = 0; e < P2; ++e) {
-        const float2 oa = ffma2(xa[e], fac[e], fmul2(xb[e], fas[e]));
-        xb[e] = ffma2(xb[e], fbc[e], fmul2(xa[e], fbs[e]));
-        xa[e] = oa;
+        for (int e = 0; e < P2; ++e) {
+          const float2 oa = ffma2(xa[e], fac[e], fmul2(xb[e], fas[e]));
+          xb[e] = ffma2(xb[e], fbc[e], fmul2(xa[e], fbs[e]));
+          xa[e] = oa;
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < P2; ++e) {
+          xa[e] = fmul2(xa[e], fac[e]);
+          xb[e] = fmul2(xb[e], fbc[e]);
+        }
       }
       a[u] = narrow<T, VEC>(xa);
       b[u] = narrow<T, VEC>(xb);

@@ -1074,7 +1074,7 @@ int tc_paged_write(const void* k_src, const void* v_src, void* k_pool, void* v_p
 
 namespace {
 // Whether rows, tables and weights are whole 16-byte chunks on 16-byte boundaries and a row is a power of
-// two of chunk pairs: what paged_append_vec_kernel takes (16,384 tokens of 48 bf16 heads of 128: 79 us, where
+// two of chunk pairs: what paged_append_vec_kernel takes (16,384 tokens of 48 bf16 heads of 128: 77 us, where
 // paged_append_kernel takes 443).
 bool paged_append_vec(PagedAppendParams& p, int dtype) {
   const int vec = dtype == TC_F32 ? 4 : 8, tab = p.table_f32 ? TC_F32 : dtype;
@@ -1096,8 +1096,8 @@ template <typename T, typename TT>
 cudaError_t launch_paged_append_vec(const PagedAppendParams& p, cudaStream_t st) {
   const int heads = 32 / p.pairs * kAppendRows;  // query heads a warp takes; keys (and their values): half
   const int64_t warps = p.t * (cdiv(p.hq, heads) + cdiv(2 * p.hkv, heads));
-  return launch_ex(paged_append_vec_kernel<T, TT>, dim3((unsigned)cdiv(warps, kAppendThreads / 32)),
-                   dim3(kAppendThreads), 0, st, p);
+  return launch_ex(p.rot < p.d ? paged_append_vec_kernel<T, TT, true> : paged_append_vec_kernel<T, TT, false>,
+                   dim3((unsigned)cdiv(warps, kAppendThreads / 32)), dim3(kAppendThreads), 0, st, p);
 }
 
 template <typename T>
