@@ -1,0 +1,61 @@
+"""The attention plugin's reading of masks, on the CPU: which masks count as the causal one or as a window, also for
+tensors made under torch.inference_mode(), which have no version counter."""
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+from threadcut_b200 import attention as A
+from threadcut_b200.prefill import causal_offset_mask
+
+
+@pytest.fixture(autouse=True)
+def _fresh(monkeypatch):
+    monkeypatch.setattr(A, "_mask_seen", {})
+    monkeypatch.setattr(A, "_window_seen", {})
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+
+
+def window_mask(lq, lk, w):
+    at = (lk - lq + torch.arange(lq))[:, None]
+    j = torch.arange(lk)
+    return ((j <= at) & (j > at - w))[None, None]
+
+
+def window_of(mask, lq, lk, w):
+    """_window_of for a query that looks like one on the GPU."""
+    query = SimpleNamespace(shape=(1, 8, lq, 128), is_cuda=True, dtype=torch.bfloat16, requires_grad=False)
+    return A._window_of(query, mask, lq, lk, 0.1, dict(sliding_window=w))
+
+
+@pytest.mark.parametrize("mode", [torch.no_grad, torch.inference_mode])
+@pytest.mark.parametrize("lq,lk,w", [(1, 30, 7), (5, 30, 7), (30, 30, 40)])
+def test_a_window_is_known_in_either_mode(mode, lq, lk, w):
+    with mode():
+        mask = window_mask(lq, lk, w)
+        for _ in range(2):
+            assert window_of(mask, lq, lk, w) == w
+        assert window_of(mask, lq, lk, 3) is None  # another window than the mask's
+        mask[0, 0, 0, 0 if w < lk else 1] ^= True  # changed in place: compared anew
+        assert window_of(mask, lq, lk, w) is None
+
+
+@pytest.mark.parametrize("mode", [torch.no_grad, torch.inference_mode])
+@pytest.mark.parametrize("lq,lk", [(1, 30), (5, 30), (30, 30)])
+def test_the_causal_mask_is_known_in_either_mode(mode, lq, lk):
+    with mode():
+        mask = causal_offset_mask(lq, lk, "cpu")[None, None].clone()
+        for _ in range(2):
+            assert A._is_causal_offset(mask, lq, lk)
+        mask[0, 0, 0, 0] ^= True
+        assert not A._is_causal_offset(mask, lq, lk)
+        assert not A._is_causal_offset(mask[:, :, :, 1:], lq, lk)
+
+
+def test_a_mask_of_one_mode_used_in_the_other():
+    normal = window_mask(5, 30, 7)
+    with torch.inference_mode():
+        made_there = window_mask(5, 30, 7)
+        assert window_of(normal, 5, 30, 7) == 7
+    assert window_of(made_there, 5, 30, 7) == 7
+    assert window_of(normal, 5, 30, 7) == 7

@@ -17,7 +17,8 @@ the pages (PagedKV.prefill), and other branches get a contiguous copy.
 A sliding-window layer (transformers passes its `sliding_window`, and a mask that hides older keys) runs
 the windowed kernels when the mask is that window and nothing else: decode_attention_window for one token,
 prefill_attention_window for a chunk, or their forms over the pages. The comparison reads the mask back
-once per mask tensor, so a step under stream capture keeps the SDPA branch.
+once per mask tensor (once per call in torch.inference_mode()), so a step under stream capture keeps the
+SDPA branch.
 Decode on a non-CUDA tensor raises: there is no CPU path.
 Prefill (q > 1 or a mask): a causal prefill over the cache (query p sees keys up to lk - lq + p;
 b == 1, 4 query heads per KV head, head_dim 128, 16-bit) runs the tcgen05 kernel of
@@ -49,23 +50,30 @@ def repeat_kv(x, n):
     return x.unsqueeze(2).expand(b, h, n, s, d).reshape(b, h * n, s, d)
 
 
+def _version(mask):
+    """The version counter by which a mask compared before is known to be unchanged; None for a tensor made under
+    torch.inference_mode(), which has no counter: it is compared anew each time."""
+    return None if mask.is_inference() else mask._version
+
+
 _mask_seen = {}  # the last mask tensor found to be the causal-offset mask (weak reference) + version
 
 
 def _is_causal_offset(mask, lq, lk):
     """True when `mask` means query p sees keys [0, lk - lq + p]: None with lq == lk (HF drops the
     mask of a plain causal prefill), or the boolean [1, 1, lq, lk] mask HF builds for a prefill over
-    a cache. The comparison runs once per mask tensor (HF passes one mask to every layer)."""
+    a cache. The comparison runs once per mask tensor (HF passes one mask to every layer), in
+    torch.inference_mode() once per call."""
     if mask is None:
         return lq == lk
     if mask.dtype != torch.bool or tuple(mask.shape) != (1, 1, lq, lk):
         return False
-    hit = _mask_seen.get("last")
-    if hit is not None and hit[0]() is mask and hit[1] == mask._version:
+    hit, version = _mask_seen.get("last"), _version(mask)
+    if hit is not None and version is not None and hit[0]() is mask and hit[1] == version:
         return True
     ok = bool(torch.equal(mask[0, 0], _prefill.causal_offset_mask(lq, lk, mask.device)))
-    if ok:
-        _mask_seen["last"] = (weakref.ref(mask), mask._version)
+    if ok and version is not None:
+        _mask_seen["last"] = (weakref.ref(mask), version)
     return ok
 
 
@@ -83,14 +91,15 @@ def _window_of(query, mask, lq, lk, scaling, kwargs):
             or kwargs.get("softcap") is not None or kwargs.get("s_aux") is not None
             or torch.cuda.is_current_stream_capturing()):
         return None
-    hit = _window_seen.get("last")
-    if hit is None or hit[0]() is not mask or hit[1:3] != (mask._version, w):
+    hit, version = _window_seen.get("last"), _version(mask)
+    if hit is None or version is None or hit[0]() is not mask or hit[1:3] != (version, w):
         seen = _prefill.causal_offset_mask(lq, lk, mask.device)
         if w < lk:
             seen = seen & (torch.arange(lk, device=mask.device)[None, :]
                            > (lk - lq - w) + torch.arange(lq, device=mask.device)[:, None])
-        hit = (weakref.ref(mask), mask._version, w, bool(torch.equal(mask[0, 0], seen)))
-        _window_seen["last"] = hit
+        hit = (weakref.ref(mask), version, w, bool(torch.equal(mask[0, 0], seen)))
+        if version is not None:
+            _window_seen["last"] = hit
     return w if hit[3] else None
 
 
