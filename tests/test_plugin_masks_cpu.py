@@ -25,7 +25,8 @@ def window_mask(lq, lk, w):
 def window_of(mask, lq, lk, w):
     """_window_of for a query that looks like one on the GPU."""
     query = SimpleNamespace(shape=(1, 8, lq, 128), is_cuda=True, dtype=torch.bfloat16, requires_grad=False)
-    return A._window_of(query, mask, lq, lk, 0.1, dict(sliding_window=w))
+    key = SimpleNamespace(shape=(1, 2, lk, 128), requires_grad=False)
+    return A._window_of(query, key, key, mask, lq, lk, 0.1, dict(sliding_window=w))
 
 
 @pytest.mark.parametrize("mode", [torch.no_grad, torch.inference_mode])

@@ -57,3 +57,34 @@ def test_a_model_with_sliding_layers_in_inference_mode(paged):
         runs.append(out)
     for a, b in zip(*runs):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("d,hq", [(128, 8), (64, 6)])
+def test_a_recorded_call_of_a_sliding_layer_has_gradients(d, hq):
+    """The gradients of SDPA over the same mask, for each input that asks for them; without recording, the same
+    windowed result as ever."""
+    gen = torch.Generator(device=DEV).manual_seed(d)
+    x = [torch.randn(1, h, n, d, generator=gen, device=DEV).to(torch.bfloat16) for h, n in ((hq, 30), (2, 60), (2, 60))]
+    mask = window_mask(30, 60, 12)
+    up = torch.randn(1, 30, hq, d, generator=gen, device=DEV).to(torch.bfloat16)
+
+    def ours(*a):
+        return tc_attention.attention(None, *a, mask, scaling=0.1, sliding_window=12)[0]
+
+    def sdpa(*a):
+        return torch.nn.functional.scaled_dot_product_attention(*a, attn_mask=mask, scale=0.1, enable_gqa=True).transpose(1, 2)
+
+    plain = ours(*x)
+    assert plain.grad_fn is None
+    for asks in ((0, 1, 2), (0,), (1,), (2,)):
+        grads = []
+        for fn in (ours, sdpa):
+            leaves = [t.clone().requires_grad_(i in asks) for i, t in enumerate(x)]
+            out = fn(*leaves)
+            out.backward(up)
+            grads.append([out.detach()] + [t.grad for t in leaves if t.requires_grad])
+        assert len(grads[0]) == 1 + len(asks)
+        for a, b in zip(*grads):  # the same pass twice; fp32 sums in another order may move a rounding by one step
+            assert torch.allclose(a.float(), b.float(), rtol=torch.finfo(torch.bfloat16).eps, atol=1e-5)
+        with torch.no_grad():
+            assert torch.equal(ours(*leaves), plain)

@@ -16,7 +16,8 @@ over the pages (PagedKV.decode, fused append), a causal prefill chunk runs the t
 the pages (PagedKV.prefill), and other branches get a contiguous copy.
 A sliding-window layer (transformers passes its `sliding_window`, and a mask that hides older keys) runs
 the windowed kernels when the mask is that window and nothing else: decode_attention_window for one token,
-prefill_attention_window for a chunk, or their forms over the pages. The comparison reads the mask back
+prefill_attention_window for a chunk, or their forms over the pages. A call that autograd records keeps the SDPA
+branch, which has a backward pass. The comparison reads the mask back
 once per mask tensor (once per call in torch.inference_mode()), so a step under stream capture keeps the
 SDPA branch.
 Decode on a non-CUDA tensor raises: there is no CPU path.
@@ -80,15 +81,17 @@ def _is_causal_offset(mask, lq, lk):
 _window_seen = {}  # the last mask tensor compared with a window's: (weak reference, version, window, result)
 
 
-def _window_of(query, mask, lq, lk, scaling, kwargs):
+def _window_of(query, key, value, mask, lq, lk, scaling, kwargs):
     """The window W of a sliding-window layer whose mask means exactly "query p sees the last W keys up to
-    its own", if the windowed kernels take the call; else None."""
+    its own", if the windowed kernels take the call; else None. They have no backward pass, so a call that autograd
+    records keeps the SDPA branch."""
     w = kwargs.get("sliding_window")
     d = query.shape[-1]
     if (not isinstance(w, int) or w < 1 or mask is None or mask.dtype != torch.bool or tuple(mask.shape) != (1, 1, lq, lk)
             or lq > lk or query.shape[0] != 1 or not query.is_cuda or not scaling > 0
             or query.dtype not in (torch.bfloat16, torch.float16) or d not in (64, 128)
             or kwargs.get("softcap") is not None or kwargs.get("s_aux") is not None
+            or (torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad))
             or torch.cuda.is_current_stream_capturing()):
         return None
     hit, version = _window_seen.get("last"), _version(mask)
@@ -110,7 +113,7 @@ def attention(module, query, key, value, attention_mask, dropout=0.0, scaling=No
     scaling = scaling if scaling is not None else d ** -0.5
     paged = paged_pending(key)
     if paged is not None:
-        w = _window_of(query, attention_mask, q, paged.get_seq_length(), scaling, kwargs)
+        w = _window_of(query, key, value, attention_mask, q, paged.get_seq_length(), scaling, kwargs)
         if w is not None and q == 1 and g <= 16 and paged._pending is not None:
             out = paged.decode(query.reshape(hkv, g, d), scaling, window=w).reshape(1, hq, 1, d)
             return out.transpose(1, 2).contiguous(), None
@@ -134,7 +137,7 @@ def attention(module, query, key, value, attention_mask, dropout=0.0, scaling=No
         return out.transpose(1, 2).contiguous(), None
     if layer is not None:
         layer._flush()
-    w = _window_of(query, attention_mask, q, key.shape[2], scaling, kwargs)
+    w = _window_of(query, key, value, attention_mask, q, key.shape[2], scaling, kwargs)
     if w is not None and q == 1 and g <= 16:
         out = decode_attention_window(query.reshape(hkv, g, d), key[0], value[0], scaling, w).reshape(1, hq, 1, d)
         return out.transpose(1, 2).contiguous(), None
