@@ -60,3 +60,12 @@ def test_a_mask_of_one_mode_used_in_the_other():
         assert window_of(normal, 5, 30, 7) == 7
     assert window_of(made_there, 5, 30, 7) == 7
     assert window_of(normal, 5, 30, 7) == 7
+
+
+def test_values_of_another_head_size_are_no_window():
+    """The windowed kernels take keys and values of one shape; SDPA does not need that."""
+    query = SimpleNamespace(shape=(1, 8, 5, 128), is_cuda=True, dtype=torch.bfloat16, requires_grad=False)
+    key, value, same = (SimpleNamespace(shape=(1, 2, 30, d), requires_grad=False) for d in (128, 64, 128))
+    mask, kw = window_mask(5, 30, 7), dict(sliding_window=7)
+    assert A._window_of(query, key, same, mask, 5, 30, 0.1, kw) == 7
+    assert A._window_of(query, key, value, mask, 5, 30, 0.1, kw) is None

@@ -88,3 +88,14 @@ def test_a_recorded_call_of_a_sliding_layer_has_gradients(d, hq):
             assert torch.allclose(a.float(), b.float(), rtol=torch.finfo(torch.bfloat16).eps, atol=1e-5)
         with torch.no_grad():
             assert torch.equal(ours(*leaves), plain)
+
+
+@pytest.mark.parametrize("lq", [1, 40])
+def test_a_sliding_layer_with_values_of_another_head_size(lq):
+    gen = torch.Generator(device=DEV).manual_seed(lq)
+    q, k, v = (torch.randn(1, h, n, d, generator=gen, device=DEV).to(torch.bfloat16)
+               for h, n, d in ((8, lq, 128), (2, 100, 128), (2, 100, 64)))
+    mask = window_mask(lq, 100, 33)
+    out, _ = tc_attention.attention(None, q, k, v, mask, scaling=0.1, sliding_window=33)
+    want = torch.nn.functional.scaled_dot_product_attention(q, k, v, attn_mask=mask, scale=0.1, enable_gqa=True)
+    assert torch.equal(out, want.transpose(1, 2))

@@ -88,8 +88,8 @@ def _window_of(query, key, value, mask, lq, lk, scaling, kwargs):
     w = kwargs.get("sliding_window")
     d = query.shape[-1]
     if (not isinstance(w, int) or w < 1 or mask is None or mask.dtype != torch.bool or tuple(mask.shape) != (1, 1, lq, lk)
-            or lq > lk or query.shape[0] != 1 or not query.is_cuda or not scaling > 0
-            or query.dtype not in (torch.bfloat16, torch.float16) or d not in (64, 128)
+            or lq > lk or query.shape[0] != 1 or value.shape != key.shape or not query.is_cuda or not scaling > 0
+            or query.dtype not in (torch.bfloat16, torch.float16) or d not in (64, 128) or key.shape[-1] != d
             or kwargs.get("softcap") is not None or kwargs.get("s_aux") is not None
             or (torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad))
             or torch.cuda.is_current_stream_capturing()):
