@@ -6,7 +6,7 @@
 //
 // One CTA per query row; each of its warps takes every kRowsWarps-th group of 32 keys, a lane per key for
 // the scores (the row is in shared memory as fp32), then a lane per element for P V, with a running
-// maximum and sum; the warps' states are joined in shared memory. No visible key: zeros.
+// maximum and sum; the warps' states are joined in shared memory. No visible key, or only scores of -inf: zeros.
 #pragma once
 
 #include <stdint.h>
@@ -80,7 +80,8 @@ __global__ void __launch_bounds__(32 * kRowsWarps) rows_attn_kernel(const __grid
     }
     const float mn = fmaxf(m, warp_max(s));
     const float a = m == -INFINITY ? 0.f : exp2f(m - mn);
-    const float w = j < total ? exp2f(s - mn) : 0.f;
+    // a group of scores that are all -inf (the first ones of a warp) has weights 0, not exp2(inf - inf)
+    const float w = j < total ? exp2f(s - (mn == -INFINITY ? 0.f : mn)) : 0.f;
     l = l * a + warp_sum(w);
 #pragma unroll
     for (int x = 0; x < E; ++x) acc[x] *= a;
@@ -107,7 +108,7 @@ __global__ void __launch_bounds__(32 * kRowsWarps) rows_attn_kernel(const __grid
   for (int w = 0; w < kRowsWarps; ++w) M = fmaxf(M, s_m[w]);
 #pragma unroll
   for (int w = 0; w < kRowsWarps; ++w) {
-    f[w] = s_l[w] == 0.f ? 0.f : exp2f(s_m[w] - M);  // a warp with no keys has l = 0
+    f[w] = s_l[w] == 0.f ? 0.f : exp2f(s_m[w] - M);  // a warp with no keys, or all at -inf, has l = 0
     L += f[w] * s_l[w];
   }
   T* out = static_cast<T*>(p.out) + b * p.so_b + h * p.so_h + i * p.so_g + pos * p.so_p;
@@ -115,7 +116,7 @@ __global__ void __launch_bounds__(32 * kRowsWarps) rows_attn_kernel(const __grid
     float o = 0.f;
 #pragma unroll
     for (int w = 0; w < kRowsWarps; ++w) o += f[w] * s_o[w][e];
-    out[e] = from_f32<T>(total > 0 ? o / L : 0.f);
+    out[e] = from_f32<T>(L == 0.f ? 0.f : o / L);
   }
 }
 
