@@ -189,6 +189,9 @@ __device__ __forceinline__ float warp_sum(float x) {
   for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
   return x;
 }
+// What a running maximum is subtracted as: 0 while every score so far is -inf (or none was seen), so that such a
+// score's weight is 2^-inf = 0 and not 2^(inf - inf).
+__device__ __forceinline__ float max_ref(float m) { return m == -INFINITY ? 0.f : m; }
 __device__ __forceinline__ float lse_nat(float m2, float l) {
   return l > 0.f ? (m2 + __log2f(l)) * kLn2 : -INFINITY;
 }
@@ -306,7 +309,7 @@ __device__ void merge_last(const DecodeParams& p, uint8_t* scratch, int b, int h
         At.z += wt * v.z;
         At.w += wt * v.w;
       }
-      const float inv = Lt > 0.f ? 1.f / Lt : 0.f;
+      const float inv = Lt == 0.f ? 0.f : 1.f / Lt;
       const int64_t o = out0 + i * p.so_g + (c0 + c - i * Q) * 4;
       put_out<T>(p, o, At.x * inv);
       put_out<T>(p, o + 1, At.y * inv);
@@ -354,9 +357,9 @@ __device__ void finish_cta(const DecodeParams& p, uint8_t* regions, int region_s
   if (tid < g) {
     float M = -INFINITY;
     for (int w = 0; w < nregions; ++w) M = fmaxf(M, R::m(region(w))[tid]);
+    const float ref = max_ref(M);
     float L = 0.f;
-    if (M != -INFINITY)
-      for (int w = 0; w < nregions; ++w) L += R::l(region(w))[tid] * fast_exp2(R::m(region(w))[tid] - M);
+    for (int w = 0; w < nregions; ++w) L += R::l(region(w))[tid] * fast_exp2(R::m(region(w))[tid] - ref);
     s_M[tid] = M;
     s_L[tid] = L;
     if (nsplit > 1) p.ws_ml[(bh * p.max_splits + split) * g + tid] = make_float2(M, L);
@@ -365,13 +368,12 @@ __device__ void finish_cta(const DecodeParams& p, uint8_t* regions, int region_s
   float* wo = p.ws_o + (bh * p.max_splits + split) * g * D;
   for (int idx = tid; idx < g * D; idx += nthr) {
     const int i = idx / D, d = idx - i * D;
-    const float M = s_M[i];
+    const float ref = max_ref(s_M[i]);
     float o = 0.f;
-    if (M != -INFINITY)
-      for (int w = 0; w < nregions; ++w) o += R::acc(region(w), i)[d] * fast_exp2(R::m(region(w))[i] - M);
+    for (int w = 0; w < nregions; ++w) o += R::acc(region(w), i)[d] * fast_exp2(R::m(region(w))[i] - ref);
     if (nsplit == 1) {
-      const float L = s_L[i];
-      put_out<T>(p, out0 + i * p.so_g + d, L > 0.f ? o / L : 0.f);
+      const float L = s_L[i];  // 0: nothing seen, or scores of -inf alone; NaN scores give NaN
+      put_out<T>(p, out0 + i * p.so_g + d, L == 0.f ? 0.f : o / L);
     } else {
       wo[idx] = o;
     }
@@ -486,7 +488,7 @@ __device__ void finish_cta(const DecodeParams& p, uint8_t* regions, int region_s
         At.z += wt * v.z;
         At.w += wt * v.w;
       }
-      const float inv = Lt > 0.f ? 1.f / Lt : 0.f;
+      const float inv = Lt == 0.f ? 0.f : 1.f / Lt;
       const int64_t o = out0 + i * p.so_g + (c - i * Q) * 4;
       put_out<T>(p, o, At.x * inv);
       put_out<T>(p, o + 1, At.y * inv);
@@ -886,10 +888,11 @@ __global__ void __launch_bounds__(32 * (kCWarps + 1), 1)
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
           const float mnew = fmaxf(m_run[nt][e], mx);
-          alpha[nt][e] = fast_exp2(m_run[nt][e] - mnew);
+          const float mref = max_ref(mnew);
+          alpha[nt][e] = fast_exp2(m_run[nt][e] - mref);
           m_run[nt][e] = mnew;
-          const float p0 = fast_exp2(x0 - mnew), p1 = fast_exp2(x1 - mnew);
-          const float p2 = fast_exp2(x2 - mnew), p3 = fast_exp2(x3 - mnew);
+          const float p0 = fast_exp2(x0 - mref), p1 = fast_exp2(x1 - mref);
+          const float p2 = fast_exp2(x2 - mref), p3 = fast_exp2(x3 - mref);
           l_run[nt][e] = l_run[nt][e] * alpha[nt][e] + ((p0 + p1) + (p2 + p3));
           sacc[0][nt][e] = p0;
           sacc[0][nt][2 + e] = p1;
@@ -1061,8 +1064,9 @@ __global__ void __launch_bounds__(32 * kGenWarps) decode_generic_kernel(const __
         for (int j = 0; j < DPL; ++j) s = fmaf(qv[i][j], kv[j], s);
         s = warp_sum(s) * p.c;
         const float mn = fmaxf(m[i], s);
-        const float al = fast_exp2(m[i] - mn);
-        const float pp = fast_exp2(s - mn);
+        const float mref = max_ref(mn);
+        const float al = fast_exp2(m[i] - mref);
+        const float pp = fast_exp2(s - mref);
         l[i] = l[i] * al + pp;
 #pragma unroll
         for (int j = 0; j < DPL; ++j) acc[i][j] = fmaf(pp, vv[j], acc[i][j] * al);
