@@ -2143,8 +2143,10 @@ void plan_shared_parts(SharedPlan& w, int64_t groups, int64_t tails, int64_t tp,
   double best = 0.0;
   bool first = true;
   for (int parts = 1; parts <= kShMaxParts; ++parts) {
-    // tiles a part: the prefix's share, or, without a prefix, the suffix's
-    const int64_t x = cdiv(tp > 0 ? tp : (ts > 0 ? ts : 1), parts);
+    // tiles a part, of either source: a share of the longer one, so that long suffixes behind a short prefix are not
+    // cut to its length. 256 sequences, 64 + 4,096: 637 us and 8.5 MB of workspace; with shares of the prefix
+    // 1,966 us and 277 MB. 48 sequences, 64 + 1,500: 57 us, 150; 1,000 + 1,500: 60 us, 57.
+    const int64_t x = cdiv(tp > ts ? tp : (ts > 0 ? ts : 1), parts);
     if (x < 2 && !first) break;
     const int np = parts_of(tp, x), ns = parts_of(ts, x);
     const double a = (double)x + kShCtaTiles, s = (ns > 0 ? 0.6 * (double)ts / ns : 0.0) + kShCtaTiles;
