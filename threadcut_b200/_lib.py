@@ -188,6 +188,16 @@ def dtype_code(t, what):
         raise TypeError(f"threadcut_b200.{what}: unsupported dtype {t.dtype}") from None
 
 
+def rows16(x):
+    """x itself if a tensor map can describe it (rows that start on 16-byte boundaries, no broadcast dimension), else
+    a copy that one can. The strides of extents of 1 count too, since the library checks them all."""
+    es = x.element_size()
+    if (x.stride(-1) == 1 and x.data_ptr() % 16 == 0
+            and all(s * es % 16 == 0 and (s > 0 or n <= 1) for n, s in zip(x.shape[:-1], x.stride()[:-1]))):
+        return x
+    return x.clone(memory_format=torch.contiguous_format)
+
+
 def stream_ptr(device):
     """Raw cudaStream_t of torch's current stream on `device` (what every launch goes to)."""
     return torch._C._cuda_getCurrentRawStream(device.index if device.index is not None

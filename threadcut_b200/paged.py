@@ -25,7 +25,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._lib import check, dtype_code, lib, require_cuda, stream_ptr, workspaces
+from ._lib import check, dtype_code, lib, require_cuda, rows16, stream_ptr, workspaces
 from .match import Split
 
 __all__ = ["PageTable", "PagedKV", "TILE_ROWS", "append_rope"]
@@ -307,14 +307,6 @@ def append_rope(k, v, cos, sin, k_pool, v_pool, slots, *, q=None, q_norm=None, k
     return out[None] if batched and out is not None else out
 
 
-def _rows16(x):
-    """x itself if its rows start on 16-byte boundaries (the tensor-map rule), else a contiguous copy."""
-    es = x.element_size()
-    if x.stride(-1) == 1 and x.data_ptr() % 16 == 0 and all(s * es % 16 == 0 for s in x.stride()[:-1]):
-        return x
-    return x.contiguous()
-
-
 class PagedKV:
     """Paged K/V of `layers` attention layers of one sequence on one GPU.
 
@@ -492,7 +484,7 @@ class PagedKV:
                             f"{k.dtype}, {v.dtype}")
         if not scale > 0:
             raise ValueError(f"{what}: needs scale > 0, got {scale}")
-        q, k, v = (_rows16(x) for x in (q, k, v))
+        q, k, v = (rows16(x) for x in (q, k, v))
         lens_ptr = None
         if lengths is not None:
             if lengths.dtype != torch.int32 or lengths.device != q.device or not lengths.is_contiguous():
@@ -547,7 +539,7 @@ class PagedKV:
         qb[:, 0] = np.searchsorted(tile_starts, np.maximum(p0 + 1 - window, 0), side="right") - 1
         qb[:, 1] = np.searchsorted(tile_starts, np.minimum(p0 + block, n), side="left")
         qb_tiles = torch.from_numpy(qb).to(self.device)
-        q = _rows16(query[0])
+        q = rows16(query[0])
         out = torch.empty((1, lq, hq, d), dtype=query.dtype, device=query.device)
         L = lib()
         n_sub = ktab.shape[0]
