@@ -160,6 +160,16 @@ bool plain_lengths(const OptTensor& n, const c10::Device& dev, int64_t b) {
 }
 const int32_t* lengths_ptr(const OptTensor& n) { return n ? n->data_ptr<int32_t>() : nullptr; }
 
+// x itself if a tensor map can describe it (rows on 16-byte boundaries, no broadcast dimension), else a copy that one
+// can; the strides of extents of 1 count too, since the library checks them all. (rows16 of the Python side.)
+at::Tensor rows16(const at::Tensor& x) {
+  const int64_t es = x.element_size();
+  bool ok = reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0;
+  for (int64_t i = 0; i + 1 < x.dim(); ++i)
+    ok = ok && x.stride(i) * es % 16 == 0 && (x.stride(i) > 0 || x.size(i) <= 1);
+  return ok ? x : x.clone(at::MemoryFormat::Contiguous);
+}
+
 // Scratch with no initial contents.
 at::Tensor scratch(size_t bytes, const at::Tensor& like) {
   return at::empty({(int64_t)bytes}, like.options().dtype(at::kByte));
@@ -252,18 +262,19 @@ py::object window_decode(const at::Tensor& q, const at::Tensor& k, const at::Ten
   return py::cast(out);
 }
 
-py::object window_prefill(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, double scale, int64_t window,
+py::object window_prefill(const at::Tensor& q_in, const at::Tensor& k, const at::Tensor& v, double scale, int64_t window,
                           int64_t sinks, int64_t splits) {
-  if (g_prefill == nullptr || !q.is_cuda() || q.dim() != 4 || k.dim() != 4 || v.sizes() != k.sizes()) return py::none();
-  const auto dev = q.device();
-  const auto dt = q.scalar_type();
+  if (g_prefill == nullptr || !q_in.is_cuda() || q_in.dim() != 4 || k.dim() != 4 || v.sizes() != k.sizes()) return py::none();
+  const auto dev = q_in.device();
+  const auto dt = q_in.scalar_type();
   const int code = dtype_code(dt);
-  const int64_t b = q.size(0), hq = q.size(1), lq = q.size(2), d = q.size(3), hkv = k.size(1), lk = k.size(2);
+  const int64_t b = q_in.size(0), hq = q_in.size(1), lq = q_in.size(2), d = q_in.size(3), hkv = k.size(1), lk = k.size(2);
   if (code < 0 || k.size(0) != b || k.size(3) != d || hkv < 1 || hq % hkv != 0 || lq < 1 || lq > lk || lk > INT32_MAX ||
-      !plain(q, dev, dt) || !plain(k, dev, dt) || !plain(v, dev, dt) || window < 1 || sinks < 0 || b < 1 || b > 65535 ||
+      !plain(q_in, dev, dt) || !plain(k, dev, dt) || !plain(v, dev, dt) || window < 1 || sinks < 0 || b < 1 || b > 65535 ||
       hq > 65535 || d > 65535 || splits < 0 || splits > 65535)
     return py::none();
   c10::cuda::CUDAGuard guard(dev);
+  const at::Tensor q = rows16(q_in);
   const cudaStream_t st = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
   window = std::min(window, lk);
   sinks = std::min(sinks, lk);
@@ -279,20 +290,21 @@ py::object window_prefill(const at::Tensor& q, const at::Tensor& k, const at::Te
   return py::cast(out);
 }
 
-py::object shared_decode(const at::Tensor& q, const at::Tensor& kp, const at::Tensor& vp, const at::Tensor& k,
+py::object shared_decode(const at::Tensor& q_in, const at::Tensor& kp, const at::Tensor& vp, const at::Tensor& k,
                          const at::Tensor& v, double scale, const OptTensor& lengths) {
-  if (g_shared == nullptr || !q.is_cuda() || q.dim() != 4 || kp.dim() != 3 || k.dim() != 4 || vp.sizes() != kp.sizes() ||
+  if (g_shared == nullptr || !q_in.is_cuda() || q_in.dim() != 4 || kp.dim() != 3 || k.dim() != 4 || vp.sizes() != kp.sizes() ||
       v.sizes() != k.sizes())
     return py::none();
-  const auto dev = q.device();
-  const auto dt = q.scalar_type();
+  const auto dev = q_in.device();
+  const auto dt = q_in.scalar_type();
   const int code = dtype_code(dt);
-  const int64_t b = q.size(0), hkv = q.size(1), g = q.size(2), d = q.size(3), n = kp.size(1), m = k.size(2);
+  const int64_t b = q_in.size(0), hkv = q_in.size(1), g = q_in.size(2), d = q_in.size(3), n = kp.size(1), m = k.size(2);
   if (code < 0 || kp.size(0) != hkv || kp.size(2) != d || k.size(0) != b || k.size(1) != hkv || k.size(3) != d ||
-      !plain(q, dev, dt) || !plain(kp, dev, dt) || !plain(vp, dev, dt) || !plain(k, dev, dt) || !plain(v, dev, dt) ||
+      !plain(q_in, dev, dt) || !plain(kp, dev, dt) || !plain(vp, dev, dt) || !plain(k, dev, dt) || !plain(v, dev, dt) ||
       !plain_lengths(lengths, dev, b) || b < 1 || b > 65535 || hkv > 65535 || g > 65535 || d > 65535)
     return py::none();
   c10::cuda::CUDAGuard guard(dev);
+  const at::Tensor q = rows16(q_in);
   const cudaStream_t st = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
   at::Tensor out = at::empty({b, hkv, g, d}, q.options());
   const size_t nb = g_shared_size((int)b, (int)hkv, (int)g, (int)d, n, m, code);

@@ -19,7 +19,7 @@ import ctypes
 import torch
 
 from . import _lib
-from ._lib import check, dtype_code, lib, require_cuda, stream_ptr, workspaces
+from ._lib import check, dtype_code, lib, require_cuda, rows16, stream_ptr, workspaces
 
 __all__ = ["decode_attention", "decode_attention_append", "decode_attention_lse", "decode_attention_partial", "decode_attention_batched",
            "decode_attention_ragged", "decode_attention_shared", "decode_attention_window", "merge_partials", "RaggedKV"]
@@ -317,7 +317,11 @@ def decode_attention_shared(q, k_prefix, v_prefix, k, v, scale, lengths=None):
     view without its batch dimension), k/v [b, hkv, m, d] of which sequence i's first lengths[i] rows count
     (int32 CUDA [b], clamped into [0, m]; None: all m). Returns [b, hkv, g, d], attention over the prefix
     and then the suffix. The prefix is read once for the whole batch. An empty prefix or suffix is fine;
-    with neither the result is zeros."""
+    with neither the result is zeros.
+
+    The tensor cores take 16-bit types, d in {64, 128, 256}, scale > 0, and prefix and suffixes whose rows start on
+    16-byte boundaries and are not broadcast (queries are copied where they are not so); anything else runs on a plain
+    kernel that reads the prefix once for every query row, many times slower."""
     what = "decode_attention_shared"
     hb = _lib.host()
     if hb is not None:
@@ -336,7 +340,7 @@ def decode_attention_shared(q, k_prefix, v_prefix, k, v, scale, lengths=None):
     n, m = k_prefix.shape[1], k.shape[2]
     if k_prefix.shape != (hkv, n, d) or k.shape != (b, hkv, m, d):
         raise ValueError(f"{what}: k_prefix {tuple(k_prefix.shape)} / k {tuple(k.shape)} do not match q {tuple(q.shape)}")
-    q, k_prefix, v_prefix, k, v = (_last_contig(x) for x in (q, k_prefix, v_prefix, k, v))
+    q, (k_prefix, v_prefix, k, v) = rows16(q), (_last_contig(x) for x in (k_prefix, v_prefix, k, v))
     dev = q.device
     lens_ptr = None
     if lengths is not None:

@@ -10,7 +10,7 @@ whether the kernel takes the inputs; the plugin keeps torch SDPA for everything 
 import torch
 
 from . import _lib
-from ._lib import check, dtype_code, lib, require_cuda, stream_ptr, workspaces
+from ._lib import check, dtype_code, lib, require_cuda, rows16, stream_ptr, workspaces
 
 __all__ = ["prefill_attention", "prefill_attention_window", "supported", "causal_offset_mask"]
 
@@ -63,7 +63,11 @@ def prefill_attention_window(query, key, value, scale, window, sinks=0, *, split
     """Causal attention of a chunk over the cache that ends with it, with a sliding window and sinks: query
     [b, hq, lq, d], key/value [b, hkv, lk, d] (hq a multiple of hkv, d <= 256, any dtype of the package).
     Query position p sees the keys j <= lk - lq + p with j < sinks or j > lk - lq + p - window (window >= 1
-    counts the query's own token). Returns [b, lq, hq, d] contiguous."""
+    counts the query's own token). Returns [b, lq, hq, d] contiguous.
+
+    The tensor cores take 16-bit types, d of 64 or 128, up to 128 query heads per KV head, scale > 0, and keys and values
+    whose rows start on 16-byte boundaries and are not broadcast (queries are copied where they are not so); anything
+    else runs on a plain kernel, a CTA a query row, many times slower."""
     what = "prefill_attention_window"
     hb = _lib.host()
     if hb is not None:
@@ -86,7 +90,7 @@ def prefill_attention_window(query, key, value, scale, window, sinks=0, *, split
         raise ValueError(f"{what}: needs window >= 1 and sinks >= 0, got {window} and {sinks}")
     window, sinks = min(window, lk), min(sinks, lk)
     code = dtype_code(query, what)
-    q, k, v = (x if x.stride(-1) == 1 else x.contiguous() for x in (query, key, value))
+    q, (k, v) = rows16(query), (x if x.stride(-1) == 1 else x.contiguous() for x in (key, value))
     dev = query.device
     out = torch.empty((b, lq, hq, d), dtype=query.dtype, device=dev)
     L = lib()
