@@ -25,7 +25,7 @@ def window_mask(lq, lk, w):
 def window_of(mask, lq, lk, w):
     """_window_of for a query that looks like one on the GPU."""
     query = SimpleNamespace(shape=(1, 8, lq, 128), is_cuda=True, dtype=torch.bfloat16, requires_grad=False)
-    key = SimpleNamespace(shape=(1, 2, lk, 128), requires_grad=False)
+    key = torch.empty(1, 2, lk, 128)
     return A._window_of(query, key, key, mask, lq, lk, 0.1, dict(sliding_window=w))
 
 
@@ -65,7 +65,18 @@ def test_a_mask_of_one_mode_used_in_the_other():
 def test_values_of_another_head_size_are_no_window():
     """The windowed kernels take keys and values of one shape; SDPA does not need that."""
     query = SimpleNamespace(shape=(1, 8, 5, 128), is_cuda=True, dtype=torch.bfloat16, requires_grad=False)
-    key, value, same = (SimpleNamespace(shape=(1, 2, 30, d), requires_grad=False) for d in (128, 64, 128))
+    key, value, same = (torch.empty(1, 2, 30, d) for d in (128, 64, 128))
     mask, kw = window_mask(5, 30, 7), dict(sliding_window=7)
     assert A._window_of(query, key, same, mask, 5, 30, 0.1, kw) == 7
     assert A._window_of(query, key, value, mask, 5, 30, 0.1, kw) is None
+
+
+def test_broadcast_keys_are_no_window():
+    """The windowed prefill runs them on its plain kernel, which SDPA beats."""
+    query = SimpleNamespace(shape=(1, 8, 5, 128), is_cuda=True, dtype=torch.bfloat16, requires_grad=False)
+    mask, kw = window_mask(5, 30, 7), dict(sliding_window=7)
+    own, shared = torch.empty(1, 2, 30, 128), torch.empty(1, 1, 30, 128).expand(1, 2, 30, 128)
+    assert A._window_of(query, own, own, mask, 5, 30, 0.1, kw) == 7
+    assert A._window_of(query, own.as_strided(own.shape, (0,) + own.stride()[1:]), own, mask, 5, 30, 0.1, kw) == 7
+    for k, v in ((shared, own), (own, shared)):
+        assert A._window_of(query, k, v, mask, 5, 30, 0.1, kw) is None

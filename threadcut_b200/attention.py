@@ -81,14 +81,18 @@ def _is_causal_offset(mask, lq, lk):
 _window_seen = {}  # the last mask tensor compared with a window's: (weak reference, version, window, result)
 
 
+def _broadcast(x):
+    return any(s == 0 and n > 1 for n, s in zip(x.shape, x.stride()))
+
+
 def _window_of(query, key, value, mask, lq, lk, scaling, kwargs):
     """The window W of a sliding-window layer whose mask means exactly "query p sees the last W keys up to
     its own", if the windowed kernels take the call; else None. They have no backward pass, so a call that autograd
-    records keeps the SDPA branch."""
+    records keeps the SDPA branch, and they are slow on broadcast keys and values, which keep it too."""
     w = kwargs.get("sliding_window")
     d = query.shape[-1]
     if (not isinstance(w, int) or w < 1 or mask is None or mask.dtype != torch.bool or tuple(mask.shape) != (1, 1, lq, lk)
-            or lq > lk or query.shape[0] != 1 or value.shape != key.shape or not query.is_cuda or not scaling > 0
+            or lq > lk or query.shape[0] != 1 or value.shape != key.shape or _broadcast(key) or _broadcast(value) or not query.is_cuda or not scaling > 0
             or query.dtype not in (torch.bfloat16, torch.float16) or d not in (64, 128) or key.shape[-1] != d
             or kwargs.get("softcap") is not None or kwargs.get("s_aux") is not None
             or (torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad))

@@ -170,6 +170,12 @@ at::Tensor rows16(const at::Tensor& x) {
   return ok ? x : x.clone(at::MemoryFormat::Contiguous);
 }
 
+bool broadcast(const at::Tensor& x) {
+  for (int64_t i = 0; i < x.dim(); ++i)
+    if (x.stride(i) == 0 && x.size(i) > 1) return true;
+  return false;
+}
+
 // Scratch with no initial contents.
 at::Tensor scratch(size_t bytes, const at::Tensor& like) {
   return at::empty({(int64_t)bytes}, like.options().dtype(at::kByte));
@@ -262,19 +268,22 @@ py::object window_decode(const at::Tensor& q, const at::Tensor& k, const at::Ten
   return py::cast(out);
 }
 
-py::object window_prefill(const at::Tensor& q_in, const at::Tensor& k, const at::Tensor& v, double scale, int64_t window,
+py::object window_prefill(const at::Tensor& q_in, const at::Tensor& k_in, const at::Tensor& v_in, double scale, int64_t window,
                           int64_t sinks, int64_t splits) {
-  if (g_prefill == nullptr || !q_in.is_cuda() || q_in.dim() != 4 || k.dim() != 4 || v.sizes() != k.sizes()) return py::none();
+  if (g_prefill == nullptr || !q_in.is_cuda() || q_in.dim() != 4 || k_in.dim() != 4 || v_in.sizes() != k_in.sizes()) return py::none();
   const auto dev = q_in.device();
   const auto dt = q_in.scalar_type();
   const int code = dtype_code(dt);
-  const int64_t b = q_in.size(0), hq = q_in.size(1), lq = q_in.size(2), d = q_in.size(3), hkv = k.size(1), lk = k.size(2);
-  if (code < 0 || k.size(0) != b || k.size(3) != d || hkv < 1 || hq % hkv != 0 || lq < 1 || lq > lk || lk > INT32_MAX ||
-      !plain(q_in, dev, dt) || !plain(k, dev, dt) || !plain(v, dev, dt) || window < 1 || sinks < 0 || b < 1 || b > 65535 ||
+  const int64_t b = q_in.size(0), hq = q_in.size(1), lq = q_in.size(2), d = q_in.size(3), hkv = k_in.size(1), lk = k_in.size(2);
+  if (code < 0 || k_in.size(0) != b || k_in.size(3) != d || hkv < 1 || hq % hkv != 0 || lq < 1 || lq > lk || lk > INT32_MAX ||
+      !plain(q_in, dev, dt) || !plain(k_in, dev, dt) || !plain(v_in, dev, dt) || window < 1 || sinks < 0 || b < 1 || b > 65535 ||
       hq > 65535 || d > 65535 || splits < 0 || splits > 65535)
     return py::none();
   c10::cuda::CUDAGuard guard(dev);
   const at::Tensor q = rows16(q_in);
+  // for the tensor cores, as on the Python side
+  const bool map = code != dtype_code(at::kFloat) && (d == 64 || d == 128);
+  const at::Tensor k = map && !broadcast(k_in) ? rows16(k_in) : k_in, v = map && !broadcast(v_in) ? rows16(v_in) : v_in;
   const cudaStream_t st = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
   window = std::min(window, lk);
   sinks = std::min(sinks, lk);

@@ -66,8 +66,8 @@ def prefill_attention_window(query, key, value, scale, window, sinks=0, *, split
     counts the query's own token). Returns [b, lq, hq, d] contiguous.
 
     The tensor cores take 16-bit types, d of 64 or 128, up to 128 query heads per KV head, scale > 0, and keys and values
-    whose rows start on 16-byte boundaries and are not broadcast (queries are copied where they are not so); anything
-    else runs on a plain kernel, a CTA a query row, many times slower."""
+    that are not broadcast; a tensor whose rows do not start on 16-byte boundaries, and a broadcast query, is copied
+    first. Anything else runs on a plain kernel, a CTA a query row, many times slower."""
     what = "prefill_attention_window"
     hb = _lib.host()
     if hb is not None:
@@ -91,6 +91,10 @@ def prefill_attention_window(query, key, value, scale, window, sinks=0, *, split
     window, sinks = min(window, lk), min(sinks, lk)
     code = dtype_code(query, what)
     q, (k, v) = rows16(query), (x if x.stride(-1) == 1 else x.contiguous() for x in (key, value))
+    if code != _lib.DTYPE_CODE[torch.float32] and d in (64, 128):
+        # off a 16-byte boundary: a copy costs its bytes, the plain kernel a hundred times that. A broadcast tensor
+        # stays: its copy could be any size.
+        k, v = (x if any(s == 0 and n > 1 for n, s in zip(x.shape, x.stride())) else rows16(x) for x in (k, v))
     dev = query.device
     out = torch.empty((b, lq, hq, d), dtype=query.dtype, device=dev)
     L = lib()
