@@ -113,19 +113,23 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const __grid_con
   const int p0 = qb * pq * kPfTiles;    // first position of Q tile 0; tile x starts at p0 + pq*x
   const int off = p.lk - p.lq;          // key j is visible to position pos iff j <= off + pos
   const int kend = p.lk < off + p0 + pq * kPfTiles ? p.lk : off + p0 + pq * kPfTiles;
-  // window: tile t of the list is key tile t for the first sink_tiles, then key tile t + skip
-  int sink_tiles = 0, skip = 0, first = 0;
-  if constexpr (kWindow) {
-    first = off + p0 + 1 - p.window;  // the block's first window key
-    const int wt = kPaged ? p.qb_tiles[2 * qb] : (first > 0 ? first / kPfKeys : 0);
-    sink_tiles = p.sink_tiles < wt ? p.sink_tiles : wt;
-    skip = wt - sink_tiles;
-  }
-  // >= 1: key 0 is visible to every position (window: the block's first query sees its own token)
-  const int ntot = (kPaged ? p.qb_tiles[kWindow ? 2 * qb + 1 : qb] : (kend + kPfKeys - 1) / kPfKeys) - skip;
+  // The block's key tiles, of which this split takes ntile from t_lo on. window: tile t of the list is key tile t for
+  // the first sink_tiles, then key tile t + skip.
+  const int first = kWindow ? off + p0 + 1 - p.window : 0;  // window: the block's first window key
+  int sink_tiles = 0, skip = 0, t_lo = 0, ntile = 0;
+  auto plan_tiles = [&] {
+    if constexpr (kWindow) {
+      const int wt = kPaged ? p.qb_tiles[2 * qb] : (first > 0 ? first / kPfKeys : 0);
+      sink_tiles = p.sink_tiles < wt ? p.sink_tiles : wt;
+      skip = wt - sink_tiles;
+    }
+    // >= 1: key 0 is visible to every position (window: the block's first query sees its own token)
+    const int ntot = (kPaged ? p.qb_tiles[kWindow ? 2 * qb + 1 : qb] : (kend + kPfKeys - 1) / kPfKeys) - skip;
+    t_lo = (int)((int64_t)ntot * split / p.nsplit);
+    ntile = (int)((int64_t)ntot * (split + 1) / p.nsplit) - t_lo;
+  };
   auto key_tile = [&](int t) { return kWindow && t >= sink_tiles ? t + skip : t; };
-  const int t_lo = (int)((int64_t)ntot * split / p.nsplit);
-  const int ntile = (int)((int64_t)ntot * (split + 1) / p.nsplit) - t_lo;
+  if constexpr (!kPaged) plan_tiles();
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
 
   if (threadIdx.x == 0) {
@@ -154,6 +158,8 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const __grid_con
     pdl_launch();
     pdl_wait();
   }
+
+  if constexpr (kPaged) plan_tiles();  // the tables may be the previous kernel's work: behind the wait
 
   if (warp >= 8) {
     reg_dealloc<kPfRegsOther>();
