@@ -216,7 +216,8 @@ int tc_prefill_attention_window(const void* q, const void* k, const void* v, voi
  * [4j, 4j + 4), qb_tiles (DEVICE int32 [blocks][2], a block being 2 * floor(128 / (hq / hkv)) queries) holds,
  * for block i from query p0 on, the last key tile with a logical start at or below
  * max(0, lk - lq + p0 + 1 - window) and the number of key tiles with a logical start below
- * min(lk, lk - lq + p0 + block); sink_tiles = the key tiles with a logical start below `sinks`. 16-bit, d in
+ * min(lk, lk - lq + p0 + block); values that name no tile, or leave the block none, are taken as the nearest that
+ * do. sink_tiles = the key tiles with a logical start below `sinks`. 16-bit, d in
  * {64, 128}, hq <= 128 hkv, scale > 0. Workspace as tc_prefill_window_workspace_size(1, hq, hkv, lq,
  * max(lq, 128 * ceil(n_sub / 4)), d, window, sinks, splits). */
 int tc_prefill_attention_window_paged(const void* q, const void* k_pool, const void* v_pool, void* out, int hq, int hkv,

@@ -1,9 +1,10 @@
-"""The block table of a windowed prefill over pages (tc_prefill_attention_window_paged) on a B200, when the launch just
-before writes it."""
+"""The block table of a windowed prefill over pages (tc_prefill_attention_window_paged) on a B200: written by
+the launch just before, and with values outside the tiles that there are."""
 import numpy as np
 import pytest
 import torch
 
+from attn_bounds import assert_within, attend64
 from threadcut_b200 import _lib
 from threadcut_b200.paged import PagedKV, append_rope
 
@@ -66,3 +67,31 @@ def test_a_table_that_the_previous_launch_writes():
         outs.append(prefill(kv, q, qb))
     for out in outs:
         assert torch.equal(out, want)
+
+
+def test_table_values_outside_the_tiles_are_held_within_them():
+    """Each block sees the keys of its window that lie in its tiles, a first tile below 0 being tile 0, an end past the
+    last tile that tile's, and no end before the second tile or first tile past the end's."""
+    gen = torch.Generator(device=DEV).manual_seed(10)
+    n = 1500
+    kv = PagedKV(1, HKV, D, max_tokens=n, device=DEV)
+    kv.reserve(n)
+    kv.write(0, *(torch.randn(HKV, n, D, generator=gen, device=DEV).to(torch.bfloat16) for _ in range(2)))
+    q = torch.randn(HKV * G, LQ, D, generator=gen, device=DEV).to(torch.bfloat16)
+    starts = kv._prefill_table()[1]
+    right = block_table(starts, n, WINDOW)
+    tiles = -(-len(starts) // 4)
+    edges = torch.tensor([int(x) for x in starts[::4]] + [n], device=DEV)
+    most = 2 ** 31 - 1
+    bad = right.copy()
+    bad[0], bad[1, 0], bad[2, 1], bad[3] = (-most - 1, most), -5, 10 ** 6, (0, most)
+    bad[4], bad[5], bad[6] = (most, most), (10, 10), (3, -7)
+    held = [(0, tiles), (0, right[1, 1]), (right[2, 0], tiles), (0, tiles), (tiles - 1, tiles), (9, 10), (0, 1), tuple(right[7])]
+    at = (n - LQ + torch.arange(LQ, device=DEV))[:, None]
+    j = torch.arange(n, device=DEV)
+    lo, hi = (edges[torch.tensor([int(h[i]) for h in held], device=DEV)].repeat_interleave(64)[:, None] for i in (0, 1))
+    k, v = (x.repeat_interleave(G, 0) for x in kv.gather(0))
+    seen = (j <= at) & (j > at - WINDOW) & (j >= lo) & (j < hi)
+    assert not seen[384:448].any()  # a block without a key gives zeros
+    ref, tol = attend64(q, k, v, 0.1, seen)
+    assert_within(prefill(kv, q, torch.from_numpy(bad).to(DEV))[0], ref.transpose(0, 1), tol.transpose(0, 1))

@@ -118,13 +118,23 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(const __grid_con
   const int first = kWindow ? off + p0 + 1 - p.window : 0;  // window: the block's first window key
   int sink_tiles = 0, skip = 0, t_lo = 0, ntile = 0;
   auto plan_tiles = [&] {
+    // >= 1: key 0 is visible to every position (window: the block's first query sees its own token). Device tables are
+    // held within the tiles that there are, so that no value of theirs reads past them or makes the loops run on.
+    int end = (kend + kPfKeys - 1) / kPfKeys;
+    if constexpr (kPaged) {
+      const int tiles = (p.n_sub + 3) / 4, t = p.qb_tiles[kWindow ? 2 * qb + 1 : qb];
+      end = t < 1 ? 1 : (t > tiles ? tiles : t);
+    }
     if constexpr (kWindow) {
-      const int wt = kPaged ? p.qb_tiles[2 * qb] : (first > 0 ? first / kPfKeys : 0);
+      int wt = first > 0 ? first / kPfKeys : 0;
+      if constexpr (kPaged) {
+        const int t = p.qb_tiles[2 * qb];
+        wt = t < 0 ? 0 : (t >= end ? end - 1 : t);
+      }
       sink_tiles = p.sink_tiles < wt ? p.sink_tiles : wt;
       skip = wt - sink_tiles;
     }
-    // >= 1: key 0 is visible to every position (window: the block's first query sees its own token)
-    const int ntot = (kPaged ? p.qb_tiles[kWindow ? 2 * qb + 1 : qb] : (kend + kPfKeys - 1) / kPfKeys) - skip;
+    const int ntot = end - skip;
     t_lo = (int)((int64_t)ntot * split / p.nsplit);
     ntile = (int)((int64_t)ntot * (split + 1) / p.nsplit) - t_lo;
   };
