@@ -233,7 +233,8 @@ int tc_prefill_attention_window_paged(const void* q, const void* k_pool, const v
  * [batch, hkv, m, d] of which the first lengths[b] rows count (DEVICE int32, NULL: m; clamped into
  * [0, m]), out [batch, hkv, g, d] = softmax(scale q [prefix ; suffix_b]^T) [prefix ; suffix_b]; n == 0,
  * m == 0 and empty suffixes are fine, nothing at all gives zeros. The prefix is read once for the whole
- * batch: its rows meet all batch*g queries of a KV head in one matrix product. g <= 128, d <= 256, every
+ * batch: its rows meet all batch*g queries of a KV head in one matrix product, which takes the softmax
+ * weights as one 16-bit number each (the other decode entries: as two). g <= 128, d <= 256, every
  * dtype, any strides with a contiguous last dimension; 16-bit, d in {64, 128, 256}, scale > 0 and 16-byte
  * aligned bases and strides run on the tcgen05 tensor cores, the rest a plain kernel. Workspace of
  * tc_decode_attention_shared_workspace_size() bytes, 32-byte aligned, with no initial contents (nothing is

@@ -24,6 +24,9 @@
 //                      row's 128 scores, causal mask with the cache offset, exp2, P packed to 16 bits
 //                      and tcgen05.st back over S; the row max is kept stale until a tile's max
 //                      exceeds it by 2^8, so O_x is rescaled in TMEM (tcgen05.ld/st) only on jumps.
+//                      P is rounded once to the 16-bit type that the product takes, its row sums add it
+//                      unrounded: half a step of a weight (bf16 2^-8), where a second part of P would double
+//                      the P V products of a kernel that these and the softmax hold.
 //                      The epilogue divides by l and stores (or, with KV splits, writes fp32
 //                      partials and the natural-log LSE for a merge).
 // kWindow (a sliding window with sinks) is the same pipeline over another list of key tiles: those holding

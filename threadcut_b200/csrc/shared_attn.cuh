@@ -16,6 +16,12 @@
 //                      is there when a softmax ends), O += P V with P from TMEM.
 //   warps 0-3:         softmax, a thread per query row; warps without live rows leave at once (a suffix has g
 //                      rows). The maximum is kept until a tile passes it by 2^8, so O is rescaled rarely.
+// The weights 2^(s_j - m_p) enter O += P V rounded once to T, as in the causal prefill; the sums l_p add them unrounded.
+// (The split-KV decode kernels hand them over in two 16-bit parts.) Half a step of bf16 is 2^-8 of a weight: against
+// float64 the result is off by 2.2e-3 of its norm, of which its own rounding to bf16 makes 1.65e-3 (fp16 2.9e-4 of
+// 2.1e-4). Two parts, the second in the other half of the S buffer, bring the 1.65e-3 and double the products of P:
+// 2 sequences of 1,536 + 40 tokens 9.0 us instead of 8.6, 8 of 16,384 + 700 23.2 instead of 20.0, 64 of 98,304 + 1,024
+// 165 instead of 139. A caller who needs the last bits has decode_attention_batched.
 // Up to 128 rows the loop runs at the DRAM's pace (b = 1 over 98,304 rows: 66 us, 6.1 TB/s); with more, each row tile
 // fetches the tiles from L2 again and 256 rows take 118 us for 98,304 keys. One CTA an SM that multiplied each tile
 // with two row tiles moved half the bytes from L2 and took 125 us: its two chains of softmax and products, not

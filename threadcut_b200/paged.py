@@ -469,7 +469,7 @@ class PagedKV:
         """flash_decode.decode_attention_shared with this sequence as the prefix, straight over its pages:
         q [b, hkv, g, d], the continuations' suffixes k/v [b, hkv, m, d] of which the first lengths[i] rows
         count (int32 CUDA [b], clamped into [0, m]; None: all m). 16-bit, d in {64, 128, 256}, g <= 128,
-        scale > 0. Returns [b, hkv, g, d]."""
+        scale > 0; weights rounded to 16 bits, as there. Returns [b, hkv, g, d]."""
         what = "PagedKV.decode_shared"
         require_cuda(q, k, v, what=what)
         if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape:

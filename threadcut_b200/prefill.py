@@ -63,7 +63,8 @@ def prefill_attention_window(query, key, value, scale, window, sinks=0, *, split
     """Causal attention of a chunk over the cache that ends with it, with a sliding window and sinks: query
     [b, hq, lq, d], key/value [b, hkv, lk, d] (hq a multiple of hkv, d <= 256, any dtype of the package).
     Query position p sees the keys j <= lk - lq + p with j < sinks or j > lk - lq + p - window (window >= 1
-    counts the query's own token). Returns [b, lq, hq, d] contiguous.
+    counts the query's own token). Returns [b, lq, hq, d] contiguous. The softmax weights meet the values rounded to the
+    16-bit type, as in prefill_attention.
 
     The tensor cores take 16-bit types, d of 64 or 128, up to 128 query heads per KV head, scale > 0, and keys and values
     that are not broadcast; a tensor whose rows do not start on 16-byte boundaries, and a broadcast query, is copied
