@@ -80,3 +80,26 @@ def test_broadcast_keys_are_no_window():
     assert A._window_of(query, own.as_strided(own.shape, (0,) + own.stride()[1:]), own, mask, 5, 30, 0.1, kw) == 7
     for k, v in ((shared, own), (own, shared)):
         assert A._window_of(query, k, v, mask, 5, 30, 0.1, kw) is None
+
+
+@pytest.mark.parametrize("d,pad", [(64, 1), (64, 8), (128, 3), (20, 1)])
+def test_sdpa_gets_rows_on_their_boundaries(monkeypatch, d, pad):
+    """Views that start between two 16-byte boundaries are copied, others and rows of an odd length go as they are."""
+    seen = []
+    real = torch.nn.functional.scaled_dot_product_attention
+    monkeypatch.setattr(A.F, "scaled_dot_product_attention", lambda *a, **k: (seen.extend(a), real(*a, **k))[1])
+    torch.manual_seed(0)
+    full = [torch.randn(1, h, n, d + pad, dtype=torch.bfloat16) for h, n in ((8, 5), (2, 30), (2, 30))]
+    x = [t[..., pad:] for t in full]
+    mask = window_mask(5, 30, 7)
+    out, _ = A.attention(None, *x, mask, scaling=0.1)
+    want = real(*(t.contiguous() for t in x), attn_mask=mask, scale=0.1, enable_gqa=True)
+    assert torch.equal(out, want.transpose(1, 2))
+    for given, used in zip(x, seen):
+        if d * 2 % 16 == 0:
+            assert used.data_ptr() % 16 == 0 and all(s * 2 % 16 == 0 for s in used.stride()[:-1])
+        if d * 2 % 16 or pad == 8:
+            assert used.data_ptr() == given.data_ptr()
+    leaf = x[1].detach().requires_grad_()  # the copy carries gradients
+    A.attention(None, x[0], leaf, x[2], mask, scaling=0.1)[0].float().sum().backward()
+    assert leaf.grad is not None and leaf.grad.abs().sum() > 0

@@ -85,6 +85,14 @@ def _broadcast(x):
     return any(s == 0 and n > 1 for n, s in zip(x.shape, x.stride()))
 
 
+def _aligned(x):
+    """x with rows on 16-byte boundaries, copied if its own are not although rows of its length could be: SDPA's CUDA
+    kernels raised "misaligned address" on a view that began between two boundaries."""
+    es = x.element_size()
+    off = x.data_ptr() % 16 or any(s * es % 16 for n, s in zip(x.shape[:-1], x.stride()) if n > 1)
+    return x.clone(memory_format=torch.contiguous_format) if off and x.shape[-1] * es % 16 == 0 else x
+
+
 def _window_of(query, key, value, mask, lq, lk, scaling, kwargs):
     """The window W of a sliding-window layer whose mask means exactly "query p sees the last W keys up to
     its own", if the windowed kernels take the call; else None. They have no backward pass, so a call that autograd
@@ -159,6 +167,7 @@ def attention(module, query, key, value, attention_mask, dropout=0.0, scaling=No
         # the reference expands K/V with repeat_kv first (attention.py:43-46); SDPA's own GQA mode
         # computes the same attention without materialising the expansion (4x the cache per layer)
         is_causal = attention_mask is None and q > 1 and q == key.shape[2]
+        query, key, value = (_aligned(x) for x in (query, key, value))
         out = F.scaled_dot_product_attention(query, key, value, attn_mask=attention_mask, scale=scaling,
                                              is_causal=is_causal, enable_gqa=g > 1)
     return out.transpose(1, 2).contiguous(), None
