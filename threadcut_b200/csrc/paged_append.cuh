@@ -130,8 +130,9 @@ __device__ __forceinline__ Chunk<T, VEC> narrow(const float2 (&x)[VEC / 2]) {
 //   out_a = (r x_a) (w_a cos_a) - (r x_b) (w_b sin_a),   out_b = (r x_b) (w_b cos_b) + (r x_a) (w_a sin_b),
 // a row costs three packed operations an output pair beside its conversions.
 // Bound by bytes for long chunks, by latency for short ones: resident warps count in both. 16,384 tokens of
-// 48 bf16 heads of 128 (411 MB): 2 rows a thread and 7 CTAs an SM (72 registers) 76.7 us, 5.4 TB/s; before the split below 78.6, 6 CTAs 81.8,
-// 8 CTAs (spills) 83.7; 4 rows 86.9, 8 rows 102; with the formula's own order of operations, unpacked, 106.
+// 48 bf16 heads of 128 (411 MB): 2 rows a thread and 7 CTAs an SM (72 registers) 76.7 us, 5.4 TB/s. Before the split
+// below: 78.6, with 6 CTAs 81.8, 8 CTAs (spills) 83.7, 4 rows 86.9, 8 rows 102; with the formula's own order of
+// operations, unpacked, 106.
 // kPartial: rot < d, some threads hold chunks that pass through. Full rotations have a kernel without their branch
 // (32 bytes of spills a thread instead of 56): the prompt above takes 76.7 us, with one kernel for both 80.4.
 template <typename T, typename TT, bool kPartial>

@@ -51,7 +51,7 @@ constexpr int kPfTiles = 2;       // Q tiles per CTA (ping-pong softmax warpgrou
 constexpr int kPfKeys = 128;      // keys per K/V tile
 constexpr int kPfThreads = 384;   // warps 0-3 / 4-7 softmax of Q tile 0 / 1, 8 TMA, 9 MMA, 10-11 idle
 // Registers per thread after the warpgroup split (setmaxnreg): the launch gives 384 x 168 = 64512,
-// softmax warpgroups 2 x 128 x 232 + the TMA/MMA warpgroup 128 x 40 = 64512.
+// softmax warpgroups 2 x 128 x 224 + the TMA/MMA warpgroup 128 x 56 = 64512 (with 40 the MMA lane spills).
 constexpr int kPfRegsSoftmax = 224;
 constexpr int kPfRegsOther = 56;
 constexpr int kPfGroup = 4;       // query heads per KV head handled by the kernel

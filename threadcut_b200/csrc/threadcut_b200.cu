@@ -184,9 +184,9 @@ int64_t window_plan_rows(int64_t n, int64_t window, int64_t sinks) {
 
 // KV partition of a windowed decode. Nearly every sequence reads the same rows, so every (sequence, head)
 // gets equal slices, as many as are resident at once, but none below kWindowSliceTiles tiles. Measured at
-// bf16 d = 128, 8 KV heads, 4,100 visible rows of one sequence: 16 slices of 8 tiles 10.1 us, 4 slices 15.2, 24
+// bf16 d = 128, 8 KV heads, 4,100 visible rows of one sequence: 15 slices of 8 or 9 tiles 10.1 us, 4 slices 15.2, 22
 // slices (a second wave) 16.3; 64 sequences of 2,064 rows: 1 slice 89.6 us, 2 slices 101.5, 4 slices 119; 28
-// (sequence, head)s of 11 tiles: 1 slice 6.7 us, 2 slices 7.9.
+// (sequence, head)s of 12 tiles: 1 slice 6.7 us, 2 slices 7.9.
 constexpr int64_t kWindowSliceTiles = 8;
 
 DecodePlan plan_window(int batch, int hkv, int64_t plan_n, int splits_req, int d, int dtype, int sms) {
@@ -2190,7 +2190,7 @@ cudaError_t launch_shared_t(const SharedParams& p, SharedMergeParams& mp, int64_
   if (e == cudaSuccess && ctas > 0) e = launch_ex(fn, dim3((unsigned)ctas), dim3(kShThreads), smem, st, p);
   if (e != cudaSuccess) return e;
   const int64_t rows = (int64_t)p.batch * p.hkv * p.g;
-  // Each warp takes about four parts, one round of loads: 8 sequences of 16,384 + 700 tokens (28 parts) 25.0 us
+  // Each warp takes about four parts, one round of loads: 8 sequences of 16,384 + 700 tokens in 28 parts 25.0 us
   // with 4 or 8 warps a row, 27.1 with 2, 28.5 with 1; 2 sequences of 1,536 + 40 (13 parts) 7.8 with 4, 9.1 with 1.
   mp.wpr = 1;
   while (mp.wpr < 8 && mp.wpr * 4 < p.np + p.ns) mp.wpr *= 2;

@@ -262,7 +262,8 @@ def decode_attention_window(q, k, v, scale, window, sinks=0, lengths=None, *, sp
     j >= n_b - window (window >= 1 counts the newest row; only visible rows are read).
 
     q: [b, hkv, g, d]; k, v: [b, hkv, n, d]; lengths: optional int32 CUDA tensor [b] of valid lengths
-    (clamped into [0, n]; 0 gives zeros). One sequence may come without the batch dimension (q
+    (clamped into [0, n]; 0 gives zeros). Types, head sizes and groups are decode_attention_batched's (g <= 16; d of 16,
+    32, 64 or 128, in 16 bits also 256). One sequence may come without the batch dimension (q
     [hkv, g, d], k/v [hkv, n, d]). Returns q's shape."""
     what = "decode_attention_window"
     hb = _lib.host()
@@ -317,7 +318,7 @@ def decode_attention_shared(q, k_prefix, v_prefix, k, v, scale, lengths=None):
     view without its batch dimension), k/v [b, hkv, m, d] of which sequence i's first lengths[i] rows count
     (int32 CUDA [b], clamped into [0, m]; None: all m). Returns [b, hkv, g, d], attention over the prefix
     and then the suffix. The prefix is read once for the whole batch. An empty prefix or suffix is fine;
-    with neither the result is zeros.
+    with neither the result is zeros. g <= 128, d <= 256, every type of the package.
 
     On the tensor cores the softmax weights are multiplied with the values as one 16-bit number each (bf16: off by up to
     2^-8 of the weight), where decode_attention_batched hands them over in two: bf16 results differ from float64 by
