@@ -89,7 +89,7 @@ def _aligned(x):
     """x with rows on 16-byte boundaries, copied if its own are not although rows of its length could be: SDPA's CUDA
     kernels raised "misaligned address" on a view that began between two boundaries."""
     es = x.element_size()
-    off = x.data_ptr() % 16 or any(s * es % 16 for n, s in zip(x.shape[:-1], x.stride()) if n > 1)
+    off = x.storage_offset() * es % 16 or any(s * es % 16 for n, s in zip(x.shape[:-1], x.stride()) if n > 1)
     return x.clone(memory_format=torch.contiguous_format) if off and x.shape[-1] * es % 16 == 0 else x
 
 
