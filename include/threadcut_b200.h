@@ -20,6 +20,9 @@
  *                             step (no reference code): decode over pages (flash_decode.py:57-69 semantics),
  *                             splice as page drop + in-place key rotation (kv.py:28-41,83-92 semantics),
  *                             append into page slots (kv.py:64-77 GrowingLayer.update semantics)
+ *   tc_int4_append_rope, tc_int4_gather, tc_int4_rotate_keys, tc_decode_attention_int4*, tc_gemv_int4
+ *                             (no reference code): the same cache, splice, decode and projections with
+ *                             rows and weights held in 4 bits
  *   tc_add_rmsnorm, tc_qk_norm_rope, tc_silu_mul, tc_gemv, tc_gemv_swiglu
  *                             threadcut/engine.py:66-73         the per-token model call, run by
  *                             transformers' Qwen3 layer (RMSNorm, q/k norm + RoPE, SwiGLU) there; here
@@ -557,6 +560,67 @@ int tc_gemv_swiglu(const void* gate_up, const void* w, void* out, int64_t n, int
 /* tc_silu_mul: out[r][i] = dtype(silu(gate_up[r][i])) * gate_up[r][inter + i] for `rows` rows
  * (Qwen3MLP: act_fn(gate_proj(x)) * up_proj(x), gate and up side by side in one row). */
 int tc_silu_mul(const void* gate_up, void* out, int64_t rows, int inter, int dtype, void* stream);
+
+/* ---- rows and weights held in 4 bits ----------------------------------------------------
+ * A group of neighbouring elements has a scale S and an offset z of the 16-bit type T (dtype: TC_F16 or TC_BF16), and
+ * each element a code of 0..15 that stands for S (1 + code / 16) + z; S = T((hi - lo) / 0.9375) and z = T(lo - S) of
+ * the group's extremes, codes of the nearest levels (ties to the even one, 0 where S = 0). A group with a NaN or an
+ * infinity, or whose S or z overflows T, reads back as NaN.
+ * A cache row of d elements (64, 128 or 256) is d / 2 bytes of codes (element e in byte e / 2, the even one in the low
+ * half) and d / 32 pairs (S, z): 5 d / 8 bytes; its values are rounded to T. Rows start on 16-byte boundaries (d = 64:
+ * 8-byte), else TC_ERR_ALIGN. Strides of such rows are in BYTES, all others in elements. */
+
+/* tc_paged_append_rope into pools of 4-bit rows: q, k [heads][t][d] (normalised and) rotated and rounded to T, q to q_out,
+ * k and v quantised into the slots [t][2] = (page, row) of k_pool / v_pool. rot = 0 (cos_t, sin_t NULL): no
+ * rotation. table_dtype: dtype or TC_F32. hq = 0: no queries. Slots outside the pool are skipped. */
+int tc_int4_append_rope(const void* q, const void* k, const void* v, void* q_out, void* k_pool, void* v_pool, int hq,
+                        int hkv, int d, int64_t t, int64_t q_stride_h, int64_t q_stride_t, int64_t k_stride_h,
+                        int64_t k_stride_t, int64_t v_stride_h, int64_t v_stride_t, int64_t q_out_stride_h,
+                        int64_t q_out_stride_t, const void* q_norm_weight, const void* k_norm_weight, float eps,
+                        const void* cos_t, const void* sin_t, int rot, int64_t cos_stride_t, int64_t sin_stride_t,
+                        int table_dtype, int64_t page_rows, int64_t num_pages, int64_t pool_stride_page,
+                        int64_t pool_stride_h, int64_t pool_stride_row, const int32_t* slots, int dtype, void* stream);
+
+/* Rows as 16-bit keys and values [hkv][n][d] (16-byte aligned): tiles [n_tiles][4] = (page, first row, rows <= 32,
+ * position of the first row), 16-byte aligned. Rows outside the pool or positions outside [0, n) are skipped. */
+int tc_int4_gather(const void* k_pool, const void* v_pool, void* k_out, void* v_out, int hkv, int d, int64_t n,
+                   int64_t out_stride_h, int64_t out_stride_n, int64_t page_rows, int64_t num_pages,
+                   int64_t pool_stride_page, int64_t pool_stride_h, int64_t pool_stride_row, const int32_t* tiles,
+                   int64_t n_tiles, int dtype, void* stream);
+
+/* Key rows of every pool re-rotated where they lie (tc_paged_rotate_keys over 4-bit rows): values, rotated in fp32 by
+ * cos_sin (host, d floats as tc_shift_keys), rounded to T and quantised again. tiles [n_tiles][tile_cols >= 3] =
+ * (page, first row, rows <= 32, ...), no row twice. */
+int tc_int4_rotate_keys(void* const* k_pools, int layers, int hkv, int d, int64_t page_rows, int64_t num_pages,
+                        int64_t pool_stride_page, int64_t pool_stride_h, int64_t pool_stride_row, const int32_t* tiles,
+                        int tile_cols, int64_t n_tiles, const float* cos_sin, int dtype, void* stream);
+
+/* Decode attention over 4-bit rows, g <= 16 query heads a KV head. Contiguous: k, v [batch][hkv][n] rows, lengths
+ * device int32 [batch] clamped into [0, n] or NULL. Paged: tiles [n_tiles][tile_cols >= 3] of k_pool / v_pool in order;
+ * tiles outside the pool are skipped. Sequences of no rows give zeros. The workspace (of the size that the function
+ * gives for batch 1 and 32 n_tiles rows when paged; 0: none needed) is zeroed before its first use and left so. */
+size_t tc_decode_attention_int4_workspace_size(int batch, int hkv, int g, int d, int64_t rows, int splits);
+int tc_decode_attention_int4(const void* q, const void* k, const void* v, void* out, int batch, int hkv, int g, int d,
+                             int64_t n, const int32_t* lengths, int64_t q_stride_b, int64_t q_stride_h,
+                             int64_t q_stride_g, int64_t k_stride_b, int64_t k_stride_h, int64_t k_stride_n,
+                             int64_t v_stride_b, int64_t v_stride_h, int64_t v_stride_n, int64_t out_stride_b,
+                             int64_t out_stride_h, int64_t out_stride_g, float scale, int splits, int dtype,
+                             void* workspace, size_t workspace_bytes, void* stream);
+int tc_decode_attention_int4_paged(const void* q, const void* k_pool, const void* v_pool, void* out, int hkv, int g, int d,
+                                   int64_t page_rows, int64_t num_pages, int64_t pool_stride_page, int64_t pool_stride_h,
+                                   int64_t pool_stride_row, const int32_t* tiles, int tile_cols, int64_t n_tiles,
+                                   int64_t q_stride_h, int64_t q_stride_g, int64_t out_stride_h, int64_t out_stride_g,
+                                   float scale, int splits, int dtype, void* workspace, size_t workspace_bytes,
+                                   void* stream);
+
+/* out [m][n] = x [m][k] . w^T for 4-bit weights w [n][k], sums in fp32; group 32, 64 or 128 neighbours of a row share
+ * (S, z), not rounded further. codes [ceil(n/16)][ceil(k/64)][512 bytes]: bytes 16 (4r + c).. of a tile are the words of
+ * (row r, columns 8c..8c+7), (row r + 8, the same), (row r, columns 32 + 8c..), (row r + 8, the same); code j of a word
+ * is column 2j, code 4 + j column 2j + 1. params [ceil(n/16)][ceil(k/group)][8][2][2] of T: (S, z) of rows r, r + 8. Both 0
+ * behind n and k, and 16-byte aligned. swiglu: x is [m][2k] (gate | up), the tokens silu(gate) * up. k up to
+ * 65,536; more tokens than fit shared memory (32 at most) are taken in turns. */
+int tc_gemv_int4(const void* x, const void* codes, const void* params, void* out, int64_t n, int k, int64_t m, int group,
+                 int64_t x_stride, int64_t out_stride, int swiglu, int dtype, void* stream);
 
 /* ---- sums over the GPUs of a tensor-parallel step, through peer memory ------------------
  * No counterpart in the reference (threadcut runs one GPU); they replace the collective library's

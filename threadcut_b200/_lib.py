@@ -89,6 +89,15 @@ SIGNATURES = {
     "tc_paged_write": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i64] + [_i64] * 4 + [_i64] * 5 + [_vp, _i, _vp]),
     "tc_paged_append_rope": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i64] + [_i64] * 8
                              + [_vp, _vp, _f, _vp, _vp, _i, _i64, _i64, _i] + [_i64] * 5 + [_vp, _i, _vp]),
+    "tc_int4_append_rope": (_i, [_vp] * 6 + [_i, _i, _i, _i64] + [_i64] * 8 + [_vp, _vp, _f, _vp, _vp, _i, _i64, _i64, _i]
+                            + [_i64] * 5 + [_vp, _i, _vp]),
+    "tc_int4_gather": (_i, [_vp] * 4 + [_i, _i] + [_i64] * 8 + [_vp, _i64, _i, _vp]),
+    "tc_int4_rotate_keys": (_i, [ctypes.POINTER(_vp), _i, _i, _i] + [_i64] * 5 + [_vp, _i, _i64, _fp, _i, _vp]),
+    "tc_decode_attention_int4_workspace_size": (_sz, [_i, _i, _i, _i, _i64, _i]),
+    "tc_decode_attention_int4": (_i, [_vp] * 4 + [_i] * 4 + [_i64, _vp] + [_i64] * 12 + [_f, _i, _i, _vp, _sz, _vp]),
+    "tc_decode_attention_int4_paged": (_i, [_vp] * 4 + [_i] * 3 + [_i64] * 5 + [_vp, _i, _i64] + [_i64] * 4
+                                       + [_f, _i, _i, _vp, _sz, _vp]),
+    "tc_gemv_int4": (_i, [_vp] * 4 + [_i64, _i, _i64, _i, _i64, _i64, _i, _i, _vp]),
     "tc_peer_handle_bytes": (_sz, []),
     "tc_peer_alloc": (_i, [_sz, ctypes.POINTER(_vp), _vp]),
     "tc_peer_open": (_i, [_vp, ctypes.POINTER(_vp)]),
@@ -154,6 +163,9 @@ def host():
                         "tc_paged_append_rope", "tc_decode_attention_window", "tc_decode_attention_window_workspace_size",
                         "tc_prefill_attention_window", "tc_prefill_window_workspace_size", "tc_decode_attention_shared",
                         "tc_decode_attention_shared_workspace_size")))
+                    mod.init_int4(*(ctypes.cast(getattr(handle, name), ctypes.c_void_p).value for name in (
+                        "tc_int4_append_rope", "tc_int4_gather", "tc_decode_attention_int4",
+                        "tc_decode_attention_int4_paged", "tc_decode_attention_int4_workspace_size", "tc_gemv_int4")))
                 _host = mod
     return _host or None
 

@@ -11,8 +11,10 @@
 // the checked Python path, which raises the documented exception for that case.
 //
 // append_rope, window_decode, window_prefill and shared_decode do the same for paged.append_rope,
-// flash_decode.decode_attention_window / decode_attention_shared and prefill.prefill_attention_window.
+// flash_decode.decode_attention_window / decode_attention_shared and prefill.prefill_attention_window;
+// int4_append, int4_gather, int4_decode and int4_gemv for the functions of int4.py.
 #include <torch/extension.h>
+#include <torch/csrc/Dtype.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -328,6 +330,194 @@ py::object shared_decode(const at::Tensor& q_in, const at::Tensor& kp, const at:
   return py::cast(out);
 }
 
+// ---- the 4-bit cache and projections
+using Int4AppendFn = AppendFn;
+using Int4GatherFn = int (*)(const void*, const void*, void*, void*, int, int, int64_t, int64_t, int64_t, int64_t, int64_t,
+                             int64_t, int64_t, int64_t, const int32_t*, int64_t, int, void*);
+using Int4DecodeFn = int (*)(const void*, const void*, const void*, void*, int, int, int, int, int64_t, const int32_t*,
+                             int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t,
+                             int64_t, int64_t, float, int, int, void*, size_t, void*);
+using Int4PagedFn = int (*)(const void*, const void*, const void*, void*, int, int, int, int64_t, int64_t, int64_t, int64_t,
+                            int64_t, const int32_t*, int, int64_t, int64_t, int64_t, int64_t, int64_t, float, int, int,
+                            void*, size_t, void*);
+using Int4SizeFn = size_t (*)(int, int, int, int, int64_t, int);
+using Int4GemvFn = int (*)(const void*, const void*, const void*, void*, int64_t, int, int64_t, int, int64_t, int64_t, int,
+                           int, void*);
+
+Int4AppendFn g_int4_append = nullptr;
+Int4GatherFn g_int4_gather = nullptr;
+Int4DecodeFn g_int4_decode = nullptr;
+Int4PagedFn g_int4_paged = nullptr;
+Int4SizeFn g_int4_size = nullptr;
+Int4GemvFn g_int4_gemv = nullptr;
+
+void init_int4(int64_t append, int64_t gather, int64_t decode, int64_t paged, int64_t size, int64_t gemv) {
+  g_int4_append = reinterpret_cast<Int4AppendFn>(append);
+  g_int4_gather = reinterpret_cast<Int4GatherFn>(gather);
+  g_int4_decode = reinterpret_cast<Int4DecodeFn>(decode);
+  g_int4_paged = reinterpret_cast<Int4PagedFn>(paged);
+  g_int4_size = reinterpret_cast<Int4SizeFn>(size);
+  g_int4_gemv = reinterpret_cast<Int4GemvFn>(gemv);
+}
+
+int64_t int4_row(int64_t d) { return d / 2 + d / 8; }
+bool int4_head(int64_t d) { return d == 64 || d == 128 || d == 256; }
+
+// Rows of 4 bits [outer, hkv, rows, row bytes] on `dev`; their starts are checked by the library.
+bool int4_rows(const at::Tensor& x, const c10::Device& dev, int64_t hkv, int64_t d) {
+  return x.device() == dev && x.scalar_type() == at::kByte && x.dim() == 4 && x.stride(3) == 1 && x.size(1) == hkv &&
+         x.size(3) == int4_row(d);
+}
+bool int4_pools(const at::Tensor& k, const at::Tensor& v, const c10::Device& dev, int64_t hkv, int64_t d) {
+  return int4_rows(k, dev, hkv, d) && int4_rows(v, dev, hkv, d) && v.sizes() == k.sizes() && v.strides() == k.strides();
+}
+bool int4_tiles(const at::Tensor& t, const c10::Device& dev, int64_t cols) {
+  return t.device() == dev && t.scalar_type() == at::kInt && t.dim() == 2 && t.size(1) >= cols && t.size(1) <= 65535 &&
+         t.is_contiguous();
+}
+
+// (whether it was done, the rotated queries or None)
+py::tuple int4_append(const at::Tensor& k, const at::Tensor& v, const OptTensor& cos, const OptTensor& sin,
+                      const at::Tensor& k_pool, const at::Tensor& v_pool, const at::Tensor& slots, const OptTensor& q,
+                      const OptTensor& q_norm, const OptTensor& k_norm, double eps) {
+  const py::tuple no = py::make_tuple(false, py::none());
+  if (g_int4_append == nullptr || !k.is_cuda()) return no;
+  const auto dev = k.device();
+  const auto dt = k.scalar_type();
+  const int code = dtype_code(dt);
+  const int64_t o = k.dim() - 3;
+  if (code < 1 || (o != 0 && o != 1) || v.sizes() != k.sizes() || (o == 1 && k.size(0) != 1)) return no;
+  const int64_t hkv = k.size(o), t = k.size(o + 1), d = k.size(o + 2);
+  if (!int4_head(d) || !plain(k, dev, dt) || !plain(v, dev, dt) || !int4_pools(k_pool, v_pool, dev, hkv, d)) return no;
+  int64_t hq = 0;
+  if (q) {
+    if (q->dim() != k.dim() || !plain(*q, dev, dt) || (o == 1 && q->size(0) != 1) || q->size(o + 1) != t ||
+        q->size(o + 2) != d)
+      return no;
+    hq = q->size(o);
+  }
+  int64_t rot = 0, cos_st = 0, sin_st = 0;
+  auto tab = dt;
+  if (cos.has_value() != sin.has_value()) return no;
+  if (cos) {
+    tab = cos->scalar_type();
+    const int64_t c = cos->dim() - 2, s = sin->dim() - 2;
+    if ((tab != dt && tab != at::kFloat) || (c != 0 && c != 1) || (s != 0 && s != 1) || (c == 1 && cos->size(0) != 1) ||
+        (s == 1 && sin->size(0) != 1) || !plain(*cos, dev, tab) || !plain(*sin, dev, tab))
+      return no;
+    rot = cos->size(c + 1);
+    if (cos->size(c) != t || sin->size(s) != t || sin->size(s + 1) != rot || rot < 2) return no;
+    cos_st = cos->stride(c);
+    sin_st = sin->stride(s);
+  }
+  if (slots.device() != dev || slots.scalar_type() != at::kInt || slots.dim() != 2 || slots.size(0) != t ||
+      slots.size(1) != 2 || !slots.is_contiguous())
+    return no;
+  for (const OptTensor* w : {&q_norm, &k_norm})
+    if (*w && (!plain(**w, dev, dt) || (*w)->dim() != 1 || (*w)->size(0) != d)) return no;
+  if (hq > 65535 || hkv > 65535 || rot > 65535) return no;
+  c10::cuda::CUDAGuard guard(dev);
+  at::Tensor out;
+  if (q)
+    out = o == 0 ? at::empty_strided({hq, t, d}, {d, hq * d, 1}, q->options())
+                 : at::empty_strided({1, hq, t, d}, {t * hq * d, d, hq * d, 1}, q->options());
+  const cudaStream_t st = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
+  const int rc = g_int4_append(
+      q ? q->data_ptr() : nullptr, k.data_ptr(), v.data_ptr(), q ? out.data_ptr() : nullptr, k_pool.data_ptr(),
+      v_pool.data_ptr(), (int)hq, (int)hkv, (int)d, t, q ? q->stride(o) : 0, q ? q->stride(o + 1) : 0, k.stride(o),
+      k.stride(o + 1), v.stride(o), v.stride(o + 1), d, hq * d, q_norm ? q_norm->data_ptr() : nullptr,
+      k_norm ? k_norm->data_ptr() : nullptr, (float)eps, cos ? cos->data_ptr() : nullptr, sin ? sin->data_ptr() : nullptr,
+      (int)rot, cos_st, sin_st, dtype_code(tab), k_pool.size(2), k_pool.size(0), k_pool.stride(0), k_pool.stride(1),
+      k_pool.stride(2), slots.data_ptr<int32_t>(), code, st);
+  if (rc != 0) return no;
+  return py::make_tuple(true, q ? py::cast(out) : py::none());
+}
+
+py::object int4_gather(const at::Tensor& k_pool, const at::Tensor& v_pool, const at::Tensor& tiles, int64_t n,
+                       py::object dtype) {
+  if (g_int4_gather == nullptr || !k_pool.is_cuda() || k_pool.dim() != 4 || n < 0 || !THPDtype_Check(dtype.ptr()))
+    return py::none();
+  const auto dev = k_pool.device();
+  const auto dt = reinterpret_cast<THPDtype*>(dtype.ptr())->scalar_type;
+  const int code = dtype_code(dt);
+  const int64_t hkv = k_pool.size(1), d = k_pool.size(3) * 8 / 5;
+  if (code < 1 || !int4_head(d) || !int4_pools(k_pool, v_pool, dev, hkv, d) || !int4_tiles(tiles, dev, 4) ||
+      tiles.size(1) != 4 || hkv > 65535)
+    return py::none();
+  c10::cuda::CUDAGuard guard(dev);
+  at::Tensor k = at::empty({hkv, n, d}, k_pool.options().dtype(dt)), v = at::empty_like(k);
+  const int rc = g_int4_gather(k_pool.data_ptr(), v_pool.data_ptr(), k.data_ptr(), v.data_ptr(), (int)hkv, (int)d, n,
+                               k.stride(0), k.stride(1), k_pool.size(2), k_pool.size(0), k_pool.stride(0), k_pool.stride(1),
+                               k_pool.stride(2), tiles.data_ptr<int32_t>(), tiles.size(0), code,
+                               c10::cuda::getCurrentCUDAStream(dev.index()).stream());
+  if (rc != 0) return py::none();
+  return py::make_tuple(k, v);
+}
+
+py::object int4_decode(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, double scale, const OptTensor& lengths,
+                       const OptTensor& tiles, int64_t splits) {
+  if (g_int4_decode == nullptr || !q.is_cuda() || q.dim() != (tiles ? 3 : 4)) return py::none();
+  const auto dev = q.device();
+  const auto dt = q.scalar_type();
+  const int code = dtype_code(dt);
+  const int64_t o = tiles ? 0 : 1, b = tiles ? 1 : q.size(0), hkv = q.size(o), g = q.size(o + 1), d = q.size(o + 2);
+  if (code < 1 || !int4_head(d) || g < 1 || g > 16 || b < 1 || b > 65535 || hkv < 1 || hkv > 65535 || splits < 0 ||
+      splits > 65535 || !plain(q, dev, dt) || !int4_rows(k, dev, hkv, d) || !int4_rows(v, dev, hkv, d) ||
+      v.sizes() != k.sizes())
+    return py::none();
+  if (tiles ? (lengths.has_value() || v.strides() != k.strides() || !int4_tiles(*tiles, dev, 3))
+            : (k.size(0) != b || !plain_lengths(lengths, dev, b)))
+    return py::none();
+  c10::cuda::CUDAGuard guard(dev);
+  const cudaStream_t st = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
+  const int64_t rows = tiles ? 32 * tiles->size(0) : k.size(2);
+  const size_t nb = g_int4_size((int)b, (int)hkv, (int)g, (int)d, rows, (int)splits);
+  void* ws = nullptr;
+  if (nb > 0) {
+    // a captured call gets a workspace of its graph's own
+    if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) return py::none();
+    ws = decode_workspace(dev, st, b * hkv, nb, q).data_ptr();
+  }
+  at::Tensor out = at::empty(q.sizes(), q.options());
+  int rc;
+  if (tiles)
+    rc = g_int4_paged(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), (int)hkv, (int)g, (int)d, k.size(2),
+                      k.size(0), k.stride(0), k.stride(1), k.stride(2), tiles->data_ptr<int32_t>(), (int)tiles->size(1),
+                      tiles->size(0), q.stride(0), q.stride(1), out.stride(0), out.stride(1), (float)scale, (int)splits,
+                      code, ws, nb, st);
+  else
+    rc = g_int4_decode(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), (int)b, (int)hkv, (int)g, (int)d, rows,
+                       lengths_ptr(lengths), q.stride(0), q.stride(1), q.stride(2), k.stride(0), k.stride(1), k.stride(2),
+                       v.stride(0), v.stride(1), v.stride(2), out.stride(0), out.stride(1), out.stride(2), (float)scale,
+                       (int)splits, code, ws, nb, st);
+  if (rc != 0) return py::none();
+  return py::cast(out);
+}
+
+py::object int4_gemv(const at::Tensor& x, const at::Tensor& codes, const at::Tensor& params, int64_t n, int64_t k,
+                     int64_t group, bool swiglu) {
+  if (g_int4_gemv == nullptr || !x.is_cuda() || (x.dim() != 1 && x.dim() != 2)) return py::none();
+  const auto dev = x.device();
+  const auto dt = x.scalar_type();
+  const int code = dtype_code(dt);
+  if (code < 1 || n < 1 || n > INT32_MAX || k < 1 || k > INT32_MAX / 2 || (group != 32 && group != 64 && group != 128) ||
+      !plain(x, dev, dt) || x.size(-1) != (swiglu ? 2 * k : k) || codes.device() != dev ||
+      codes.scalar_type() != at::kByte || codes.dim() != 3 || codes.size(0) != (n + 15) / 16 ||
+      codes.size(1) != (k + 63) / 64 || codes.size(2) != 512 || !codes.is_contiguous() || params.device() != dev ||
+      params.scalar_type() != dt || params.dim() != 5 || params.size(0) != (n + 15) / 16 ||
+      params.size(1) != (k + group - 1) / group || params.size(2) != 8 || params.size(3) != 2 || params.size(4) != 2 ||
+      !params.is_contiguous())
+    return py::none();
+  c10::cuda::CUDAGuard guard(dev);
+  const int64_t m = x.dim() == 2 ? x.size(0) : 1;
+  at::Tensor out = x.dim() == 2 ? at::empty({m, n}, x.options()) : at::empty({n}, x.options());
+  const int rc = g_int4_gemv(x.data_ptr(), codes.data_ptr(), params.data_ptr(), out.data_ptr(), n, (int)k, m, (int)group,
+                             x.dim() == 2 ? x.stride(0) : 0, n, swiglu, code,
+                             c10::cuda::getCurrentCUDAStream(dev.index()).stream());
+  if (rc != 0) return py::none();
+  return py::cast(out);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -339,5 +529,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("window_decode", &window_decode, "checked decode_attention_window fast path; None means: take the Python path");
   m.def("window_prefill", &window_prefill, "checked prefill_attention_window fast path; None means: take the Python path");
   m.def("shared_decode", &shared_decode, "checked decode_attention_shared fast path; None means: take the Python path");
+  m.def("init_int4", &init_int4, "set the addresses of the 4-bit entry points");
+  m.def("int4_append", &int4_append, "checked int4.append_rope_int4 / write_int4 fast path: (done, queries)");
+  m.def("int4_gather", &int4_gather, "checked int4.gather_int4 fast path; None means: take the Python path");
+  m.def("int4_decode", &int4_decode, "checked int4.decode_attention_int4 fast path; None means: take the Python path");
+  m.def("int4_gemv", &int4_gemv, "checked int4.gemv_int4 fast path; None means: take the Python path");
   m.def("partial", &partial, "checked decode_attention_partial fast path; None means: take the Python path");
 }

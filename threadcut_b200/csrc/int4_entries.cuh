@@ -1,0 +1,393 @@
+// C entry points of the 4-bit cache and the 4-bit projections (kernels: int4.cuh, int4_attn.cuh, int4_gemv.cuh).
+// Included at the end of threadcut_b200.cu, whose host helpers it uses.
+#pragma once
+
+namespace {
+
+bool i4_dtype(int dtype) { return dtype == TC_BF16 || dtype == TC_F16; }
+
+// Rows of 4-bit caches are copied and stored in whole 16-byte (d = 64: 8-byte) units.
+bool i4_aligned(const void* base, int64_t s0, int64_t s1, int64_t s2, int d) {
+  const int64_t unit = d == 64 ? 8 : 16;
+  return reinterpret_cast<uintptr_t>(base) % unit == 0 && s0 % unit == 0 && s1 % unit == 0 && s2 % unit == 0;
+}
+
+bool i4_pool(int hkv, int d, int64_t page_rows, int64_t num_pages) {
+  return hkv >= 1 && hkv <= 65535 && mma_dim(d) && page_rows >= 1 && page_rows <= (1 << 30) && num_pages >= 1 &&
+         num_pages <= (1 << 30);
+}
+
+// fn<T, D>(args...) for the type and head size
+#define TC_INT4_DISPATCH(fn, dtype, d, ...)                                                                     \
+  ((dtype) == TC_BF16 ? ((d) == 64    ? fn<__nv_bfloat16, 64>(__VA_ARGS__)                                      \
+                         : (d) == 128 ? fn<__nv_bfloat16, 128>(__VA_ARGS__)                                     \
+                                      : fn<__nv_bfloat16, 256>(__VA_ARGS__))                                    \
+                      : ((d) == 64    ? fn<__half, 64>(__VA_ARGS__)                                             \
+                         : (d) == 128 ? fn<__half, 128>(__VA_ARGS__)                                            \
+                                      : fn<__half, 256>(__VA_ARGS__)))
+
+template <typename T, int D>
+cudaError_t launch_int4_append(const Int4AppendParams& p, bool table_f32, bool vec, int sms, cudaStream_t st) {
+  constexpr int RW = 256 / D;
+  const int64_t warps = p.t * (cdiv(p.hq, RW) + 2 * cdiv(p.hkv, RW));
+  const int64_t blocks = cdiv(warps, 8) < (int64_t)sms * 64 ? cdiv(warps, 8) : (int64_t)sms * 64;
+  auto fn = table_f32 ? (vec ? int4_append_kernel<T, float, D, true> : int4_append_kernel<T, float, D, false>)
+                      : (vec ? int4_append_kernel<T, T, D, true> : int4_append_kernel<T, T, D, false>);
+  return launch_ex(fn, dim3((unsigned)blocks), dim3(256), 0, st, p);
+}
+
+template <typename T, int D>
+cudaError_t launch_int4_gather(const Int4GatherParams& p, int sms, cudaStream_t st) {
+  const int64_t blocks = cdiv(p.n_tiles * p.hkv, 8);
+  return launch_ex(int4_gather_kernel<T, D>, dim3((unsigned)(blocks < (int64_t)sms * 64 ? blocks : (int64_t)sms * 64)),
+                   dim3(256), 0, st, p);
+}
+
+template <typename T, int D>
+cudaError_t launch_int4_rotate(const Int4RotateParams& p, int sms, cudaStream_t st) {
+  const int64_t blocks = cdiv(p.layers * p.n_tiles * p.hkv, 8);
+  return launch_ex(int4_rotate_kernel<T, D>, dim3((unsigned)(blocks < (int64_t)sms * 8 ? blocks : (int64_t)sms * 8)),
+                   dim3(256), 0, st, p);
+}
+
+template <typename T, int D, int NG>
+cudaError_t launch_int4_decode_ng(const Int4DecodeParams& p, dim3 grid, int dev, cudaStream_t st) {
+  auto fn = int4_decode_kernel<T, D, NG>;
+  const cudaError_t e = set_smem(reinterpret_cast<const void*>(fn), I4Geom<D>::kSmem + 1024, dev);  // beside static shared memory
+  if (e != cudaSuccess) return e;
+  return launch_ex(fn, grid, dim3(32 * kI4Warps), I4Geom<D>::kSmem, st, p);
+}
+template <typename T, int D>
+cudaError_t launch_int4_decode(const Int4DecodeParams& p, dim3 grid, int dev, cudaStream_t st) {
+  return p.g > 8 ? launch_int4_decode_ng<T, D, 2>(p, grid, dev, st) : launch_int4_decode_ng<T, D, 1>(p, grid, dev, st);
+}
+
+// KV partition: as many slices as are resident at once for one sequence, equal slices that the block scheduler
+// balances for several (their lengths are on the device); none below a tile a warp.
+DecodePlan plan_int4(int batch, int hkv, int g, int d, int64_t rows, int splits_req, int sms) {
+  const int per_sm = d * (g > 8 ? 2 : 1) <= 128 ? 2 : 1;  // the kernel's launch bounds
+  DecodePlan pl = plan_decode(batch, hkv, rows, 0, batch > 1, splits_req, per_sm, sms);
+  if (splits_req <= 0 && pl.tps < kI4Warps) {
+    const int64_t tiles = rows > 0 ? cdiv(rows, kTile) : 1;
+    pl.tps = kI4Warps;
+    pl.max_splits = cdiv(tiles, pl.tps);
+  }
+  return pl;
+}
+
+int run_int4_decode(Int4DecodeParams& p, int d, int64_t rows, float scale, int splits, int dtype, void* ws,
+                    size_t ws_bytes, cudaStream_t st) {
+  const int dev = current_device();
+  const DecodePlan pl = plan_int4(p.batch, p.hkv, p.g, d, rows, splits, sm_count(dev));
+  const WsLayout w = decode_ws_layout(p.batch, p.hkv, p.g, d, pl.max_splits);
+  if (pl.max_splits > 1) {
+    if (ws == nullptr || ws_bytes < w.total) return TC_ERR_WORKSPACE;
+    if (!aligned16(ws)) return TC_ERR_ALIGN;
+    uint8_t* wb = static_cast<uint8_t*>(ws);
+    p.counters = reinterpret_cast<unsigned int*>(wb + w.counters);
+    p.ws_ml = reinterpret_cast<float2*>(wb + w.ml);
+    p.ws_o = reinterpret_cast<float*>(wb + w.o);
+  }
+  p.tiles_per_split = (int)pl.tps;
+  p.max_splits = (int)pl.max_splits;
+  p.c = scale * kLog2e;
+  const dim3 grid((unsigned)pl.max_splits, (unsigned)p.hkv, (unsigned)p.batch);
+  const cudaError_t e = TC_INT4_DISPATCH(launch_int4_decode, dtype, d, p, grid, dev, st);
+  return e == cudaSuccess ? TC_OK : TC_ERR_CUDA;
+}
+
+// Shared memory of a launch over m tokens.
+int64_t gv_smem(int k, int m, int group) {
+  const int64_t sums = cdiv((int64_t)gv_blocks(k) * (group == 32 ? 2 : 1) * gv_sums(m) * 4, 16) * 16;
+  return kGvWarps * kGvStages * (group == 32 ? gv_stage_bytes<32>() : gv_stage_bytes<64>()) + 2 * kGvPartBytes + sums +
+         (int64_t)m * gv_x_stride(k) * 2;
+}
+constexpr int64_t kGvMaxSmem = 227 * 1024;
+constexpr int kGvMaxColumns = 65536;  // one token of them fits
+
+template <typename T, int NT, int G>
+cudaError_t launch_int4_gemv_g(const Int4GemvParams& p, int smem, int dev, cudaStream_t st) {
+  auto fn = int4_gemv_kernel<T, NT, G>;
+  // the opt-in is set once per (kernel, device): ask for the most any plan takes
+  const cudaError_t e = set_smem(reinterpret_cast<const void*>(fn), (int)kGvMaxSmem, dev);
+  if (e != cudaSuccess) return e;
+  int per_sm = (int)(kGvMaxSmem / (smem + 1024));
+  if (per_sm < 1) per_sm = 1;
+  if (per_sm > 3) per_sm = 3;
+  const int64_t tiles = cdiv(p.n, 16), slots = (int64_t)sm_count(dev) * per_sm;
+  return launch_ex(fn, dim3((unsigned)(tiles < slots ? tiles : slots)), dim3(32 * kGvWarps), smem, st, p);
+}
+template <typename T, int NT>
+cudaError_t launch_int4_gemv_nt(const Int4GemvParams& p, int group, int smem, int dev, cudaStream_t st) {
+  return group == 32   ? launch_int4_gemv_g<T, NT, 32>(p, smem, dev, st)
+         : group == 64 ? launch_int4_gemv_g<T, NT, 64>(p, smem, dev, st)
+                       : launch_int4_gemv_g<T, NT, 128>(p, smem, dev, st);
+}
+template <typename T>
+cudaError_t launch_int4_gemv(const Int4GemvParams& p, int group, int smem, int dev, cudaStream_t st) {
+  return p.m <= 8    ? launch_int4_gemv_nt<T, 1>(p, group, smem, dev, st)
+         : p.m <= 16 ? launch_int4_gemv_nt<T, 2>(p, group, smem, dev, st)
+                     : launch_int4_gemv_nt<T, 4>(p, group, smem, dev, st);
+}
+
+}  // namespace
+
+extern "C" {
+
+int tc_int4_append_rope(const void* q, const void* k, const void* v, void* q_out, void* k_pool, void* v_pool, int hq,
+                        int hkv, int d, int64_t t, int64_t q_stride_h, int64_t q_stride_t, int64_t k_stride_h,
+                        int64_t k_stride_t, int64_t v_stride_h, int64_t v_stride_t, int64_t q_out_stride_h,
+                        int64_t q_out_stride_t, const void* q_norm_weight, const void* k_norm_weight, float eps,
+                        const void* cos_t, const void* sin_t, int rot, int64_t cos_stride_t, int64_t sin_stride_t,
+                        int table_dtype, int64_t page_rows, int64_t num_pages, int64_t pool_stride_page,
+                        int64_t pool_stride_h, int64_t pool_stride_row, const int32_t* slots, int dtype, void* stream) {
+  if (!i4_dtype(dtype) || (table_dtype != dtype && table_dtype != TC_F32)) return TC_ERR_DTYPE;
+  if (!i4_pool(hkv, d, page_rows, num_pages) || hq < 0 || hq > 65535 || rot < 0 || rot > d || (rot & 1) || t < 0 ||
+      t > INT32_MAX || !(eps >= 0.f))
+    return TC_ERR_INVALID;
+  if (t == 0) return TC_OK;
+  if (k == nullptr || v == nullptr || k_pool == nullptr || v_pool == nullptr || slots == nullptr ||
+      (rot > 0 && (cos_t == nullptr || sin_t == nullptr)) || (hq > 0 && (q == nullptr || q_out == nullptr)))
+    return TC_ERR_INVALID;
+  if (!i4_aligned(k_pool, pool_stride_page, pool_stride_h, pool_stride_row, d) ||
+      !i4_aligned(v_pool, 0, 0, 0, d))
+    return TC_ERR_ALIGN;
+  Int4AppendParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.q = q;
+  p.k = k;
+  p.v = v;
+  p.q_out = q_out;
+  p.kp = static_cast<uint8_t*>(k_pool);
+  p.vp = static_cast<uint8_t*>(v_pool);
+  p.q_w = q_norm_weight;
+  p.k_w = k_norm_weight;
+  p.cos_t = cos_t;
+  p.sin_t = sin_t;
+  p.hq = hq;
+  p.hkv = hkv;
+  p.rot = rot;
+  p.t = t;
+  p.q_sh = q_stride_h;
+  p.q_st = q_stride_t;
+  p.k_sh = k_stride_h;
+  p.k_st = k_stride_t;
+  p.v_sh = v_stride_h;
+  p.v_st = v_stride_t;
+  p.qo_sh = q_out_stride_h;
+  p.qo_st = q_out_stride_t;
+  p.cos_st = cos_stride_t;
+  p.sin_st = sin_stride_t;
+  p.page_rows = page_rows;
+  p.num_pages = num_pages;
+  p.s_page = pool_stride_page;
+  p.s_h = pool_stride_h;
+  p.s_row = pool_stride_row;
+  p.slots = slots;
+  p.eps = eps;
+  p.inv_d = 1.f / (float)d;
+  bool vec = rot % 16 == 0 && aligned16(k) && aligned16(v) && stride16(k_stride_h, dtype) && stride16(k_stride_t, dtype) &&
+             stride16(v_stride_h, dtype) && stride16(v_stride_t, dtype);
+  if (hq > 0)
+    vec = vec && aligned16(q) && aligned16(q_out) && stride16(q_stride_h, dtype) && stride16(q_stride_t, dtype) &&
+          stride16(q_out_stride_h, dtype) && stride16(q_out_stride_t, dtype);
+  if (rot > 0)
+    vec = vec && aligned16(cos_t) && aligned16(sin_t) && stride16(cos_stride_t, table_dtype) &&
+          stride16(sin_stride_t, table_dtype);
+  vec = vec && aligned16(q_norm_weight) && aligned16(k_norm_weight);
+  const cudaError_t e = TC_INT4_DISPATCH(launch_int4_append, dtype, d, p, table_dtype == TC_F32, vec,
+                                         sm_count(current_device()), static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? TC_OK : TC_ERR_CUDA;
+}
+
+int tc_int4_gather(const void* k_pool, const void* v_pool, void* k_out, void* v_out, int hkv, int d, int64_t n,
+                   int64_t out_stride_h, int64_t out_stride_n, int64_t page_rows, int64_t num_pages,
+                   int64_t pool_stride_page, int64_t pool_stride_h, int64_t pool_stride_row, const int32_t* tiles,
+                   int64_t n_tiles, int dtype, void* stream) {
+  if (!i4_dtype(dtype)) return TC_ERR_DTYPE;
+  if (!i4_pool(hkv, d, page_rows, num_pages) || n < 0 || n_tiles < 0 || n_tiles > INT32_MAX) return TC_ERR_INVALID;
+  if (n == 0 || n_tiles == 0) return TC_OK;
+  if (k_pool == nullptr || v_pool == nullptr || k_out == nullptr || v_out == nullptr || tiles == nullptr)
+    return TC_ERR_INVALID;
+  if (!i4_aligned(k_pool, pool_stride_page, pool_stride_h, pool_stride_row, d) ||
+      !i4_aligned(v_pool, 0, 0, 0, d) ||
+      !aligned16(k_out) || !aligned16(v_out) || !stride16(out_stride_h, dtype) || !stride16(out_stride_n, dtype) ||
+      !aligned16(tiles))
+    return TC_ERR_ALIGN;
+  Int4GatherParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.kp = static_cast<const uint8_t*>(k_pool);
+  p.vp = static_cast<const uint8_t*>(v_pool);
+  p.k_out = k_out;
+  p.v_out = v_out;
+  p.hkv = hkv;
+  p.n = n;
+  p.out_sh = out_stride_h;
+  p.out_sn = out_stride_n;
+  p.page_rows = page_rows;
+  p.num_pages = num_pages;
+  p.s_page = pool_stride_page;
+  p.s_h = pool_stride_h;
+  p.s_row = pool_stride_row;
+  p.tiles = tiles;
+  p.n_tiles = n_tiles;
+  const cudaError_t e =
+      TC_INT4_DISPATCH(launch_int4_gather, dtype, d, p, sm_count(current_device()), static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? TC_OK : TC_ERR_CUDA;
+}
+
+int tc_int4_rotate_keys(void* const* k_pools, int layers, int hkv, int d, int64_t page_rows, int64_t num_pages,
+                        int64_t pool_stride_page, int64_t pool_stride_h, int64_t pool_stride_row, const int32_t* tiles,
+                        int tile_cols, int64_t n_tiles, const float* cos_sin, int dtype, void* stream) {
+  if (!i4_dtype(dtype)) return TC_ERR_DTYPE;
+  if (layers < 1 || layers > kMaxLayers || !i4_pool(hkv, d, page_rows, num_pages) || n_tiles < 0 || n_tiles > INT32_MAX ||
+      tile_cols < 3 || tile_cols > 65535 || k_pools == nullptr || cos_sin == nullptr)
+    return TC_ERR_INVALID;
+  if (n_tiles == 0) return TC_OK;
+  if (tiles == nullptr) return TC_ERR_INVALID;
+  Int4RotateParams p;
+  std::memset(&p, 0, sizeof(p));
+  for (int l = 0; l < layers; ++l) {
+    if (k_pools[l] == nullptr) return TC_ERR_INVALID;
+    if (!i4_aligned(k_pools[l], pool_stride_page, pool_stride_h, pool_stride_row, d)) return TC_ERR_ALIGN;
+    p.kp[l] = static_cast<uint8_t*>(k_pools[l]);
+  }
+  p.layers = layers;
+  p.hkv = hkv;
+  p.page_rows = page_rows;
+  p.num_pages = num_pages;
+  p.s_page = pool_stride_page;
+  p.s_h = pool_stride_h;
+  p.s_row = pool_stride_row;
+  p.tiles = tiles;
+  p.tile_cols = tile_cols;
+  p.n_tiles = n_tiles;
+  load_cos_sin(p.cs, cos_sin, d);
+  const cudaError_t e =
+      TC_INT4_DISPATCH(launch_int4_rotate, dtype, d, p, sm_count(current_device()), static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? TC_OK : TC_ERR_CUDA;
+}
+
+size_t tc_decode_attention_int4_workspace_size(int batch, int hkv, int g, int d, int64_t rows, int splits) {
+  if (batch < 1 || batch > 65535 || hkv < 1 || hkv > 65535 || g < 1 || g > 16 || !mma_dim(d) || rows < 0 || splits < 0)
+    return 0;
+  const DecodePlan pl = plan_int4(batch, hkv, g, d, rows, splits, sm_count(current_device()));
+  return pl.max_splits > 1 ? decode_ws_layout(batch, hkv, g, d, pl.max_splits).total : 0;
+}
+
+int tc_decode_attention_int4(const void* q, const void* k, const void* v, void* out, int batch, int hkv, int g, int d,
+                             int64_t n, const int32_t* lengths, int64_t q_stride_b, int64_t q_stride_h,
+                             int64_t q_stride_g, int64_t k_stride_b, int64_t k_stride_h, int64_t k_stride_n,
+                             int64_t v_stride_b, int64_t v_stride_h, int64_t v_stride_n, int64_t out_stride_b,
+                             int64_t out_stride_h, int64_t out_stride_g, float scale, int splits, int dtype,
+                             void* workspace, size_t workspace_bytes, void* stream) {
+  if (!i4_dtype(dtype)) return TC_ERR_DTYPE;
+  if (batch < 1 || batch > 65535 || hkv < 1 || hkv > 65535 || g < 1 || g > 16 || !mma_dim(d) || n < 0 || n > (1 << 30) ||
+      splits < 0 || q == nullptr || out == nullptr || (n > 0 && (k == nullptr || v == nullptr)) || !finite_scale(scale))
+    return TC_ERR_INVALID;
+  if (!i4_aligned(k, k_stride_b, k_stride_h, k_stride_n, d) || !i4_aligned(v, v_stride_b, v_stride_h, v_stride_n, d))
+    return TC_ERR_ALIGN;
+  Int4DecodeParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.q = q;
+  p.out = out;
+  p.k = k;
+  p.v = v;
+  p.lengths = lengths;
+  p.n = n;
+  p.sq_b = q_stride_b;
+  p.sq_h = q_stride_h;
+  p.sq_g = q_stride_g;
+  p.so_b = out_stride_b;
+  p.so_h = out_stride_h;
+  p.so_g = out_stride_g;
+  p.sk_b = k_stride_b;
+  p.sk_h = k_stride_h;
+  p.sk_n = k_stride_n;
+  p.sv_b = v_stride_b;
+  p.sv_h = v_stride_h;
+  p.sv_n = v_stride_n;
+  p.hkv = hkv;
+  p.g = g;
+  p.batch = batch;
+  return run_int4_decode(p, d, n, scale, splits, dtype, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+}
+
+int tc_decode_attention_int4_paged(const void* q, const void* k_pool, const void* v_pool, void* out, int hkv, int g, int d,
+                                   int64_t page_rows, int64_t num_pages, int64_t pool_stride_page, int64_t pool_stride_h,
+                                   int64_t pool_stride_row, const int32_t* tiles, int tile_cols, int64_t n_tiles,
+                                   int64_t q_stride_h, int64_t q_stride_g, int64_t out_stride_h, int64_t out_stride_g,
+                                   float scale, int splits, int dtype, void* workspace, size_t workspace_bytes,
+                                   void* stream) {
+  if (!i4_dtype(dtype)) return TC_ERR_DTYPE;
+  if (!i4_pool(hkv, d, page_rows, num_pages) || g < 1 || g > 16 || n_tiles < 0 || n_tiles > (1 << 25) || tile_cols < 3 ||
+      tile_cols > 65535 || splits < 0 || q == nullptr || out == nullptr || k_pool == nullptr || v_pool == nullptr ||
+      (n_tiles > 0 && tiles == nullptr) || !finite_scale(scale))
+    return TC_ERR_INVALID;
+  if (!i4_aligned(k_pool, pool_stride_page, pool_stride_h, pool_stride_row, d) ||
+      !i4_aligned(v_pool, 0, 0, 0, d))
+    return TC_ERR_ALIGN;
+  Int4DecodeParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.q = q;
+  p.out = out;
+  p.k = k_pool;
+  p.v = v_pool;
+  p.paged = 1;
+  p.tiles = tiles;
+  p.tile_cols = tile_cols;
+  p.n_tiles = n_tiles;
+  p.page_rows = page_rows;
+  p.num_pages = num_pages;
+  p.sq_h = q_stride_h;
+  p.sq_g = q_stride_g;
+  p.so_h = out_stride_h;
+  p.so_g = out_stride_g;
+  p.sk_b = p.sv_b = pool_stride_page;
+  p.sk_h = p.sv_h = pool_stride_h;
+  p.sk_n = p.sv_n = pool_stride_row;
+  p.hkv = hkv;
+  p.g = g;
+  p.batch = 1;
+  return run_int4_decode(p, d, n_tiles * kTile, scale, splits, dtype, workspace, workspace_bytes,
+                         static_cast<cudaStream_t>(stream));
+}
+
+int tc_gemv_int4(const void* x, const void* codes, const void* params, void* out, int64_t n, int k, int64_t m, int group,
+                 int64_t x_stride, int64_t out_stride, int swiglu, int dtype, void* stream) {
+  if (!i4_dtype(dtype)) return TC_ERR_DTYPE;
+  if (n < 0 || n > INT32_MAX || k < 1 || m < 0 || m > (1 << 20) || (group != 32 && group != 64 && group != 128) ||
+      k > kGvMaxColumns)
+    return TC_ERR_INVALID;
+  if (n == 0 || m == 0) return TC_OK;
+  if (x == nullptr || codes == nullptr || params == nullptr || out == nullptr) return TC_ERR_INVALID;
+  if (!aligned16(codes) || !aligned16(params)) return TC_ERR_ALIGN;
+  int most = 32;  // tokens a launch, as many as fit
+  while (gv_smem(k, most, group) > kGvMaxSmem) --most;
+  const int dev = current_device();
+  for (int64_t m0 = 0; m0 < m; m0 += most) {
+    Int4GemvParams p;
+    std::memset(&p, 0, sizeof(p));
+    p.x = static_cast<const uint16_t*>(x) + m0 * x_stride;
+    p.codes = static_cast<const uint8_t*>(codes);
+    p.params = params;
+    p.out = static_cast<uint16_t*>(out) + m0 * out_stride;
+    p.n = n;
+    p.k = k;
+    p.m = (int)(m - m0 < most ? m - m0 : most);
+    p.sx = x_stride;
+    p.so = out_stride;
+    p.swiglu = swiglu != 0;
+    p.vec = aligned16(p.x) && (p.m == 1 || stride16(x_stride, dtype)) && (!p.swiglu || k % 8 == 0);
+    p.x_stride = gv_x_stride(k);
+    p.flush = kGvPartBytes / (kGvWarps * 64 * p.m);
+    const int smem = (int)gv_smem(k, p.m, group);
+    const cudaError_t e = dtype == TC_BF16
+                              ? launch_int4_gemv<__nv_bfloat16>(p, group, smem, dev, static_cast<cudaStream_t>(stream))
+                              : launch_int4_gemv<__half>(p, group, smem, dev, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return TC_ERR_CUDA;
+  }
+  return TC_OK;
+}
+
+}  // extern "C"

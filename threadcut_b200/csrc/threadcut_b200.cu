@@ -20,6 +20,7 @@
 #include "layer_ops.cuh"
 #include "peer.cuh"
 #include "gemv_stream.cuh"
+#include "int4_gemv.cuh"
 
 using namespace tc;
 
@@ -2545,3 +2546,5 @@ int tc_decode_attention_shared_paged(const void* q, const void* k_pool, const vo
 }
 
 }  // extern "C"
+
+#include "int4_entries.cuh"
