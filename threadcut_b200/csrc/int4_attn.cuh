@@ -1,16 +1,21 @@
 // Split-KV decode attention over a cache held in 4 bits (rows as in int4.cuh): softmax(scale q K^T) V of the g
-// query heads of each KV head over the values that the rows stand for, which are exactly what the products take.
+// query heads of each KV head. Keys enter as S (1 + c/16) + z, values as that rounded to T.
 //
 // Split, merge and partials are those of the 16-bit decode kernel (finish_cta). Inside a CTA each warp works
-// alone, on tiles of 32 rows that it copies into its own two shared-memory stages with cp.async: nothing waits
-// for another warp before the end. Per tile
-//   S^T[32 tok x 8 heads] = K q^T   K's fragments straight from the codes: lane (r, c) takes word c of a
-//                                   group's four, 8 neighbouring elements, as the columns of two products, so
-//                                   that every product lies within one group and q is permuted once instead
+// alone, on tiles of 32 rows that it brings into its own two shared-memory stages: nothing waits for another warp
+// before the end. What bounds it beside the bytes is the ALU pipe (half rate: masks, shifts, permutes), so each
+// part is arranged for few of those. Per tile
+//   S^T[32 tok x heads] = K q^T     on e4m3 products of the codes as they are (3 ALU instructions for 8 codes), S and z
+//                                   applied to their sums in fp32: sum_e q (S (1 + c/16) + z) over a group is
+//                                   (S / 16) sum q c + (S + z) sum q. The parts of a query head are neighbouring columns, so that
+//                                   one lane holds all sums of a head and a token
 //   online softmax                  as in the 16-bit kernel
-//   O^T[D x 8 heads] += V^T P^T     the words of two tokens are paired by byte permutes, lane r's rows of the
-//                                   products being its own D/8 neighbouring elements, all of one group
-// with P in two 16-bit parts, as there.
+//   O^T[D x heads] += V^T P^T       V^T's fragments as 16-bit values from the codes: the words of two tokens are paired by
+//                                   byte permutes, lane r's rows of the products being its own D/8 neighbouring elements, all
+//                                   of one group; P in two 16-bit parts, for up to 4 heads in neighbouring columns of one
+//                                   product
+// First form, with K's fragments as 16-bit values too, copies by cp.async and 8 heads' columns throughout: 98,304 rows of
+// 8 KV heads of 128 in 49.7 us (2.5 TB/s; 2.3 ALU instructions an element, the pipe 59 % busy).
 #pragma once
 
 #include "decode_attn.cuh"
@@ -26,14 +31,18 @@ struct Int4DecodeParams : DecodeParams {
   // stride, and tile t is rows [te[1], te[1] + te[2]) of page te[0], te = tiles + tile_cols t.
   int paged;  // (a sequence without tiles needs no table)
   int tile_cols;
+  int q_vec;  // q in 16-byte chunks
   int64_t page_rows, num_pages;
 };
 
-template <int D>
+// kBulk: a tile's rows are neighbours in memory (of one page, or of a sequence), 16-byte aligned, and come as one bulk
+// copy; else a lane copies units of 16 bytes (d = 64: 8) row by row.
+template <int D, bool kBulk>
 struct I4Geom {
   static constexpr int kRow = i4_row_bytes(D);
-  // Shared-memory row stride: the 32 words that a warp reads of 8 rows lie in different banks.
-  static constexpr int kStride = D == 64 ? 48 : D == 128 ? 80 : 176;
+  // Shared-memory row stride. Where it is free, the 32 words that a warp reads of 8 rows lie in different banks; 160 of a
+  // bulk copy at d = 256 has two to a bank.
+  static constexpr int kStride = kBulk ? kRow : D == 64 ? 48 : D == 128 ? 80 : 176;
   static constexpr int kCopy = D == 64 ? 8 : 16;  // bytes of a copy
   static constexpr int kCopies = kRow / kCopy;    // of a row
   static constexpr int kStage = 2 * kTile * kStride;
@@ -73,21 +82,39 @@ __device__ __forceinline__ void lds_words(uint32_t addr, uint32_t (&w)[N]) {
   }
 }
 
-// T in {bf16, f16}, D in {64, 128, 256}, NG tiles of 8 query heads (g <= 8 NG).
-template <typename T, int D, int NG>
-__global__ void __launch_bounds__(32 * kI4Warps, D * NG <= 128 ? 2 : 1)
+// Resident CTAs an SM, by what a lane holds (O^T's sums and the queries' parts): two within 128 registers where that spills
+// nothing that counts.
+__host__ __device__ constexpr int i4_ctas(bool bf16, int d, int nh) {
+  return d * nh <= 128 || (bf16 && d == 128 && nh == 2) ? 2 : 1;
+}
+
+// T in {bf16, f16}, D in {64, 128, 256}, NH tiles of 4 query heads (g <= 4 NH).
+template <typename T, int D, int NH, bool kBulk>
+__global__ void __launch_bounds__(32 * kI4Warps, i4_ctas(kE4Parts<T> == 2, D, NH))
     int4_decode_kernel(const __grid_constant__ Int4DecodeParams p) {
-  using G = I4Geom<D>;
-  constexpr int HP = 8 * NG;
-  constexpr int NGR = D / kI4Group;  // groups of a row
-  constexpr int WPT = D / 64;        // words of a value row that a lane takes
+  using G = I4Geom<D, kBulk>;
+  constexpr int NT = NH == 1 ? 1 : NH / 2;  // tiles of 8 columns of O^T
+  constexpr int HP = 8 * NT;
+  constexpr int NGR = D / kI4Group;      // groups of a row
+  constexpr int WPT = D / 64;            // words of a value row that a lane takes
+  constexpr int NQ = kE4Parts<T> - 1;    // products that hold a head's parts: (h, m), (l, 0)
   static_assert(Region<D, HP>::kFloats * 4 <= G::kWarpBytes, "a warp's state must fit in its stages");
   static_assert(merge_scratch_bytes(32 * kI4Warps) <= G::kSmem, "merge scratch must fit in the stages");
   extern __shared__ __align__(16) uint8_t i4_smem[];
+  __shared__ uint64_t s_full[kBulk ? kI4Warps * kI4Stages : 1];
   __shared__ int s_mi;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int r = lane >> 2, c = lane & 3;
   const int split = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
+  uint64_t* full = s_full + (kBulk ? warp * kI4Stages : 0);
+  if constexpr (kBulk) {
+    if (lane == 0) {
+#pragma unroll
+      for (int i = 0; i < kI4Stages; ++i) mbar_init(&full[i], 1);
+      fence_mbar_init();
+    }
+    __syncwarp();
+  }
   pdl_launch();
   pdl_wait();
   const int64_t n = seq_length<true>(p, b);  // clamped into [0, p.n]
@@ -106,178 +133,243 @@ __global__ void __launch_bounds__(32 * kI4Warps, D * NG <= 128 ? 2 : 1)
   const uint8_t* kb = static_cast<const uint8_t*>(p.k) + h * p.sk_h;
   const uint8_t* vb = static_cast<const uint8_t*>(p.v) + h * p.sv_h;
 
-  // Valid rows of tile j, and where they begin.
-  auto locate = [&](int j, const uint8_t*& ks, const uint8_t*& vs) -> int {
+  // Where tile j lies: (page or sequence, first row, rows), read a tile ahead of its use.
+  auto entry = [&](int j) -> int3 {
     const int64_t t = tt0 + j;
-    int64_t outer = b, row = t * kTile, rows = n - row;
     if (paged) {
       const int32_t* te = p.tiles + p.tile_cols * t;
-      outer = te[0];
-      row = te[1];
-      rows = te[2];
-      if (outer < 0 || outer >= p.num_pages || row < 0 || row >= p.page_rows) rows = 0;
-      if (rows > p.page_rows - row) rows = p.page_rows - row;
+      return make_int3(te[0], te[1], te[2]);
     }
-    if (rows <= 0) {
-      ks = kb;
-      vs = vb;
-      return 0;
-    }
-    ks = kb + outer * p.sk_b + row * p.sk_n;
-    vs = vb + outer * p.sv_b + row * p.sv_n;
-    return rows < kTile ? (int)rows : kTile;
+    return make_int3(b, (int)(t * kTile), (int)(n - t * kTile));
   };
-  // Starts the copies of tile j into stage s; rows behind the valid ones become zeros (code 0, S = z = 0).
-  auto fetch = [&](int j, int s) -> int {
-    const uint8_t *ks, *vs;
-    const int valid = locate(j, ks, vs);
+  // Starts the copies of a tile into stage s and returns its valid rows. What lies behind them: zeros (cp.async), or
+  // whatever was there (bulk).
+  const uint64_t pol = policy_evict_first();
+  auto fetch = [&](int3 te, int s) -> int {
+    int valid = te.z;
+    if (paged) {
+      if (te.x < 0 || te.x >= p.num_pages || te.y < 0 || te.y >= p.page_rows) valid = 0;
+      if (valid > p.page_rows - te.y) valid = (int)(p.page_rows - te.y);
+    }
+    valid = valid < 0 ? 0 : valid > kTile ? kTile : valid;
+    const uint8_t* ks = kb + te.x * p.sk_b + te.y * p.sk_n;
+    const uint8_t* vs = vb + te.x * p.sv_b + te.y * p.sv_n;
     const uint32_t dst = ring_s + s * G::kStage;
+    if constexpr (kBulk) {
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&full[s], 2 * valid * G::kRow);
+        if (valid > 0) {
+          bulk_g2s(ring + s * G::kStage, ks, valid * G::kRow, &full[s], pol);
+          bulk_g2s(ring + s * G::kStage + kTile * G::kStride, vs, valid * G::kRow, &full[s], pol);
+        }
+      }
+    } else {
 #pragma unroll
-    for (int u = 0; u < G::kCopies; ++u) {
-      const int x = lane + 32 * u;
-      const int row = x / G::kCopies, ch = x - row * G::kCopies;
-      const bool in = row < valid;
-      const uint32_t d = dst + row * G::kStride + ch * G::kCopy;
-      copy_async<G::kCopy>(d, in ? ks + row * p.sk_n + ch * G::kCopy : kb, in);
-      copy_async<G::kCopy>(d + kTile * G::kStride, in ? vs + row * p.sv_n + ch * G::kCopy : vb, in);
+      for (int u = 0; u < G::kCopies; ++u) {
+        const int x = lane + 32 * u;
+        const int row = x / G::kCopies, ch = x - row * G::kCopies;
+        const bool in = row < valid;
+        const uint32_t d = dst + row * G::kStride + ch * G::kCopy;
+        copy_async<G::kCopy>(d, in ? ks + row * p.sk_n + ch * G::kCopy : kb, in);
+        copy_async<G::kCopy>(d + kTile * G::kStride, in ? vs + row * p.sv_n + ch * G::kCopy : vb, in);
+      }
     }
     return valid;
   };
 
   int valid_next = 0;
-  if (warp < ntiles) valid_next = fetch(warp, 0);
-  copy_commit();
+  int3 ahead = make_int3(0, 0, 0);
+  if (warp < ntiles) valid_next = fetch(entry(warp), 0);
+  if constexpr (!kBulk) copy_commit();
+  if (warp + kI4Warps < ntiles) ahead = entry(warp + kI4Warps);
 
-  // q^T fragments: product 2 grp + m takes of each group's word c the codes (2m, 2m + 4) and (2m + 1, 2m + 5)
-  uint32_t bq[NG][2 * NGR][2];
+  // q^T as e4m3 parts. Column 2i of a tile's products is the first part of its head i, column 2i + 1 the second; a lane
+  // holds column r, of each group the bytes of elements 8c, 8c + 2, .. (the words' even codes) and 8c + 1, ...
+  uint32_t bq[NH][NQ][NGR][2];
+  float qsum[NH][NGR], qdown[NH];  // of head c: sums over the groups, the power of two of its parts
   {
-    const T* qb = static_cast<const T*>(p.q) + b * p.sq_b + h * p.sq_h;
-    const T zero = from_f32<T>(0.f);
 #pragma unroll
-    for (int nt = 0; nt < NG; ++nt) {
-      const int i = nt * 8 + r;
+    for (int t = 0; t < NH; ++t) {
+      const int i = 4 * t + (r >> 1);
       const bool ok = i < p.g;
-      const T* qr = qb + (ok ? i : 0) * p.sq_g;
+      const T* qr = static_cast<const T*>(p.q) + b * p.sq_b + h * p.sq_h + (ok ? i : 0) * p.sq_g + 8 * c;
+      auto elements = [&](int gr, float (&x)[8]) {
+        if (p.q_vec) {
+          load8(qr + gr * kI4Group, x);
+        } else {
 #pragma unroll
-      for (int ks = 0; ks < 2 * NGR; ++ks) {
-        const int e = (ks >> 1) * kI4Group + 8 * c + 2 * (ks & 1);
-        bq[nt][ks][0] = pack_raw<T>(ok ? qr[e] : zero, ok ? qr[e + 4] : zero);
-        bq[nt][ks][1] = pack_raw<T>(ok ? qr[e + 1] : zero, ok ? qr[e + 5] : zero);
+          for (int e = 0; e < 8; ++e) x[e] = to_f32(qr[gr * kI4Group + e]);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = ok ? x[e] : 0.f;
+      };
+      float most = 0.f;
+#pragma unroll
+      for (int gr = 0; gr < NGR; ++gr) {
+        float x[8], sum = 0.f;
+        elements(gr, x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          most = max_nan(most, fabsf(x[e]));
+          sum += x[e];
+        }
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        qsum[t][gr] = __shfl_sync(0xffffffffu, sum, 8 * c);
+      }
+      most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, 1));
+      most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, 2));
+      float up, down;
+      e4m3_scale(most, up, down);
+      qdown[t] = 32.f * __shfl_sync(0xffffffffu, down, 8 * c);
+#pragma unroll
+      for (int gr = 0; gr < NGR; ++gr) {
+        float x[8];
+        elements(gr, x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] *= up;
+        uint32_t even[NQ + 1], odd[NQ + 1];
+        e4m3_parts<NQ + 1>(x[0], x[2], x[4], x[6], even);
+        e4m3_parts<NQ + 1>(x[1], x[3], x[5], x[7], odd);
+        bq[t][0][gr][0] = r & 1 ? even[1] : even[0];
+        bq[t][0][gr][1] = r & 1 ? odd[1] : odd[0];
+        if constexpr (NQ == 2) {
+          bq[t][1][gr][0] = r & 1 ? 0u : even[2];
+          bq[t][1][gr][1] = r & 1 ? 0u : odd[2];
+        }
       }
     }
   }
-  float m_run[NG][2], l_run[NG][2];
-  float oacc[4 * WPT][NG][4];
+  float m_run[NH], l_run[NH];
+  float oacc[4 * WPT][NT][4];
 #pragma unroll
-  for (int nt = 0; nt < NG; ++nt)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      m_run[nt][e] = -INFINITY;
-      l_run[nt][e] = 0.f;
-    }
+  for (int t = 0; t < NH; ++t) {
+    m_run[t] = -INFINITY;
+    l_run[t] = 0.f;
+  }
 #pragma unroll
   for (int i = 0; i < 4 * WPT; ++i)
 #pragma unroll
-    for (int nt = 0; nt < NG; ++nt)
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int e = 0; e < 4; ++e) oacc[i][nt][e] = 0.f;
 
-  int s = 0;
-  for (int j = warp; j < ntiles; j += kI4Warps, s ^= 1) {
+  int s = 0, phase = 0;
+  for (int j = warp; j < ntiles; j += kI4Warps) {
     const int valid = valid_next;
-    if (j + kI4Warps < ntiles) valid_next = fetch(j + kI4Warps, s ^ 1);
-    copy_commit();
-    copy_wait<1>();
-    __syncwarp();
+    if (j + kI4Warps < ntiles) valid_next = fetch(ahead, s ^ 1);
+    if (j + 2 * kI4Warps < ntiles) ahead = entry(j + 2 * kI4Warps);
     const uint32_t kst = ring_s + s * G::kStage, vst = kst + kTile * G::kStride;
+    if constexpr (kBulk) {
+      if (!mbar_wait(&full[s], phase, TC_DEVERR_PIPE_TIMEOUT)) break;
+      if (valid < kTile) {
+        // values of rows that the tile does not have: S = z = 0, so that a weight of 0 never meets a NaN
+        if (lane >= valid) {
+          uint4* param = reinterpret_cast<uint4*>(ring + s * G::kStage + (kTile + lane) * G::kStride + D / 2);
+#pragma unroll
+          for (int i = 0; i < D / 128; ++i) param[i] = make_uint4(0u, 0u, 0u, 0u);
+        }
+        __syncwarp();
+      }
+    } else {
+      copy_commit();
+      copy_wait<1>();
+      __syncwarp();
+    }
 
-    float sacc[2][NG][4];
+    // scores of tokens r, r + 8, r + 16, r + 24 (index 2 mt + half) and head c of each tile of heads
+    float sc[4][NH];
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt) {
-#pragma unroll
-      for (int nt = 0; nt < NG; ++nt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sacc[mt][nt][e] = 0.f;
       const uint32_t k0 = kst + (mt * 16 + r) * G::kStride, k1 = k0 + 8 * G::kStride;
       uint32_t p0[NGR], p1[NGR];
       lds_words(k0 + D / 2, p0);
       lds_words(k1 + D / 2, p1);
+      float f0[NH], f1[NH], g0[NH], g1[NH];  // sums of S P and of (S + z) sum q
+#pragma unroll
+      for (int t = 0; t < NH; ++t) f0[t] = f1[t] = g0[t] = g1[t] = 0.f;
 #pragma unroll
       for (int gr = 0; gr < NGR; ++gr) {
         uint32_t w0[1], w1[1], a[4];
         lds_words(k0 + 16 * gr + 4 * c, w0);
         lds_words(k1 + 16 * gr + 4 * c, w1);
-        const uint32_t s0 = i4_low2(p0[gr], p0[gr]), z0 = i4_high2(p0[gr], p0[gr]);
-        const uint32_t s1 = i4_low2(p1[gr], p1[gr]), z1 = i4_high2(p1[gr], p1[gr]);
-        a[0] = I4<T>::fma2(i4_mant<T, 0>(w0[0]), s0, z0);
-        a[1] = I4<T>::fma2(i4_mant<T, 0>(w1[0]), s1, z1);
-        a[2] = I4<T>::fma2(i4_mant<T, 1>(w0[0]), s0, z0);
-        a[3] = I4<T>::fma2(i4_mant<T, 1>(w1[0]), s1, z1);
+        i4_bytes(w0[0], w1[0], a);
+        const float s0 = Mma<T>::lo(p0[gr]), s1 = Mma<T>::lo(p1[gr]);
+        const float o0 = s0 + Mma<T>::hi(p0[gr]), o1 = s1 + Mma<T>::hi(p1[gr]);
 #pragma unroll
-        for (int nt = 0; nt < NG; ++nt) Mma<T>::run(sacc[mt][nt], a, bq[nt][2 * gr][0], bq[nt][2 * gr][1]);
-        a[0] = I4<T>::fma2(i4_mant<T, 2>(w0[0]), s0, z0);
-        a[1] = I4<T>::fma2(i4_mant<T, 2>(w1[0]), s1, z1);
-        a[2] = I4<T>::fma2(i4_mant<T, 3>(w0[0]), s0, z0);
-        a[3] = I4<T>::fma2(i4_mant<T, 3>(w1[0]), s1, z1);
+        for (int t = 0; t < NH; ++t) {
+          float d[4] = {0.f, 0.f, 0.f, 0.f};
+          mma_e4m3(d, a, bq[t][0][gr][0], bq[t][0][gr][1]);
+          float x0 = fmaf(d[1], 0.0625f, d[0]), x1 = fmaf(d[3], 0.0625f, d[2]);
+          if constexpr (NQ == 2) {
+            float l[4] = {0.f, 0.f, 0.f, 0.f};
+            mma_e4m3(l, a, bq[t][1][gr][0], bq[t][1][gr][1]);
+            x0 = fmaf(l[0], 0.00390625f, x0);
+            x1 = fmaf(l[2], 0.00390625f, x1);
+          }
+          f0[t] = fmaf(s0, x0, f0[t]);
+          f1[t] = fmaf(s1, x1, f1[t]);
+          g0[t] = fmaf(o0, qsum[t][gr], g0[t]);
+          g1[t] = fmaf(o1, qsum[t][gr], g1[t]);
+        }
+      }
 #pragma unroll
-        for (int nt = 0; nt < NG; ++nt) Mma<T>::run(sacc[mt][nt], a, bq[nt][2 * gr + 1][0], bq[nt][2 * gr + 1][1]);
+      for (int t = 0; t < NH; ++t) {
+        sc[2 * mt][t] = fmaf(f0[t], qdown[t], g0[t]) * p.c;
+        sc[2 * mt + 1][t] = fmaf(f1[t], qdown[t], g1[t]) * p.c;
       }
     }
 
-    // online softmax; this lane holds tokens {r, r+8, r+16, r+24} x heads {2c, 2c+1}
-    float alpha[NG][2];
+    // online softmax
+    float alpha[NH];
 #pragma unroll
-    for (int nt = 0; nt < NG; ++nt) {
+    for (int t = 0; t < NH; ++t) {
+      if (valid < kTile) {
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float x0 = sacc[0][nt][e] * p.c, x1 = sacc[0][nt][2 + e] * p.c;
-        float x2 = sacc[1][nt][e] * p.c, x3 = sacc[1][nt][2 + e] * p.c;
-        if (r >= valid) x0 = -INFINITY;
-        if (r + 8 >= valid) x1 = -INFINITY;
-        if (r + 16 >= valid) x2 = -INFINITY;
-        if (r + 24 >= valid) x3 = -INFINITY;
-        float mx = fmaxf(fmaxf(x0, x1), fmaxf(x2, x3));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-        const float mnew = fmaxf(m_run[nt][e], mx);
-        const float mref = max_ref(mnew);
-        alpha[nt][e] = fast_exp2(m_run[nt][e] - mref);
-        m_run[nt][e] = mnew;
-        const float e0 = fast_exp2(x0 - mref), e1 = fast_exp2(x1 - mref);
-        const float e2 = fast_exp2(x2 - mref), e3 = fast_exp2(x3 - mref);
-        l_run[nt][e] = l_run[nt][e] * alpha[nt][e] + ((e0 + e1) + (e2 + e3));
-        sacc[0][nt][e] = e0;
-        sacc[0][nt][2 + e] = e1;
-        sacc[1][nt][e] = e2;
-        sacc[1][nt][2 + e] = e3;
+        for (int i = 0; i < 4; ++i)
+          if (r + 8 * i >= valid) sc[i][t] = -INFINITY;
       }
+      float mx = fmaxf(fmaxf(sc[0][t], sc[1][t]), fmaxf(sc[2][t], sc[3][t]));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+      const float mnew = fmaxf(m_run[t], mx);
+      const float mref = max_ref(mnew);
+      alpha[t] = fast_exp2(m_run[t] - mref);
+      m_run[t] = mnew;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sc[i][t] = fast_exp2(sc[i][t] - mref);
+      l_run[t] = l_run[t] * alpha[t] + ((sc[0][t] + sc[1][t]) + (sc[2][t] + sc[3][t]));
     }
+    // columns 2c, 2c + 1 of O^T: the two parts of head c (NH == 1), else heads c and c + 4 of a tile of 8
 #pragma unroll
     for (int i = 0; i < 4 * WPT; ++i)
 #pragma unroll
-      for (int nt = 0; nt < NG; ++nt) {
-        oacc[i][nt][0] *= alpha[nt][0];
-        oacc[i][nt][1] *= alpha[nt][1];
-        oacc[i][nt][2] *= alpha[nt][0];
-        oacc[i][nt][3] *= alpha[nt][1];
+      for (int nt = 0; nt < NT; ++nt) {
+        const float a0 = alpha[NH == 1 ? 0 : 2 * nt], a1 = alpha[NH == 1 ? 0 : 2 * nt + 1];
+        oacc[i][nt][0] *= a0;
+        oacc[i][nt][1] *= a1;
+        oacc[i][nt][2] *= a0;
+        oacc[i][nt][3] *= a1;
       }
 
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) {
-      // P^T fragments of 16 tokens, in two 16-bit parts
-      uint32_t hi[NG][2], lo[NG][2];
+      // P^T fragments of 16 tokens
+      uint32_t hi[NT][2], lo[NT][2];
 #pragma unroll
-      for (int nt = 0; nt < NG; ++nt) {
-        const float* sp = sacc[kk][nt];
-        const uint32_t x0 = Mma<T>::pack(sp[0], sp[1]), x1 = Mma<T>::pack(sp[2], sp[3]);
-        const uint32_t y0 = Mma<T>::pack(sp[0] - Mma<T>::lo(x0), sp[1] - Mma<T>::hi(x0));
-        const uint32_t y1 = Mma<T>::pack(sp[2] - Mma<T>::lo(x1), sp[3] - Mma<T>::hi(x1));
-        hi[nt][0] = movm_t(x0);
-        hi[nt][1] = movm_t(x1);
-        lo[nt][0] = movm_t(y0);
-        lo[nt][1] = movm_t(y1);
-      }
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float* x = sc[2 * kk + e];
+          if constexpr (NH == 1) {
+            hi[nt][e] = movm_t(Mma<T>::pack(x[0], x[0] - Mma<T>::lo(Mma<T>::pack(x[0], 0.f))));
+          } else {
+            const uint32_t y = Mma<T>::pack(x[2 * nt], x[2 * nt + 1]);
+            hi[nt][e] = movm_t(y);
+            lo[nt][e] = movm_t(Mma<T>::pack(x[2 * nt] - Mma<T>::lo(y), x[2 * nt + 1] - Mma<T>::hi(y)));
+          }
+        }
       // this lane's tokens 2c, 2c+1, 2c+8, 2c+9 of the 16: its D/8 elements and their group's (S, z)
       uint32_t w[4][WPT], q[4][1];
 #pragma unroll
@@ -296,47 +388,50 @@ __global__ void __launch_bounds__(32 * kI4Warps, D * NG <= 128 ? 2 : 1)
           const uint32_t a[4] = {I4<T>::fma2(m0, s01, z01), I4<T>::fma2(m1, s01, z01), I4<T>::fma2(m2, s23, z23),
                                  I4<T>::fma2(m3, s23, z23)};
 #pragma unroll
-          for (int nt = 0; nt < NG; ++nt) {
+          for (int nt = 0; nt < NT; ++nt) {
             Mma<T>::run(oacc[i][nt], a, hi[nt][0], hi[nt][1]);
-            Mma<T>::run(oacc[i][nt], a, lo[nt][0], lo[nt][1]);
+            if constexpr (NH > 1) Mma<T>::run(oacc[i][nt], a, lo[nt][0], lo[nt][1]);
           }
         };
-        product(4 * x, i4_mant<T, 0>(l01), i4_mant<T, 0>(h01), i4_mant<T, 0>(l23), i4_mant<T, 0>(h23));
-        product(4 * x + 1, i4_mant<T, 1>(l01), i4_mant<T, 1>(h01), i4_mant<T, 1>(l23), i4_mant<T, 1>(h23));
-        product(4 * x + 2, i4_mant<T, 2>(l01), i4_mant<T, 2>(h01), i4_mant<T, 2>(l23), i4_mant<T, 2>(h23));
-        product(4 * x + 3, i4_mant<T, 3>(l01), i4_mant<T, 3>(h01), i4_mant<T, 3>(l23), i4_mant<T, 3>(h23));
+        product(4 * x, i4_ones<T, 0>(l01), i4_ones<T, 0>(h01), i4_ones<T, 0>(l23), i4_ones<T, 0>(h23));
+        product(4 * x + 1, i4_ones<T, 1>(l01), i4_ones<T, 1>(h01), i4_ones<T, 1>(l23), i4_ones<T, 1>(h23));
+        product(4 * x + 2, i4_ones<T, 2>(l01), i4_ones<T, 2>(h01), i4_ones<T, 2>(l23), i4_ones<T, 2>(h23));
+        product(4 * x + 3, i4_ones<T, 3>(l01), i4_ones<T, 3>(h01), i4_ones<T, 3>(l23), i4_ones<T, 3>(h23));
       }
     }
+    if (kBulk && valid < kTile) fence_proxy_async_smem();  // the zeros above precede the next copy into the stage
     __syncwarp();  // the stage may be filled again
+    s ^= 1;
+    phase ^= s == 0;
   }
-  copy_wait<0>();
+  if constexpr (!kBulk) copy_wait<0>();
   __syncwarp();
 
   // this warp's state -> its own (now idle) stages
   using R = Region<D, HP>;
   float* reg = reinterpret_cast<float*>(ring);
 #pragma unroll
-  for (int nt = 0; nt < NG; ++nt)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      float l = l_run[nt][e];
-      l += __shfl_xor_sync(0xffffffffu, l, 4);
-      l += __shfl_xor_sync(0xffffffffu, l, 8);
-      l += __shfl_xor_sync(0xffffffffu, l, 16);
-      const int head = nt * 8 + 2 * c + e;
-      if (r == 0) {
-        R::m(reg)[head] = m_run[nt][e];
-        R::l(reg)[head] = l;
-      }
-#pragma unroll
-      for (int x = 0; x < WPT; ++x)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float* acc = R::acc(reg, head) + 8 * WPT * r + 8 * x + i;
-          acc[0] = oacc[4 * x + i][nt][e];
-          acc[4] = oacc[4 * x + i][nt][2 + e];
-        }
+  for (int t = 0; t < NH; ++t) {
+    float l = l_run[t];
+    l += __shfl_xor_sync(0xffffffffu, l, 4);
+    l += __shfl_xor_sync(0xffffffffu, l, 8);
+    l += __shfl_xor_sync(0xffffffffu, l, 16);
+    const int head = 4 * t + c;
+    if (r == 0) {
+      R::m(reg)[head] = m_run[t];
+      R::l(reg)[head] = l;
     }
+    const int nt = NH == 1 ? 0 : t / 2, e = NH == 1 ? 0 : t & 1;
+#pragma unroll
+    for (int x = 0; x < WPT; ++x)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float* o = oacc[4 * x + i][nt];
+        float* acc = R::acc(reg, head) + 8 * WPT * r + 8 * x + i;
+        acc[0] = NH == 1 ? o[0] + o[1] : o[e];
+        acc[4] = NH == 1 ? o[2] + o[3] : o[2 + e];
+      }
+  }
   __syncthreads();
   finish_cta<T, D, HP>(p, i4_smem, G::kWarpBytes, kI4Warps, b, h, split, nsplit, s_mi);
 }

@@ -50,22 +50,34 @@ cudaError_t launch_int4_rotate(const Int4RotateParams& p, int sms, cudaStream_t 
                    dim3(256), 0, st, p);
 }
 
-template <typename T, int D, int NG>
-cudaError_t launch_int4_decode_ng(const Int4DecodeParams& p, dim3 grid, int dev, cudaStream_t st) {
-  auto fn = int4_decode_kernel<T, D, NG>;
-  const cudaError_t e = set_smem(reinterpret_cast<const void*>(fn), I4Geom<D>::kSmem + 1024, dev);  // beside static shared memory
+template <typename T, int D, int NH, bool kBulk>
+cudaError_t launch_int4_decode_nh(const Int4DecodeParams& p, dim3 grid, int dev, cudaStream_t st) {
+  auto fn = int4_decode_kernel<T, D, NH, kBulk>;
+  constexpr int smem = I4Geom<D, kBulk>::kSmem;
+  const cudaError_t e = set_smem(reinterpret_cast<const void*>(fn), smem + 1024, dev);  // beside static shared memory
   if (e != cudaSuccess) return e;
-  return launch_ex(fn, grid, dim3(32 * kI4Warps), I4Geom<D>::kSmem, st, p);
+  return launch_ex(fn, grid, dim3(32 * kI4Warps), smem, st, p);
+}
+template <typename T, int D, bool kBulk>
+cudaError_t launch_int4_decode_bulk(const Int4DecodeParams& p, dim3 grid, int dev, cudaStream_t st) {
+  return p.g <= 4   ? launch_int4_decode_nh<T, D, 1, kBulk>(p, grid, dev, st)
+         : p.g <= 8 ? launch_int4_decode_nh<T, D, 2, kBulk>(p, grid, dev, st)
+                    : launch_int4_decode_nh<T, D, 4, kBulk>(p, grid, dev, st);
 }
 template <typename T, int D>
 cudaError_t launch_int4_decode(const Int4DecodeParams& p, dim3 grid, int dev, cudaStream_t st) {
-  return p.g > 8 ? launch_int4_decode_ng<T, D, 2>(p, grid, dev, st) : launch_int4_decode_ng<T, D, 1>(p, grid, dev, st);
+  if constexpr (D > 64) {  // (rows of d = 64 are 40 bytes, and begin off 16-byte boundaries)
+    if (p.sk_n == i4_row_bytes(D) && p.sv_n == i4_row_bytes(D))
+      return launch_int4_decode_bulk<T, D, true>(p, grid, dev, st);
+  }
+  return launch_int4_decode_bulk<T, D, false>(p, grid, dev, st);
 }
 
 // KV partition: as many slices as are resident at once for one sequence, equal slices that the block scheduler
 // balances for several (their lengths are on the device); none below a tile a warp.
 DecodePlan plan_int4(int batch, int hkv, int g, int d, int64_t rows, int splits_req, int sms) {
-  const int per_sm = d * (g > 8 ? 2 : 1) <= 128 ? 2 : 1;  // the kernel's launch bounds
+  // (one plan for both types: the workspace is sized without the type)
+  const int per_sm = i4_ctas(true, d, g <= 4 ? 1 : g <= 8 ? 2 : 4);
   DecodePlan pl = plan_decode(batch, hkv, rows, 0, batch > 1, splits_req, per_sm, sms);
   if (splits_req <= 0 && pl.tps < kI4Warps) {
     const int64_t tiles = rows > 0 ? cdiv(rows, kTile) : 1;
@@ -91,6 +103,7 @@ int run_int4_decode(Int4DecodeParams& p, int d, int64_t rows, float scale, int s
   p.tiles_per_split = (int)pl.tps;
   p.max_splits = (int)pl.max_splits;
   p.c = scale * kLog2e;
+  p.q_vec = aligned16(p.q) && stride16(p.sq_b, dtype) && stride16(p.sq_h, dtype) && stride16(p.sq_g, dtype);
   const dim3 grid((unsigned)pl.max_splits, (unsigned)p.hkv, (unsigned)p.batch);
   const cudaError_t e = TC_INT4_DISPATCH(launch_int4_decode, dtype, d, p, grid, dev, st);
   return e == cudaSuccess ? TC_OK : TC_ERR_CUDA;
