@@ -29,16 +29,11 @@ def rows_of(x):
     return pack_rows(*quantise64(x))
 
 
-def exact_of(rows, d, dtype):
-    """What 4-bit rows stand for, S (1 + code/16) + z, in float64."""
+def values_of(rows, d, dtype):
+    """The values of 4-bit rows, of `dtype`: one rounding of the exact S (1 + code/16) + z."""
     codes = torch.stack((rows[..., :d // 2] & 15, rows[..., :d // 2] >> 4), -1).flatten(-2).double()
     p = rows[..., d // 2:].contiguous().view(dtype).double().unflatten(-1, (-1, 2)).repeat_interleave(GROUP, -2)
-    return p[..., 0] * (1 + codes / 16) + p[..., 1]
-
-
-def values_of(rows, d, dtype):
-    """The values of 4-bit rows as they are read back: that rounded once to `dtype`."""
-    return exact_of(rows, d, dtype).to(dtype)
+    return (p[..., 0] * (1 + codes / 16) + p[..., 1]).to(dtype)
 
 
 def rotate32(x, cos, sin):

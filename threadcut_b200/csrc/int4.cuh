@@ -15,7 +15,7 @@
 
 #include <stdint.h>
 
-#include "tc_common.cuh"
+#include "rope_splice.cuh"  // kMaxLayers, kMaxRopeDim
 
 namespace tc {
 
@@ -48,12 +48,20 @@ struct I4<__half> {
   }
 };
 
+// (w & kMask) | kSet as one instruction: written with operators it becomes two.
+template <uint32_t kMask, uint32_t kSet>
+__device__ __forceinline__ uint32_t mask_set(uint32_t w) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(d) : "r"(w), "n"(kMask), "n"(kSet));
+  return d;
+}
+
 // 1 + c/16 for codes J (low half) and J + 4 (high half) of a word.
 template <typename T, int J>
 __device__ __forceinline__ uint32_t i4_mant(uint32_t w) {
   constexpr int up = I4<T>::kBit - 4 * J;
   const uint32_t s = up >= 0 ? w << (up >= 0 ? up : 0) : w >> (up >= 0 ? 0 : -up);
-  return (s & I4<T>::kMask) | I4<T>::kOne;
+  return mask_set<I4<T>::kMask, I4<T>::kOne>(s);
 }
 __device__ __forceinline__ uint32_t i4_low2(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x5410); }
 __device__ __forceinline__ uint32_t i4_high2(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x7632); }
@@ -78,72 +86,15 @@ template <typename T, int J>
 __device__ __forceinline__ uint32_t i4_ones(uint32_t w) {
   constexpr bool bf = I4<T>::kBit == 3;
   if constexpr (J == 0) {
-    const uint32_t x = (w & 0x000f000fu) | (bf ? 0x43004300u : 0x64006400u);
+    const uint32_t x = mask_set<0x000f000fu, bf ? 0x43004300u : 0x64006400u>(w);
     return bf ? I4<T>::fma2(x, 0x3d803d80u, 0xc0e0c0e0u)   // x / 16 - 7
               : I4<T>::fma2(x, 0x2c002c00u, 0xd3e0d3e0u);  // x / 16 - 63
   } else if constexpr (J == 1) {
     return bf ? I4<T>::fma2(w & 0x00f000f0u, 0x7e007e00u, 0x3f803f80u)                    // x 2^125 + 1
-              : I4<T>::fma2((w & 0x00f000f0u) | 0x64006400u, 0x1c001c00u, 0xc200c200u);  // x / 256 - 3
+              : I4<T>::fma2(mask_set<0x00f000f0u, 0x64006400u>(w), 0x1c001c00u, 0xc200c200u);  // x / 256 - 3
   } else {
     return i4_mant<T, J>(w);
   }
-}
-
-// ---- products with the codes themselves. A byte 0..15 is the e4m3 number code * 2^-9 (subnormal up to 7, linear on
-// through the first binade): two masks and a shift turn a word's 8 codes into the operands of an e4m3 product, whose sums
-// are exact (measured: 256,000 sums of 32 products with random e4m3 numbers, none off). The other operand, of 8 or 11
-// significant bits, is scaled by a power of two and split into parts of 4 bits: q = h + m / 16 (+ l / 256).
-__device__ __forceinline__ void mma_e4m3(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-// The operands (rows r and r + 8) of a product with the codes of two words: even codes, then odd ones.
-__device__ __forceinline__ void i4_bytes(uint32_t w0, uint32_t w1, uint32_t (&a)[4]) {
-  a[0] = w0 & 0x0f0f0f0fu;
-  a[1] = w1 & 0x0f0f0f0fu;
-  a[2] = (w0 >> 4) & 0x0f0f0f0fu;
-  a[3] = (w1 >> 4) & 0x0f0f0f0fu;
-}
-__device__ __forceinline__ uint32_t e4m3_pair(float lo, float hi) {  // saturating
-  uint16_t r;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-__device__ __forceinline__ float e4m3_low(uint32_t pair) {
-  uint32_t h;
-  asm("{\n\t.reg .b16 p;\n\tmov.b16 p, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, p;\n\t}" : "=r"(h) : "h"((uint16_t)pair));
-  return Mma<__half>::lo(h);
-}
-__device__ __forceinline__ float e4m3_high(uint32_t pair) {
-  uint32_t h;
-  asm("{\n\t.reg .b16 p;\n\tmov.b16 p, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, p;\n\t}" : "=r"(h) : "h"((uint16_t)pair));
-  return Mma<__half>::hi(h);
-}
-// Parts of 4 numbers (scaled into +-256): bytes in order, each part 16 times the one before.
-template <int kParts>
-__device__ __forceinline__ void e4m3_parts(float x0, float x1, float x2, float x3, uint32_t (&part)[kParts]) {
-#pragma unroll
-  for (int i = 0; i < kParts; ++i) {
-    const uint32_t a = e4m3_pair(x0, x1), b = e4m3_pair(x2, x3);
-    part[i] = a | (b << 16);
-    x0 = 16.f * (x0 - e4m3_low(a));
-    x1 = 16.f * (x1 - e4m3_high(a));
-    x2 = 16.f * (x2 - e4m3_low(b));
-    x3 = 16.f * (x3 - e4m3_high(b));
-  }
-}
-// Parts that hold a number of type T: bf16 has 8 significant bits (h + m / 16 is exact), fp16 11.
-template <typename T>
-constexpr int kE4Parts = I4<T>::kBit == 3 ? 2 : 3;
-// The power of two that brings a largest magnitude into [128, 256), and its inverse; NaN as the inverse where it is not
-// finite, so that it shows (the parts saturate).
-__device__ __forceinline__ void e4m3_scale(float most, float& up, float& down) {
-  int e = 134 - (int)(__float_as_uint(most) >> 23);
-  e = e > 100 ? 100 : e;
-  up = __uint_as_float((uint32_t)(127 + e) << 23);
-  down = most < INFINITY ? __uint_as_float((uint32_t)(127 - e) << 23) : __uint_as_float(0x7fffffffu);
 }
 
 __device__ __forceinline__ float min_nan(float a, float b) {

@@ -1,21 +1,19 @@
 // Split-KV decode attention over a cache held in 4 bits (rows as in int4.cuh): softmax(scale q K^T) V of the g
-// query heads of each KV head. Keys enter as S (1 + c/16) + z, values as that rounded to T.
+// query heads of each KV head over the values that the rows stand for, which are exactly what the products take.
 //
-// Split, merge and partials are those of the 16-bit decode kernel (finish_cta). Inside a CTA each warp works
-// alone, on tiles of 32 rows that it brings into its own two shared-memory stages: nothing waits for another warp
-// before the end. What bounds it beside the bytes is the ALU pipe (half rate: masks, shifts, permutes), so each
-// part is arranged for few of those. Per tile
-//   S^T[32 tok x heads] = K q^T     on e4m3 products of the codes as they are (3 ALU instructions for 8 codes), S and z
-//                                   applied to their sums in fp32: sum_e q (S (1 + c/16) + z) over a group is
-//                                   (S / 16) sum q c + (S + z) sum q. The parts of a query head are neighbouring columns, so that
-//                                   one lane holds all sums of a head and a token
-//   online softmax                  as in the 16-bit kernel
-//   O^T[D x heads] += V^T P^T       V^T's fragments as 16-bit values from the codes: the words of two tokens are paired by
-//                                   byte permutes, lane r's rows of the products being its own D/8 neighbouring elements, all
-//                                   of one group; P in two 16-bit parts, for up to 4 heads in neighbouring columns of one
-//                                   product
-// First form, with K's fragments as 16-bit values too, copies by cp.async and 8 heads' columns throughout: 98,304 rows of
-// 8 KV heads of 128 in 49.7 us (2.5 TB/s; 2.3 ALU instructions an element, the pipe 59 % busy).
+// Partials and their merge are those of the 16-bit decode kernel (finish_cta). Inside a CTA each warp works alone, on
+// tiles of 32 rows that it brings into its own two shared-memory stages: nothing waits for another warp before the end.
+// Per tile
+//   S^T[32 tok x heads] = K q^T     K's fragments straight from the codes: lane (r, c) takes word c of a group's four, 8
+//                                   neighbouring elements, as the columns of two products, so that every product lies
+//                                   within one group and q is permuted once instead
+//   online softmax                  as in the 16-bit kernel, the sums so far rescaled only where a maximum grew
+//   O^T[D x heads] += V^T P^T       the words of two tokens are paired by byte permutes, lane r's rows of the products being
+//                                   its own D/8 neighbouring elements, all of one group
+// P enters in two 16-bit parts; for up to 4 query heads a KV head (NH = 1) these are neighbouring columns of one product.
+//
+// Beside the bytes, instruction issue bounds it: about 5 instructions for each element a lane turns into an operand, most of
+// them on the half-rate ALU pipe (masks, shifts, permutes).
 #pragma once
 
 #include "decode_attn.cuh"
@@ -23,7 +21,6 @@
 
 namespace tc {
 
-constexpr int kI4Warps = 8;
 constexpr int kI4Stages = 2;
 
 struct Int4DecodeParams : DecodeParams {
@@ -37,7 +34,7 @@ struct Int4DecodeParams : DecodeParams {
 
 // kBulk: a tile's rows are neighbours in memory (of one page, or of a sequence), 16-byte aligned, and come as one bulk
 // copy; else a lane copies units of 16 bytes (d = 64: 8) row by row.
-template <int D, bool kBulk>
+template <int D, bool kBulk, int kWarps>
 struct I4Geom {
   static constexpr int kRow = i4_row_bytes(D);
   // Shared-memory row stride. Where it is free, the 32 words that a warp reads of 8 rows lie in different banks; 160 of a
@@ -47,7 +44,7 @@ struct I4Geom {
   static constexpr int kCopies = kRow / kCopy;    // of a row
   static constexpr int kStage = 2 * kTile * kStride;
   static constexpr int kWarpBytes = kI4Stages * kStage;
-  static constexpr int kSmem = kI4Warps * kWarpBytes;
+  static constexpr int kSmem = kWarps * kWarpBytes;
 };
 
 // Asynchronous copy of kBytes; without `in`, zeros (src is not read).
@@ -82,26 +79,24 @@ __device__ __forceinline__ void lds_words(uint32_t addr, uint32_t (&w)[N]) {
   }
 }
 
-// Resident CTAs an SM, by what a lane holds (O^T's sums and the queries' parts): two within 128 registers where that spills
-// nothing that counts.
-__host__ __device__ constexpr int i4_ctas(bool bf16, int d, int nh) {
-  return d * nh <= 128 || (bf16 && d == 128 && nh == 2) ? 2 : 1;
-}
+// Warps an SM holds, by what a lane holds (O^T's sums and q's fragments): 16 within 128 registers, where that spills nothing.
+__host__ __device__ constexpr int i4_warps(int d, int nh) { return d * nh <= 256 && d <= 128 ? 16 : 8; }
 
-// T in {bf16, f16}, D in {64, 128, 256}, NH tiles of 4 query heads (g <= 4 NH).
-template <typename T, int D, int NH, bool kBulk>
-__global__ void __launch_bounds__(32 * kI4Warps, i4_ctas(kE4Parts<T> == 2, D, NH))
+// T in {bf16, f16}, D in {64, 128, 256}, NH tiles of 4 query heads (g <= 4 NH), kWarps of a CTA.
+template <typename T, int D, int NH, bool kBulk, int kWarps>
+__global__ void __launch_bounds__(32 * kWarps, i4_warps(D, NH) / kWarps)
     int4_decode_kernel(const __grid_constant__ Int4DecodeParams p) {
-  using G = I4Geom<D, kBulk>;
-  constexpr int NT = NH == 1 ? 1 : NH / 2;  // tiles of 8 columns of O^T
+  using G = I4Geom<D, kBulk, kWarps>;
+  constexpr int NT = NH == 1 ? 1 : NH / 2;  // tiles of 8 columns
   constexpr int HP = 8 * NT;
-  constexpr int NGR = D / kI4Group;      // groups of a row
-  constexpr int WPT = D / 64;            // words of a value row that a lane takes
-  constexpr int NQ = kE4Parts<T> - 1;    // products that hold a head's parts: (h, m), (l, 0)
-  static_assert(Region<D, HP>::kFloats * 4 <= G::kWarpBytes, "a warp's state must fit in its stages");
-  static_assert(merge_scratch_bytes(32 * kI4Warps) <= G::kSmem, "merge scratch must fit in the stages");
+  constexpr int NGR = D / kI4Group;  // groups of a row
+  constexpr int WPT = D / 64;        // words of a value row that a lane takes
+  using R = Region<D, HP>;
+  static_assert(R::kFloats * 4 <= G::kWarpBytes, "a warp's state must fit in its stages");
+  static_assert(merge_scratch_bytes(32 * kWarps) <= G::kSmem, "merge scratch must fit in the stages");
   extern __shared__ __align__(16) uint8_t i4_smem[];
-  __shared__ uint64_t s_full[kBulk ? kI4Warps * kI4Stages : 1];
+  __shared__ uint64_t s_full[kBulk ? kWarps * kI4Stages : 1];
+  __shared__ float s_weight[kWarps][HP];
   __shared__ int s_mi;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int r = lane >> 2, c = lane & 3;
@@ -117,53 +112,58 @@ __global__ void __launch_bounds__(32 * kI4Warps, i4_ctas(kE4Parts<T> == 2, D, NH
   }
   pdl_launch();
   pdl_wait();
-  const int64_t n = seq_length<true>(p, b);  // clamped into [0, p.n]
+  const int n = (int)seq_length<true>(p, b);  // clamped into [0, p.n], below 2^30
   const bool paged = p.paged;
-  const int64_t seq_tiles = paged ? p.n_tiles : (n + kTile - 1) / kTile;
-  const int nsplit = seq_tiles > 0 ? (int)((seq_tiles + p.tiles_per_split - 1) / p.tiles_per_split) : 1;
+  const int seq_tiles = paged ? (int)p.n_tiles : (n + kTile - 1) / kTile;
+  const int nsplit = seq_tiles > 0 ? (seq_tiles + p.tiles_per_split - 1) / p.tiles_per_split : 1;
   if (split >= nsplit) return;
-  int64_t tt0, tt1;
-  split_range(seq_tiles, split, nsplit, tt0, tt1);
-  const int ntiles = (int)(tt1 - tt0);
-  if (threadIdx.x == 0)
-    s_mi = nsplit > 1 && !last_arrival_merge(nsplit, blockDim.x) ? merger_index(p, b, h, nsplit, p.g * (D / 4)) : -1;
+  // as even as whole tiles allow
+  const int share = seq_tiles / nsplit, more = seq_tiles - share * nsplit;
+  const int tt0 = split * share + (split < more ? split : more);
+  const int ntiles = share + (split < more);
 
   uint8_t* ring = i4_smem + warp * G::kWarpBytes;
   const uint32_t ring_s = smem_u32(ring);
-  const uint8_t* kb = static_cast<const uint8_t*>(p.k) + h * p.sk_h;
-  const uint8_t* vb = static_cast<const uint8_t*>(p.v) + h * p.sv_h;
+  const uint64_t pol = policy_evict_first();
 
   // Where tile j lies: (page or sequence, first row, rows), read a tile ahead of its use.
   auto entry = [&](int j) -> int3 {
-    const int64_t t = tt0 + j;
+    const int t = tt0 + j;
     if (paged) {
-      const int32_t* te = p.tiles + p.tile_cols * t;
+      const int32_t* te = p.tiles + p.tile_cols * (int64_t)t;
       return make_int3(te[0], te[1], te[2]);
     }
-    return make_int3(b, (int)(t * kTile), (int)(n - t * kTile));
+    return make_int3(b, t * kTile, n - t * kTile);
   };
-  // Starts the copies of a tile into stage s and returns its valid rows. What lies behind them: zeros (cp.async), or
-  // whatever was there (bulk).
-  const uint64_t pol = policy_evict_first();
-  auto fetch = [&](int3 te, int s) -> int {
+  // Valid rows of a tile.
+  auto rows_of = [&](int3 te) -> int {
     int valid = te.z;
     if (paged) {
       if (te.x < 0 || te.x >= p.num_pages || te.y < 0 || te.y >= p.page_rows) valid = 0;
       if (valid > p.page_rows - te.y) valid = (int)(p.page_rows - te.y);
     }
-    valid = valid < 0 ? 0 : valid > kTile ? kTile : valid;
-    const uint8_t* ks = kb + te.x * p.sk_b + te.y * p.sk_n;
-    const uint8_t* vs = vb + te.x * p.sv_b + te.y * p.sv_n;
-    const uint32_t dst = ring_s + s * G::kStage;
+    return valid < 0 ? 0 : valid > kTile ? kTile : valid;
+  };
+  // Starts the copies of a tile's valid rows into stage s. What lies behind them: zeros (cp.async), or whatever was
+  // there (bulk).
+  auto fetch = [&](int3 te, int valid, int s) {
     if constexpr (kBulk) {
       if (lane == 0) {
         mbar_arrive_expect_tx(&full[s], 2 * valid * G::kRow);
         if (valid > 0) {
-          bulk_g2s(ring + s * G::kStage, ks, valid * G::kRow, &full[s], pol);
-          bulk_g2s(ring + s * G::kStage + kTile * G::kStride, vs, valid * G::kRow, &full[s], pol);
+          bulk_g2s(ring + s * G::kStage, static_cast<const uint8_t*>(p.k) + h * p.sk_h + te.x * p.sk_b + te.y * p.sk_n,
+                   valid * G::kRow, &full[s], pol);
+          bulk_g2s(ring + s * G::kStage + kTile * G::kStride,
+                   static_cast<const uint8_t*>(p.v) + h * p.sv_h + te.x * p.sv_b + te.y * p.sv_n, valid * G::kRow, &full[s],
+                   pol);
         }
       }
     } else {
+      const uint8_t* kb = static_cast<const uint8_t*>(p.k) + h * p.sk_h;
+      const uint8_t* vb = static_cast<const uint8_t*>(p.v) + h * p.sv_h;
+      const uint8_t* ks = kb + te.x * p.sk_b + te.y * p.sk_n;
+      const uint8_t* vs = vb + te.x * p.sv_b + te.y * p.sv_n;
+      const uint32_t dst = ring_s + s * G::kStage;
 #pragma unroll
       for (int u = 0; u < G::kCopies; ++u) {
         const int x = lane + 32 * u;
@@ -174,70 +174,45 @@ __global__ void __launch_bounds__(32 * kI4Warps, i4_ctas(kE4Parts<T> == 2, D, NH
         copy_async<G::kCopy>(d + kTile * G::kStride, in ? vs + row * p.sv_n + ch * G::kCopy : vb, in);
       }
     }
-    return valid;
   };
 
   int valid_next = 0;
   int3 ahead = make_int3(0, 0, 0);
-  if (warp < ntiles) valid_next = fetch(entry(warp), 0);
+  if (warp < ntiles) {
+    const int3 te = entry(warp);
+    valid_next = rows_of(te);
+    fetch(te, valid_next, 0);
+  }
   if constexpr (!kBulk) copy_commit();
-  if (warp + kI4Warps < ntiles) ahead = entry(warp + kI4Warps);
+  if (warp + kWarps < ntiles) ahead = entry(warp + kWarps);
+  if (threadIdx.x == 0)
+    s_mi = nsplit > 1 && !last_arrival_merge(nsplit, blockDim.x) ? merger_index(p, b, h, nsplit, p.g * (D / 4)) : -1;
 
-  // q^T as e4m3 parts. Column 2i of a tile's products is the first part of its head i, column 2i + 1 the second; a lane
-  // holds column r, of each group the bytes of elements 8c, 8c + 2, .. (the words' even codes) and 8c + 1, ...
-  uint32_t bq[NH][NQ][NGR][2];
-  float qsum[NH][NGR], qdown[NH];  // of head c: sums over the groups, the power of two of its parts
-  {
+  // q^T fragments: product 2 gr + m takes of each group's word c the codes (2m, 2m + 4) and (2m + 1, 2m + 5). Column 2i of
+  // tile nt is query head 8 nt + i, column 2i + 1 head 8 nt + 4 + i (NH = 1: nothing, P's second part goes there)
+  uint32_t bq[NT][2 * NGR][2];
 #pragma unroll
-    for (int t = 0; t < NH; ++t) {
-      const int i = 4 * t + (r >> 1);
-      const bool ok = i < p.g;
-      const T* qr = static_cast<const T*>(p.q) + b * p.sq_b + h * p.sq_h + (ok ? i : 0) * p.sq_g + 8 * c;
-      auto elements = [&](int gr, float (&x)[8]) {
+  for (int nt = 0; nt < NT; ++nt) {
+    const int i = 8 * nt + (r >> 1) + 4 * (r & 1);
+    const bool ok = i < p.g && (NH > 1 || !(r & 1));
+    const T* qr = static_cast<const T*>(p.q) + b * p.sq_b + h * p.sq_h + (ok ? i : 0) * p.sq_g + 8 * c;
+#pragma unroll
+    for (int gr = 0; gr < NGR; ++gr) {
+      uint4 x = make_uint4(0u, 0u, 0u, 0u);
+      if (ok) {
         if (p.q_vec) {
-          load8(qr + gr * kI4Group, x);
+          x = *reinterpret_cast<const uint4*>(qr + gr * kI4Group);
         } else {
+          T e[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] = to_f32(qr[gr * kI4Group + e]);
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = ok ? x[e] : 0.f;
-      };
-      float most = 0.f;
-#pragma unroll
-      for (int gr = 0; gr < NGR; ++gr) {
-        float x[8], sum = 0.f;
-        elements(gr, x);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          most = max_nan(most, fabsf(x[e]));
-          sum += x[e];
-        }
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        qsum[t][gr] = __shfl_sync(0xffffffffu, sum, 8 * c);
-      }
-      most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, 1));
-      most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, 2));
-      float up, down;
-      e4m3_scale(most, up, down);
-      qdown[t] = 32.f * __shfl_sync(0xffffffffu, down, 8 * c);
-#pragma unroll
-      for (int gr = 0; gr < NGR; ++gr) {
-        float x[8];
-        elements(gr, x);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] *= up;
-        uint32_t even[NQ + 1], odd[NQ + 1];
-        e4m3_parts<NQ + 1>(x[0], x[2], x[4], x[6], even);
-        e4m3_parts<NQ + 1>(x[1], x[3], x[5], x[7], odd);
-        bq[t][0][gr][0] = r & 1 ? even[1] : even[0];
-        bq[t][0][gr][1] = r & 1 ? odd[1] : odd[0];
-        if constexpr (NQ == 2) {
-          bq[t][1][gr][0] = r & 1 ? 0u : even[2];
-          bq[t][1][gr][1] = r & 1 ? 0u : odd[2];
+          for (int u = 0; u < 8; ++u) e[u] = qr[gr * kI4Group + u];
+          memcpy(&x, e, 16);
         }
       }
+      bq[nt][2 * gr][0] = i4_low2(x.x, x.z);
+      bq[nt][2 * gr][1] = i4_high2(x.x, x.z);
+      bq[nt][2 * gr + 1][0] = i4_low2(x.y, x.w);
+      bq[nt][2 * gr + 1][1] = i4_high2(x.y, x.w);
     }
   }
   float m_run[NH], l_run[NH];
@@ -255,10 +230,13 @@ __global__ void __launch_bounds__(32 * kI4Warps, i4_ctas(kE4Parts<T> == 2, D, NH
       for (int e = 0; e < 4; ++e) oacc[i][nt][e] = 0.f;
 
   int s = 0, phase = 0;
-  for (int j = warp; j < ntiles; j += kI4Warps) {
+  for (int j = warp; j < ntiles; j += kWarps) {
     const int valid = valid_next;
-    if (j + kI4Warps < ntiles) valid_next = fetch(ahead, s ^ 1);
-    if (j + 2 * kI4Warps < ntiles) ahead = entry(j + 2 * kI4Warps);
+    if (j + kWarps < ntiles) {
+      valid_next = rows_of(ahead);
+      fetch(ahead, valid_next, s ^ 1);
+    }
+    if (j + 2 * kWarps < ntiles) ahead = entry(j + 2 * kWarps);
     const uint32_t kst = ring_s + s * G::kStage, vst = kst + kTile * G::kStride;
     if constexpr (kBulk) {
       if (!mbar_wait(&full[s], phase, TC_DEVERR_PIPE_TIMEOUT)) break;
@@ -277,7 +255,7 @@ __global__ void __launch_bounds__(32 * kI4Warps, i4_ctas(kE4Parts<T> == 2, D, NH
       __syncwarp();
     }
 
-    // scores of tokens r, r + 8, r + 16, r + 24 (index 2 mt + half) and head c of each tile of heads
+    // scores of tokens r, r + 8, r + 16, r + 24 (index 2 mt + half), of head 4 t + c
     float sc[4][NH];
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt) {
@@ -285,73 +263,78 @@ __global__ void __launch_bounds__(32 * kI4Warps, i4_ctas(kE4Parts<T> == 2, D, NH
       uint32_t p0[NGR], p1[NGR];
       lds_words(k0 + D / 2, p0);
       lds_words(k1 + D / 2, p1);
-      float f0[NH], f1[NH], g0[NH], g1[NH];  // sums of S P and of (S + z) sum q
+      float acc[NT][4];
 #pragma unroll
-      for (int t = 0; t < NH; ++t) f0[t] = f1[t] = g0[t] = g1[t] = 0.f;
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[nt][e] = 0.f;
 #pragma unroll
       for (int gr = 0; gr < NGR; ++gr) {
-        uint32_t w0[1], w1[1], a[4];
+        uint32_t w0[1], w1[1];
         lds_words(k0 + 16 * gr + 4 * c, w0);
         lds_words(k1 + 16 * gr + 4 * c, w1);
-        i4_bytes(w0[0], w1[0], a);
-        const float s0 = Mma<T>::lo(p0[gr]), s1 = Mma<T>::lo(p1[gr]);
-        const float o0 = s0 + Mma<T>::hi(p0[gr]), o1 = s1 + Mma<T>::hi(p1[gr]);
+        const uint32_t s0 = i4_low2(p0[gr], p0[gr]), z0 = i4_high2(p0[gr], p0[gr]);
+        const uint32_t s1 = i4_low2(p1[gr], p1[gr]), z1 = i4_high2(p1[gr], p1[gr]);
+        const uint32_t a[4] = {I4<T>::fma2(i4_ones<T, 0>(w0[0]), s0, z0), I4<T>::fma2(i4_ones<T, 0>(w1[0]), s1, z1),
+                               I4<T>::fma2(i4_ones<T, 1>(w0[0]), s0, z0), I4<T>::fma2(i4_ones<T, 1>(w1[0]), s1, z1)};
+        const uint32_t a2[4] = {I4<T>::fma2(i4_ones<T, 2>(w0[0]), s0, z0), I4<T>::fma2(i4_ones<T, 2>(w1[0]), s1, z1),
+                                I4<T>::fma2(i4_ones<T, 3>(w0[0]), s0, z0), I4<T>::fma2(i4_ones<T, 3>(w1[0]), s1, z1)};
 #pragma unroll
-        for (int t = 0; t < NH; ++t) {
-          float d[4] = {0.f, 0.f, 0.f, 0.f};
-          mma_e4m3(d, a, bq[t][0][gr][0], bq[t][0][gr][1]);
-          float x0 = fmaf(d[1], 0.0625f, d[0]), x1 = fmaf(d[3], 0.0625f, d[2]);
-          if constexpr (NQ == 2) {
-            float l[4] = {0.f, 0.f, 0.f, 0.f};
-            mma_e4m3(l, a, bq[t][1][gr][0], bq[t][1][gr][1]);
-            x0 = fmaf(l[0], 0.00390625f, x0);
-            x1 = fmaf(l[2], 0.00390625f, x1);
-          }
-          f0[t] = fmaf(s0, x0, f0[t]);
-          f1[t] = fmaf(s1, x1, f1[t]);
-          g0[t] = fmaf(o0, qsum[t][gr], g0[t]);
-          g1[t] = fmaf(o1, qsum[t][gr], g1[t]);
+        for (int nt = 0; nt < NT; ++nt) {
+          Mma<T>::run(acc[nt], a, bq[nt][2 * gr][0], bq[nt][2 * gr][1]);
+          Mma<T>::run(acc[nt], a2, bq[nt][2 * gr + 1][0], bq[nt][2 * gr + 1][1]);
         }
       }
 #pragma unroll
       for (int t = 0; t < NH; ++t) {
-        sc[2 * mt][t] = fmaf(f0[t], qdown[t], g0[t]) * p.c;
-        sc[2 * mt + 1][t] = fmaf(f1[t], qdown[t], g1[t]) * p.c;
+        sc[2 * mt][t] = acc[t / 2][t & 1] * p.c;
+        sc[2 * mt + 1][t] = acc[t / 2][2 + (t & 1)] * p.c;
       }
     }
 
     // online softmax
-    float alpha[NH];
+    if (valid < kTile) {
 #pragma unroll
-    for (int t = 0; t < NH; ++t) {
-      if (valid < kTile) {
+      for (int t = 0; t < NH; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           if (r + 8 * i >= valid) sc[i][t] = -INFINITY;
-      }
+    }
+    float mref[NH], alpha[NH];
+    bool grew = false;
+#pragma unroll
+    for (int t = 0; t < NH; ++t) {
       float mx = fmaxf(fmaxf(sc[0][t], sc[1][t]), fmaxf(sc[2][t], sc[3][t]));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
       const float mnew = fmaxf(m_run[t], mx);
-      const float mref = max_ref(mnew);
-      alpha[t] = fast_exp2(m_run[t] - mref);
+      grew = grew || mnew > m_run[t];
+      mref[t] = max_ref(mnew);
+      alpha[t] = fast_exp2(m_run[t] - mref[t]);
       m_run[t] = mnew;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) sc[i][t] = fast_exp2(sc[i][t] - mref);
-      l_run[t] = l_run[t] * alpha[t] + ((sc[0][t] + sc[1][t]) + (sc[2][t] + sc[3][t]));
     }
-    // columns 2c, 2c + 1 of O^T: the two parts of head c (NH == 1), else heads c and c + 4 of a tile of 8
+    if (__any_sync(0xffffffffu, grew)) {
+      // columns 2c, 2c + 1 of O^T: the two parts of head c (NH = 1), else heads c and c + 4 of a tile
 #pragma unroll
-    for (int i = 0; i < 4 * WPT; ++i)
+      for (int t = 0; t < NH; ++t) l_run[t] *= alpha[t];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const float a0 = alpha[NH == 1 ? 0 : 2 * nt], a1 = alpha[NH == 1 ? 0 : 2 * nt + 1];
-        oacc[i][nt][0] *= a0;
-        oacc[i][nt][1] *= a1;
-        oacc[i][nt][2] *= a0;
-        oacc[i][nt][3] *= a1;
-      }
+      for (int i = 0; i < 4 * WPT; ++i)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const float a0 = alpha[NH == 1 ? 0 : 2 * nt], a1 = alpha[NH == 1 ? 0 : 2 * nt + 1];
+          oacc[i][nt][0] *= a0;
+          oacc[i][nt][1] *= a1;
+          oacc[i][nt][2] *= a0;
+          oacc[i][nt][3] *= a1;
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < NH; ++t) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sc[i][t] = fast_exp2(sc[i][t] - mref[t]);
+      l_run[t] += (sc[0][t] + sc[1][t]) + (sc[2][t] + sc[3][t]);
+    }
 
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) {
@@ -408,7 +391,6 @@ __global__ void __launch_bounds__(32 * kI4Warps, i4_ctas(kE4Parts<T> == 2, D, NH
   __syncwarp();
 
   // this warp's state -> its own (now idle) stages
-  using R = Region<D, HP>;
   float* reg = reinterpret_cast<float*>(ring);
 #pragma unroll
   for (int t = 0; t < NH; ++t) {
@@ -433,7 +415,31 @@ __global__ void __launch_bounds__(32 * kI4Warps, i4_ctas(kE4Parts<T> == 2, D, NH
       }
   }
   __syncthreads();
-  finish_cta<T, D, HP>(p, i4_smem, G::kWarpBytes, kI4Warps, b, h, split, nsplit, s_mi);
+  // the warps' states as one, in the first warp's place: a head's maximum, weights and sum by the lanes of one warp, then an
+  // output a thread
+  auto region = [&](int w) { return reinterpret_cast<float*>(i4_smem + w * G::kWarpBytes); };
+  for (int i = warp; i < p.g; i += kWarps) {
+    const float m = lane < kWarps ? R::m(region(lane))[i] : -INFINITY;
+    const float M = warp_max(m);
+    const float w = fast_exp2(m - max_ref(M));
+    const float L = warp_sum(lane < kWarps ? w * R::l(region(lane))[i] : 0.f);
+    if (lane < kWarps) s_weight[lane][i] = w;
+    __syncwarp();
+    if (lane == 0) {
+      R::m(reg = region(0))[i] = M;
+      R::l(reg)[i] = L;
+    }
+  }
+  __syncthreads();
+  for (int idx = threadIdx.x; idx < p.g * D; idx += 32 * kWarps) {
+    const int i = idx / D, d = idx - i * D;
+    float o = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) o += R::acc(region(w), i)[d] * s_weight[w][i];
+    R::acc(region(0), i)[d] = o;
+  }
+  __syncthreads();
+  finish_cta<T, D, HP>(p, i4_smem, G::kWarpBytes, 1, b, h, split, nsplit, s_mi);
 }
 
 }  // namespace tc

@@ -50,40 +50,66 @@ cudaError_t launch_int4_rotate(const Int4RotateParams& p, int sms, cudaStream_t 
                    dim3(256), 0, st, p);
 }
 
-template <typename T, int D, int NH, bool kBulk>
-cudaError_t launch_int4_decode_nh(const Int4DecodeParams& p, dim3 grid, int dev, cudaStream_t st) {
-  auto fn = int4_decode_kernel<T, D, NH, kBulk>;
-  constexpr int smem = I4Geom<D, kBulk>::kSmem;
-  const cudaError_t e = set_smem(reinterpret_cast<const void*>(fn), smem + 1024, dev);  // beside static shared memory
-  if (e != cudaSuccess) return e;
-  return launch_ex(fn, grid, dim3(32 * kI4Warps), smem, st, p);
-}
-template <typename T, int D, bool kBulk>
-cudaError_t launch_int4_decode_bulk(const Int4DecodeParams& p, dim3 grid, int dev, cudaStream_t st) {
-  return p.g <= 4   ? launch_int4_decode_nh<T, D, 1, kBulk>(p, grid, dev, st)
-         : p.g <= 8 ? launch_int4_decode_nh<T, D, 2, kBulk>(p, grid, dev, st)
-                    : launch_int4_decode_nh<T, D, 4, kBulk>(p, grid, dev, st);
-}
-template <typename T, int D>
-cudaError_t launch_int4_decode(const Int4DecodeParams& p, dim3 grid, int dev, cudaStream_t st) {
-  if constexpr (D > 64) {  // (rows of d = 64 are 40 bytes, and begin off 16-byte boundaries)
-    if (p.sk_n == i4_row_bytes(D) && p.sv_n == i4_row_bytes(D))
-      return launch_int4_decode_bulk<T, D, true>(p, grid, dev, st);
-  }
-  return launch_int4_decode_bulk<T, D, false>(p, grid, dev, st);
+int i4_head_tiles(int g) { return g <= 4 ? 1 : g <= 8 ? 2 : 4; }
+// Warps of a CTA. The slices of one long sequence end together, so that one large CTA an SM has the least to merge; short
+// ones leave a large CTA's warps with too little each, and those of several sequences end at different times, so that a second
+// CTA on the SM works while one begins or ends. One sequence, 8 KV heads of 128, 16 against 8 warps: 4,096 rows 10.4 and
+// 8.8 us, 8,192 rows 12.4 and 12.4, 16,384 rows 14.4 and 16.3, 98,304 rows 34.3 and 35.2.
+int i4_cta_warps(int batch, int hkv, int64_t rows, int d, int nh, int sms) {
+  return batch == 1 && hkv * cdiv(rows, kTile) >= 14 * (int64_t)sms ? i4_warps(d, nh) : 8;
 }
 
-// KV partition: as many slices as are resident at once for one sequence, equal slices that the block scheduler
-// balances for several (their lengths are on the device); none below a tile a warp.
-DecodePlan plan_int4(int batch, int hkv, int g, int d, int64_t rows, int splits_req, int sms) {
-  // (one plan for both types: the workspace is sized without the type)
-  const int per_sm = i4_ctas(true, d, g <= 4 ? 1 : g <= 8 ? 2 : 4);
-  DecodePlan pl = plan_decode(batch, hkv, rows, 0, batch > 1, splits_req, per_sm, sms);
-  if (splits_req <= 0 && pl.tps < kI4Warps) {
-    const int64_t tiles = rows > 0 ? cdiv(rows, kTile) : 1;
-    pl.tps = kI4Warps;
-    pl.max_splits = cdiv(tiles, pl.tps);
+template <typename T, int D, int NH, bool kBulk, int kWarps>
+cudaError_t launch_int4_decode_w(const Int4DecodeParams& p, dim3 grid, int dev, cudaStream_t st) {
+  auto fn = int4_decode_kernel<T, D, NH, kBulk, kWarps>;
+  constexpr int smem = I4Geom<D, kBulk, kWarps>::kSmem;
+  const cudaError_t e = set_smem(reinterpret_cast<const void*>(fn), smem + 1024, dev);  // beside static shared memory
+  if (e != cudaSuccess) return e;
+  return launch_ex(fn, grid, dim3(32 * kWarps), smem, st, p);
+}
+template <typename T, int D, int NH, bool kBulk>
+cudaError_t launch_int4_decode_nh(const Int4DecodeParams& p, int warps, dim3 grid, int dev, cudaStream_t st) {
+  if constexpr (i4_warps(D, NH) == 16) {
+    if (warps == 16) return launch_int4_decode_w<T, D, NH, kBulk, 16>(p, grid, dev, st);
   }
+  return launch_int4_decode_w<T, D, NH, kBulk, 8>(p, grid, dev, st);
+}
+template <typename T, int D, bool kBulk>
+cudaError_t launch_int4_decode_bulk(const Int4DecodeParams& p, int warps, dim3 grid, int dev, cudaStream_t st) {
+  switch (i4_head_tiles(p.g)) {
+    case 1: return launch_int4_decode_nh<T, D, 1, kBulk>(p, warps, grid, dev, st);
+    case 2: return launch_int4_decode_nh<T, D, 2, kBulk>(p, warps, grid, dev, st);
+  }
+  return launch_int4_decode_nh<T, D, 4, kBulk>(p, warps, grid, dev, st);
+}
+template <typename T, int D>
+cudaError_t launch_int4_decode(const Int4DecodeParams& p, int warps, dim3 grid, int dev, cudaStream_t st) {
+  if constexpr (D > 64) {  // (rows of d = 64 are 40 bytes, and begin off 16-byte boundaries)
+    if (p.sk_n == i4_row_bytes(D) && p.sv_n == i4_row_bytes(D))
+      return launch_int4_decode_bulk<T, D, true>(p, warps, grid, dev, st);
+  }
+  return launch_int4_decode_bulk<T, D, false>(p, warps, grid, dev, st);
+}
+
+// KV partition. One sequence: as many slices as are resident at once, none below a tile a warp. Several, whose lengths are
+// on the device: slices for about two rounds of CTAs, of 2 to 16 tiles a warp, that the block scheduler balances (64
+// sequences of 8,704 rows, 8 KV heads of 128: slices of 32 tiles 191 us, 64 172, 136 154, 272 162; 8 of 2,000 rows:
+// slices of 8 tiles 17.1 us, 16 and 32 14.4, 64 16.5).
+DecodePlan plan_int4(int batch, int hkv, int g, int d, int64_t rows, int splits_req, int sms) {
+  const int nh = i4_head_tiles(g), warps = i4_cta_warps(batch, hkv, rows, d, nh, sms);
+  const int per_sm = i4_warps(d, nh) / warps;
+  const int64_t tiles = rows > 0 ? cdiv(rows, kTile) : 1;
+  if (splits_req > 0) return plan_decode(batch, hkv, rows, 0, false, splits_req, per_sm, sms);
+  DecodePlan pl;
+  if (batch == 1) {
+    pl = plan_decode(1, hkv, rows, 0, false, 0, per_sm, sms);
+    if (pl.tps < warps) pl.tps = warps;
+  } else {
+    const int64_t share = (int64_t)batch * hkv * tiles / (2 * (int64_t)sms * per_sm);
+    pl.tps = share < 2 * warps ? 2 * warps : share > 16 * warps ? 16 * warps : share;
+    if (pl.tps < cdiv(tiles, kMaxSplits)) pl.tps = cdiv(tiles, kMaxSplits);
+  }
+  pl.max_splits = cdiv(tiles, pl.tps);
   return pl;
 }
 
@@ -105,7 +131,8 @@ int run_int4_decode(Int4DecodeParams& p, int d, int64_t rows, float scale, int s
   p.c = scale * kLog2e;
   p.q_vec = aligned16(p.q) && stride16(p.sq_b, dtype) && stride16(p.sq_h, dtype) && stride16(p.sq_g, dtype);
   const dim3 grid((unsigned)pl.max_splits, (unsigned)p.hkv, (unsigned)p.batch);
-  const cudaError_t e = TC_INT4_DISPATCH(launch_int4_decode, dtype, d, p, grid, dev, st);
+  const cudaError_t e = TC_INT4_DISPATCH(
+      launch_int4_decode, dtype, d, p, i4_cta_warps(p.batch, p.hkv, rows, d, i4_head_tiles(p.g), sm_count(dev)), grid, dev, st);
   return e == cudaSuccess ? TC_OK : TC_ERR_CUDA;
 }
 
