@@ -36,6 +36,16 @@ struct I4<__nv_bfloat16> {
     asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
     return d;
   }
+  __device__ __forceinline__ static uint32_t max2(uint32_t a, uint32_t b) {  // NaN if either is
+    uint32_t d;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+  }
+  __device__ __forceinline__ static uint32_t min2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+  }
 };
 template <>
 struct I4<__half> {
@@ -44,6 +54,16 @@ struct I4<__half> {
   __device__ __forceinline__ static uint32_t fma2(uint32_t a, uint32_t b, uint32_t c) {
     uint32_t d;
     asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+    return d;
+  }
+  __device__ __forceinline__ static uint32_t max2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+  }
+  __device__ __forceinline__ static uint32_t min2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
     return d;
   }
 };
@@ -97,17 +117,6 @@ __device__ __forceinline__ uint32_t i4_ones(uint32_t w) {
   }
 }
 
-__device__ __forceinline__ float min_nan(float a, float b) {
-  float d;
-  asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-  return d;
-}
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float d;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-  return d;
-}
-
 template <typename X>
 __device__ __forceinline__ void load8(const X* p, float (&x)[8]) {
   constexpr int V = 16 / sizeof(X);
@@ -121,53 +130,57 @@ __device__ __forceinline__ void load8(const X* p, float (&x)[8]) {
   }
 }
 
-// Codes of this lane's 8 elements (values of T) of a group that four neighbouring lanes (aligned to 4) hold, and
-// the group's (S, z). Every lane of the warp calls it.
-// The nearest level is found through the reciprocal of a step, and decided by the exact distance from it: many
-// elements of coarse 16-bit data lie on a border between two levels, where the reciprocal's error would show.
+// x / 0.9375, correctly rounded: a product with the rounded reciprocal, corrected by its exact remainder (Markstein 1990).
+__device__ __forceinline__ float by_15_16(float x) {
+  constexpr float kUnit = 16.f / 15.f;
+  const float q = x * kUnit;
+  return fmaf(fmaf(-q, 0.9375f, x), kUnit, q);
+}
+
+// Codes of this lane's 8 elements (w: pairs of T) of a group that four neighbouring lanes (aligned to 4) hold, and the
+// group's (S, z). Every lane of the warp calls it.
+// The extremes as packed maxima and minima. A code is 15 u rounded, u = (16/15) (x - z) / S - 16/15 saturated into [0, 1] as the
+// fma goes. Many elements of coarse 16-bit data lie exactly on a border between two levels, and the even one is theirs: 15 u is
+// off by 7e-6 at most (1 ulp of the reciprocal, two roundings, times 2.1 * 15), so it is first rounded to a multiple of
+// 2^-16, which a border is. (An element 2^-17 of a level beside one counts as on it.) Nearly all of that runs on the fma pipe;
+// the codes are collected as the floats' bits, whose exponents add up to a constant.
+// With the border decided by the exact remainder, comparisons and fp32 extremes instead, a 16,384-token prompt of 48 heads of
+// 128 took 45 instructions an element and 170 us.
 template <typename T>
-__device__ __forceinline__ uint32_t quantise8(const float (&x)[8], uint32_t& param) {
-  float lo = x[0], hi = x[0];
-#pragma unroll
-  for (int e = 1; e < 8; ++e) {
-    lo = min_nan(lo, x[e]);
-    hi = max_nan(hi, x[e]);
+__device__ __forceinline__ uint32_t quantise8(const uint32_t (&w)[4], uint32_t& param) {
+  const uint32_t hi2 = I4<T>::max2(I4<T>::max2(w[0], w[1]), I4<T>::max2(w[2], w[3]));
+  const uint32_t lo2 = I4<T>::min2(I4<T>::min2(w[0], w[1]), I4<T>::min2(w[2], w[3])) ^ 0x80008000u;
+  uint32_t m = I4<T>::max2(i4_low2(hi2, lo2), i4_high2(hi2, lo2));  // (largest, largest negative)
+  m = I4<T>::max2(m, __shfl_xor_sync(0xffffffffu, m, 1));
+  m = I4<T>::max2(m, __shfl_xor_sync(0xffffffffu, m, 2));
+  const float hi = Mma<T>::lo(m), lo = -Mma<T>::hi(m);
+  const uint32_t st = Mma<T>::pack(by_15_16(__fsub_rn(hi, lo)), 0.f);
+  float s = Mma<T>::lo(st);
+  const uint32_t both = Mma<T>::pack(s, __fsub_rn(lo, s));
+  float z = Mma<T>::hi(both);
+  param = fabsf(z) == INFINITY ? both | 0x7fffu : both;  // S NaN: a finite S would leave infinities that look like data
+  float by = 1.f;
+  if constexpr (I4<T>::kBit == 3) {
+    // where (in bf16) the reciprocal or x - z would overflow: the same levels, a power of two larger or smaller
+    by = s < 1e-30f ? 18446744073709551616.f : s > 1e30f ? 1.f / 18446744073709551616.f : 1.f;
+    s *= by;
+    z *= by;
   }
-#pragma unroll
-  for (int o = 1; o < 4; o <<= 1) {
-    lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-  }
-  const T st = from_f32<T>(__fdiv_rn(__fsub_rn(hi, lo), 0.9375f));
-  float s = to_f32(st);
-  const T zt = from_f32<T>(__fsub_rn(lo, s));
-  float z = to_f32(zt);
-  uint16_t sb, zb;
-  memcpy(&sb, &st, 2);
-  memcpy(&zb, &zt, 2);
-  if (fabsf(z) == INFINITY) sb = 0x7fffu;  // NaN: a finite S would leave infinities that look like data
-  param = (uint32_t)sb | ((uint32_t)zb << 16);
-  // (bf16) where the reciprocal or x - z would overflow: the same levels, a power of two larger or smaller
-  const float by = s < 1e-30f ? 18446744073709551616.f : s > 1e30f ? 1.f / 18446744073709551616.f : 1.f;
-  s *= by;
-  z *= by;
-  const float r = s > 0.f ? __fdividef(16.f, s) : 0.f;
-  const float step = 0.0625f * s, half = 0.03125f * s;
+  constexpr float kUnit = 16.f / 15.f;
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
+  r = s > 0.f ? kUnit * r : 0.f;
   constexpr float kWhole = 12582912.f;  // 1.5 * 2^23: adding it leaves a whole number in the low bits
-  uint32_t word = 0;
+  constexpr float kSnap = 192.f;        // 1.5 * 2^7: adding it leaves multiples of 2^-16
+  uint32_t word = 0u - 0x4b400000u * 0x11111111u;  // the bits of kWhole, as often as they come in
+  uint32_t sum = 0u;
 #pragma unroll
   for (int e = 7; e >= 0; --e) {
-    const float t = fmaf(x[e], by, -z);  // by 1: x - z
-    const float y = fmaf(t, r, kWhole);
-    float k = y - kWhole;  // 16 + code, or its neighbour near a border
-    const float off = fmaf(-k, step, t);
-    const bool odd = __float_as_uint(y) & 1u;
-    if (odd ? off >= half : off > half) k += 1.f;
-    if (odd ? off <= -half : off < -half) k -= 1.f;
-    k = fminf(fmaxf(k, 16.f), 31.f);
-    word = (word << 4) | (__float_as_uint(k + kWhole) & 15u);
+    const float x = e & 1 ? Mma<T>::hi(w[e / 2]) : Mma<T>::lo(w[e / 2]);
+    const float u = __saturatef(fmaf(I4<T>::kBit == 3 ? fmaf(x, by, -z) : x - z, r, -kUnit));  // NaN gives 0
+    sum = sum * 16u + __float_as_uint(fmaf(u, 15.f, kSnap) + (kWhole - kSnap));
   }
-  return word;
+  return sum + word;
 }
 
 // ------------------------------------------------------------------------------------------------ writing
@@ -191,13 +204,27 @@ struct Int4AppendParams {
   float eps, inv_d;
 };
 
-// A lane holds 8 neighbouring elements of a row, so a row is D/8 lanes, a group four of them, and a warp 256/D
-// heads of one token, all of them queries, keys or values. The elements that an element is rotated with are
-// loaded a second time (they are in L1: another lane of the row holds them). Arithmetic of the rotation as
-// elementary fp32 operations give it (no contraction), then one rounding to T, whose result is quantised (keys)
-// or stored (queries).
-// kVec: rows, tables and weights on 16-byte boundaries, rot a multiple of 16.
-template <typename T, typename TT, int D, bool kVec>
+// Rotation of 8 elements (fp32, first element i0) with the 8 they are paired with, by elementary fp32 operations (no
+// contraction), rounded to T; elements from rot on pass through.
+template <typename T>
+__device__ __forceinline__ void rotate8(const float (&x)[8], const float (&y)[8], const float (&cs)[8], const float (&sn)[8],
+                                        int i0, int rot, uint32_t (&w)[4]) {
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    float o[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int i = i0 + e + u;
+      const float a = __fmul_rn(x[e + u], cs[e + u]), b = __fmul_rn(y[e + u], sn[e + u]);
+      o[u] = i >= rot ? x[e + u] : i < rot / 2 ? __fsub_rn(a, b) : __fadd_rn(a, b);
+    }
+    w[e / 2] = Mma<T>::pack(o[0], o[1]);
+  }
+}
+
+// Any strides, alignment and rot: a lane holds 8 neighbouring elements of a row, loaded one by one, so a row is D/8 lanes and a
+// group four of them; a warp takes 256/D heads of one token, all of them queries, keys or values.
+template <typename T, typename TT, int D>
 __global__ void __launch_bounds__(256) int4_append_kernel(const __grid_constant__ Int4AppendParams p) {
   constexpr int L = D / 8;
   constexpr int RW = 32 / L;
@@ -223,93 +250,41 @@ __global__ void __launch_bounds__(256) int4_append_kernel(const __grid_constant_
       use = use && page >= 0 && page < p.num_pages && r >= 0 && r < p.page_rows;
       row = (isv ? p.vp : p.kp) + page * p.s_page + h * p.s_h + r * p.s_row;
     }
-    float x[8], o[8];
+    const int rot = isv ? 0 : p.rot;
+    const T* w = static_cast<const T*>(isq ? p.q_w : isv ? nullptr : p.k_w);
+    const TT* ct = static_cast<const TT*>(p.cos_t) + tok * p.cos_st;
+    const TT* st = static_cast<const TT*>(p.sin_t) + tok * p.sin_st;
+    float x[8], y[8], cs[8], sn[8], ss = 0.f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = 0.f;
-    if (use) {
-      if constexpr (kVec) {
-        load8(src + i0, x);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = to_f32(src[i0 + e]);
-      }
+    for (int e = 0; e < 8; ++e) {
+      const int i = i0 + e;
+      const bool turns = use && i < rot;
+      x[e] = use ? to_f32(src[i]) : 0.f;
+      y[e] = turns ? to_f32(src[i < rot / 2 ? i + rot / 2 : i - rot / 2]) : 0.f;
+      cs[e] = turns ? to_f32(ct[i]) : 0.f;
+      sn[e] = turns ? to_f32(st[i]) : 0.f;
+      ss += x[e] * x[e];
     }
-    if (isv) {
+    if (w != nullptr) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) o[e] = x[e];
-    } else {
-      const T* w = static_cast<const T*>(isq ? p.q_w : p.k_w);
-      const int half = p.rot / 2;
-      float y[8], cs[8], sn[8], r = 1.f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        y[e] = sn[e] = 0.f;
-        cs[e] = 1.f;
-      }
-      const TT* ct = static_cast<const TT*>(p.cos_t) + tok * p.cos_st;
-      const TT* st = static_cast<const TT*>(p.sin_t) + tok * p.sin_st;
-      // the partner of element i: i + half in the first half, i - half in the second
-      if constexpr (kVec) {
-        if (use && i0 < p.rot) {
-          load8(src + (i0 < half ? i0 + half : i0 - half), y);
-          load8(ct + i0, cs);
-          load8(st + i0, sn);
-        }
-      } else {
-        if (use) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int i = i0 + e;
-            if (i < p.rot) {
-              y[e] = to_f32(src[i < half ? i + half : i - half]);
-              cs[e] = to_f32(ct[i]);
-              sn[e] = to_f32(st[i]);
-            }
-          }
-        }
-      }
-      if (w != nullptr) {
-        float ss = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) ss += x[e] * x[e];
-#pragma unroll
-        for (int a = 1; a < L; a <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, a);
-        r = rsqrtf(ss * p.inv_d + p.eps);
-        float wx[8], wy[8];
-        if constexpr (kVec) {
-          load8(w + i0, wx);
-          load8(w + (i0 >= p.rot ? i0 : i0 < half ? i0 + half : i0 - half), wy);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int i = i0 + e;
-            wx[e] = to_f32(w[i]);
-            wy[e] = to_f32(w[i >= p.rot ? i : i < half ? i + half : i - half]);
-          }
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          x[e] = x[e] * r * wx[e];
-          y[e] = y[e] * r * wy[e];
-        }
-      }
+      for (int a = 1; a < L; a <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, a);
+      const float r = rsqrtf(ss * p.inv_d + p.eps);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const int i = i0 + e;
-        const float turned = __fadd_rn(__fmul_rn(x[e], cs[e]), __fmul_rn(i < half ? -y[e] : y[e], sn[e]));
-        o[e] = to_f32(from_f32<T>(i < p.rot ? turned : x[e]));
+        x[e] = x[e] * r * to_f32(w[i]);
+        if (i < rot) y[e] = y[e] * r * to_f32(w[i < rot / 2 ? i + rot / 2 : i - rot / 2]);
       }
     }
+    uint32_t o[4];
+    rotate8<T>(x, y, cs, sn, i0, rot, o);
     if (isq) {
       if (use) {
+        T v[8];
+        memcpy(v, o, 16);
         T* out = static_cast<T*>(p.q_out) + h * p.qo_sh + tok * p.qo_st + i0;
-        if constexpr (kVec) {
-          *reinterpret_cast<uint4*>(out) = make_uint4(Mma<T>::pack(o[0], o[1]), Mma<T>::pack(o[2], o[3]),
-                                                      Mma<T>::pack(o[4], o[5]), Mma<T>::pack(o[6], o[7]));
-        } else {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) out[e] = from_f32<T>(o[e]);
-        }
+        for (int e = 0; e < 8; ++e) out[e] = v[e];
       }
       continue;
     }
@@ -319,6 +294,141 @@ __global__ void __launch_bounds__(256) int4_append_kernel(const __grid_constant_
       *reinterpret_cast<uint32_t*>(row + 4 * c) = word;
       if ((c & 3) == 0) *reinterpret_cast<uint32_t*>(row + D / 2 + c) = param;
     }
+  }
+}
+
+// Rows, tables and weights on 16-byte boundaries, rot a multiple of 16: the same with 16-byte accesses. A warp stays with its
+// heads (256/D times U of them, queries, keys or values) and goes through tokens; a lane has the same 8 elements of U heads,
+// for which it converts a token's cos and sin once. The elements that it rotates them with are loaded a second time (they are
+// in L1: another lane of the row holds them).
+// kKind: 0 queries, 1 keys, 2 values. kNorm: with a norm weight.
+template <typename T, typename TT, int D, int U, int kKind, bool kNorm>
+__device__ __forceinline__ void append_tokens(const Int4AppendParams& p, int grp, uint32_t tok0, uint32_t step) {
+  constexpr int L = D / 8;
+  constexpr int RW = 32 / L;
+  const int lane = threadIdx.x & 31, c = lane % L, i0 = 8 * c;
+  const int h0 = grp * RW * U + lane / L, heads = kKind == 0 ? p.hq : p.hkv;
+  const int64_t sh = kKind == 0 ? p.q_sh : kKind == 1 ? p.k_sh : p.v_sh;
+  const int64_t st = kKind == 0 ? p.q_st : kKind == 1 ? p.k_st : p.v_st;
+  const T* src0 = static_cast<const T*>(kKind == 0 ? p.q : kKind == 1 ? p.k : p.v) + h0 * sh + i0;
+  const bool turns = kKind < 2 && i0 < p.rot;
+  const bool first = i0 < p.rot / 2;
+  const int other = turns ? (first ? p.rot / 2 : -(p.rot / 2)) : 0;  // where its elements' partners are
+  const T* w = static_cast<const T*>(kKind == 0 ? p.q_w : p.k_w);
+  for (uint32_t tok = tok0; tok < p.t; tok += step) {
+    const T* src = src0 + tok * st;
+    uint4 a[U], b[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      a[u] = b[u] = make_uint4(0u, 0u, 0u, 0u);
+      if (h0 + u * RW < heads) {
+        a[u] = *reinterpret_cast<const uint4*>(src + u * RW * sh);
+        if (turns) b[u] = *reinterpret_cast<const uint4*>(src + u * RW * sh + other);
+      }
+    }
+    uint8_t* row = nullptr;
+    if constexpr (kKind > 0) {
+      const int2 slot = *reinterpret_cast<const int2*>(p.slots + 2 * (int64_t)tok);
+      if (slot.x >= 0 && slot.x < p.num_pages && slot.y >= 0 && slot.y < p.page_rows)
+        row = (kKind == 1 ? p.kp : p.vp) + slot.x * p.s_page + slot.y * p.s_row + h0 * p.s_h;
+    }
+    float2 cs[4], sn[4];
+    if constexpr (kKind < 2) {
+      if (turns) {
+        float x[8], y[8];
+        load8(static_cast<const TT*>(p.cos_t) + tok * p.cos_st + i0, x);
+        load8(static_cast<const TT*>(p.sin_t) + tok * p.sin_st + i0, y);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          cs[e] = make_float2(x[2 * e], x[2 * e + 1]);
+          sn[e] = first ? make_float2(-y[2 * e], -y[2 * e + 1]) : make_float2(y[2 * e], y[2 * e + 1]);
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      uint32_t o[4] = {a[u].x, a[u].y, a[u].z, a[u].w};
+      if constexpr (kKind < 2) {
+        const uint32_t q[4] = {b[u].x, b[u].y, b[u].z, b[u].w};
+        float2 x[4], y[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x[e] = make_float2(Mma<T>::lo(o[e]), Mma<T>::hi(o[e]));
+          y[e] = make_float2(Mma<T>::lo(q[e]), Mma<T>::hi(q[e]));
+        }
+        if constexpr (kNorm) {
+          float2 s2 = fmul2(x[0], x[0]);
+#pragma unroll
+          for (int e = 1; e < 4; ++e) s2 = ffma2(x[e], x[e], s2);
+          float ss = s2.x + s2.y;
+#pragma unroll
+          for (int i = 1; i < L; i <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, i);
+          const float r = rsqrtf(ss * p.inv_d + p.eps);
+          float wx[8], wy[8];
+          load8(w + i0, wx);
+          load8(w + i0 + other, wy);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            x[e] = fmul2(fmul2(x[e], make_float2(r, r)), make_float2(wx[2 * e], wx[2 * e + 1]));
+            y[e] = fmul2(fmul2(y[e], make_float2(r, r)), make_float2(wy[2 * e], wy[2 * e + 1]));
+            if (!turns) o[e] = Mma<T>::pack(x[e].x, x[e].y);
+          }
+        }
+        if (turns) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            // (not packed: those products and sums are contracted)
+            o[e] = Mma<T>::pack(__fadd_rn(__fmul_rn(x[e].x, cs[e].x), __fmul_rn(y[e].x, sn[e].x)),
+                                __fadd_rn(__fmul_rn(x[e].y, cs[e].y), __fmul_rn(y[e].y, sn[e].y)));
+          }
+        }
+      }
+      if constexpr (kKind == 0) {
+        if (h0 + u * RW < heads)
+          *reinterpret_cast<uint4*>(static_cast<T*>(p.q_out) + tok * p.qo_st + (h0 + u * RW) * p.qo_sh + i0) =
+              make_uint4(o[0], o[1], o[2], o[3]);
+      } else {
+        uint32_t param;
+        const uint32_t word = quantise8<T>(o, param);
+        if (row != nullptr && h0 + u * RW < heads) {
+          uint8_t* at = row + u * RW * p.s_h;
+          *reinterpret_cast<uint32_t*>(at + 4 * c) = word;
+          if ((c & 3) == 0) *reinterpret_cast<uint32_t*>(at + D / 2 + c) = param;
+        }
+      }
+    }
+  }
+}
+
+// Keys and values take about twice the instructions of queries, so a warp has half as many of them.
+__host__ __device__ constexpr int i4_kv_heads(int u) { return u > 1 ? u / 2 : 1; }
+// Resident CTAs an SM: what spills nothing.
+__host__ __device__ constexpr int i4_append_ctas(int u, bool norm) { return u > 1 && norm ? 2 : 3; }
+
+template <typename T, typename TT, int D, int U, bool kNorm>
+__global__ void __launch_bounds__(256, i4_append_ctas(U, kNorm)) int4_append_vec_kernel(const __grid_constant__ Int4AppendParams p) {
+  constexpr int KU = i4_kv_heads(U);
+  constexpr int QW = 256 / D * U, KW = 256 / D * KU;
+  pdl_launch();
+  pdl_wait();
+  const int q_groups = (p.hq + QW - 1) / QW, kv_groups = (p.hkv + KW - 1) / KW;
+  const uint32_t groups = q_groups + 2 * kv_groups;
+  const uint32_t warp = blockIdx.x * 8 + (threadIdx.x >> 5), step = gridDim.x * 8 / groups;  // warps of a group
+  const uint32_t tok0 = warp / groups;
+  if (tok0 >= step) return;
+  const int grp = (int)(warp - tok0 * groups);
+  if (grp < q_groups) {
+    if (kNorm && p.q_w != nullptr)
+      append_tokens<T, TT, D, U, 0, true>(p, grp, tok0, step);
+    else
+      append_tokens<T, TT, D, U, 0, false>(p, grp, tok0, step);
+  } else if (grp < q_groups + kv_groups) {
+    if (kNorm && p.k_w != nullptr)
+      append_tokens<T, TT, D, KU, 1, true>(p, grp - q_groups, tok0, step);
+    else
+      append_tokens<T, TT, D, KU, 1, false>(p, grp - q_groups, tok0, step);
+  } else {
+    append_tokens<T, TT, D, KU, 2, false>(p, grp - q_groups - kv_groups, tok0, step);
   }
 }
 
@@ -337,12 +447,15 @@ struct Int4GatherParams {
   int64_t n_tiles;
 };
 
-// A warp per (tile, head): a lane turns one word of a key row and of the value row beside it into 16 bytes
-// each, a row being D/8 lanes.
+// A warp per (tile, head): a lane turns one word of a key row and of the value row beside it into 16 bytes each, a row
+// being D/8 lanes. kI4Ahead rows' words are loaded before any is turned.
+constexpr int kI4Ahead = 4;
+
 template <typename T, int D>
-__global__ void __launch_bounds__(256) int4_gather_kernel(const __grid_constant__ Int4GatherParams p) {
+__global__ void __launch_bounds__(256, 4) int4_gather_kernel(const __grid_constant__ Int4GatherParams p) {
   constexpr int L = D / 8;
   constexpr int RW = 32 / L;  // rows a warp takes at a time
+  constexpr int A = kI4Ahead;
   pdl_launch();
   pdl_wait();
   const int lane = threadIdx.x & 31, c = lane % L;
@@ -353,23 +466,37 @@ __global__ void __launch_bounds__(256) int4_gather_kernel(const __grid_constant_
     const int4 te = *reinterpret_cast<const int4*>(p.tiles + 4 * tile);
     if (te.x < 0 || te.x >= p.num_pages) continue;
     const int rows = te.z < kI4TileRows ? te.z : kI4TileRows;
-    const int64_t base = te.x * p.s_page + h * p.s_h;
-#pragma unroll 4
-    for (int r = lane / L; r < rows; r += RW) {
-      const int64_t pr = (int64_t)te.y + r, pos = (int64_t)te.w + r;
-      if (pr < 0 || pr >= p.page_rows || pos < 0 || pos >= p.n) continue;
-      const uint8_t* kr = p.kp + base + pr * p.s_row;
-      const uint8_t* vr = p.vp + base + pr * p.s_row;
-      const uint32_t kw = *reinterpret_cast<const uint32_t*>(kr + 4 * c);
-      const uint32_t vw = *reinterpret_cast<const uint32_t*>(vr + 4 * c);
-      const uint32_t kq = *reinterpret_cast<const uint32_t*>(kr + D / 2 + 4 * (c / 4));
-      const uint32_t vq = *reinterpret_cast<const uint32_t*>(vr + D / 2 + 4 * (c / 4));
-      uint32_t k4[4], v4[4];
-      i4_values<T>(kw, kq, k4);
-      i4_values<T>(vw, vq, v4);
-      const int64_t o = h * p.out_sh + pos * p.out_sn + 8 * c;
-      *reinterpret_cast<uint4*>(static_cast<T*>(p.k_out) + o) = make_uint4(k4[0], k4[1], k4[2], k4[3]);
-      *reinterpret_cast<uint4*>(static_cast<T*>(p.v_out) + o) = make_uint4(v4[0], v4[1], v4[2], v4[3]);
+    const int64_t base = te.x * p.s_page + h * p.s_h + te.y * p.s_row;
+    const int64_t out = h * p.out_sh + te.w * p.out_sn + 8 * c;
+#pragma unroll 1
+    for (int r0 = lane / L; r0 < rows; r0 += A * RW) {
+      uint32_t kw[A], vw[A], kq[A], vq[A];
+      bool use[A];
+#pragma unroll
+      for (int u = 0; u < A; ++u) {
+        const int r = r0 + u * RW;
+        const int64_t pr = (int64_t)te.y + r, pos = (int64_t)te.w + r;
+        use[u] = r < rows && pr >= 0 && pr < p.page_rows && pos >= 0 && pos < p.n;
+        if (use[u]) {
+          const uint8_t* kr = p.kp + base + r * p.s_row;
+          const uint8_t* vr = p.vp + base + r * p.s_row;
+          kw[u] = *reinterpret_cast<const uint32_t*>(kr + 4 * c);
+          vw[u] = *reinterpret_cast<const uint32_t*>(vr + 4 * c);
+          kq[u] = *reinterpret_cast<const uint32_t*>(kr + D / 2 + 4 * (c / 4));
+          vq[u] = *reinterpret_cast<const uint32_t*>(vr + D / 2 + 4 * (c / 4));
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < A; ++u) {
+        if (use[u]) {
+          const int64_t o = out + (r0 + u * RW) * p.out_sn;
+          uint32_t x[4];
+          i4_values<T>(kw[u], kq[u], x);
+          *reinterpret_cast<uint4*>(static_cast<T*>(p.k_out) + o) = make_uint4(x[0], x[1], x[2], x[3]);
+          i4_values<T>(vw[u], vq[u], x);
+          *reinterpret_cast<uint4*>(static_cast<T*>(p.v_out) + o) = make_uint4(x[0], x[1], x[2], x[3]);
+        }
+      }
     }
   }
 }
@@ -388,19 +515,24 @@ struct Int4RotateParams {
 
 // Keys re-rotated in place by one angle a frequency (the splice of threadcut/kv.py:28-41 over 4-bit rows): a row's
 // values, rotated in fp32 as the 16-bit splice rotates them, rounded to T and quantised again. A warp per
-// (layer, tile, head); a row is D/8 lanes, the partner's values come from the lane half a row away.
+// (layer, tile, head); a row is D/8 lanes, the partner's values come from the lane half a row away. kI4Ahead rows' words are
+// loaded before any is turned. Bound by instructions (29 an element).
 template <typename T, int D>
-__global__ void __launch_bounds__(256) int4_rotate_kernel(const __grid_constant__ Int4RotateParams p) {
+__global__ void __launch_bounds__(256, 3) int4_rotate_kernel(const __grid_constant__ Int4RotateParams p) {
   constexpr int L = D / 8;
   constexpr int RW = 32 / L;
+  constexpr int A = kI4Ahead;
+  __shared__ float s_cs[D];
+  for (int i = threadIdx.x; i < D; i += blockDim.x) s_cs[i] = p.cs[i];
+  __syncthreads();
   const int lane = threadIdx.x & 31, c = lane % L;
   const bool first = c < L / 2;
   float cs[8], sn[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     const int i = 8 * (c % (L / 2)) + e;
-    cs[e] = p.cs[i];
-    sn[e] = first ? -p.cs[D / 2 + i] : p.cs[D / 2 + i];
+    cs[e] = s_cs[i];
+    sn[e] = first ? -s_cs[D / 2 + i] : s_cs[D / 2 + i];
   }
   pdl_launch();
   pdl_wait();
@@ -412,34 +544,45 @@ __global__ void __launch_bounds__(256) int4_rotate_kernel(const __grid_constant_
     const int64_t tile = th / p.hkv;
     const int h = (int)(th - tile * p.hkv);
     const int32_t* te = p.tiles + p.tile_cols * tile;
-    const int64_t page = te[0], r0 = te[1];
+    const int64_t page = te[0], first_row = te[1];
     const int rows = te[2] < kI4TileRows ? te[2] : kI4TileRows;
     if (page < 0 || page >= p.num_pages) continue;
-    uint8_t* base = p.kp[layer] + page * p.s_page + h * p.s_h;
-#pragma unroll 2
-    for (int rb = 0; rb < rows; rb += RW) {  // the whole warp: the lanes exchange values
-      const int64_t pr = r0 + rb + lane / L;
-      const bool use = rb + lane / L < rows && pr >= 0 && pr < p.page_rows;
-      uint8_t* row = base + pr * p.s_row;
-      uint32_t v[4] = {0u, 0u, 0u, 0u}, u[4];
-      if (use)
-        i4_values<T>(*reinterpret_cast<const uint32_t*>(row + 4 * c),
-                     *reinterpret_cast<const uint32_t*>(row + D / 2 + 4 * (c / 4)), v);
+    uint8_t* base = p.kp[layer] + page * p.s_page + h * p.s_h + first_row * p.s_row;
+#pragma unroll 1
+    for (int r0 = 0; r0 < rows; r0 += A * RW) {  // the whole warp: the lanes exchange values
+      uint32_t word[A], param[A];
+      bool use[A];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) u[i] = __shfl_xor_sync(0xffffffffu, v[i], L / 2);
-      float o[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float x = e & 1 ? Mma<T>::hi(v[e / 2]) : Mma<T>::lo(v[e / 2]);
-        const float y = e & 1 ? Mma<T>::hi(u[e / 2]) : Mma<T>::lo(u[e / 2]);
-        o[e] = to_f32(from_f32<T>(__fadd_rn(__fmul_rn(x, cs[e]), __fmul_rn(y, sn[e]))));
+      for (int u = 0; u < A; ++u) {
+        const int r = r0 + u * RW + lane / L;
+        const int64_t pr = first_row + r;
+        use[u] = r < rows && pr >= 0 && pr < p.page_rows;
+        word[u] = param[u] = 0u;
+        if (use[u]) {
+          word[u] = *reinterpret_cast<const uint32_t*>(base + r * p.s_row + 4 * c);
+          param[u] = *reinterpret_cast<const uint32_t*>(base + r * p.s_row + D / 2 + 4 * (c / 4));
+        }
       }
-      uint32_t param;
-      const uint32_t word = quantise8<T>(o, param);
-      // every lane of the row has read it: the exchange above waited for them
-      if (use) {
-        *reinterpret_cast<uint32_t*>(row + 4 * c) = word;
-        if ((c & 3) == 0) *reinterpret_cast<uint32_t*>(row + D / 2 + c) = param;
+#pragma unroll
+      for (int u = 0; u < A; ++u) {
+        if (r0 + u * RW >= rows) break;  // (the same for every lane)
+        uint32_t v[4], y[4], o[4];
+        i4_values<T>(word[u], param[u], v);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = __shfl_xor_sync(0xffffffffu, v[i], L / 2);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          o[e] = Mma<T>::pack(
+              __fadd_rn(__fmul_rn(Mma<T>::lo(v[e]), cs[2 * e]), __fmul_rn(Mma<T>::lo(y[e]), sn[2 * e])),
+              __fadd_rn(__fmul_rn(Mma<T>::hi(v[e]), cs[2 * e + 1]), __fmul_rn(Mma<T>::hi(y[e]), sn[2 * e + 1])));
+        uint32_t q;
+        const uint32_t w = quantise8<T>(o, q);
+        // every lane of the row has read it: the exchange above waited for them
+        if (use[u]) {
+          uint8_t* row = base + (r0 + u * RW + lane / L) * p.s_row;
+          *reinterpret_cast<uint32_t*>(row + 4 * c) = w;
+          if ((c & 3) == 0) *reinterpret_cast<uint32_t*>(row + D / 2 + c) = q;
+        }
       }
     }
   }

@@ -26,14 +26,29 @@ bool i4_pool(int hkv, int d, int64_t page_rows, int64_t num_pages) {
                          : (d) == 128 ? fn<__half, 128>(__VA_ARGS__)                                            \
                                       : fn<__half, 256>(__VA_ARGS__)))
 
+template <typename T, int D, int U>
+cudaError_t launch_int4_append_vec(const Int4AppendParams& p, bool table_f32, int sms, cudaStream_t st) {
+  const int64_t groups = cdiv(p.hq, 256 / D * U) + 2 * cdiv(p.hkv, 256 / D * i4_kv_heads(U));
+  // warps of a token's groups, the tokens shared out evenly over those that are resident at once
+  const bool norm = p.q_w != nullptr || p.k_w != nullptr;
+  const int64_t resident = (int64_t)sms * 8 * i4_append_ctas(U, norm) / groups;
+  const int64_t rounds = cdiv(p.t, resident < 1 ? 1 : resident);
+  const dim3 grid((unsigned)cdiv(cdiv(p.t, rounds) * groups, 8));
+  auto fn = table_f32 ? (norm ? int4_append_vec_kernel<T, float, D, U, true> : int4_append_vec_kernel<T, float, D, U, false>)
+                      : (norm ? int4_append_vec_kernel<T, T, D, U, true> : int4_append_vec_kernel<T, T, D, U, false>);
+  return launch_ex(fn, grid, dim3(256), 0, st, p);
+}
+
 template <typename T, int D>
 cudaError_t launch_int4_append(const Int4AppendParams& p, bool table_f32, bool vec, int sms, cudaStream_t st) {
   constexpr int RW = 256 / D;
   const int64_t warps = p.t * (cdiv(p.hq, RW) + 2 * cdiv(p.hkv, RW));
-  const int64_t blocks = cdiv(warps, 8) < (int64_t)sms * 64 ? cdiv(warps, 8) : (int64_t)sms * 64;
-  auto fn = table_f32 ? (vec ? int4_append_kernel<T, float, D, true> : int4_append_kernel<T, float, D, false>)
-                      : (vec ? int4_append_kernel<T, T, D, true> : int4_append_kernel<T, T, D, false>);
-  return launch_ex(fn, dim3((unsigned)blocks), dim3(256), 0, st, p);
+  if (vec)
+    return warps < (int64_t)sms * 64 ? launch_int4_append_vec<T, D, 1>(p, table_f32, sms, st)
+                                     : launch_int4_append_vec<T, D, 4>(p, table_f32, sms, st);
+  const int64_t blocks = cdiv(warps, 8);
+  return launch_ex(table_f32 ? int4_append_kernel<T, float, D> : int4_append_kernel<T, T, D>,
+                   dim3((unsigned)(blocks < (int64_t)sms * 64 ? blocks : (int64_t)sms * 64)), dim3(256), 0, st, p);
 }
 
 template <typename T, int D>
@@ -234,7 +249,7 @@ int tc_int4_append_rope(const void* q, const void* k, const void* v, void* q_out
   if (rot > 0)
     vec = vec && aligned16(cos_t) && aligned16(sin_t) && stride16(cos_stride_t, table_dtype) &&
           stride16(sin_stride_t, table_dtype);
-  vec = vec && aligned16(q_norm_weight) && aligned16(k_norm_weight);
+  vec = vec && aligned16(q_norm_weight) && aligned16(k_norm_weight) && (reinterpret_cast<uintptr_t>(slots) & 7u) == 0;
   const cudaError_t e = TC_INT4_DISPATCH(launch_int4_append, dtype, d, p, table_dtype == TC_F32, vec,
                                          sm_count(current_device()), static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? TC_OK : TC_ERR_CUDA;
