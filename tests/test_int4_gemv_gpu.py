@@ -14,13 +14,19 @@ def randn(*shape, dtype, seed=0, scale=1.0):
 
 
 def bound(x, w, out):
-    """Products are exact; S P + z X takes sums of up to 16 columns an instruction, then of groups and of 8 parts, each
-    off by 2^-23 of what has been added up so far (|x| (2 S + |z|) at most); one rounding to the output's type."""
+    """Sums of products are off by 2^-23 of what has been added up (|x| (2 S + |z|) at most) for each of their steps: 16 or
+    64 columns, then groups, then up to 16 parts. One or two tokens enter as whole numbers of at most 1 / 524,288 of the
+    largest of each 64 columns: half of that off, for an S of 15/16. One rounding to the output's type."""
     half = torch.finfo(out.dtype).eps / 2
     p = w.params.double().permute(0, 3, 2, 1, 4).reshape(-1, w.params.shape[1], 2)[:w.n]
-    size = (2 * p[..., 0] + p[..., 1].abs()).repeat_interleave(w.group, 1)[:, :w.k]
+    scale = p[..., 0].repeat_interleave(w.group, 1)[:, :w.k]
+    size = 2 * scale + p[..., 1].abs().repeat_interleave(w.group, 1)[:, :w.k]
     tiny = 2.0 ** -25 if out.dtype == HF else 0.0
-    return (w.k / 8 + 64) * 2.0 ** -23 * (x.double().abs() @ size.t()) * (1 + half) + half * out.double().abs() * 1.01 + tiny
+    x = x.double().abs()
+    pad = torch.nn.functional.pad(x, (0, -w.k % 64)).view(x.shape[0], -1, 64)
+    step = (pad.amax(-1, keepdim=True) / 524288).expand_as(pad).reshape(x.shape[0], -1)[:, :w.k]
+    off = (w.k / 8 + 64) * 2.0 ** -23 * (x @ size.t()) + (step / 2) @ scale.t()
+    return off * (1 + half) + half * out.double().abs() * 1.01 + tiny
 
 
 def check(got, x, w):
@@ -48,6 +54,20 @@ def test_long_rows_take_fewer_tokens_a_launch(group):
     w = quantize_weight(randn(20, 60001, dtype=BF, seed=1, scale=0.02), group)
     x = randn(3, 60001, dtype=BF, seed=2)
     check(gemv_int4(x, w), x, w)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_tokens_of_very_different_sizes(dtype):
+    w = quantize_weight(randn(300, 640, dtype=dtype, seed=1, scale=0.02), 64)
+    x = randn(2, 640, dtype=dtype, seed=2)
+    x[0, 5], x[0, 300] = 3000.0, -900.0
+    x[1] *= 2.0 ** -12
+    x[1, 64:128] = 0
+    x[1, 200] = 1.0
+    for t in (x, x[:1], x[1:]):
+        check(gemv_int4(t, w), t, w)
+    x = x * 0
+    assert not gemv_int4(x[:1], w).any()
 
 
 def test_many_rows():

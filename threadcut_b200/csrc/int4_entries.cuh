@@ -151,38 +151,57 @@ int run_int4_decode(Int4DecodeParams& p, int d, int64_t rows, float scale, int s
   return e == cudaSuccess ? TC_OK : TC_ERR_CUDA;
 }
 
-// Shared memory of a launch over m tokens.
-int64_t gv_smem(int k, int m, int group) {
-  const int64_t sums = cdiv((int64_t)gv_blocks(k) * (group == 32 ? 2 : 1) * gv_sums(m) * 4, 16) * 16;
-  return kGvWarps * kGvStages * (group == 32 ? gv_stage_bytes<32>() : gv_stage_bytes<64>()) + 2 * kGvPartBytes + sums +
-         (int64_t)m * gv_x_stride(k) * 2;
-}
-constexpr int64_t kGvMaxSmem = 227 * 1024;
+constexpr int kGvMaxSmem = 226 * 1024;
 constexpr int kGvMaxColumns = 65536;  // one token of them fits
+constexpr int kGvIntTokens = 2;       // up to these, tokens as digits
 
-template <typename T, int NT, int G>
-cudaError_t launch_int4_gemv_g(const Int4GemvParams& p, int smem, int dev, cudaStream_t st) {
-  auto fn = int4_gemv_kernel<T, NT, G>;
-  // the opt-in is set once per (kernel, device): ask for the most any plan takes
-  const cudaError_t e = set_smem(reinterpret_cast<const void*>(fn), (int)kGvMaxSmem, dev);
-  if (e != cudaSuccess) return e;
-  int per_sm = (int)(kGvMaxSmem / (smem + 1024));
-  if (per_sm < 1) per_sm = 1;
-  if (per_sm > 3) per_sm = 3;
-  const int64_t tiles = cdiv(p.n, 16), slots = (int64_t)sm_count(dev) * per_sm;
-  return launch_ex(fn, dim3((unsigned)(tiles < slots ? tiles : slots)), dim3(32 * kGvWarps), smem, st, p);
+// Two row tiles at a time, 8 warps on each, or (few row tiles) all 16 on one.
+int gv_streams(int64_t n, int sms) { return cdiv(n, 16) > 2 * (int64_t)sms ? 2 : 1; }
+int gv_part_bytes(int m, int streams) {
+  const int least = kGvWarps * 64 * m;  // a row tile of each stream
+  return least > kGvPartBytes ? least : kGvPartBytes;
 }
-template <typename T, int NT>
+// Shared memory of a launch over m tokens beside the rings.
+int64_t gv_fixed(int k, int m, int group, int streams, bool digits) {
+  return 2 * gv_part_bytes(m, streams) + gv_sum_bytes(k, m, group, digits) +
+         (int64_t)m * (digits ? kGvDigits : 1) * gv_x_bytes(k, digits);
+}
+// The largest ring that fits beside that; false where none does.
+bool gv_ring(int64_t fixed, int group, int& chunk, int& stages) {
+  const int plans[4][2] = {{4, 3}, {4, 2}, {2, 2}, {1, 2}};
+  for (const auto& p : plans) {
+    chunk = p[0];
+    stages = p[1];
+    if (fixed + (int64_t)kGvWarps * chunk * stages * gv_tile_bytes(group) <= kGvMaxSmem) return true;
+  }
+  return false;
+}
+
+template <typename T, int NT, int G, bool kInt>
+cudaError_t launch_int4_gemv_g(Int4GemvParams p, int smem, int dev, cudaStream_t st) {
+  auto fn = int4_gemv_kernel<T, NT, G, kInt>;
+  // the opt-in is set once per (kernel, device): ask for the most any plan takes
+  const cudaError_t e = set_smem(reinterpret_cast<const void*>(fn), kGvMaxSmem, dev);
+  if (e != cudaSuccess) return e;
+  const int tiles = (int)cdiv(p.n, 16), sms = sm_count(dev);
+  int ctas = (int)cdiv(tiles, p.streams);
+  if (ctas > sms) ctas = sms;
+  p.share = tiles / ctas;
+  p.more = tiles - p.share * ctas;
+  return launch_ex(fn, dim3((unsigned)ctas), dim3(32 * kGvWarps), smem, st, p);
+}
+template <typename T, int NT, bool kInt>
 cudaError_t launch_int4_gemv_nt(const Int4GemvParams& p, int group, int smem, int dev, cudaStream_t st) {
-  return group == 32   ? launch_int4_gemv_g<T, NT, 32>(p, smem, dev, st)
-         : group == 64 ? launch_int4_gemv_g<T, NT, 64>(p, smem, dev, st)
-                       : launch_int4_gemv_g<T, NT, 128>(p, smem, dev, st);
+  return group == 32   ? launch_int4_gemv_g<T, NT, 32, kInt>(p, smem, dev, st)
+         : group == 64 ? launch_int4_gemv_g<T, NT, 64, kInt>(p, smem, dev, st)
+                       : launch_int4_gemv_g<T, NT, 128, kInt>(p, smem, dev, st);
 }
 template <typename T>
-cudaError_t launch_int4_gemv(const Int4GemvParams& p, int group, int smem, int dev, cudaStream_t st) {
-  return p.m <= 8    ? launch_int4_gemv_nt<T, 1>(p, group, smem, dev, st)
-         : p.m <= 16 ? launch_int4_gemv_nt<T, 2>(p, group, smem, dev, st)
-                     : launch_int4_gemv_nt<T, 4>(p, group, smem, dev, st);
+cudaError_t launch_int4_gemv(const Int4GemvParams& p, int group, bool digits, int smem, int dev, cudaStream_t st) {
+  return digits              ? launch_int4_gemv_nt<T, 1, true>(p, group, smem, dev, st)
+         : p.m <= 8          ? launch_int4_gemv_nt<T, 1, false>(p, group, smem, dev, st)
+         : p.m <= 16         ? launch_int4_gemv_nt<T, 2, false>(p, group, smem, dev, st)
+                             : launch_int4_gemv_nt<T, 4, false>(p, group, smem, dev, st);
 }
 
 }  // namespace
@@ -417,29 +436,41 @@ int tc_gemv_int4(const void* x, const void* codes, const void* params, void* out
   if (n == 0 || m == 0) return TC_OK;
   if (x == nullptr || codes == nullptr || params == nullptr || out == nullptr) return TC_ERR_INVALID;
   if (!aligned16(codes) || !aligned16(params)) return TC_ERR_ALIGN;
-  int most = 32;  // tokens a launch, as many as fit
-  while (gv_smem(k, most, group) > kGvMaxSmem) --most;
   const int dev = current_device();
-  for (int64_t m0 = 0; m0 < m; m0 += most) {
+  const int streams = gv_streams(n, sm_count(dev));
+  for (int64_t m0 = 0; m0 < m;) {
     Int4GemvParams p;
     std::memset(&p, 0, sizeof(p));
+    // as many tokens a launch as fit, 32 at most; one always does as 16-bit numbers
+    int now = (int)(m - m0 < 32 ? m - m0 : 32);
+    bool digits = now <= kGvIntTokens;
+    while (!gv_ring(gv_fixed(k, now, group, streams, digits), group, p.chunk, p.stages)) {
+      if (digits) {
+        digits = false;
+      } else if (--now == 0) {
+        return TC_ERR_INVALID;
+      }
+    }
     p.x = static_cast<const uint16_t*>(x) + m0 * x_stride;
     p.codes = static_cast<const uint8_t*>(codes);
     p.params = params;
     p.out = static_cast<uint16_t*>(out) + m0 * out_stride;
     p.n = n;
     p.k = k;
-    p.m = (int)(m - m0 < most ? m - m0 : most);
+    p.m = now;
     p.sx = x_stride;
     p.so = out_stride;
     p.swiglu = swiglu != 0;
     p.vec = aligned16(p.x) && (p.m == 1 || stride16(x_stride, dtype)) && (!p.swiglu || k % 8 == 0);
-    p.x_stride = gv_x_stride(k);
-    p.flush = kGvPartBytes / (kGvWarps * 64 * p.m);
-    const int smem = (int)gv_smem(k, p.m, group);
-    const cudaError_t e = dtype == TC_BF16
-                              ? launch_int4_gemv<__nv_bfloat16>(p, group, smem, dev, static_cast<cudaStream_t>(stream))
-                              : launch_int4_gemv<__half>(p, group, smem, dev, static_cast<cudaStream_t>(stream));
+    p.streams = streams;
+    p.part_bytes = gv_part_bytes(p.m, streams);
+    p.flush = p.part_bytes / (kGvWarps * 64 * p.m) * streams;
+    const int smem = (int)(gv_fixed(k, now, group, streams, digits) +
+                           (int64_t)kGvWarps * p.chunk * p.stages * gv_tile_bytes(group));
+    const cudaError_t e =
+        dtype == TC_BF16 ? launch_int4_gemv<__nv_bfloat16>(p, group, digits, smem, dev, static_cast<cudaStream_t>(stream))
+                         : launch_int4_gemv<__half>(p, group, digits, smem, dev, static_cast<cudaStream_t>(stream));
+    m0 += now;
     if (e != cudaSuccess) return TC_ERR_CUDA;
   }
   return TC_OK;

@@ -6,20 +6,28 @@
 // the same); in a word, code j is column 2j and code j + 4 column 2j + 1. (S, z) as [row tile][group][r][row r | row r + 8].
 // Rows and columns behind the matrix have codes and (S, z) of 0.
 //
-// Products on the tensor cores, the weights as the 16-row operand straight from registers, the tokens as its 8
-// columns: with one token seven of them idle, which costs nothing, as the bytes of the weights are the bound.
-// 1 + code/16 goes into the product as it is; S and z are applied to the sums in fp32:
-//   sum_k x (S (1 + code/16) + z) = S P + z X,     P = sum_k x (1 + code/16),  X = sum_k x over the group's columns.
-// A warp takes every 8th tile of a row of tiles; the 8 warps' sums are added in shared memory in warp order.
+// Products on the tensor cores, a tile's weights being the 16-row operand straight from shared memory and the tokens its 8
+// columns. S and z are applied to the sums in fp32:
+//   sum_k x (S (1 + code/16) + z) = S P + (S + z) X,   P = sum_k x code/16,  X = sum_k x, over the group's columns in a tile.
+// One or two tokens: P as an integer product of the codes, bytes after two masks and a shift (12 instructions for a lane's 32
+// codes), with the digits of x, which are otherwise idle columns: x of each 64 columns, scaled by a power of two and rounded
+// to a whole number below 2^20, is 65536 h + 256 m + l. More tokens: 1 + code/16 and x as they are, 16-bit operands (24 and
+// 8; S P + z X then), 8 tokens a product.
+//
+// A CTA an SM takes neighbouring row tiles, in one or two streams of warps. A stream's warps share out the columns in
+// neighbouring runs, each bringing in its run of a row tile, and of the next ones, by bulk copies of a few tiles; their sums are
+// added in shared memory in warp order.
 #pragma once
 
 #include "int4_attn.cuh"
 
 namespace tc {
 
-constexpr int kGvWarps = 8;
-constexpr int kGvStages = 8;     // tiles in flight a warp
-constexpr int kGvPartBytes = 16 * 1024;  // one of the two buffers of sums
+constexpr int kGvWarps = 16;
+constexpr int kGvMaxStages = 3;          // of a warp's ring
+constexpr int kGvPreWait = 1;            // stages filled before the previous kernel has ended
+constexpr int kGvPartBytes = 8 * 1024;   // one of the two buffers of sums, at least a row tile's
+constexpr int kGvDigits = 3;
 
 struct Int4GemvParams {
   const void* x;  // [m][k], row stride sx (swiglu: [m][2k], gate | up)
@@ -30,84 +38,131 @@ struct Int4GemvParams {
   int k, m;
   int64_t sx, so;
   int swiglu;
-  int vec;       // x in 16-byte chunks
-  int x_stride;  // elements between the tokens' rows in shared memory
-  int flush;     // row tiles whose sums a buffer holds
+  int vec;         // x in 16-byte chunks
+  int streams;     // 1 or 2
+  int share, more; // row tiles of a CTA: share, and one more for the first `more` CTAs
+  int flush;       // row tiles whose sums a buffer holds
+  int part_bytes;  // of a buffer
+  int chunk;       // tiles a stage holds
+  int stages;
 };
 
 __host__ __device__ __forceinline__ int gv_blocks(int k) { return (k + 63) / 64; }
 
-// Elements of a token's row in shared memory: whole tiles, and 16 bytes more, so that the 8 tokens' chunks that a
-// warp reads together lie in different banks.
-__host__ __device__ __forceinline__ int gv_x_stride(int k) { return 64 * gv_blocks(k) + 8; }
-
-// Sums X kept for each group: the tokens, in pairs as a lane reads them.
+// Bytes of a token's row in shared memory. 16-bit tokens: 16 bytes beside whole tiles, so that the 8 tokens' chunks that a warp
+// reads together lie in different banks. Digits: a row for each, an odd number of 64-byte blocks.
+__host__ __device__ __forceinline__ int gv_x_bytes(int k, bool digits) {
+  return digits ? 64 * (gv_blocks(k) | 1) : 128 * gv_blocks(k) + 16;
+}
+// Tokens that sums are kept for: in pairs, as a lane reads them.
 __host__ __device__ __forceinline__ int gv_sums(int m) { return (m + 1) & ~1; }
 
-template <int G>
-__host__ __device__ constexpr int gv_stage_bytes() {
-  return 512 + (G == 32 ? 128 : 64);
+// Bytes a tile takes in a stage, its (S, z) included.
+__host__ __device__ constexpr int gv_tile_bytes(int g) { return 512 + (g == 32 ? 128 : 64); }
+// Sums X: [block of 64 columns][1 or 2 groups][token]; with digits [..][lane c of an operand's four] with a factor beside each.
+__host__ __device__ __forceinline__ int gv_sum_bytes(int k, int m, int g, bool digits) {
+  return (gv_blocks(k) * (g == 32 ? 2 : 1) * (digits ? 32 : 4 * gv_sums(m)) + 15) / 16 * 16;
 }
 
-template <typename T, int NT, int G>
-__global__ void __launch_bounds__(32 * kGvWarps) int4_gemv_kernel(const __grid_constant__ Int4GemvParams p) {
-  constexpr int kParamBytes = G == 32 ? 128 : 64;
-  constexpr int kStage = gv_stage_bytes<G>();
+__device__ __forceinline__ void mma_u8s8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Codes of two words (rows r and r + 8) as bytes: codes 0, 2, 4, 6, then 1, 3, 5, 7.
+__device__ __forceinline__ void i4_bytes(uint32_t w0, uint32_t w1, uint32_t (&a)[4]) {
+  a[0] = w0 & 0x0f0f0f0fu;
+  a[1] = w1 & 0x0f0f0f0fu;
+  a[2] = (w0 >> 4) & 0x0f0f0f0fu;
+  a[3] = (w1 >> 4) & 0x0f0f0f0fu;
+}
+// The digits (l, m, h) of 4 whole numbers below 2^20, as 4 signed bytes each. V: the numbers + 0x8080, whose bytes are the digits
+// above 128 less than themselves.
+__device__ __forceinline__ void digits4(int v0, int v1, int v2, int v3, uint32_t (&d)[kGvDigits]) {
+  d[0] = __byte_perm(__byte_perm(v0, v1, 0x0040), __byte_perm(v2, v3, 0x0040), 0x5410) ^ 0x80808080u;
+  d[1] = __byte_perm(__byte_perm(v0, v1, 0x0051), __byte_perm(v2, v3, 0x0051), 0x5410) ^ 0x80808080u;
+  d[2] = __byte_perm(__byte_perm(v0, v1, 0x0062), __byte_perm(v2, v3, 0x0062), 0x5410);
+}
+// The power of two that brings a largest magnitude into [2^19, 2^20), and its inverse; NaN as the inverse where it is not
+// finite, so that it shows.
+__device__ __forceinline__ void digit_scale(float most, float& up, float& down) {
+  int e = 146 - (int)(__float_as_uint(most) >> 23);
+  e = e > 100 ? 100 : e;
+  up = __uint_as_float((uint32_t)(127 + e) << 23);
+  down = most < INFINITY ? __uint_as_float((uint32_t)(127 - e) << 23) : __uint_as_float(0x7fffffffu);
+}
+
+// NT tiles of 8 tokens, or (kInt) up to 2 tokens as digits.
+template <typename T, int NT, int G, bool kInt>
+__global__ void __launch_bounds__(32 * kGvWarps, 1) int4_gemv_kernel(const __grid_constant__ Int4GemvParams p) {
   constexpr int kXw = G == 32 ? 32 : 64;  // columns of a sum X
   constexpr int XS = 64 / kXw;            // sums a tile
   extern __shared__ __align__(16) uint8_t gv_smem[];
+  __shared__ uint64_t s_full[kGvWarps][kGvMaxStages];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int r = lane >> 2, c = lane & 3;
+  // warps that share a row tile's columns (kGvWarps / streams)
+  const int slice_bits = p.streams == 2 ? 3 : 4, slices = 1 << slice_bits;
+  static_assert(kGvWarps == 16, "");
+  const int stream = warp >> slice_bits, slice = warp & (slices - 1);
   const int KT = gv_blocks(p.k);
   const int groups = (p.k + G - 1) / G;
-  uint8_t* ring = gv_smem + warp * (kGvStages * kStage);
-  float* part = reinterpret_cast<float*>(gv_smem + kGvWarps * kGvStages * kStage);
-  float* xsum = part + 2 * (kGvPartBytes / 4);  // [KT * XS][xw]
+  const int stage_bytes = p.chunk * gv_tile_bytes(G);
+  uint8_t* ring = gv_smem + warp * (p.stages * stage_bytes);
+  float* part = reinterpret_cast<float*>(gv_smem + kGvWarps * p.stages * stage_bytes);
+  float* xsum = part + 2 * (p.part_bytes / 4);
   const int xw = gv_sums(p.m);
-  T* xs = reinterpret_cast<T*>(reinterpret_cast<uint8_t*>(xsum) + (KT * XS * xw * 4 + 15) / 16 * 16);
+  uint8_t* xs = reinterpret_cast<uint8_t*>(xsum) + gv_sum_bytes(p.k, p.m, G, kInt);
+  const int x_bytes = gv_x_bytes(p.k, kInt);
+  uint64_t* full = s_full[warp];
+  if (lane == 0) {
+    for (int i = 0; i < p.stages; ++i) mbar_init(&full[i], 1);
+    fence_mbar_init();
+  }
+  __syncwarp();
 
-  const int64_t row_tiles = (p.n + 15) / 16;
-  const int64_t rt0 = row_tiles * blockIdx.x / gridDim.x, rt1 = row_tiles * (blockIdx.x + 1) / gridDim.x;
-  const int nk = warp < KT ? (KT - warp + kGvWarps - 1) / kGvWarps : 0;  // this warp's tiles of a row
-  const uint8_t* params = static_cast<const uint8_t*>(p.params);
-  const uint32_t ring_s = smem_u32(ring);
+  const int cta = blockIdx.x;
+  const int rt0 = cta * p.share + (cta < p.more ? cta : p.more), rt1 = rt0 + p.share + (cta < p.more);
+  // this warp's run of columns, in tiles
+  const int per = KT >> slice_bits, over = KT - (per << slice_bits);
+  const int kt0 = slice * per + (slice < over ? slice : over), nk = per + (slice < over);
 
-  // The weights do not depend on the previous kernel: the first tiles are fetched before waiting for it.
-  int64_t f_rt = rt0;
-  int f_kt = warp, f_s = 0;
+  // Lane 0 fetches: its runs of the stream's row tiles, chunk by chunk.
+  int f_rt = rt0 + stream, f_kt = kt0, f_s = 0;
+  const uint64_t pol = policy_evict_first();
   auto fetch = [&]() {
-    if (f_rt < rt1 && nk > 0) {
-      const uint32_t dst = ring_s + f_s * kStage;
-      copy_async<16>(dst + 16 * lane, p.codes + (f_rt * KT + f_kt) * 512 + 16 * lane, true);
-      const int g0 = G == 32 ? 2 * f_kt : f_kt * 64 / G;
-      if (lane < kParamBytes / 16) {
-        // (G = 32: the last tile's second half may lie behind the last group)
-        const bool in = G != 32 || g0 + lane / 4 < groups;
-        copy_async<16>(dst + 512 + 16 * lane, params + (f_rt * groups + g0) * 64 + (in ? 16 * lane : 0), in);
+    if (lane == 0 && f_rt < rt1 && nk > 0) {
+      const int left = kt0 + nk - f_kt, nt = left < p.chunk ? left : p.chunk;
+      const int g0 = f_kt * 64 / G;
+      int g1 = ((f_kt + nt) * 64 + G - 1) / G;
+      g1 = g1 < groups ? g1 : groups;
+      uint8_t* dst = ring + f_s * stage_bytes;
+      mbar_arrive_expect_tx(&full[f_s], nt * 512 + (g1 - g0) * 64);
+      bulk_g2s(dst, p.codes + ((int64_t)f_rt * KT + f_kt) * 512, nt * 512, &full[f_s], pol);
+      bulk_g2s(dst + p.chunk * 512, static_cast<const uint8_t*>(p.params) + ((int64_t)f_rt * groups + g0) * 64,
+               (g1 - g0) * 64, &full[f_s], pol);
+      f_kt += nt;
+      if (f_kt == kt0 + nk) {
+        f_kt = kt0;
+        f_rt += p.streams;
       }
-      f_kt += kGvWarps;
-      if (f_kt >= KT) {
-        f_kt = warp;
-        ++f_rt;
-      }
-      f_s = f_s + 1 == kGvStages ? 0 : f_s + 1;
+      f_s = f_s + 1 == p.stages ? 0 : f_s + 1;
     }
-    copy_commit();
   };
-#pragma unroll
-  for (int i = 0; i < kGvStages - 1; ++i) fetch();
-
+  // The weights do not depend on the previous kernel: the first tiles are fetched before waiting for it.
+  for (int i = 0; i < kGvPreWait; ++i) fetch();
   pdl_launch();
   pdl_wait();
+  for (int i = kGvPreWait; i < p.stages; ++i) fetch();
   {
     // tokens into shared memory, 8 elements a thread, with their groups' sums
-    const int chunks = 8 * KT;
+    const int chunks = 8 * KT, total = p.m * chunks;
     const T zero = from_f32<T>(0.f);
-    const int total = p.m * chunks;
-    for (int base = 0; base < total; base += 32 * kGvWarps) {  // every thread: neighbours add up their sums
-      const int idx = base + threadIdx.x;
+    for (int base = 32 * warp; base < total; base += 32 * kGvWarps) {  // whole warps: neighbours work out their sums together
+      const int idx = base + lane;
       const bool use = idx < total;
-      const int m = use ? idx / chunks : 0, k0 = use ? 8 * (idx - m * chunks) : 0;
+      const int m = !use || p.m == 1 ? 0 : idx / chunks, k0 = use ? 8 * (idx - m * chunks) : 0;
       const T* xr = static_cast<const T*>(p.x) + m * p.sx;
       T v[8], u[8];
       if (use && p.vec && k0 + 8 <= p.k) {
@@ -124,119 +179,204 @@ __global__ void __launch_bounds__(32 * kGvWarps) int4_gemv_kernel(const __grid_c
           u[e] = use && p.swiglu && k0 + e < p.k ? xr[p.k + k0 + e] : zero;
         }
       }
-      float sum = 0.f;
+      float f[8], sum = 0.f;
+      if (p.swiglu) {
+        // the arithmetic of the 16-bit projection's staging
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        if (p.swiglu) {
-          // the arithmetic of the 16-bit projection's staging
+        for (int e = 0; e < 8; ++e) {
           const float g = to_f32(v[e]);
           v[e] = from_f32<T>(to_f32(from_f32<T>(g / (1.0f + expf(-g)))) * to_f32(u[e]));
         }
-        sum += to_f32(v[e]);
       }
-      if (use) {
-        uint4 a;
-        memcpy(&a, v, 16);
-        *reinterpret_cast<uint4*>(xs + (int64_t)m * p.x_stride + k0) = a;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        f[e] = to_f32(v[e]);
+        sum += f[e];
       }
 #pragma unroll
       for (int o = 1; o < kXw / 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if (use && (k0 & (kXw - 1)) == 0) xsum[(k0 / kXw) * xw + m] = sum;
+      const bool writes = use && (k0 & (kXw - 1)) == 0;
+      if constexpr (kInt) {
+        float most = fabsf(f[0]);
+#pragma unroll
+        for (int e = 1; e < 8; ++e) most = fmaxf(most, fabsf(f[e]));
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+        float up, down;
+        digit_scale(sum * 0.f == 0.f ? most : INFINITY, up, down);
+        constexpr float kWhole = 12582912.f;  // 1.5 * 2^23: adding it leaves a whole number in the low bits
+        int q[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) q[e] = __float_as_int(fmaf(f[e], up, kWhole)) + (0x8080 - 0x4b400000);
+        uint32_t even[kGvDigits], odd[kGvDigits];
+        // bytes in the order of a word's codes 0, 2, 4, 6 (columns 0, 4, 1, 5) and 1, 3, 5, 7 (columns 2, 6, 3, 7)
+        digits4(q[0], q[4], q[1], q[5], even);
+        digits4(q[2], q[6], q[3], q[7], odd);
+        if (use) {
+          const int chunk = k0 / 8;
+          uint8_t* to = xs + m * kGvDigits * x_bytes + (chunk / 8) * 64 + (chunk & 3) * 16 + ((chunk >> 2) & 1) * 8;
+#pragma unroll
+          for (int i = 0; i < kGvDigits; ++i)
+            *reinterpret_cast<uint2*>(to + i * x_bytes) = make_uint2(even[kGvDigits - 1 - i], odd[kGvDigits - 1 - i]);
+        }
+        if (writes) {
+          // lane c's sums of a token are 256 h + m (c even), and 256 l; the products are with codes, 16 times code/16
+          float2* to = reinterpret_cast<float2*>(xsum) + (k0 / kXw) * 4 + 2 * m;
+          to[0] = make_float2(sum, 16.f * down);
+          to[1] = make_float2(0.f, 0.000244140625f * down);
+        }
+      } else {
+        if (use) {
+          uint4 a;
+          memcpy(&a, v, 16);
+          *reinterpret_cast<uint4*>(xs + m * x_bytes + 2 * k0) = a;
+        }
+        if (writes) xsum[(k0 / kXw) * xw + m] = sum;
+      }
     }
-    if (p.m < xw)  // the pair's other column
-      for (int idx = threadIdx.x; idx < KT * XS; idx += 32 * kGvWarps) xsum[idx * xw + p.m] = 0.f;
+    if (p.m < xw) {  // the pair's other token
+      for (int idx = threadIdx.x; idx < KT * XS; idx += 32 * kGvWarps) {
+        if constexpr (kInt)
+          reinterpret_cast<float4*>(xsum)[idx * 2 + 1] = make_float4(0.f, 0.f, 0.f, 0.f);
+        else
+          xsum[idx * xw + p.m] = 0.f;
+      }
+    }
   }
   __syncthreads();
 
-  int s = 0, buf = 0;
-  for (int64_t f0 = rt0; f0 < rt1; f0 += p.flush, buf ^= 1) {
-    const int nf = rt1 - f0 < p.flush ? (int)(rt1 - f0) : p.flush;
-    float* pb = part + buf * (kGvPartBytes / 4);  // [nf][warps][m][16]
-    for (int f = 0; f < nf; ++f) {
+  // kInt: column 4 token + digit; this lane's operand is of digit r & 3 of token r / 4, its sums of token c / 2
+  const bool has = kInt ? (r & 3) < kGvDigits && r / 4 < p.m : true;
+  const uint32_t xa0 = smem_u32(xs) + (kInt ? ((r / 4) * kGvDigits + (r & 3)) * x_bytes + 16 * c : r * x_bytes + 16 * c);
+  int s = 0, phase = 0, buf = 0;
+  for (int f0 = rt0; f0 < rt1; f0 += p.flush, buf ^= 1) {
+    const int nf = rt1 - f0 < p.flush ? rt1 - f0 : p.flush;  // (flush is a multiple of streams)
+    float* pb = part + buf * (p.part_bytes / 4);             // [nf][slices][m][16]
+    for (int f = stream; f < nf; f += p.streams) {
       float acc[NT][4];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[nt][e] = 0.f;
-      for (int i = 0, kt = warp; i < nk; ++i, kt += kGvWarps) {
-        fetch();
-        copy_wait<kGvStages - 1>();
-        __syncwarp();  // the (S, z) came through other lanes
-        const uint32_t st = ring_s + s * kStage;
-        uint32_t w[4], q[XS][2];
-        lds_words(st + 16 * lane, w);
-#pragma unroll
-        for (int x = 0; x < XS; ++x) lds_words(st + 512 + 64 * x + 8 * r, q[x]);
-        uint32_t a[4][4];
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          a[2 * x][0] = i4_mant<T, 0>(w[2 * x]);
-          a[2 * x][1] = i4_mant<T, 0>(w[2 * x + 1]);
-          a[2 * x][2] = i4_mant<T, 1>(w[2 * x]);
-          a[2 * x][3] = i4_mant<T, 1>(w[2 * x + 1]);
-          a[2 * x + 1][0] = i4_mant<T, 2>(w[2 * x]);
-          a[2 * x + 1][1] = i4_mant<T, 2>(w[2 * x + 1]);
-          a[2 * x + 1][2] = i4_mant<T, 3>(w[2 * x]);
-          a[2 * x + 1][3] = i4_mant<T, 3>(w[2 * x + 1]);
-        }
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          const int m = nt * 8 + r;
-          uint32_t b0[4] = {0u, 0u, 0u, 0u}, b1[4] = {0u, 0u, 0u, 0u};
-          if (m < p.m) {
-            const uint32_t xa = smem_u32(xs + (int64_t)m * p.x_stride + 64 * kt + 8 * c);
-            lds_words(xa, b0);
-            lds_words(xa + 64, b1);
-          }
-          float d[XS][4];
+      for (int kt = kt0; kt < kt0 + nk;) {
+        if (!mbar_wait(&full[s], phase, TC_DEVERR_PIPE_TIMEOUT)) break;
+        const uint32_t st = smem_u32(ring) + s * stage_bytes;
+        const int end = kt + p.chunk < kt0 + nk ? kt + p.chunk : kt0 + nk;
+        uint32_t code = st + 16 * lane, param = st + p.chunk * 512 + 8 * r;
+        const int odd = G == 128 ? kt & 1 : 0;  // (two tiles a group)
+        for (int t = 0; kt < end; ++kt, ++t, code += 512) {
+          uint32_t w[4], q[XS][2];
+          lds_words(code, w);
 #pragma unroll
           for (int x = 0; x < XS; ++x)
+            lds_words(param + (G == 32 ? 128 * t + 64 * x : G == 64 ? 64 * t : 64 * ((t + odd) >> 1)), q[x]);
+          if (G == 32 && 2 * kt + 1 >= groups) q[XS - 1][0] = q[XS - 1][1] = 0u;  // (no such group: nothing was copied)
+          if constexpr (kInt) {
+            uint32_t b[4] = {0u, 0u, 0u, 0u}, a[4];
+            if (has) lds_words(xa0 + 64 * kt, b);
+            int d[XS][4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) d[x][e] = 0.f;
-          Mma<T>::run(d[0], a[0], b0[0], b0[1]);
-          Mma<T>::run(d[0], a[1], b0[2], b0[3]);
-          Mma<T>::run(d[XS - 1], a[2], b1[0], b1[1]);
-          Mma<T>::run(d[XS - 1], a[3], b1[2], b1[3]);
+            for (int x = 0; x < XS; ++x)
 #pragma unroll
-          for (int x = 0; x < XS; ++x) {
-            float2 X = make_float2(0.f, 0.f);
-            if (nt * 8 + 2 * c < xw) X = *reinterpret_cast<const float2*>(xsum + (kt * XS + x) * xw + nt * 8 + 2 * c);
-            const float s0 = Mma<T>::lo(q[x][0]), z0 = Mma<T>::hi(q[x][0]);
-            const float s1 = Mma<T>::lo(q[x][1]), z1 = Mma<T>::hi(q[x][1]);
-            acc[nt][0] = fmaf(z0, X.x, fmaf(s0, d[x][0], acc[nt][0]));
-            acc[nt][1] = fmaf(z0, X.y, fmaf(s0, d[x][1], acc[nt][1]));
-            acc[nt][2] = fmaf(z1, X.x, fmaf(s1, d[x][2], acc[nt][2]));
-            acc[nt][3] = fmaf(z1, X.y, fmaf(s1, d[x][3], acc[nt][3]));
+              for (int e = 0; e < 4; ++e) d[x][e] = 0;
+            i4_bytes(w[0], w[1], a);
+            mma_u8s8(d[0], a, b[0], b[1]);
+            i4_bytes(w[2], w[3], a);
+            mma_u8s8(d[XS - 1], a, b[2], b[3]);
+#pragma unroll
+            for (int x = 0; x < XS; ++x) {
+              const float2 X = reinterpret_cast<const float2*>(xsum)[(kt * XS + x) * 4 + c];
+              // (at most 64 * 15 * (256 * 16 + 128) < 2^24)
+              const float P0 = X.y * (float)(256 * d[x][0] + d[x][1]), P1 = X.y * (float)(256 * d[x][2] + d[x][3]);
+              const float s0 = Mma<T>::lo(q[x][0]), s1 = Mma<T>::lo(q[x][1]);
+              acc[0][0] = fmaf(s0 + Mma<T>::hi(q[x][0]), X.x, fmaf(s0, P0, acc[0][0]));
+              acc[0][2] = fmaf(s1 + Mma<T>::hi(q[x][1]), X.x, fmaf(s1, P1, acc[0][2]));
+            }
+          } else {
+            uint32_t a[4][4];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              a[2 * x][0] = i4_ones<T, 0>(w[2 * x]);
+              a[2 * x][1] = i4_ones<T, 0>(w[2 * x + 1]);
+              a[2 * x][2] = i4_ones<T, 1>(w[2 * x]);
+              a[2 * x][3] = i4_ones<T, 1>(w[2 * x + 1]);
+              a[2 * x + 1][0] = i4_ones<T, 2>(w[2 * x]);
+              a[2 * x + 1][1] = i4_ones<T, 2>(w[2 * x + 1]);
+              a[2 * x + 1][2] = i4_ones<T, 3>(w[2 * x]);
+              a[2 * x + 1][3] = i4_ones<T, 3>(w[2 * x + 1]);
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              uint32_t b0[4] = {0u, 0u, 0u, 0u}, b1[4] = {0u, 0u, 0u, 0u};
+              if (nt * 8 + r < p.m) {
+                const uint32_t xa = xa0 + nt * 8 * x_bytes + 128 * kt;
+                lds_words(xa, b0);
+                lds_words(xa + 64, b1);
+              }
+              float d[XS][4];
+#pragma unroll
+              for (int x = 0; x < XS; ++x)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) d[x][e] = 0.f;
+              Mma<T>::run(d[0], a[0], b0[0], b0[1]);
+              Mma<T>::run(d[0], a[1], b0[2], b0[3]);
+              Mma<T>::run(d[XS - 1], a[2], b1[0], b1[1]);
+              Mma<T>::run(d[XS - 1], a[3], b1[2], b1[3]);
+#pragma unroll
+              for (int x = 0; x < XS; ++x) {
+                float2 X = make_float2(0.f, 0.f);
+                if (nt * 8 + 2 * c < xw) X = *reinterpret_cast<const float2*>(xsum + (kt * XS + x) * xw + nt * 8 + 2 * c);
+                const float s0 = Mma<T>::lo(q[x][0]), z0 = Mma<T>::hi(q[x][0]);
+                const float s1 = Mma<T>::lo(q[x][1]), z1 = Mma<T>::hi(q[x][1]);
+                acc[nt][0] = fmaf(z0, X.x, fmaf(s0, d[x][0], acc[nt][0]));
+                acc[nt][1] = fmaf(z0, X.y, fmaf(s0, d[x][1], acc[nt][1]));
+                acc[nt][2] = fmaf(z1, X.x, fmaf(s1, d[x][2], acc[nt][2]));
+                acc[nt][3] = fmaf(z1, X.y, fmaf(s1, d[x][3], acc[nt][3]));
+              }
+            }
           }
         }
         __syncwarp();  // the stage may be filled again
-        s = s + 1 == kGvStages ? 0 : s + 1;
-      }
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int m = nt * 8 + 2 * c + e;
-          if (m < p.m) {
-            float* o = pb + ((f * kGvWarps + warp) * p.m + m) * 16 + r;
-            o[0] = acc[nt][e];
-            o[8] = acc[nt][2 + e];
-          }
+        fetch();
+        if (++s == p.stages) {
+          s = 0;
+          phase ^= 1;
         }
+      }
+      float* o = pb + (f * slices + slice) * p.m * 16 + r;
+      if constexpr (kInt) {
+        const float a0 = acc[0][0] + __shfl_xor_sync(0xffffffffu, acc[0][0], 1);
+        const float a1 = acc[0][2] + __shfl_xor_sync(0xffffffffu, acc[0][2], 1);
+        if ((c & 1) == 0 && c / 2 < p.m) {
+          o[c / 2 * 16] = a0;
+          o[c / 2 * 16 + 8] = a1;
+        }
+      } else {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int m = nt * 8 + 2 * c + e;
+            if (m < p.m) {
+              o[m * 16] = acc[nt][e];
+              o[m * 16 + 8] = acc[nt][2 + e];
+            }
+          }
+      }
     }
     __syncthreads();  // (the other buffer's readers are a barrier ahead of its next writers)
     const int outs = nf * p.m * 16;
     for (int idx = threadIdx.x; idx < outs; idx += 32 * kGvWarps) {
       const int rr = idx & 15, fm = idx >> 4;
-      const int f = fm / p.m, m = fm - f * p.m;
-      const int64_t row = (f0 + f) * 16 + rr;
+      const int f = p.m == 1 ? fm : fm / p.m, m = fm - f * p.m;
+      const int64_t row = (int64_t)(f0 + f) * 16 + rr;
+      const float* o = pb + (f * slices * p.m + m) * 16 + rr;
       float sum = 0.f;
-#pragma unroll
-      for (int w = 0; w < kGvWarps; ++w) sum += pb[((f * kGvWarps + w) * p.m + m) * 16 + rr];
+#pragma unroll 8
+      for (int w = 0; w < slices; ++w) sum += o[w * p.m * 16];
       if (row < p.n) static_cast<T*>(p.out)[m * p.so + row] = from_f32<T>(sum);
     }
   }
-  copy_wait<0>();
 }
 
 }  // namespace tc
