@@ -155,8 +155,14 @@ constexpr int kGvMaxSmem = 226 * 1024;
 constexpr int kGvMaxColumns = 65536;  // one token of them fits
 constexpr int kGvIntTokens = 2;       // up to these, tokens as digits
 
-// Two row tiles at a time, 8 warps on each, or (few row tiles) all 16 on one.
-int gv_streams(int64_t n, int sms) { return cdiv(n, 16) > 2 * (int64_t)sms ? 2 : 1; }
+// Row tiles a CTA works on at a time, 16 warps between them: as many as leave each stream 8 to go through, so that few sums
+// are added across warps and the streams end together; two at least where there are enough row tiles.
+int gv_streams(int64_t n, int sms) {
+  const int64_t tiles = cdiv(n, 16);
+  int streams = tiles > 2 * (int64_t)sms ? 2 : 1;
+  while (streams < 8 && tiles >= 16 * (int64_t)streams * sms) streams *= 2;
+  return streams;
+}
 int gv_part_bytes(int m, int streams) {
   const int least = kGvWarps * 64 * m;  // a row tile of each stream
   return least > kGvPartBytes ? least : kGvPartBytes;
@@ -166,14 +172,14 @@ int64_t gv_fixed(int k, int m, int group, int streams, bool digits) {
   return 2 * gv_part_bytes(m, streams) + gv_sum_bytes(k, m, group, digits) +
          (int64_t)m * (digits ? kGvDigits : 1) * gv_x_bytes(k, digits);
 }
-// The largest ring that fits beside that; false where none does.
-bool gv_ring(int64_t fixed, int group, int& chunk, int& stages) {
-  const int plans[4][2] = {{4, 3}, {4, 2}, {2, 2}, {1, 2}};
-  for (const auto& p : plans) {
-    chunk = p[0];
-    stages = p[1];
-    if (fixed + (int64_t)kGvWarps * chunk * stages * gv_tile_bytes(group) <= kGvMaxSmem) return true;
-  }
+// The largest ring that fits beside that; false where none does. A stage holds a warp's run of columns, or an even part of it.
+bool gv_ring(int64_t fixed, int k, int group, int streams, int& chunk, int& stages) {
+  const int64_t run = cdiv((int64_t)gv_blocks(k) * streams, kGvWarps);
+  for (int most = kGvMaxChunk; most >= 1; --most)
+    for (stages = kGvMaxStages; stages >= 2; --stages) {
+      chunk = (int)cdiv(run, cdiv(run, most));
+      if (fixed + (int64_t)kGvWarps * chunk * stages * gv_tile_bytes(group) <= kGvMaxSmem) return true;
+    }
   return false;
 }
 
@@ -444,7 +450,7 @@ int tc_gemv_int4(const void* x, const void* codes, const void* params, void* out
     // as many tokens a launch as fit, 32 at most; one always does as 16-bit numbers
     int now = (int)(m - m0 < 32 ? m - m0 : 32);
     bool digits = now <= kGvIntTokens;
-    while (!gv_ring(gv_fixed(k, now, group, streams, digits), group, p.chunk, p.stages)) {
+    while (!gv_ring(gv_fixed(k, now, group, streams, digits), k, group, streams, p.chunk, p.stages)) {
       if (digits) {
         digits = false;
       } else if (--now == 0) {
@@ -463,6 +469,7 @@ int tc_gemv_int4(const void* x, const void* codes, const void* params, void* out
     p.swiglu = swiglu != 0;
     p.vec = aligned16(p.x) && (p.m == 1 || stride16(x_stride, dtype)) && (!p.swiglu || k % 8 == 0);
     p.streams = streams;
+    for (p.slice_bits = 4; (kGvWarps >> p.slice_bits) < streams;) --p.slice_bits;
     p.part_bytes = gv_part_bytes(p.m, streams);
     p.flush = p.part_bytes / (kGvWarps * 64 * p.m) * streams;
     const int smem = (int)(gv_fixed(k, now, group, streams, digits) +

@@ -14,7 +14,7 @@
 // to a whole number below 2^20, is 65536 h + 256 m + l. More tokens: 1 + code/16 and x as they are, 16-bit operands (24 and
 // 8; S P + z X then), 8 tokens a product.
 //
-// A CTA an SM takes neighbouring row tiles, in one or two streams of warps. A stream's warps share out the columns in
+// A CTA an SM takes neighbouring row tiles, in one or more streams of warps. A stream's warps share out the columns in
 // neighbouring runs, each bringing in its run of a row tile, and of the next ones, by bulk copies of a few tiles; their sums are
 // added in shared memory in warp order.
 #pragma once
@@ -24,9 +24,10 @@
 namespace tc {
 
 constexpr int kGvWarps = 16;
-constexpr int kGvMaxStages = 3;          // of a warp's ring
+constexpr int kGvMaxStages = 2;          // of a warp's ring (a third gains nothing)
 constexpr int kGvPreWait = 1;            // stages filled before the previous kernel has ended
-constexpr int kGvPartBytes = 8 * 1024;   // one of the two buffers of sums, at least a row tile's
+constexpr int kGvPartBytes = 16 * 1024;  // one of the two buffers of sums, at least a row tile's of each stream
+constexpr int kGvMaxChunk = 5;           // tiles of a stage
 constexpr int kGvDigits = 3;
 
 struct Int4GemvParams {
@@ -39,7 +40,8 @@ struct Int4GemvParams {
   int64_t sx, so;
   int swiglu;
   int vec;         // x in 16-byte chunks
-  int streams;     // 1 or 2
+  int streams;     // a power of two, 8 at most
+  int slice_bits;  // kGvWarps / streams warps share a row tile's columns: 2^slice_bits
   int share, more; // row tiles of a CTA: share, and one more for the first `more` CTAs
   int flush;       // row tiles whose sums a buffer holds
   int part_bytes;  // of a buffer
@@ -64,11 +66,24 @@ __host__ __device__ __forceinline__ int gv_sum_bytes(int k, int m, int g, bool d
   return (gv_blocks(k) * (g == 32 ? 2 : 1) * (digits ? 32 : 4 * gv_sums(m)) + 15) / 16 * 16;
 }
 
+// Products into d, from 0 (kFirst) or from what is there.
+template <bool kFirst>
 __device__ __forceinline__ void mma_u8s8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  if constexpr (kFirst)
+    asm volatile(
+        "mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(0));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float2 lds_float2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr));
+  return v;
 }
 // Codes of two words (rows r and r + 8) as bytes: codes 0, 2, 4, 6, then 1, 3, 5, 7.
 __device__ __forceinline__ void i4_bytes(uint32_t w0, uint32_t w1, uint32_t (&a)[4]) {
@@ -102,10 +117,8 @@ __global__ void __launch_bounds__(32 * kGvWarps, 1) int4_gemv_kernel(const __gri
   __shared__ uint64_t s_full[kGvWarps][kGvMaxStages];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int r = lane >> 2, c = lane & 3;
-  // warps that share a row tile's columns (kGvWarps / streams)
-  const int slice_bits = p.streams == 2 ? 3 : 4, slices = 1 << slice_bits;
-  static_assert(kGvWarps == 16, "");
-  const int stream = warp >> slice_bits, slice = warp & (slices - 1);
+  const int slices = 1 << p.slice_bits;
+  const int stream = warp >> p.slice_bits, slice = warp & (slices - 1);
   const int KT = gv_blocks(p.k);
   const int groups = (p.k + G - 1) / G;
   const int stage_bytes = p.chunk * gv_tile_bytes(G);
@@ -125,7 +138,7 @@ __global__ void __launch_bounds__(32 * kGvWarps, 1) int4_gemv_kernel(const __gri
   const int cta = blockIdx.x;
   const int rt0 = cta * p.share + (cta < p.more ? cta : p.more), rt1 = rt0 + p.share + (cta < p.more);
   // this warp's run of columns, in tiles
-  const int per = KT >> slice_bits, over = KT - (per << slice_bits);
+  const int per = KT >> p.slice_bits, over = KT - (per << p.slice_bits);
   const int kt0 = slice * per + (slice < over ? slice : over), nk = per + (slice < over);
 
   // Lane 0 fetches: its runs of the stream's row tiles, chunk by chunk.
@@ -220,10 +233,10 @@ __global__ void __launch_bounds__(32 * kGvWarps, 1) int4_gemv_kernel(const __gri
             *reinterpret_cast<uint2*>(to + i * x_bytes) = make_uint2(even[kGvDigits - 1 - i], odd[kGvDigits - 1 - i]);
         }
         if (writes) {
-          // lane c's sums of a token are 256 h + m (c even), and 256 l; the products are with codes, 16 times code/16
+          // lane c's sums of a token are 256 h + m (c even), and 256 l + l; the products are with codes, 16 times code/16
           float2* to = reinterpret_cast<float2*>(xsum) + (k0 / kXw) * 4 + 2 * m;
           to[0] = make_float2(sum, 16.f * down);
-          to[1] = make_float2(0.f, 0.000244140625f * down);
+          to[1] = make_float2(0.f, (0.0625f / 257.f) * down);
         }
       } else {
         if (use) {
@@ -245,9 +258,23 @@ __global__ void __launch_bounds__(32 * kGvWarps, 1) int4_gemv_kernel(const __gri
   }
   __syncthreads();
 
-  // kInt: column 4 token + digit; this lane's operand is of digit r & 3 of token r / 4, its sums of token c / 2
-  const bool has = kInt ? (r & 3) < kGvDigits && r / 4 < p.m : true;
-  const uint32_t xa0 = smem_u32(xs) + (kInt ? ((r / 4) * kGvDigits + (r & 3)) * x_bytes + 16 * c : r * x_bytes + 16 * c);
+  // This lane's operand is column r of the tokens: token nt 8 + r, or (kInt) digit r & 3 of token r / 4, the fourth column being
+  // the last digit again. Columns that no token has repeat another's: nothing reads their sums.
+  uint32_t xa0[NT];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int token = kInt ? r / 4 : nt * 8 + r, last = p.m - 1;
+    const int digit = (r & 3) < kGvDigits ? r & 3 : kGvDigits - 1;
+    xa0[nt] = smem_u32(xs) + ((token < last ? token : last) * (kInt ? kGvDigits : 1) + (kInt ? digit : 0)) * x_bytes + 16 * c;
+  }
+  // and its sums are those of columns 2c and 2c + 1
+  uint32_t sum0[NT];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int token = nt * 8 + 2 * c;
+    sum0[nt] = smem_u32(xsum) + (kInt ? 8 * c : 4 * (token < xw ? token : 0));
+  }
+  const uint32_t sum_step = kInt ? 32 : 4 * xw;
   int s = 0, phase = 0, buf = 0;
   for (int f0 = rt0; f0 < rt1; f0 += p.flush, buf ^= 1) {
     const int nf = rt1 - f0 < p.flush ? rt1 - f0 : p.flush;  // (flush is a multiple of streams)
@@ -262,30 +289,26 @@ __global__ void __launch_bounds__(32 * kGvWarps, 1) int4_gemv_kernel(const __gri
         if (!mbar_wait(&full[s], phase, TC_DEVERR_PIPE_TIMEOUT)) break;
         const uint32_t st = smem_u32(ring) + s * stage_bytes;
         const int end = kt + p.chunk < kt0 + nk ? kt + p.chunk : kt0 + nk;
-        uint32_t code = st + 16 * lane, param = st + p.chunk * 512 + 8 * r;
-        const int odd = G == 128 ? kt & 1 : 0;  // (two tiles a group)
-        for (int t = 0; kt < end; ++kt, ++t, code += 512) {
+        uint32_t code = st + 16 * lane, param = st + p.chunk * 512 + 8 * r, xk = kt * (kInt ? 64 : 128), xx = kt * XS * sum_step;
+#pragma unroll 2
+        for (; kt < end; ++kt, code += 512, xk += kInt ? 64 : 128, xx += XS * sum_step) {
           uint32_t w[4], q[XS][2];
           lds_words(code, w);
 #pragma unroll
-          for (int x = 0; x < XS; ++x)
-            lds_words(param + (G == 32 ? 128 * t + 64 * x : G == 64 ? 64 * t : 64 * ((t + odd) >> 1)), q[x]);
+          for (int x = 0; x < XS; ++x) lds_words(param + 64 * x, q[x]);
+          param += G == 32 ? 128 : G == 64 ? 64 : (kt & 1) * 64;  // (G = 128: two tiles a group)
           if (G == 32 && 2 * kt + 1 >= groups) q[XS - 1][0] = q[XS - 1][1] = 0u;  // (no such group: nothing was copied)
           if constexpr (kInt) {
-            uint32_t b[4] = {0u, 0u, 0u, 0u}, a[4];
-            if (has) lds_words(xa0 + 64 * kt, b);
+            uint32_t b[4], a[4];
+            lds_words(xa0[0] + xk, b);
             int d[XS][4];
-#pragma unroll
-            for (int x = 0; x < XS; ++x)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) d[x][e] = 0;
             i4_bytes(w[0], w[1], a);
-            mma_u8s8(d[0], a, b[0], b[1]);
+            mma_u8s8<true>(d[0], a, b[0], b[1]);
             i4_bytes(w[2], w[3], a);
-            mma_u8s8(d[XS - 1], a, b[2], b[3]);
+            mma_u8s8<XS == 2>(d[XS - 1], a, b[2], b[3]);
 #pragma unroll
             for (int x = 0; x < XS; ++x) {
-              const float2 X = reinterpret_cast<const float2*>(xsum)[(kt * XS + x) * 4 + c];
+              const float2 X = lds_float2(sum0[0] + xx + x * 32);
               // (at most 64 * 15 * (256 * 16 + 128) < 2^24)
               const float P0 = X.y * (float)(256 * d[x][0] + d[x][1]), P1 = X.y * (float)(256 * d[x][2] + d[x][3]);
               const float s0 = Mma<T>::lo(q[x][0]), s1 = Mma<T>::lo(q[x][1]);
@@ -307,12 +330,9 @@ __global__ void __launch_bounds__(32 * kGvWarps, 1) int4_gemv_kernel(const __gri
             }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-              uint32_t b0[4] = {0u, 0u, 0u, 0u}, b1[4] = {0u, 0u, 0u, 0u};
-              if (nt * 8 + r < p.m) {
-                const uint32_t xa = xa0 + nt * 8 * x_bytes + 128 * kt;
-                lds_words(xa, b0);
-                lds_words(xa + 64, b1);
-              }
+              uint32_t b0[4], b1[4];
+              lds_words(xa0[nt] + xk, b0);
+              lds_words(xa0[nt] + xk + 64, b1);
               float d[XS][4];
 #pragma unroll
               for (int x = 0; x < XS; ++x)
@@ -324,8 +344,7 @@ __global__ void __launch_bounds__(32 * kGvWarps, 1) int4_gemv_kernel(const __gri
               Mma<T>::run(d[XS - 1], a[3], b1[2], b1[3]);
 #pragma unroll
               for (int x = 0; x < XS; ++x) {
-                float2 X = make_float2(0.f, 0.f);
-                if (nt * 8 + 2 * c < xw) X = *reinterpret_cast<const float2*>(xsum + (kt * XS + x) * xw + nt * 8 + 2 * c);
+                const float2 X = lds_float2(sum0[nt] + xx + x * sum_step);
                 const float s0 = Mma<T>::lo(q[x][0]), z0 = Mma<T>::hi(q[x][0]);
                 const float s1 = Mma<T>::lo(q[x][1]), z1 = Mma<T>::hi(q[x][1]);
                 acc[nt][0] = fmaf(z0, X.x, fmaf(s0, d[x][0], acc[nt][0]));
