@@ -32,6 +32,7 @@ __all__ = ["Int4Weight", "append_rope_int4", "decode_attention_int4", "dequantiz
 
 GROUP = 32  # elements of a cache row that share a scale
 HEAD_SIZES = (64, 128, 256)
+MAX_LAYERS = 128  # of a rotation's launch
 
 
 def row_bytes(d):
@@ -187,8 +188,8 @@ def gather_int4(k_pool, v_pool, tiles, n, dtype):
 
 
 def rotate_keys_int4(k_pools, tiles, delta, inv_freq, dtype):
-    """Moves the keys that `tiles` lists by `delta` positions, in place and in every pool (one a layer), in one launch
-    (tc_int4_rotate_keys): each row's values, rotated as kv.shift_keys rotates them and quantised again. tiles: int32
+    """Moves the keys that `tiles` lists by `delta` positions, in place and in every pool (one a layer), in one launch for
+    128 layers (tc_int4_rotate_keys): each row's values, rotated as kv.shift_keys rotates them and quantised again. tiles: int32
     [T, >= 3] (page, first row, rows <= 32, ...), no row twice; rows outside the pools are skipped. inv_freq:
     [d / 2]. dtype: the 16-bit type the rows were written from. All pools of one shape and strides."""
     what = "rotate_keys_int4"
@@ -207,11 +208,13 @@ def rotate_keys_int4(k_pools, tiles, delta, inv_freq, dtype):
     if inv_freq.numel() * 2 != d:
         raise ValueError(f"{what}: inv_freq has {inv_freq.numel()} entries, keys need {d // 2}")
     tab, tab_ptr = cos_sin_table(int(delta), inv_freq)
-    pools = (ctypes.c_void_p * len(k_pools))(*[p.data_ptr() for p in k_pools])
     with torch.cuda.device(first.device):
-        check("tc_int4_rotate_keys", lib().tc_int4_rotate_keys(
-            pools, len(k_pools), first.shape[1], d, first.shape[2], first.shape[0], *first.stride()[:3], tiles.data_ptr(),
-            tiles.shape[1], tiles.shape[0], tab_ptr, code, stream_ptr(first.device)))
+        for i in range(0, len(k_pools), MAX_LAYERS):
+            some = k_pools[i:i + MAX_LAYERS]
+            check("tc_int4_rotate_keys", lib().tc_int4_rotate_keys(
+                (ctypes.c_void_p * len(some))(*[p.data_ptr() for p in some]), len(some), first.shape[1], d, first.shape[2],
+                first.shape[0], *first.stride()[:3], tiles.data_ptr(), tiles.shape[1], tiles.shape[0], tab_ptr, code,
+                stream_ptr(first.device)))
     del tab  # the table is copied into the launch parameters
 
 

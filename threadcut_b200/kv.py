@@ -266,18 +266,20 @@ class _PagedState:
     """The PagedKV shared by the PagedLayers of one cache, created at the first update (when the
     head count, head size, dtype and device are known)."""
 
-    def __init__(self, layers, max_tokens, page_rows, fuse):
+    def __init__(self, layers, max_tokens, page_rows, fuse, bits=16):
         self.kv = None
         self.layers, self.max_tokens, self.page_rows, self.fuse = layers, max_tokens, page_rows, fuse
+        self.bits = bits
         self.members = []
 
     def ensure(self, key_states):
         if self.kv is None:
-            from .paged import PagedKV
+            from .paged import PagedKV, PagedKVInt4
             _, hkv, _, d = key_states.shape
             pages = -(-self.max_tokens // self.page_rows)
-            self.kv = PagedKV(self.layers, hkv, d, max_tokens=self.max_tokens, page_rows=self.page_rows,
-                              dtype=key_states.dtype, device=key_states.device, spare_pages=max(64, pages // 4))
+            store = PagedKVInt4 if self.bits == 4 else PagedKV
+            self.kv = store(self.layers, hkv, d, max_tokens=self.max_tokens, page_rows=self.page_rows,
+                            dtype=key_states.dtype, device=key_states.device, spare_pages=max(64, pages // 4))
             self.fuse = (self.fuse and key_states.is_cuda and key_states.dtype in (torch.bfloat16, torch.float16)
                          and d in (64, 128, 256))
 
@@ -292,7 +294,8 @@ class PagedLayer(DynamicLayer):
     into page slots (layer 0 reserves them for every layer of the step), a splice drops B's pages
     and re-rotates C's keys in place (kv.splice), and a one-token step with the threadcut attention
     leaves the new row pending: the plugin's decode branch writes it in the launch that attends over
-    the pages. Prefill chunks (and any other reader) get a contiguous copy of the layer's K/V."""
+    the pages. Prefill chunks (and any other reader) get a contiguous copy of the layer's K/V. Over a store of
+    4-bit rows (PagedKVInt4) the same calls quantise what they write and read it back."""
 
     def __init__(self, state, index):
         super().__init__()
@@ -401,29 +404,36 @@ def paged_pending(key):
 # Layout of the caches new_cache(config) builds when the caller does not say: the reference's
 # engine calls new_cache(self.model.config) (threadcut/engine.py:53), so a process that wants the
 # paged layout under that unchanged caller selects it here (use_paged_cache) instead.
-_LAYOUT = {"paged": False, "max_tokens": 32768, "page_rows": 64}
+_LAYOUT = {"paged": False, "max_tokens": 32768, "page_rows": 64, "bits": 16}
 
 
-def use_paged_cache(enabled=True, max_tokens=32768, page_rows=64):
+def use_paged_cache(enabled=True, max_tokens=32768, page_rows=64, bits=16):
     """Make new_cache(config) build paged caches (PagedLayers over one PagedKV of max_tokens rows in
-    page_rows-row pages) from now on, or contiguous GrowingLayer caches again (enabled=False)."""
+    page_rows-row pages) from now on, or contiguous GrowingLayer caches again (enabled=False). bits=4: rows of 4 bits
+    (PagedKVInt4) instead of the model's type."""
     if max_tokens < 1 or page_rows < 1:
         raise ValueError("use_paged_cache: max_tokens and page_rows must be positive")
-    _LAYOUT.update(paged=bool(enabled), max_tokens=int(max_tokens), page_rows=int(page_rows))
+    if bits not in (4, 16):
+        raise ValueError(f"use_paged_cache: rows have 4 or 16 bits, got {bits}")
+    _LAYOUT.update(paged=bool(enabled), max_tokens=int(max_tokens), page_rows=int(page_rows), bits=int(bits))
 
 
-def new_cache(config, paged=None, max_tokens=None, page_rows=None):
+def new_cache(config, paged=None, max_tokens=None, page_rows=None, bits=None):
     """A DynamicCache of GrowingLayers (the reference's layout, threadcut/kv.py:44-98) or, with
     paged=True, of PagedLayers over one PagedKV sized for max_tokens (plus spare pages for the
-    partly used pages splices leave; a full pool is re-packed by PagedKV.compact). Arguments left
-    None take the process-wide choice of use_paged_cache (default: contiguous, 32768, 64)."""
+    partly used pages splices leave; a full pool is re-packed by PagedKV.compact). bits=4 (paged only): rows of 4 bits.
+    Arguments left None take the process-wide choice of use_paged_cache (default: contiguous, 32768, 64, 16)."""
     paged = _LAYOUT["paged"] if paged is None else paged
     max_tokens = _LAYOUT["max_tokens"] if max_tokens is None else max_tokens
     page_rows = _LAYOUT["page_rows"] if page_rows is None else page_rows
+    bits = (_LAYOUT["bits"] if paged else 16) if bits is None else bits
+    if bits not in (4, 16) or (bits == 4 and not paged):
+        raise ValueError(f"new_cache: rows have 4 (paged caches) or 16 bits, got {bits} for a "
+                         f"{'paged' if paged else 'contiguous'} cache")
     cache = DynamicCache(config=config)
     fused = getattr(config, "_attn_implementation", None) == FUSED_ATTENTION
     if paged:
-        state = _PagedState(len(cache.layers), int(max_tokens), int(page_rows), fused)
+        state = _PagedState(len(cache.layers), int(max_tokens), int(page_rows), fused, bits)
         cache.layers = [PagedLayer(state, i) for i in range(len(cache.layers))]
         return cache
     cache.layers = [GrowingLayer() for _ in cache.layers]
@@ -438,7 +448,7 @@ def cache_bytes(cache):
     layers = cache.layers
     if layers and isinstance(layers[0], PagedLayer):
         kv = layers[0].state.kv
-        return 0 if kv is None else 2 * kv.n * kv.hkv * kv.d * kv.k[0].element_size() * kv.layers
+        return 0 if kv is None else 2 * kv.n * kv.hkv * kv.row_bytes * kv.layers
     n = cache.get_seq_length()
     layer = layers[0]
     return 2 * n * layer.keys[0, :, 0].numel() * layer.keys.element_size() * len(layers)

@@ -24,11 +24,12 @@ import ctypes
 import numpy as np
 import torch
 
-from . import _lib
+from . import _lib, int4
 from ._lib import check, dtype_code, lib, require_cuda, rows16, stream_ptr, workspaces
 from .match import Split
+from .prefill import prefill_attention, prefill_attention_window
 
-__all__ = ["PageTable", "PagedKV", "TILE_ROWS", "append_rope"]
+__all__ = ["PageTable", "PagedKV", "PagedKVInt4", "TILE_ROWS", "append_rope"]
 
 TILE_ROWS = 32  # rows per tile-table entry (the decode kernel's tile height)
 
@@ -325,9 +326,10 @@ class PagedKV:
         pages = -(-int(max_tokens) // self.page_rows) + int(spare_pages)
         self.table = PageTable(pages, self.page_rows)
         self.dtype, self.device = dtype, dev
-        shape = (pages, self.hkv, self.page_rows, self.d)
-        self.k = [torch.zeros(shape, dtype=dtype, device=dev) for _ in range(self.layers)]
-        self.v = [torch.zeros(shape, dtype=dtype, device=dev) for _ in range(self.layers)]
+        row, kind = self._row()
+        shape = (pages, self.hkv, self.page_rows, row)
+        self.k = [torch.zeros(shape, dtype=kind, device=dev) for _ in range(self.layers)]
+        self.v = [torch.zeros(shape, dtype=kind, device=dev) for _ in range(self.layers)]
         self._kptrs = (ctypes.c_void_p * self.layers)(*[t.data_ptr() for t in self.k])
         self._slots = None       # device int32 [t, 2] of the step reserved last
         self._tiles_dev = None   # device int32 [capacity, 3]: the tile table, rows [0, n) valid
@@ -337,6 +339,15 @@ class PagedKV:
         self._ktab = None        # device int32 [T, 4]: tiles + logical start, for prefill
         self._ktab_starts = None
         self._ktab_ver = -1
+
+    def _row(self):
+        """Elements and type of a pool's row."""
+        return self.d, self.dtype
+
+    @property
+    def row_bytes(self):
+        """Bytes of a token's key (or value) of one head."""
+        return self._row()[0] * self._row()[1].itemsize
 
     @property
     def n(self):
@@ -441,15 +452,8 @@ class PagedKV:
                 k_new, v_new = k_new.contiguous(), v_new.contiguous()
         if q.stride(-1) != 1:
             q = q.contiguous()
-        if window is None:
-            (tiles, nt), n = self._tiles(), self.table.n
-            if sinks:
-                raise ValueError("PagedKV.decode: sinks go with a window")
-        else:
-            if window < 1 or sinks < 0:
-                raise ValueError(f"PagedKV.decode: needs window >= 1 and sinks >= 0, got {window} and {sinks}")
-            tiles, nt, n = self._window_tiles(int(window), int(sinks))
-            stable_tiles = 0
+        tiles, nt, n = self._decode_tiles(window, sinks, "PagedKV.decode")
+        stable_tiles = 0 if window is not None else stable_tiles
         out = torch.empty((hkv, g, d), dtype=q.dtype, device=q.device)
         code = dtype_code(q, "PagedKV.decode")
         ws = workspaces.get(("decode", hkv), q.device, _lib.decode_workspace_bound(1, hkv, g, d, code))
@@ -508,6 +512,16 @@ class PagedKV:
                 stream_ptr(q.device))
         check("tc_decode_attention_shared_paged", st)
         return out
+
+    def _decode_tiles(self, window, sinks, what):
+        """Device tile table of a decode, its length and the tokens it lists, for all tokens or a window's."""
+        if window is None:
+            if sinks:
+                raise ValueError(f"{what}: sinks go with a window")
+            return (*self._tiles(), self.table.n)
+        if window < 1 or sinks < 0:
+            raise ValueError(f"{what}: needs window >= 1 and sinks >= 0, got {window} and {sinks}")
+        return self._window_tiles(int(window), int(sinks))
 
     def _prefill_table(self):
         """Device int32 [T, 4] = (page, first row, rows, logical position of the first row) of the
@@ -651,3 +665,114 @@ class PagedKV:
                 k.stride(0), k.stride(1), self.page_rows, self.table.num_pages, sp, sh, sr, ktab.data_ptr(),
                 ktab.shape[0], _lib.DTYPE_CODE[self.dtype], stream_ptr(self.device)))
         return k, v
+
+
+class PagedKVInt4(PagedKV):
+    """PagedKV whose rows are held in 4 bits (threadcut_b200.int4: 5 d / 8 bytes a row instead of 2 d): the same steps,
+    splices and reads over uint8 pools [pages, hkv, page_rows, row_bytes(d)]. dtype (bf16 or fp16) is the type that keys and
+    values come in and are read back as; d 64, 128 or 256.
+
+    Keys that a splice rotates are quantised again: each splice that moves a key may move its elements by half a level.
+    The shared decode has no form over such rows: gather the context once and use decode_attention_shared."""
+
+    def __init__(self, layers, hkv, d, *, dtype=torch.bfloat16, **kwargs):
+        if d not in int4.HEAD_SIZES or dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError(f"PagedKVInt4: needs bf16 or fp16 and heads of 64, 128 or 256, got {dtype} and {d}")
+        super().__init__(layers, hkv, d, dtype=dtype, **kwargs)
+
+    def _row(self):
+        return int4.row_bytes(self.d), torch.uint8
+
+    def _step(self, k, what):
+        t = k.shape[-2]
+        if self._slots is None or self._slots.shape[0] != t:
+            raise ValueError(f"{what}: reserve(t) the step's slots first (same t)")
+        if tuple(k.shape[-3:]) != (self.hkv, t, self.d) or k.dtype != self.dtype:
+            raise ValueError(f"{what}: expected [{self.hkv}, t, {self.d}] {self.dtype}, got {tuple(k.shape)} {k.dtype}")
+
+    def write(self, layer, k, v):
+        """Quantises and writes the reserved step's rows of one layer: k, v [hkv, t, d] (or [1, hkv, t, d])."""
+        self._step(k, "PagedKVInt4.write")
+        int4.write_int4(k, v, self.k[layer], self.v[layer], self._slots)
+
+    def append(self, layer, k, v, cos, sin, *, q=None, q_norm=None, k_norm=None, eps=1e-6):
+        """PagedKV.append with the keys and values quantised: int4.append_rope_int4 into this layer's pools."""
+        self._step(k, "PagedKVInt4.append")
+        return int4.append_rope_int4(k, v, cos, sin, self.k[layer], self.v[layer], self._slots, q=q, q_norm=q_norm,
+                                     k_norm=k_norm, eps=eps)
+
+    def decode(self, layer, q, scale, *, k_new=None, v_new=None, splits=None, stable_tiles=0, window=None, sinks=0):
+        """PagedKV.decode over the 4-bit rows (decode_attention_int4): q [hkv, g, d], at most 16 query heads a KV head.
+        k_new / v_new [hkv, d] (or [hkv, 1, d]) are written first, in a launch of their own. stable_tiles changes nothing."""
+        what = "PagedKVInt4.decode"
+        require_cuda(q, what=what)
+        if q.dim() != 3 or q.shape[0] != self.hkv or q.shape[2] != self.d or q.dtype != self.dtype:
+            raise ValueError(f"{what}: q {tuple(q.shape)} {q.dtype} does not match the cache")
+        if (k_new is None) != (v_new is None):
+            raise ValueError(f"{what}: k_new and v_new go together")
+        if k_new is not None:
+            if self._slots is None or self._slots.shape[0] != 1:
+                raise ValueError(f"{what}: reserve(1) the step's slot first")
+            self.write(layer, k_new.reshape(self.hkv, 1, self.d), v_new.reshape(self.hkv, 1, self.d))
+        tiles, nt, _ = self._decode_tiles(window, sinks, what)
+        if nt == 0:
+            return torch.zeros_like(q)
+        return int4.decode_attention_int4(q, self.k[layer], self.v[layer], scale, tiles=tiles[:nt], splits=splits)
+
+    def decode_shared(self, layer, q, k, v, scale, lengths=None):
+        raise ValueError("PagedKVInt4.decode_shared: no shared decode over 4-bit rows; gather(layer) the context once and use "
+                         "flash_decode.decode_attention_shared")
+
+    def prefill(self, layer, query, scale, *, splits=None, window=None, sinks=0):
+        """PagedKV.prefill: the rows that the chunk's queries see are read back as 16-bit keys and values (gather_int4)
+        and the contiguous kernels run over them."""
+        what = "PagedKVInt4.prefill"
+        require_cuda(query, what=what)
+        n = self.n
+        if (query.dim() != 4 or query.shape[0] != 1 or query.shape[3] != self.d or query.dtype != self.dtype
+                or not 1 <= query.shape[2] <= n):
+            raise ValueError(f"{what}: query {tuple(query.shape)} {query.dtype} does not fit the cache")
+        if window is None:
+            if sinks:
+                raise ValueError(f"{what}: sinks go with a window")
+            k, v = self.gather(layer)
+            return prefill_attention(query, k[None], v[None], scale, splits=splits)
+        if window < 1 or sinks < 0:
+            raise ValueError(f"{what}: needs window >= 1 and sinks >= 0, got {window} and {sinks}")
+        first = max(0, n - query.shape[2] - int(window) + 1) if sinks == 0 else 0
+        k, v = self.gather(layer, first)
+        return prefill_attention_window(query, k[None], v[None], scale, int(window), int(sinks), splits=splits)
+
+    def splice(self, s: Split, inv_freq):
+        """A.B.C -> A.C on every layer: B's pages return to the pool, C's keys are rotated by -(c0 - a) positions and
+        quantised again where they lie (int4.rotate_keys_int4)."""
+        runs_c, _ = self.table.splice(s)
+        gap = int(s.c0) - int(s.a)
+        if gap and runs_c.shape[0]:
+            tiles = torch.from_numpy(PageTable.tiles_of(runs_c)).to(self.device)
+            int4.rotate_keys_int4(self.k, tiles, -gap, inv_freq, self.dtype)
+
+    def compact(self):
+        """PagedKV.compact; the rows' bytes are moved as they are."""
+        at = torch.from_numpy(self.table.positions()).to(self.device)
+        new = PagedKVInt4(self.layers, self.hkv, self.d, max_tokens=self.table.num_pages * self.page_rows,
+                          page_rows=self.page_rows, dtype=self.dtype, device=self.device, spare_pages=0)
+        if self.n:
+            to = new.reserve(self.n).long()
+            for l in range(self.layers):
+                for pools, fresh in ((self.k, new.k), (self.v, new.v)):
+                    fresh[l][to[:, 0], :, to[:, 1]] = pools[l][at[:, 0], :, at[:, 1]]
+                    pools[l] = None  # free the old pools layer by layer
+        self.__dict__.update(new.__dict__)
+
+    def gather(self, layer, first=0):
+        """Contiguous (K, V) [hkv, n - first, d] of the tokens from `first` on, in logical order and of the cache's dtype."""
+        n = self.n
+        if first == 0:
+            tiles = self._prefill_table()[0] if n else torch.zeros((0, 4), dtype=torch.int32, device=self.device)
+        else:
+            tab = self.table._span(first, n, *self.table._index())[1]
+            start = np.cumsum(tab[:, 2], dtype=np.int64) - tab[:, 2]
+            tab = np.concatenate((tab, start[:, None].astype(np.int32)), axis=1)
+            tiles = torch.from_numpy(np.ascontiguousarray(tab)).to(self.device)
+        return int4.gather_int4(self.k[layer], self.v[layer], tiles, n - first, self.dtype)

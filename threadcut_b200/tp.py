@@ -37,6 +37,8 @@ import torch.distributed as dist
 from . import kv as _kv
 from ._lib import check, dtype_code, lib, require_cuda, stream_ptr
 from .flash_decode import decode_attention_append, decode_attention_append_rope
+from .int4 import Int4Weight, gemv_int4, quantize_weight
+from .paged import PagedKVInt4
 from .sharded import head_shard
 
 __all__ = ["TPDecoder", "accelerate"]
@@ -73,7 +75,9 @@ def _silu_mul(gu, out):
 def _gemv(x, w):
     """x [1, K] @ w[N, K]^T -> [1, N] for the one-token projections: tc_gemv (HBM-bound, fp32
     accumulation) for contiguous 16-bit operands with K a multiple of 8 and 16-byte aligned; other
-    operands take the GPU library matmul. CPU tensors raise."""
+    operands take the GPU library matmul. A 4-bit w (Int4Weight) takes gemv_int4. CPU tensors raise."""
+    if isinstance(w, Int4Weight):
+        return gemv_int4(x, w)
     require_cuda(x, w, what="gemv")
     n, k = w.shape
     if (x.dtype in (torch.bfloat16, torch.float16) and w.dtype == x.dtype and x.is_contiguous() and w.is_contiguous()
@@ -87,7 +91,9 @@ def _gemv(x, w):
 
 def _gemv_swiglu(gu, w):
     """silu(gate) * up from gu [1, 2I] (gate | up) times w[N, I]^T -> [1, N]: the SwiGLU activation
-    computed while the GEMV stages its input (tc_gemv_swiglu, one launch)."""
+    computed while the GEMV stages its input (tc_gemv_swiglu, one launch; a 4-bit w: gemv_int4)."""
+    if isinstance(w, Int4Weight):
+        return gemv_int4(gu, w, swiglu=True)
     require_cuda(gu, w, what="gemv_swiglu")
     n, k = w.shape
     if not (gu.dtype == w.dtype and gu.dtype in (torch.bfloat16, torch.float16) and gu.is_contiguous()
@@ -121,10 +127,27 @@ def _attend_rope(layer, q, k, v, wq, wk, cos, sin, eps, scale):
                                         stable_rows=stable)
 
 
-class _Shard:
-    """One layer's weights on this rank."""
+def _attend_paged(layer, q, k, v, wq, wk, cos, sin, eps, scale):
+    """_attend_rope over a paged cache layer (kv.PagedLayer): q/k norm, RoPE and the row's write in
+    one launch, attention over the pages in the next. Layer 0 takes the step's slot for every layer."""
+    kv = layer.state.kv
+    if layer.index == 0:
+        layer.state.flush_all()
+        try:
+            kv.reserve(1)
+        except MemoryError:
+            kv.compact()
+            kv.reserve(1)
+    hr, g, d = q.shape
+    q = kv.append(layer.index, k[:, None], v[:, None], cos[None], sin[None], q=q.reshape(hr * g, 1, d), q_norm=wq, k_norm=wk,
+                  eps=eps)
+    return kv.decode(layer.index, q.reshape(hr, g, d), scale)
 
-    def __init__(self, layer, h0, h1, g, d, i0, i1, dev, interleave_gu=False):
+
+class _Shard:
+    """One layer's weights on this rank, the projections in 16 bits or (bits=4) as Int4Weights."""
+
+    def __init__(self, layer, h0, h1, g, d, i0, i1, dev, interleave_gu=False, bits=16):
         at, mlp = layer.self_attn, layer.mlp
 
         def rows(w, lo, hi):
@@ -149,6 +172,8 @@ class _Shard:
                     if interleave_gu else torch.cat((gate, up)))
         del gate, up
         self.wd = cols(mlp.down_proj.weight, i0, i1)
+        if bits == 4:
+            self.wqkv, self.wo, self.wgu, self.wd = (quantize_weight(w) for w in (self.wqkv, self.wo, self.wgu, self.wd))
         for name in ("q_proj", "k_proj", "v_proj", "o_proj"):
             if getattr(at, name).bias is not None:
                 raise ValueError(f"TPDecoder: {name} with a bias is not supported (Qwen3 has none)")
@@ -161,10 +186,19 @@ class TPDecoder:
     model: the full HF model (any device; only this rank's slices are copied to `device`).
     step(token, pos) -> next token id (int64 device tensor [1]); appends the token's K/V row.
     load(layer, k, v): fill layer's cache from full-head K/V [1 or -, hkv, n, d] (own heads kept).
-    splice(s, inv_freq): kv.splice on the local heads.  crop(n): drop rows past n."""
+    splice(s, inv_freq): kv.splice on the local heads.  crop(n): drop rows past n.
+    weight_bits=4: the projections and lm_head in 4 bits (int4.quantize_weight, groups of 64), multiplied by gemv_int4; the
+    sums then go through launches of their own (as with peer_sums=False)."""
 
-    def __init__(self, model, device, group=None, world=None, rank=None, peer_sums=True):
+    def __init__(self, model, device, group=None, world=None, rank=None, peer_sums=True, weight_bits=16):
         cfg = model.config
+        if weight_bits not in (4, 16):
+            raise ValueError(f"TPDecoder: weights have 4 or 16 bits, got {weight_bits}")
+        if weight_bits == 4:
+            if model.model.embed_tokens.weight.dtype not in (torch.bfloat16, torch.float16):
+                raise ValueError("TPDecoder: 4-bit weights need a bf16 or fp16 model")
+            peer_sums = False
+        self.weight_bits = weight_bits
         kinds = set(getattr(cfg, "layer_types", None) or ["full_attention"])
         if getattr(cfg, "use_sliding_window", False) or kinds != {"full_attention"}:
             raise ValueError("TPDecoder: sliding-window attention layers are not supported")
@@ -188,10 +222,13 @@ class TPDecoder:
         base = model.model
         peer_capable = self.dev.type == "cuda" and base.embed_tokens.weight.dtype in (torch.bfloat16, torch.float16)
         self.layers_w = [_Shard(layer, self.h0, self.h1, self.g, self.d, i0, i1, self.dev,
-                                interleave_gu=peer_sums and peer_capable) for layer in base.layers]
+                                interleave_gu=peer_sums and peer_capable, bits=weight_bits)
+                         for layer in base.layers]
         self.embed = base.embed_tokens.weight.detach().to(self.dev)
         self.final_norm = base.norm.weight.detach().to(self.dev)
         self.lm_head = model.lm_head.weight.detach()[self.v0:v1].to(self.dev).contiguous()
+        if weight_bits == 4:
+            self.lm_head = quantize_weight(self.lm_head)
         self.inv_freq = base.rotary_emb.inv_freq.detach().float().to(self.dev)
         self.attn_scaling = float(getattr(base.rotary_emb, "attention_scaling", 1.0))
         self.scale = model.model.layers[0].self_attn.scaling
@@ -259,7 +296,9 @@ class TPDecoder:
         hr, d, g = self.h1 - self.h0, self.d, self.g
         nq = hr * g
         q, k, v = qkv[:nq * d].view(nq, d), qkv[nq * d:(nq + hr) * d].view(hr, d), qkv[(nq + hr) * d:].view(hr, d)
-        if self.fuse_rope:
+        if isinstance(layer, _kv.PagedLayer):
+            o = _attend_paged(layer, q.view(hr, g, d), k, v, w.q_norm, w.k_norm, cos, sin, self.eps, self.scale)
+        elif self.fuse_rope:
             o = _attend_rope(layer, q.view(hr, g, d), k, v, w.q_norm, w.k_norm, cos, sin, self.eps, self.scale)
         else:
             _qk_norm_rope(q, k, w.q_norm, w.k_norm, cos, sin, self.eps)
@@ -403,12 +442,18 @@ class TPDecoder:
 
 
 def _fusable(cache, dec):
-    """True when `cache` is this package's contiguous cache of the model `dec` decodes: every layer a
-    GrowingLayer holding rows, with the fused append on, in the model's dtype, on its device, with
-    the local head count."""
+    """True when `cache` is this package's cache of the model `dec` decodes: every layer a GrowingLayer holding
+    rows, with the fused append on, or a PagedLayer of one store of 4-bit rows, in the model's dtype, on its device,
+    with the local head count."""
     layers = getattr(cache, "layers", None)
     if not layers or len(layers) != len(dec.layers_w):
         return False
+    if all(isinstance(ly, _kv.PagedLayer) for ly in layers):
+        state = layers[0].state
+        kv = state.kv
+        return (isinstance(kv, PagedKVInt4) and state.fuse and kv.n > 0 and all(ly.state is state for ly in layers)
+                and kv.dtype == dec.dtype and kv.device == dec.embed.device and kv.hkv == dec.h1 - dec.h0 and kv.d == dec.d
+                and dec.g <= 16)
     for ly in layers:
         if not (isinstance(ly, _kv.GrowingLayer) and ly.fuse_append and ly.is_initialized
                 and getattr(ly, "kbuf", None) is not None and ly.n > 0):
@@ -419,20 +464,21 @@ def _fusable(cache, dec):
     return True
 
 
-def accelerate(model, device=None):
+def accelerate(model, device=None, weight_bits=16):
     """Route the one-token decode steps of a one-GPU Qwen3 model through the fused step of this
     module, behind the model's own call: after accelerate(model), model(input_ids=[[t]],
     past_key_values=cache, use_cache=True) over a cache of this package (kv.new_cache with the
-    threadcut attention: GrowingLayers with the fused append, holding rows) returns HF's output type
-    with `.logits` [1, 1, vocab] computed by TPDecoder at world 1 (7 launches per layer instead
+    threadcut attention: GrowingLayers with the fused append, or a paged cache of 4-bit rows, holding rows) returns
+    HF's output type with `.logits` [1, 1, vocab] computed by TPDecoder at world 1 (7 launches per layer instead
     of transformers' ~50), appending the token's K/V row to the same cache. Every other call (a
     prefill chunk, another cache, extra arguments) goes to the model's own forward. The reference's
     engine (threadcut/engine.py:66-73, 88-95) makes exactly such calls, so it runs unchanged on the
     fused step. Returns the TPDecoder doing the work (it shares the model's weights where no copy is
-    needed: the q|k|v and gate|up rows are concatenated copies). bf16/fp16 models only."""
+    needed: the q|k|v and gate|up rows are concatenated copies). weight_bits=4: the fused step's own copies of the
+    projections are held in 4 bits (the model's forward, and so a prefill, keeps the 16-bit ones). bf16/fp16 models only."""
     from transformers.modeling_outputs import CausalLMOutputWithPast
     dev = torch.device(device) if device is not None else next(model.parameters()).device
-    dec = TPDecoder(model, dev, world=1, rank=0)
+    dec = TPDecoder(model, dev, world=1, rank=0, weight_bits=weight_bits)
     if dec.dtype not in (torch.bfloat16, torch.float16):
         raise ValueError("accelerate: the fused step needs a bf16 or fp16 model")
     inner = model.forward
