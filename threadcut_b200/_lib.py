@@ -164,7 +164,7 @@ def host():
                         "tc_prefill_attention_window", "tc_prefill_window_workspace_size", "tc_decode_attention_shared",
                         "tc_decode_attention_shared_workspace_size")))
                     mod.init_int4(*(ctypes.cast(getattr(handle, name), ctypes.c_void_p).value for name in (
-                        "tc_int4_append_rope", "tc_int4_gather", "tc_decode_attention_int4",
+                        "tc_int4_append_rope", "tc_int4_gather", "tc_int4_rotate_keys", "tc_decode_attention_int4",
                         "tc_decode_attention_int4_paged", "tc_decode_attention_int4_workspace_size", "tc_gemv_int4")))
                 _host = mod
     return _host or None

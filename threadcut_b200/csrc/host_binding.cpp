@@ -12,7 +12,7 @@
 //
 // append_rope, window_decode, window_prefill and shared_decode do the same for paged.append_rope,
 // flash_decode.decode_attention_window / decode_attention_shared and prefill.prefill_attention_window;
-// int4_append, int4_gather, int4_decode and int4_gemv for the functions of int4.py.
+// int4_append, int4_gather, int4_rotate, int4_decode and int4_gemv for the functions of int4.py.
 #include <torch/extension.h>
 #include <torch/csrc/Dtype.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
@@ -24,6 +24,7 @@
 #include <map>
 #include <optional>
 #include <tuple>
+#include <vector>
 
 namespace {
 
@@ -334,6 +335,8 @@ py::object shared_decode(const at::Tensor& q_in, const at::Tensor& kp, const at:
 using Int4AppendFn = AppendFn;
 using Int4GatherFn = int (*)(const void*, const void*, void*, void*, int, int, int64_t, int64_t, int64_t, int64_t, int64_t,
                              int64_t, int64_t, int64_t, const int32_t*, int64_t, int, void*);
+using Int4RotateFn = int (*)(void* const*, int, int, int, int64_t, int64_t, int64_t, int64_t, int64_t, const int32_t*, int,
+                             int64_t, const float*, int, void*);
 using Int4DecodeFn = int (*)(const void*, const void*, const void*, void*, int, int, int, int, int64_t, const int32_t*,
                              int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t,
                              int64_t, int64_t, float, int, int, void*, size_t, void*);
@@ -346,14 +349,16 @@ using Int4GemvFn = int (*)(const void*, const void*, const void*, void*, int64_t
 
 Int4AppendFn g_int4_append = nullptr;
 Int4GatherFn g_int4_gather = nullptr;
+Int4RotateFn g_int4_rotate = nullptr;
 Int4DecodeFn g_int4_decode = nullptr;
 Int4PagedFn g_int4_paged = nullptr;
 Int4SizeFn g_int4_size = nullptr;
 Int4GemvFn g_int4_gemv = nullptr;
 
-void init_int4(int64_t append, int64_t gather, int64_t decode, int64_t paged, int64_t size, int64_t gemv) {
+void init_int4(int64_t append, int64_t gather, int64_t rotate, int64_t decode, int64_t paged, int64_t size, int64_t gemv) {
   g_int4_append = reinterpret_cast<Int4AppendFn>(append);
   g_int4_gather = reinterpret_cast<Int4GatherFn>(gather);
+  g_int4_rotate = reinterpret_cast<Int4RotateFn>(rotate);
   g_int4_decode = reinterpret_cast<Int4DecodeFn>(decode);
   g_int4_paged = reinterpret_cast<Int4PagedFn>(paged);
   g_int4_size = reinterpret_cast<Int4SizeFn>(size);
@@ -454,6 +459,37 @@ py::object int4_gather(const at::Tensor& k_pool, const at::Tensor& v_pool, const
   return py::make_tuple(k, v);
 }
 
+// Whether it was done: frequencies on the host, as many layers as a launch takes.
+bool int4_rotate(const std::vector<at::Tensor>& pools, const at::Tensor& tiles, int64_t delta, const at::Tensor& inv_freq,
+                 py::object dtype) {
+  if (g_int4_rotate == nullptr || pools.empty() || pools.size() > 128 || !THPDtype_Check(dtype.ptr())) return false;
+  const at::Tensor& first = pools[0];
+  const int code = dtype_code(reinterpret_cast<THPDtype*>(dtype.ptr())->scalar_type);
+  if (code < 1 || !first.is_cuda() || first.dim() != 4) return false;
+  const auto dev = first.device();
+  const int64_t hkv = first.size(1), d = first.size(3) * 8 / 5;
+  if (!int4_head(d) || hkv > 65535 || !int4_tiles(tiles, dev, 3) || !inv_freq.device().is_cpu() ||
+      inv_freq.scalar_type() != at::kFloat || inv_freq.dim() != 1 || inv_freq.size(0) * 2 != d)
+    return false;
+  void* at[128];
+  for (size_t i = 0; i < pools.size(); ++i) {
+    if (!int4_pools(first, pools[i], dev, hkv, d)) return false;
+    at[i] = pools[i].data_ptr();
+  }
+  float table[256];
+  {
+    // as the reference makes it: the angles as 32-bit numbers, then their cos and sin
+    const at::Tensor angle = inv_freq.detach().mul(at::Scalar(delta)).contiguous();
+    const at::Tensor c = angle.cos(), s = angle.sin();
+    std::copy_n(c.const_data_ptr<float>(), d / 2, table);
+    std::copy_n(s.const_data_ptr<float>(), d / 2, table + d / 2);
+  }
+  c10::cuda::CUDAGuard guard(dev);
+  return g_int4_rotate(at, (int)pools.size(), (int)hkv, (int)d, first.size(2), first.size(0), first.stride(0), first.stride(1),
+                       first.stride(2), tiles.data_ptr<int32_t>(), (int)tiles.size(1), tiles.size(0), table, code,
+                       c10::cuda::getCurrentCUDAStream(dev.index()).stream()) == 0;
+}
+
 py::object int4_decode(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, double scale, const OptTensor& lengths,
                        const OptTensor& tiles, int64_t splits) {
   if (g_int4_decode == nullptr || !q.is_cuda() || q.dim() != (tiles ? 3 : 4)) return py::none();
@@ -532,6 +568,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("init_int4", &init_int4, "set the addresses of the 4-bit entry points");
   m.def("int4_append", &int4_append, "checked int4.append_rope_int4 / write_int4 fast path: (done, queries)");
   m.def("int4_gather", &int4_gather, "checked int4.gather_int4 fast path; None means: take the Python path");
+  m.def("int4_rotate", &int4_rotate, "checked int4.rotate_keys_int4 fast path: whether it was done");
   m.def("int4_decode", &int4_decode, "checked int4.decode_attention_int4 fast path; None means: take the Python path");
   m.def("int4_gemv", &int4_gemv, "checked int4.gemv_int4 fast path; None means: take the Python path");
   m.def("partial", &partial, "checked decode_attention_partial fast path; None means: take the Python path");

@@ -117,6 +117,10 @@ __device__ __forceinline__ uint32_t i4_ones(uint32_t w) {
   }
 }
 
+// Two products, each rounded: an fma with -0, which is not merged with a sum that follows it, as packed products are. (nz is -0
+// from memory: as a constant it would make them products again.)
+__device__ __forceinline__ float2 product2(float2 a, float2 b, float2 nz) { return ffma2(a, b, nz); }
+
 template <typename X>
 __device__ __forceinline__ void load8(const X* p, float (&x)[8]) {
   constexpr int V = 16 / sizeof(X);
@@ -139,15 +143,21 @@ __device__ __forceinline__ float by_15_16(float x) {
 
 // Codes of this lane's 8 elements (w: pairs of T) of a group that four neighbouring lanes (aligned to 4) hold, and the
 // group's (S, z). Every lane of the warp calls it.
-// The extremes as packed maxima and minima. A code is 15 u rounded, u = (16/15) (x - z) / S - 16/15 saturated into [0, 1] as the
-// fma goes. Many elements of coarse 16-bit data lie exactly on a border between two levels, and the even one is theirs: 15 u is
-// off by 7e-6 at most (1 ulp of the reciprocal, two roundings, times 2.1 * 15), so it is first rounded to a multiple of
-// 2^-16, which a border is. (An element 2^-17 of a level beside one counts as on it.) Nearly all of that runs on the fma pipe;
-// the codes are collected as the floats' bits, whose exponents add up to a constant.
-// With the border decided by the exact remainder, comparisons and fp32 extremes instead, a 16,384-token prompt of 48 heads of
-// 128 took 45 instructions an element and 170 us.
+// The extremes as packed maxima and minima. A code is x (16/S) + (-16 z/S - 16) rounded. Many elements of coarse 16-bit data
+// lie exactly on a border between two levels, and the even one is theirs. That sum is off by at most 4.3e-6: 32 * 2^-24 from
+// 16/S (one Newton step behind the approximate reciprocal), 2^-19 from the offset's rounding while it is below 64, 2^-21 from
+// its own. So it is first rounded to a multiple of 2^-16, which a border is (half of one is 7.6e-6; an element 2^-17 of a level
+// beside one counts as on it), then to a whole number, both by adding constants, two elements an instruction; the codes are
+// collected as the floats' bits, whose exponents add up to a constant. No clamp: below that offset z's and S's roundings move
+// an end by 0.2 of a level at most.
+// Groups that this does not hold for (S subnormal, far from 1 or 0, values many times their spread, NaN) send their warp another way:
+// (x - z) / S by itself, scaled by a power of two where (in bf16) the reciprocal or x - z would overflow, and clamped; 15 u
+// with u of [0, 1] is off by 7e-6 there.
+// A prompt of 49,152 tokens (8 heads of 128, keys and values) is quantised in @W us so, in 76 with the other way for all, and a
+// 16,384-token prompt of 48 heads took 170 us with borders decided by exact remainders and comparisons.
 template <typename T>
 __device__ __forceinline__ uint32_t quantise8(const uint32_t (&w)[4], uint32_t& param) {
+  constexpr bool bf = I4<T>::kBit == 3;
   const uint32_t hi2 = I4<T>::max2(I4<T>::max2(w[0], w[1]), I4<T>::max2(w[2], w[3]));
   const uint32_t lo2 = I4<T>::min2(I4<T>::min2(w[0], w[1]), I4<T>::min2(w[2], w[3])) ^ 0x80008000u;
   uint32_t m = I4<T>::max2(i4_low2(hi2, lo2), i4_high2(hi2, lo2));  // (largest, largest negative)
@@ -156,31 +166,44 @@ __device__ __forceinline__ uint32_t quantise8(const uint32_t (&w)[4], uint32_t& 
   const float hi = Mma<T>::lo(m), lo = -Mma<T>::hi(m);
   const uint32_t st = Mma<T>::pack(by_15_16(__fsub_rn(hi, lo)), 0.f);
   float s = Mma<T>::lo(st);
-  const uint32_t both = Mma<T>::pack(s, __fsub_rn(lo, s));
-  float z = Mma<T>::hi(both);
-  param = fabsf(z) == INFINITY ? both | 0x7fffu : both;  // S NaN: a finite S would leave infinities that look like data
+  param = Mma<T>::pack(s, __fsub_rn(lo, s));
+  float z = Mma<T>::hi(param);
+  constexpr float kWhole = 12582912.f;  // 1.5 * 2^23: adding it leaves a whole number in the low bits
+  constexpr float kSnap = 192.f;        // 1.5 * 2^7: adding it leaves multiples of 2^-16
+  uint32_t sum = 0u - 0x4b400000u * 0x11111111u;  // the bits of kWhole, as often as they come in
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(0.0625f * s));
+  r = fmaf(r, fmaf(-0.0625f * s, r, 1.f), r);
+  const float c = fmaf(-z, r, -16.f);
+  const bool plain = s >= (bf ? 1e-30f : 6.103515625e-5f) && s <= (bf ? 1e30f : 65504.f) && fabsf(c) < 64.f;
+  if (__all_sync(0xffffffffu, plain)) {
+    uint32_t codes = 0u;
+#pragma unroll
+    for (int i = 3; i >= 0; --i) {
+      float2 t = ffma2(make_float2(Mma<T>::lo(w[i]), Mma<T>::hi(w[i])), make_float2(r, r), make_float2(c, c));
+      t = fadd2(fadd2(t, make_float2(kSnap, kSnap)), make_float2(kWhole - kSnap, kWhole - kSnap));
+      codes = (codes * 16u + __float_as_uint(t.y)) * 16u + __float_as_uint(t.x);
+    }
+    return codes + sum;
+  }
+  if (fabsf(z) == INFINITY) param |= 0x7fffu;  // S NaN: a finite S would leave infinities that look like data
   float by = 1.f;
-  if constexpr (I4<T>::kBit == 3) {
-    // where (in bf16) the reciprocal or x - z would overflow: the same levels, a power of two larger or smaller
+  if constexpr (bf) {
     by = s < 1e-30f ? 18446744073709551616.f : s > 1e30f ? 1.f / 18446744073709551616.f : 1.f;
     s *= by;
     z *= by;
   }
   constexpr float kUnit = 16.f / 15.f;
-  float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
   r = s > 0.f ? kUnit * r : 0.f;
-  constexpr float kWhole = 12582912.f;  // 1.5 * 2^23: adding it leaves a whole number in the low bits
-  constexpr float kSnap = 192.f;        // 1.5 * 2^7: adding it leaves multiples of 2^-16
-  uint32_t word = 0u - 0x4b400000u * 0x11111111u;  // the bits of kWhole, as often as they come in
-  uint32_t sum = 0u;
+  uint32_t codes = 0u;
 #pragma unroll
   for (int e = 7; e >= 0; --e) {
     const float x = e & 1 ? Mma<T>::hi(w[e / 2]) : Mma<T>::lo(w[e / 2]);
-    const float u = __saturatef(fmaf(I4<T>::kBit == 3 ? fmaf(x, by, -z) : x - z, r, -kUnit));  // NaN gives 0
-    sum = sum * 16u + __float_as_uint(fmaf(u, 15.f, kSnap) + (kWhole - kSnap));
+    const float u = __saturatef(fmaf(bf ? fmaf(x, by, -z) : x - z, r, -kUnit));  // NaN gives 0
+    codes = codes * 16u + __float_as_uint(fmaf(u, 15.f, kSnap) + (kWhole - kSnap));
   }
-  return sum + word;
+  return codes + sum;
 }
 
 // ------------------------------------------------------------------------------------------------ writing
@@ -202,6 +225,7 @@ struct Int4AppendParams {
   int64_t s_page, s_h, s_row;
   const int32_t* slots;  // [t][2]: page, row
   float eps, inv_d;
+  float minus_zero;  // -0
 };
 
 // Rotation of 8 elements (fp32, first element i0) with the 8 they are paired with, by elementary fp32 operations (no
@@ -315,6 +339,7 @@ __device__ __forceinline__ void append_tokens(const Int4AppendParams& p, int grp
   const bool first = i0 < p.rot / 2;
   const int other = turns ? (first ? p.rot / 2 : -(p.rot / 2)) : 0;  // where its elements' partners are
   const T* w = static_cast<const T*>(kKind == 0 ? p.q_w : p.k_w);
+  const float2 nz = make_float2(p.minus_zero, p.minus_zero);
   for (uint32_t tok = tok0; tok < p.t; tok += step) {
     const T* src = src0 + tok * st;
     uint4 a[U], b[U];
@@ -377,9 +402,8 @@ __device__ __forceinline__ void append_tokens(const Int4AppendParams& p, int grp
         if (turns) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            // (not packed: those products and sums are contracted)
-            o[e] = Mma<T>::pack(__fadd_rn(__fmul_rn(x[e].x, cs[e].x), __fmul_rn(y[e].x, sn[e].x)),
-                                __fadd_rn(__fmul_rn(x[e].y, cs[e].y), __fmul_rn(y[e].y, sn[e].y)));
+            const float2 r = fadd2(product2(x[e], cs[e], nz), product2(y[e], sn[e], nz));
+            o[e] = Mma<T>::pack(r.x, r.y);
           }
         }
       }
@@ -429,6 +453,59 @@ __global__ void __launch_bounds__(256, i4_append_ctas(U, kNorm)) int4_append_vec
       append_tokens<T, TT, D, KU, 1, false>(p, grp - q_groups, tok0, step);
   } else {
     append_tokens<T, TT, D, KU, 2, false>(p, grp - q_groups - kv_groups, tok0, step);
+  }
+}
+
+// Keys and values alone, as they are, many of them: the same with the next token's rows loaded before this one's are quantised
+// (it is bound by the bytes in flight otherwise).
+constexpr int kI4WriteHeads = 4;  // heads of a lane, times 256/D of a warp
+
+template <typename T, int D>
+__global__ void __launch_bounds__(256, 3) int4_write_kernel(const __grid_constant__ Int4AppendParams p) {
+  constexpr int L = D / 8;
+  constexpr int RW = 32 / L;
+  constexpr int U = kI4WriteHeads;
+  pdl_launch();
+  pdl_wait();
+  const int lane = threadIdx.x & 31, c = lane % L;
+  const uint32_t half = (p.hkv + RW * U - 1) / (RW * U);
+  const uint32_t warp = blockIdx.x * 8 + (threadIdx.x >> 5), step = gridDim.x * 8 / (2 * half);
+  if (warp / (2 * half) >= step) return;
+  const int grp = (int)(warp % (2 * half));
+  const bool isv = grp >= (int)half;
+  const int h0 = (isv ? grp - (int)half : grp) * RW * U + lane / L;
+  const int64_t sh = isv ? p.v_sh : p.k_sh, st = isv ? p.v_st : p.k_st;
+  const T* src = static_cast<const T*>(isv ? p.v : p.k) + h0 * sh + 8 * c;
+  uint8_t* pool = (isv ? p.vp : p.kp) + h0 * p.s_h;
+  uint4 next[U];
+  int2 slot;
+  uint32_t tok = warp / (2 * half);
+  const auto load = [&] {
+    slot = *reinterpret_cast<const int2*>(p.slots + 2 * (int64_t)tok);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      next[u] = h0 + u * RW < p.hkv ? *reinterpret_cast<const uint4*>(src + tok * st + u * RW * sh) : make_uint4(0u, 0u, 0u, 0u);
+  };
+  if (tok < p.t) load();
+  while (tok < p.t) {
+    uint4 now[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) now[u] = next[u];
+    const bool use = slot.x >= 0 && slot.x < p.num_pages && slot.y >= 0 && slot.y < p.page_rows;
+    uint8_t* row = pool + slot.x * p.s_page + slot.y * p.s_row;
+    tok += step;
+    if (tok < p.t) load();
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint32_t w[4] = {now[u].x, now[u].y, now[u].z, now[u].w};
+      uint32_t param;
+      const uint32_t word = quantise8<T>(w, param);
+      if (use && h0 + u * RW < p.hkv) {
+        uint8_t* at = row + u * RW * p.s_h;
+        *reinterpret_cast<uint32_t*>(at + 4 * c) = word;
+        if ((c & 3) == 0) *reinterpret_cast<uint32_t*>(at + D / 2 + c) = param;
+      }
+    }
   }
 }
 
@@ -511,29 +588,26 @@ struct Int4RotateParams {
   int tile_cols;
   int64_t n_tiles;
   float cs[kMaxRopeDim];  // cos of the D/2 angles, then sin
+  float minus_zero;       // -0
 };
 
 // Keys re-rotated in place by one angle a frequency (the splice of threadcut/kv.py:28-41 over 4-bit rows): a row's
 // values, rotated in fp32 as the 16-bit splice rotates them, rounded to T and quantised again. A warp per
-// (layer, tile, head); a row is D/8 lanes, the partner's values come from the lane half a row away. kI4Ahead rows' words are
-// loaded before any is turned. Bound by instructions (29 an element).
+// (layer, tile, head); a row is D/16 lanes, each with 8 elements of its first half and the 8 that they are paired with. kI4Ahead
+// rows' words are loaded before any is turned.
 template <typename T, int D>
 __global__ void __launch_bounds__(256, 3) int4_rotate_kernel(const __grid_constant__ Int4RotateParams p) {
-  constexpr int L = D / 8;
+  constexpr int L = D / 16;
   constexpr int RW = 32 / L;
   constexpr int A = kI4Ahead;
-  __shared__ float s_cs[D];
-  for (int i = threadIdx.x; i < D; i += blockDim.x) s_cs[i] = p.cs[i];
-  __syncthreads();
   const int lane = threadIdx.x & 31, c = lane % L;
-  const bool first = c < L / 2;
-  float cs[8], sn[8];
+  float2 cs[4], sn[4];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const int i = 8 * (c % (L / 2)) + e;
-    cs[e] = s_cs[i];
-    sn[e] = first ? -s_cs[D / 2 + i] : s_cs[D / 2 + i];
+  for (int e = 0; e < 4; ++e) {
+    cs[e] = make_float2(p.cs[8 * c + 2 * e], p.cs[8 * c + 2 * e + 1]);
+    sn[e] = make_float2(p.cs[D / 2 + 8 * c + 2 * e], p.cs[D / 2 + 8 * c + 2 * e + 1]);
   }
+  const float2 nz = make_float2(p.minus_zero, p.minus_zero);
   pdl_launch();
   pdl_wait();
   const int64_t per_layer = p.n_tiles * p.hkv;
@@ -549,39 +623,47 @@ __global__ void __launch_bounds__(256, 3) int4_rotate_kernel(const __grid_consta
     if (page < 0 || page >= p.num_pages) continue;
     uint8_t* base = p.kp[layer] + page * p.s_page + h * p.s_h + first_row * p.s_row;
 #pragma unroll 1
-    for (int r0 = 0; r0 < rows; r0 += A * RW) {  // the whole warp: the lanes exchange values
-      uint32_t word[A], param[A];
+    for (int r0 = 0; r0 < rows; r0 += A * RW) {  // the whole warp: quantise8 exchanges extremes
+      uint32_t wx[A], wy[A], qx[A], qy[A];
       bool use[A];
 #pragma unroll
       for (int u = 0; u < A; ++u) {
         const int r = r0 + u * RW + lane / L;
         const int64_t pr = first_row + r;
         use[u] = r < rows && pr >= 0 && pr < p.page_rows;
-        word[u] = param[u] = 0u;
+        wx[u] = wy[u] = qx[u] = qy[u] = 0u;
         if (use[u]) {
-          word[u] = *reinterpret_cast<const uint32_t*>(base + r * p.s_row + 4 * c);
-          param[u] = *reinterpret_cast<const uint32_t*>(base + r * p.s_row + D / 2 + 4 * (c / 4));
+          const uint32_t* row = reinterpret_cast<const uint32_t*>(base + r * p.s_row);
+          wx[u] = row[c];
+          wy[u] = row[D / 16 + c];
+          qx[u] = row[D / 8 + c / 4];
+          qy[u] = row[D / 8 + D / 64 + c / 4];
         }
       }
 #pragma unroll
       for (int u = 0; u < A; ++u) {
         if (r0 + u * RW >= rows) break;  // (the same for every lane)
-        uint32_t v[4], y[4], o[4];
-        i4_values<T>(word[u], param[u], v);
+        uint32_t vx[4], vy[4];
+        i4_values<T>(wx[u], qx[u], vx);
+        i4_values<T>(wy[u], qy[u], vy);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) y[i] = __shfl_xor_sync(0xffffffffu, v[i], L / 2);
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          o[e] = Mma<T>::pack(
-              __fadd_rn(__fmul_rn(Mma<T>::lo(v[e]), cs[2 * e]), __fmul_rn(Mma<T>::lo(y[e]), sn[2 * e])),
-              __fadd_rn(__fmul_rn(Mma<T>::hi(v[e]), cs[2 * e + 1]), __fmul_rn(Mma<T>::hi(y[e]), sn[2 * e + 1])));
-        uint32_t q;
-        const uint32_t w = quantise8<T>(o, q);
-        // every lane of the row has read it: the exchange above waited for them
+        for (int e = 0; e < 4; ++e) {
+          const float2 x = make_float2(Mma<T>::lo(vx[e]), Mma<T>::hi(vx[e])), y = make_float2(Mma<T>::lo(vy[e]), Mma<T>::hi(vy[e]));
+          const float2 a = fadd2(product2(x, cs[e], nz), product2(y, make_float2(-sn[e].x, -sn[e].y), nz));
+          const float2 b = fadd2(product2(y, cs[e], nz), product2(x, sn[e], nz));
+          vx[e] = Mma<T>::pack(a.x, a.y);
+          vy[e] = Mma<T>::pack(b.x, b.y);
+        }
+        const uint32_t ox = quantise8<T>(vx, qx[u]), oy = quantise8<T>(vy, qy[u]);
+        // every lane of a group has read its (S, z): the exchange above waited for them
         if (use[u]) {
-          uint8_t* row = base + (r0 + u * RW + lane / L) * p.s_row;
-          *reinterpret_cast<uint32_t*>(row + 4 * c) = w;
-          if ((c & 3) == 0) *reinterpret_cast<uint32_t*>(row + D / 2 + c) = q;
+          uint32_t* row = reinterpret_cast<uint32_t*>(base + (r0 + u * RW + lane / L) * p.s_row);
+          row[c] = ox;
+          row[D / 16 + c] = oy;
+          if ((c & 3) == 0) {
+            row[D / 8 + c / 4] = qx[u];
+            row[D / 8 + D / 64 + c / 4] = qy[u];
+          }
         }
       }
     }

@@ -43,6 +43,11 @@ template <typename T, int D>
 cudaError_t launch_int4_append(const Int4AppendParams& p, bool table_f32, bool vec, int sms, cudaStream_t st) {
   constexpr int RW = 256 / D;
   const int64_t warps = p.t * (cdiv(p.hq, RW) + 2 * cdiv(p.hkv, RW));
+  if (vec && p.hq == 0 && p.rot == 0 && p.k_w == nullptr && warps >= (int64_t)sms * 64) {
+    const int64_t groups = 2 * cdiv(p.hkv, RW * kI4WriteHeads), resident = (int64_t)sms * 24 / groups;
+    const int64_t rounds = cdiv(p.t, resident < 1 ? 1 : resident);
+    return launch_ex(int4_write_kernel<T, D>, dim3((unsigned)cdiv(cdiv(p.t, rounds) * groups, 8)), dim3(256), 0, st, p);
+  }
   if (vec)
     return warps < (int64_t)sms * 64 ? launch_int4_append_vec<T, D, 1>(p, table_f32, sms, st)
                                      : launch_int4_append_vec<T, D, 4>(p, table_f32, sms, st);
@@ -266,6 +271,7 @@ int tc_int4_append_rope(const void* q, const void* k, const void* v, void* q_out
   p.slots = slots;
   p.eps = eps;
   p.inv_d = 1.f / (float)d;
+  p.minus_zero = -0.f;
   bool vec = rot % 16 == 0 && aligned16(k) && aligned16(v) && stride16(k_stride_h, dtype) && stride16(k_stride_t, dtype) &&
              stride16(v_stride_h, dtype) && stride16(v_stride_t, dtype);
   if (hq > 0)
@@ -343,6 +349,7 @@ int tc_int4_rotate_keys(void* const* k_pools, int layers, int hkv, int d, int64_
   p.tile_cols = tile_cols;
   p.n_tiles = n_tiles;
   load_cos_sin(p.cs, cos_sin, d);
+  p.minus_zero = -0.f;
   const cudaError_t e =
       TC_INT4_DISPATCH(launch_int4_rotate, dtype, d, p, sm_count(current_device()), static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? TC_OK : TC_ERR_CUDA;

@@ -196,6 +196,8 @@ def rotate_keys_int4(k_pools, tiles, delta, inv_freq, dtype):
     k_pools = list(k_pools)
     if not k_pools:
         return
+    if (hb := _lib.host()) is not None and hb.int4_rotate(k_pools, tiles, int(delta), inv_freq, dtype):
+        return
     require_cuda(*k_pools, tiles, what=what)
     code = _code16(dtype, what)
     first = k_pools[0]
