@@ -618,7 +618,8 @@ int tc_decode_attention_int4_paged(const void* q, const void* k_pool, const void
  * (row r, columns 8c..8c+7), (row r + 8, the same), (row r, columns 32 + 8c..), (row r + 8, the same); code j of a word
  * is column 2j, code 4 + j column 2j + 1. params [ceil(n/16)][ceil(k/group)][8][2][2] of T: (S, z) of rows r, r + 8. Both 0
  * behind n and k, and 16-byte aligned. swiglu: x is [m][2k] (gate | up), the tokens silu(gate) * up. k up to
- * 65,536; more tokens than fit shared memory (32 at most) are taken in turns. */
+ * 65,536; more tokens than fit shared memory (32 at most) are taken in turns. Weights are constant, as tc_gemv's are: with
+ * programmatic dependent launch their first tiles are read while the kernel ahead in the stream still runs. */
 int tc_gemv_int4(const void* x, const void* codes, const void* params, void* out, int64_t n, int k, int64_t m, int group,
                  int64_t x_stride, int64_t out_stride, int swiglu, int dtype, void* stream);
 

@@ -153,8 +153,8 @@ __device__ __forceinline__ float by_15_16(float x) {
 // Groups that this does not hold for (S subnormal, far from 1 or 0, values many times their spread, NaN) send their warp another way:
 // (x - z) / S by itself, scaled by a power of two where (in bf16) the reciprocal or x - z would overflow, and clamped; 15 u
 // with u of [0, 1] is off by 7e-6 there.
-// A prompt of 49,152 tokens (8 heads of 128, keys and values) is quantised in @W us so, in 76 with the other way for all, and a
-// 16,384-token prompt of 48 heads took 170 us with borders decided by exact remainders and comparisons.
+// 49,152 keys of 8 heads of 128 are rotated in 36 us so, in 47 with the other way for all groups; a 16,384-token prompt (32
+// query and 8 KV heads) is written in 67 us, and took 170 with borders decided by exact remainders and comparisons.
 template <typename T>
 __device__ __forceinline__ uint32_t quantise8(const uint32_t (&w)[4], uint32_t& param) {
   constexpr bool bf = I4<T>::kBit == 3;
@@ -456,8 +456,8 @@ __global__ void __launch_bounds__(256, i4_append_ctas(U, kNorm)) int4_append_vec
   }
 }
 
-// Keys and values alone, as they are, many of them: the same with the next token's rows loaded before this one's are quantised
-// (it is bound by the bytes in flight otherwise).
+// Keys and values alone, as they are, many of them: the same with the next token's rows loaded before this one's are quantised,
+// as it is bound by the bytes in flight otherwise: 49,152 tokens of 8 heads of 128 in 49 us (5.4 TB/s), 74 without.
 constexpr int kI4WriteHeads = 4;  // heads of a lane, times 256/D of a warp
 
 template <typename T, int D>
@@ -594,7 +594,8 @@ struct Int4RotateParams {
 // Keys re-rotated in place by one angle a frequency (the splice of threadcut/kv.py:28-41 over 4-bit rows): a row's
 // values, rotated in fp32 as the 16-bit splice rotates them, rounded to T and quantised again. A warp per
 // (layer, tile, head); a row is D/16 lanes, each with 8 elements of its first half and the 8 that they are paired with. kI4Ahead
-// rows' words are loaded before any is turned.
+// rows' words are loaded before any is turned. Bound by instructions (18 an element, half of them on the half-rate pipe): 49,152
+// keys of 8 heads of 128 in 36 us, 47 with a lane's partners fetched by shuffles and converted twice.
 template <typename T, int D>
 __global__ void __launch_bounds__(256, 3) int4_rotate_kernel(const __grid_constant__ Int4RotateParams p) {
   constexpr int L = D / 16;

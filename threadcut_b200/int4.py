@@ -304,7 +304,9 @@ class Int4Weight(NamedTuple):
     codes: tiles of 16 rows and 64 columns. Bytes 16 (4 r + c) .. + 15 of a tile, r < 8, c < 4, are four little-endian
     words: (row r, columns 8 c .. 8 c + 7), (row r + 8, the same), (row r, columns 32 + 8 c ..), (row r + 8, the same);
     of a word's codes, number j is column 2 j and number 4 + j column 2 j + 1. params: (S, z) of rows r and r + 8.
-    Both are 0 behind row n and column k. A code stands for S (1 + code / 16) + z, not rounded further."""
+    Both are 0 behind row n and column k. A code stands for S (1 + code / 16) + z, not rounded further.
+    The tensors stay as they are: gemv_int4 may read them while the kernel ahead of it in the stream is still running, so
+    weights that change become a new Int4Weight (or wait for the kernel that writes them before the next product)."""
     codes: torch.Tensor
     params: torch.Tensor
     n: int
@@ -348,6 +350,8 @@ def quantize_weight(w, group=64):
         both = torch.zeros((16 * (r1 - r0), groups, 2), dtype=w.dtype, device=w.device)
         both[:m] = torch.stack((scale, zero), -1)
         params[r0:r1] = both.view(r1 - r0, 2, 8, groups, 2).permute(0, 3, 2, 1, 4)
+    if w.is_cuda and not torch.cuda.is_current_stream_capturing():
+        torch.cuda.current_stream(w.device).synchronize()  # products do not wait for the kernel that wrote their weights
     return Int4Weight(codes, params, n, k, group)
 
 
@@ -366,7 +370,7 @@ def dequantize_weight(w):
 def gemv_int4(x, w, *, swiglu=False):
     """x [..., k] times the transpose of an Int4Weight [n, k] -> [..., n] (tc_gemv_int4), sums in fp32: the
     projections of a decode step. x: bf16 or fp16, the type of w's params. Up to 32 tokens read the weights once (as
-    many as fit shared memory with their k columns: 8 at 12,288); more are taken in turns.
+    many as fit shared memory with their k columns: 28 at 2,560, 7 at 12,288); more are taken in turns.
     swiglu: x is [..., 2 k] (gate | up) and the tokens are silu(gate) * up, rounded after each step as
     transformers rounds them, computed on the way."""
     what = "gemv_int4"
