@@ -13,7 +13,7 @@ ROOT = os.path.dirname(HERE)
 SRC = os.path.join(HERE, "csrc", "threadcut_b200.cu")
 OUT = os.path.join(HERE, "libthreadcut_b200.so")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
-FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-shared", "--split-compile", "0", "-Xcompiler", "-fPIC", "-cudart", "static",
+FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-shared", "-Xcompiler", "-fPIC", "-cudart", "static",
          "-I", os.path.join(ROOT, "include")]
 
 

@@ -27,20 +27,19 @@ bool i4_pool(int hkv, int d, int64_t page_rows, int64_t num_pages) {
                                       : fn<__half, 256>(__VA_ARGS__)))
 
 template <typename T, int D, int U>
-cudaError_t launch_int4_append_vec(const Int4AppendParams& p, bool table_f32, int sms, cudaStream_t st) {
+cudaError_t launch_int4_append_vec(const Int4AppendParams& p, int sms, cudaStream_t st) {
   const int64_t groups = cdiv(p.hq, 256 / D * U) + 2 * cdiv(p.hkv, 256 / D * i4_kv_heads(U));
   // warps of a token's groups, the tokens shared out evenly over those that are resident at once
   const bool norm = p.q_w != nullptr || p.k_w != nullptr;
   const int64_t resident = (int64_t)sms * 8 * i4_append_ctas(U, norm) / groups;
   const int64_t rounds = cdiv(p.t, resident < 1 ? 1 : resident);
   const dim3 grid((unsigned)cdiv(cdiv(p.t, rounds) * groups, 8));
-  auto fn = table_f32 ? (norm ? int4_append_vec_kernel<T, float, D, U, true> : int4_append_vec_kernel<T, float, D, U, false>)
-                      : (norm ? int4_append_vec_kernel<T, T, D, U, true> : int4_append_vec_kernel<T, T, D, U, false>);
+  auto fn = norm ? int4_append_vec_kernel<T, D, U, true> : int4_append_vec_kernel<T, D, U, false>;
   return launch_ex(fn, grid, dim3(256), 0, st, p);
 }
 
 template <typename T, int D>
-cudaError_t launch_int4_append(const Int4AppendParams& p, bool table_f32, bool vec, int sms, cudaStream_t st) {
+cudaError_t launch_int4_append(const Int4AppendParams& p, bool vec, int sms, cudaStream_t st) {
   constexpr int RW = 256 / D;
   const int64_t warps = p.t * (cdiv(p.hq, RW) + 2 * cdiv(p.hkv, RW));
   if (vec && p.hq == 0 && p.rot == 0 && p.k_w == nullptr && warps >= (int64_t)sms * 64) {
@@ -49,10 +48,10 @@ cudaError_t launch_int4_append(const Int4AppendParams& p, bool table_f32, bool v
     return launch_ex(int4_write_kernel<T, D>, dim3((unsigned)cdiv(cdiv(p.t, rounds) * groups, 8)), dim3(256), 0, st, p);
   }
   if (vec)
-    return warps < (int64_t)sms * 64 ? launch_int4_append_vec<T, D, 1>(p, table_f32, sms, st)
-                                     : launch_int4_append_vec<T, D, 4>(p, table_f32, sms, st);
+    return warps < (int64_t)sms * 64 ? launch_int4_append_vec<T, D, 1>(p, sms, st)
+                                     : launch_int4_append_vec<T, D, 4>(p, sms, st);
   const int64_t blocks = cdiv(warps, 8);
-  return launch_ex(table_f32 ? int4_append_kernel<T, float, D> : int4_append_kernel<T, T, D>,
+  return launch_ex(int4_append_kernel<T, D>,
                    dim3((unsigned)(blocks < (int64_t)sms * 64 ? blocks : (int64_t)sms * 64)), dim3(256), 0, st, p);
 }
 
@@ -276,6 +275,7 @@ int tc_int4_append_rope(const void* q, const void* k, const void* v, void* q_out
   p.eps = eps;
   p.inv_d = 1.f / (float)d;
   p.minus_zero = -0.f;
+  p.table_f32 = table_dtype == TC_F32;
   bool vec = rot % 16 == 0 && aligned16(k) && aligned16(v) && stride16(k_stride_h, dtype) && stride16(k_stride_t, dtype) &&
              stride16(v_stride_h, dtype) && stride16(v_stride_t, dtype);
   if (hq > 0)
@@ -285,8 +285,8 @@ int tc_int4_append_rope(const void* q, const void* k, const void* v, void* q_out
     vec = vec && aligned16(cos_t) && aligned16(sin_t) && stride16(cos_stride_t, table_dtype) &&
           stride16(sin_stride_t, table_dtype);
   vec = vec && aligned16(q_norm_weight) && aligned16(k_norm_weight) && (reinterpret_cast<uintptr_t>(slots) & 7u) == 0;
-  const cudaError_t e = TC_INT4_DISPATCH(launch_int4_append, dtype, d, p, table_dtype == TC_F32, vec,
-                                         sm_count(current_device()), static_cast<cudaStream_t>(stream));
+  const cudaError_t e = TC_INT4_DISPATCH(launch_int4_append, dtype, d, p, vec, sm_count(current_device()),
+                                         static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? TC_OK : TC_ERR_CUDA;
 }
 

@@ -331,8 +331,9 @@ def quantize_weight(w, group=64):
     rows, cols, groups = -(-n // 16), -(-k // 64), -(-k // group)
     codes = torch.empty((rows, cols, 512), dtype=torch.uint8, device=w.device)
     params = torch.zeros((rows, groups, 8, 2, 2), dtype=w.dtype, device=w.device)
-    for r0 in range(0, rows, 512):  # pieces: the steps below take about 30 bytes an element
-        r1 = min(rows, r0 + 512)
+    some = max(1, 2 ** 20 // k)
+    for r0 in range(0, rows, some):  # pieces: the steps below take about 30 bytes an element
+        r1 = min(rows, r0 + some)
         piece = w[16 * r0:16 * r1].float()
         m = piece.shape[0]
         # the last group's extremes are those of its own columns
