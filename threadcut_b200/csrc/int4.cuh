@@ -121,14 +121,6 @@ __device__ __forceinline__ uint32_t i4_ones(uint32_t w) {
 // from memory: as a constant it would make them products again.)
 __device__ __forceinline__ float2 product2(float2 a, float2 b, float2 nz) { return ffma2(a, b, nz); }
 
-// 16 bytes, loaded where it stands: left to the compiler, loads of several heads end up beside their uses (a 16,384-token prompt
-// is then written in 82 us instead of 67).
-__device__ __forceinline__ uint4 load16(const void* p) {
-  uint4 v;
-  asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
-  return v;
-}
-
 template <typename X>
 __device__ __forceinline__ void load8(const X* p, float (&x)[8]) {
   constexpr int V = 16 / sizeof(X);
@@ -162,7 +154,7 @@ __device__ __forceinline__ float by_15_16(float x) {
 // (x - z) / S by itself, scaled by a power of two where (in bf16) the reciprocal or x - z would overflow, and clamped; 15 u
 // with u of [0, 1] is off by 7e-6 there.
 // 49,152 keys of 8 heads of 128 are rotated in 36 us so, in 47 with the other way for all groups; a 16,384-token prompt (32
-// query and 8 KV heads) is written in 67 us, and took 170 with borders decided by exact remainders and comparisons.
+// query and 8 KV heads) is written in 69 us, and took 170 with borders decided by exact remainders and comparisons.
 template <typename T>
 __device__ __forceinline__ uint32_t quantise8(const uint32_t (&w)[4], uint32_t& param) {
   constexpr bool bf = I4<T>::kBit == 3;
@@ -336,7 +328,9 @@ __global__ void __launch_bounds__(256) int4_append_kernel(const __grid_constant_
 // Rows, tables and weights on 16-byte boundaries, rot a multiple of 16: the same with 16-byte accesses. A warp stays with its
 // heads (256/D times U of them, queries, keys or values) and goes through tokens; a lane has the same 8 elements of U heads,
 // for which it converts a token's cos and sin once. The elements that it rotates them with are loaded a second time (they are
-// in L1: another lane of the row holds them).
+// in L1: another lane of the row holds them). A 16,384-token prompt of 32 query and 8 KV heads of 128: 69 us (5.3 TB/s); half as
+// many heads a lane 87, one CTA an SM less 83, the next token's rows loaded ahead 82, both elements of a pair in one lane 86:
+// each has fewer bytes in flight or fewer warps.
 // kKind: 0 queries, 1 keys, 2 values. kNorm: with a norm weight.
 template <typename T, int D, int U, int kKind, bool kNorm>
 __device__ __forceinline__ void append_tokens(const Int4AppendParams& p, int grp, uint32_t tok0, uint32_t step) {
@@ -359,8 +353,8 @@ __device__ __forceinline__ void append_tokens(const Int4AppendParams& p, int grp
     for (int u = 0; u < U; ++u) {
       a[u] = b[u] = make_uint4(0u, 0u, 0u, 0u);
       if (h0 + u * RW < heads) {
-        a[u] = load16(src + u * RW * sh);
-        if (turns) b[u] = load16(src + u * RW * sh + other);
+        a[u] = *reinterpret_cast<const uint4*>(src + u * RW * sh);
+        if (turns) b[u] = *reinterpret_cast<const uint4*>(src + u * RW * sh + other);
       }
     }
     uint8_t* row = nullptr;
@@ -542,7 +536,8 @@ struct Int4GatherParams {
 };
 
 // A warp per (tile, head): a lane turns one word of a key row and of the value row beside it into 16 bytes each, a row
-// being D/8 lanes. kI4Ahead rows' words are loaded before any is turned.
+// being D/8 lanes. kI4Ahead rows' words are loaded before any is turned: 16,384 tokens of 8 heads of 128 in 14.8 us (5.9 TB/s,
+// bound by memory), 29 with one row at a time.
 constexpr int kI4Ahead = 4;
 
 template <typename T, int D>

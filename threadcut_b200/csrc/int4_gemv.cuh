@@ -17,6 +17,9 @@
 // A CTA an SM takes neighbouring row tiles, in one or more streams of warps. A stream's warps share out the columns in
 // neighbouring runs, each bringing in its run of a row tile, and of the next ones, by bulk copies of a few tiles; their sums are
 // added in shared memory in warp order.
+//
+// Groups of 64, bf16: 2,560 x 4,096 with one token 3.7 us and 19,456 x 2,560 7.5 (start and end of a launch), 151,936 x 2,560
+// 34.4 (6.3 TB/s, bound by memory), with 7 tokens 51 (4.2 TB/s, bound by issue: 98 instructions a tile).
 #pragma once
 
 #include "int4_attn.cuh"
