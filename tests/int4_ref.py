@@ -13,7 +13,9 @@ def quantise64(x, group=GROUP):
     in float64, ties to the even code."""
     g = x.unflatten(-1, (-1, group))
     lo, hi = g.float().amin(-1), g.float().amax(-1)
-    s = ((hi - lo) / 0.9375).to(x.dtype)
+    # (a tensor of divisors: by a number, torch's CUDA division is a product with its rounded reciprocal, which turned an S of
+    # exactly 0x1.9dp87 into 0x1.9ep87 in bf16, where the even neighbour is 0x1.9cp87)
+    s = ((hi - lo) / torch.full_like(hi, 0.9375)).to(x.dtype)
     z = (lo - s.float()).to(x.dtype)
     sd, zd = s.double().unsqueeze(-1), z.double().unsqueeze(-1)
     c = ((g.double() - zd) / sd * 16 - 16).round().clamp(0, 15).masked_fill(sd == 0, 0).nan_to_num(0)

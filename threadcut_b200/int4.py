@@ -340,7 +340,7 @@ def quantize_weight(w, group=64):
         pad = groups * group - k
         g = torch.cat((piece, piece[:, -1:].expand(m, pad)), 1).view(m, groups, group)
         lo, hi = g.amin(-1), g.amax(-1)
-        scale = ((hi - lo) / 0.9375).to(w.dtype)
+        scale = ((hi - lo) / torch.full_like(hi, 0.9375)).to(w.dtype)  # (by a number: a product with its reciprocal on CUDA)
         zero = (lo - scale.float()).to(w.dtype)
         s, z = scale.double().unsqueeze(-1), zero.double().unsqueeze(-1)
         c = ((g.double() - z) / s * 16 - 16).round().clamp(0, 15).masked_fill(s == 0, 0).nan_to_num(0).to(torch.uint8)
