@@ -7,8 +7,8 @@
 // with lo and hi the group's extremes: 16 levels from lo to hi, S being 16 steps. In this form the codes are
 // the top four mantissa bits of numbers in [1, 2), so that a shift and one logic instruction turn two codes
 // into 16-bit floats, and one packed fma turns those into two values: no conversion, no subtraction, one
-// rounding. What the offset form costs: z's rounding, at most 2^-9 |z| (bf16), where |z| is about 23 steps for
-// data around zero: 0.05 of a step, beside the 0.5 of the code itself.
+// rounding. What the offset form costs: z's rounding, at most 2^-8 |z| (bf16), where |z| is about 23 steps for
+// data around zero: 0.09 of a step, beside the 0.5 of the code itself.
 // Each element takes its nearest level, ties to the even code (quantise8). A group with a NaN or an infinity,
 // or whose S or z overflows T (fp16: magnitudes above 20,000), reads back as NaN throughout.
 #pragma once
@@ -141,20 +141,64 @@ __device__ __forceinline__ float by_15_16(float x) {
   return fmaf(fmaf(-q, 0.9375f, x), kUnit, q);
 }
 
+// The codes of 8 elements (w0 to w3: pairs of T) under (S, z), each at its nearest level, whatever the two are (not finite: some
+// codes). A level by an approximate reciprocal, off by one at most and only beside a border, then the sign of x - z - S h against
+// the borders h around it: d = x - z rounded, its error exactly (Knuth's two-sum), and d - S h by one fma, which is 0 or larger than
+// that error, as it is a multiple of d's last bit. A bf16 S that x - z would overflow with is taken a fourth of (exact in fp32).
+// A function of its own, as it is rare and takes registers and instruction cache where it is inlined: with a costlier test for
+// it than there is now, 49,152 keys of 8 heads of 128 were rotated in 42 us so, 43 with this loop inlined, 49 unrolled.
+template <typename T>
+__device__ __noinline__ uint32_t exact_codes8(uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3, float s, float z) {
+  float by = 1.f, up = 1.f;
+  if constexpr (I4<T>::kBit == 3) {
+    by = s > 1e30f ? 0.25f : 1.f;
+    up = s > 1e30f ? 1.f / 18446744073709551616.f : s < 1e-30f ? 18446744073709551616.f : 1.f;  // 2^64: for the reciprocal
+    s *= by;
+    z *= by;
+  }
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s * up));
+  r = s > 0.f ? 16.f * r : 0.f;
+  uint32_t codes = 0u;
+#pragma unroll 1
+  for (int e = 0; e < 32; e += 4) {
+    const float x = Mma<T>::lo(w0) * by;
+    w0 = __funnelshift_r(w0, w1, 16);
+    w1 = __funnelshift_r(w1, w2, 16);
+    w2 = __funnelshift_r(w2, w3, 16);
+    w3 >>= 16;
+    const float d = __fsub_rn(x, z), back = __fsub_rn(d, x);
+    const float err = __fsub_rn(__fsub_rn(x, __fsub_rn(d, back)), __fadd_rn(z, back));
+    const float c = fminf(fmaxf(rintf(fmaf(d * up, r, -16.f)), 0.f), 15.f);  // NaN gives 0
+    float below = fmaf(-s, (c + 15.5f) * 0.0625f, d), above = fmaf(-s, (c + 16.5f) * 0.0625f, d);
+    below = below == 0.f ? err : below;
+    above = above == 0.f ? err : above;
+    int code = (int)c;
+    const bool odd = code & 1;  // on a border, the even level
+    code += (above > 0.f || (above == 0.f && odd)) - (below < 0.f || (below == 0.f && odd));
+    codes |= (uint32_t)(code < 0 ? 0 : code > 15 ? 15 : code) << e;
+  }
+  return codes;
+}
+
 // Codes of this lane's 8 elements (w: pairs of T) of a group that four neighbouring lanes (aligned to 4) hold, and the
 // group's (S, z). Every lane of the warp calls it.
 // The extremes as packed maxima and minima. A code is x (16/S) + (-16 z/S - 16) rounded. Many elements of coarse 16-bit data
 // lie exactly on a border between two levels, and the even one is theirs. That sum is off by at most 4.3e-6: 32 * 2^-24 from
 // 16/S (one Newton step behind the approximate reciprocal), 2^-19 from the offset's rounding while it is below 64, 2^-21 from
-// its own. So it is first rounded to a multiple of 2^-16, which a border is (half of one is 7.6e-6; an element 2^-17 of a level
-// beside one counts as on it), then to a whole number, both by adding constants, two elements an instruction; the codes are
-// collected as the floats' bits, whose exponents add up to a constant. No clamp: below that offset z's and S's roundings move
-// an end by 0.2 of a level at most.
-// Groups that this does not hold for (S subnormal, far from 1 or 0, values many times their spread, NaN) send their warp another way:
-// (x - z) / S by itself, scaled by a power of two where (in bf16) the reciprocal or x - z would overflow, and clamped; 15 u
-// with u of [0, 1] is off by 7e-6 there.
-// 49,152 keys of 8 heads of 128 are rotated in 36 us so, in 47 with the other way for all groups; a 16,384-token prompt (32
-// query and 8 KV heads) is written in 69 us, and took 170 with borders decided by exact remainders and comparisons.
+// its own. So it is first rounded to a multiple of 2^-16, which a border is (half of one is 7.6e-6), then to a whole number, both
+// by adding constants, two elements an instruction; the codes are collected as the floats' bits, whose exponents add up to a
+// constant. No clamp: below that offset z's and S's roundings move an end by 0.37 of a level at most (z's, 16 * 2^-8 |z|/S in
+// bf16 with |z| < 5 S, by 0.31; S's by 0.06).
+// An element beside a border but less than 2^-16 of a level from it may come out as on it. With p significant bits (8 or 11),
+// z and the borders S (33 + 2 j) / 32 + z are multiples of 2^-(p+5) S, so that such an element's last bit must be finer:
+// |x| < 2^(p-20) S, and the border lies as near to zero. That is one border at most, and the offset, which is zero's own place
+// among the levels, is within 2^(p-16) of its number. Groups with such an offset look whether anything came out on that border.
+// Warps where something did, and those with an offset of 64 or more (values many times their spread), with an S of 0 or too small
+// for the reciprocal, or with a NaN, take exact_codes8. Both ways give the nearest level, so that a row's bytes are the same in any
+// company.
+// 49,152 keys of 8 heads of 128 are rotated in 37 us in bf16 and 39 in fp16; 37 and 37 without that test, 47 and 51 with the
+// elements near such a border compared with it and both ways inlined.
 template <typename T>
 __device__ __forceinline__ uint32_t quantise8(const uint32_t (&w)[4], uint32_t& param) {
   constexpr bool bf = I4<T>::kBit == 3;
@@ -165,45 +209,41 @@ __device__ __forceinline__ uint32_t quantise8(const uint32_t (&w)[4], uint32_t& 
   m = I4<T>::max2(m, __shfl_xor_sync(0xffffffffu, m, 2));
   const float hi = Mma<T>::lo(m), lo = -Mma<T>::hi(m);
   const uint32_t st = Mma<T>::pack(by_15_16(__fsub_rn(hi, lo)), 0.f);
-  float s = Mma<T>::lo(st);
+  const float s = Mma<T>::lo(st);
   param = Mma<T>::pack(s, __fsub_rn(lo, s));
-  float z = Mma<T>::hi(param);
+  const float z = Mma<T>::hi(param);
   constexpr float kWhole = 12582912.f;  // 1.5 * 2^23: adding it leaves a whole number in the low bits
   constexpr float kSnap = 192.f;        // 1.5 * 2^7: adding it leaves multiples of 2^-16
-  uint32_t sum = 0u - 0x4b400000u * 0x11111111u;  // the bits of kWhole, as often as they come in
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(0.0625f * s));
   r = fmaf(r, fmaf(-0.0625f * s, r, 1.f), r);
   const float c = fmaf(-z, r, -16.f);
-  const bool plain = s >= (bf ? 1e-30f : 6.103515625e-5f) && s <= (bf ? 1e30f : 65504.f) && fabsf(c) < 64.f;
-  if (__all_sync(0xffffffffu, plain)) {
+  float2 t[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    t[i] = fadd2(ffma2(make_float2(Mma<T>::lo(w[i]), Mma<T>::hi(w[i])), make_float2(r, r), make_float2(c, c)),
+                 make_float2(kSnap, kSnap));
+  bool sure = fabsf(c) < 64.f;  // (false for NaN too)
+  // whether c, to a multiple of 2^(p-18), is within 2^(p-16) of a half: its fraction from 1/2 - 2^(p-16) on, as bits
+  constexpr float kFine = bf ? 12288.f : 49152.f;       // 1.5 * 2^13 or 2^15: adding it leaves multiples of 2^-10 or 2^-8
+  constexpr float kFrom = bf ? 0.49609375f : 0.46875f;  // 1/2 - 2^-8 or - 2^-5
+  constexpr uint32_t kUnit = bf ? 1024 : 256, kWide = bf ? 8 : 16;
+  if ((__float_as_uint(c + (kFine - kFrom)) & (kUnit - 1)) <= kWide) {
+    const float tie = __fsub_rn(__fadd_rn(c + 0.5f, kWhole), kWhole) + (kSnap - 0.5f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sure = sure && t[i].x != tie && t[i].y != tie;
+  }
+  if (__all_sync(0xffffffffu, sure)) {
     uint32_t codes = 0u;
 #pragma unroll
     for (int i = 3; i >= 0; --i) {
-      float2 t = ffma2(make_float2(Mma<T>::lo(w[i]), Mma<T>::hi(w[i])), make_float2(r, r), make_float2(c, c));
-      t = fadd2(fadd2(t, make_float2(kSnap, kSnap)), make_float2(kWhole - kSnap, kWhole - kSnap));
-      codes = (codes * 16u + __float_as_uint(t.y)) * 16u + __float_as_uint(t.x);
+      const float2 n = fadd2(t[i], make_float2(kWhole - kSnap, kWhole - kSnap));
+      codes = (codes * 16u + __float_as_uint(n.y)) * 16u + __float_as_uint(n.x);
     }
-    return codes + sum;
+    return codes - 0x4b400000u * 0x11111111u;  // the bits of kWhole, as often as they came in
   }
   if (fabsf(z) == INFINITY) param |= 0x7fffu;  // S NaN: a finite S would leave infinities that look like data
-  float by = 1.f;
-  if constexpr (bf) {
-    by = s < 1e-30f ? 18446744073709551616.f : s > 1e30f ? 1.f / 18446744073709551616.f : 1.f;
-    s *= by;
-    z *= by;
-  }
-  constexpr float kUnit = 16.f / 15.f;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
-  r = s > 0.f ? kUnit * r : 0.f;
-  uint32_t codes = 0u;
-#pragma unroll
-  for (int e = 7; e >= 0; --e) {
-    const float x = e & 1 ? Mma<T>::hi(w[e / 2]) : Mma<T>::lo(w[e / 2]);
-    const float u = __saturatef(fmaf(bf ? fmaf(x, by, -z) : x - z, r, -kUnit));  // NaN gives 0
-    codes = codes * 16u + __float_as_uint(fmaf(u, 15.f, kSnap) + (kWhole - kSnap));
-  }
-  return codes + sum;
+  return exact_codes8<T>(w[0], w[1], w[2], w[3], s, z);
 }
 
 // ------------------------------------------------------------------------------------------------ writing
