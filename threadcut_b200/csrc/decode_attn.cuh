@@ -341,7 +341,7 @@ __device__ void merge_last(const DecodeParams& p, uint8_t* scratch, int b, int h
 // The last merger past the wait clears the published count; the merger with the last ticket clears
 // the ticket.
 // Preconditions: every thread calls this after a __syncthreads() that follows the region writes;
-// the region area holds at least merge_scratch_bytes(blockDim.x) bytes.
+// the region area starts on a 16-byte boundary and holds at least merge_scratch_bytes(blockDim.x) bytes.
 template <typename T, int D, int HP>
 __device__ void finish_cta(const DecodeParams& p, uint8_t* regions, int region_stride_bytes, int nregions,
                            int b, int h, int split, int nsplit, int mi) {
@@ -431,9 +431,10 @@ __device__ void finish_cta(const DecodeParams& p, uint8_t* regions, int region_s
     const int nsg = nthr / w;
     const int sg = tid / w, col = cc + (tid - (tid / w) * w);
     const int hd = col / Q;
-    float* sM = reinterpret_cast<float*>(regions);  // [nsg][w] per-thread states
+    // [nsg][w] per-thread states, the float4 first: behind nsg w floats it would start off a 16-byte boundary for odd counts
+    float4* sA = reinterpret_cast<float4*>(regions);
+    float* sM = reinterpret_cast<float*>(sA + nsg * w);
     float* sL = sM + nsg * w;
-    float4* sA = reinterpret_cast<float4*>(sL + nsg * w);
     float M = -INFINITY, L = 0.f;
     float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
     if (sg < nsg) {
