@@ -102,8 +102,8 @@ __device__ __forceinline__ void digits4(int v0, int v1, int v2, int v3, uint32_t
   d[1] = __byte_perm(__byte_perm(v0, v1, 0x0051), __byte_perm(v2, v3, 0x0051), 0x5410) ^ 0x80808080u;
   d[2] = __byte_perm(__byte_perm(v0, v1, 0x0062), __byte_perm(v2, v3, 0x0062), 0x5410);
 }
-// The power of two that brings a largest magnitude into [2^19, 2^20), and its inverse; NaN as the inverse where it is not
-// finite, so that it shows.
+// The power of two that brings a largest magnitude (0, or 2^-86 at least) into [2^19, 2^20), and its inverse; NaN as the inverse where
+// it is not finite, so that it shows.
 __device__ __forceinline__ void digit_scale(float most, float& up, float& down) {
   int e = 146 - (int)(__float_as_uint(most) >> 23);
   e = e > 100 ? 100 : e;
@@ -219,8 +219,16 @@ __global__ void __launch_bounds__(32 * kGvWarps, 1) int4_gemv_kernel(const __gri
         for (int e = 1; e < 8; ++e) most = fmaxf(most, fabsf(f[e]));
 #pragma unroll
         for (int o = 1; o < 8; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+        // below the powers of two that fp32 has on both sides: as many times 2^64 (the same for the 8 lanes of a block)
+        const bool tiny = most < 0x1p-64f;
+        if (tiny) {
+          most *= 0x1p64f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) f[e] *= 0x1p64f;
+        }
         float up, down;
         digit_scale(sum * 0.f == 0.f ? most : INFINITY, up, down);
+        if (tiny) down *= 0x1p-64f;
         constexpr float kWhole = 12582912.f;  // 1.5 * 2^23: adding it leaves a whole number in the low bits
         int q[8];
 #pragma unroll
@@ -237,10 +245,11 @@ __global__ void __launch_bounds__(32 * kGvWarps, 1) int4_gemv_kernel(const __gri
             *reinterpret_cast<uint2*>(to + i * x_bytes) = make_uint2(even[kGvDigits - 1 - i], odd[kGvDigits - 1 - i]);
         }
         if (writes) {
-          // lane c's sums of a token are 256 h + m (c even), and 256 l + l; the products are with codes, 16 times code/16
+          // lane c's sums of a token are 256 h + m (c even), and l; the products are with codes, 16 times code/16. Powers of two: where
+          // they are subnormal, a tiny token's low digits, which would make them inexact, are 0
           float2* to = reinterpret_cast<float2*>(xsum) + (k0 / kXw) * 4 + 2 * m;
           to[0] = make_float2(sum, 16.f * down);
-          to[1] = make_float2(0.f, (0.0625f / 257.f) * down);
+          to[1] = make_float2(0.f, 0.0625f * down);
         }
       } else {
         if (use) {
@@ -279,6 +288,7 @@ __global__ void __launch_bounds__(32 * kGvWarps, 1) int4_gemv_kernel(const __gri
     sum0[nt] = smem_u32(xsum) + (kInt ? 8 * c : 4 * (token < xw ? token : 0));
   }
   const uint32_t sum_step = kInt ? 32 : 4 * xw;
+  const int high = c & 1 ? 0 : 256;  // (kInt) what column 2c counts: an odd lane's columns are both the last digit
   int s = 0, phase = 0, buf = 0;
   for (int f0 = rt0; f0 < rt1; f0 += p.flush, buf ^= 1) {
     const int nf = rt1 - f0 < p.flush ? rt1 - f0 : p.flush;  // (flush is a multiple of streams)
@@ -314,7 +324,7 @@ __global__ void __launch_bounds__(32 * kGvWarps, 1) int4_gemv_kernel(const __gri
             for (int x = 0; x < XS; ++x) {
               const float2 X = lds_float2(sum0[0] + xx + x * 32);
               // (at most 64 * 15 * (256 * 16 + 128) < 2^24)
-              const float P0 = X.y * (float)(256 * d[x][0] + d[x][1]), P1 = X.y * (float)(256 * d[x][2] + d[x][3]);
+              const float P0 = X.y * (float)(high * d[x][0] + d[x][1]), P1 = X.y * (float)(high * d[x][2] + d[x][3]);
               const float s0 = Mma<T>::lo(q[x][0]), s1 = Mma<T>::lo(q[x][1]);
               acc[0][0] = fmaf(s0 + Mma<T>::hi(q[x][0]), X.x, fmaf(s0, P0, acc[0][0]));
               acc[0][2] = fmaf(s1 + Mma<T>::hi(q[x][1]), X.x, fmaf(s1, P1, acc[0][2]));
