@@ -342,6 +342,7 @@ def quantize_weight(w, group=64):
         lo, hi = g.amin(-1), g.amax(-1)
         scale = ((hi - lo) / torch.full_like(hi, 0.9375)).to(w.dtype)  # (by a number: a product with its reciprocal on CUDA)
         zero = (lo - scale.float()).to(w.dtype)
+        scale.masked_fill_(~zero.isfinite(), float("nan"))  # (a finite S would leave infinities that look like data)
         s, z = scale.double().unsqueeze(-1), zero.double().unsqueeze(-1)
         c = ((g.double() - z) / s * 16 - 16).round().clamp(0, 15).masked_fill(s == 0, 0).nan_to_num(0).to(torch.uint8)
         full = torch.zeros((16 * (r1 - r0), 64 * cols), dtype=torch.uint8, device=w.device)
