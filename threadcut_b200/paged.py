@@ -616,8 +616,9 @@ class PagedKV:
     def splice(self, s: Split, inv_freq):
         """A.B.C -> A.C on every layer (threadcut/kv.py:28-41, 83-92 semantics): B's pages return to
         the pool, C's keys are re-rotated by -(c0 - a) positions where they lie, nothing moves."""
-        runs_c, _ = self.table.splice(s)
         gap = int(s.c0) - int(s.a)
+        self._rotates(s, inv_freq, "PagedKV.splice")
+        runs_c, _ = self.table.splice(s)
         if gap == 0 or runs_c.shape[0] == 0:
             return  # the reference clones C onto itself: nothing to rotate
         tab = PageTable.tiles_of(runs_c)
@@ -629,6 +630,11 @@ class PagedKV:
                 self._kptrs, self.layers, self.hkv, self.d, self.page_rows, self.table.num_pages, sp, sh, sr,
                 tiles.data_ptr(), tab.shape[0], cs_ptr, _lib.DTYPE_CODE[self.dtype], stream_ptr(self.device)))
         del cs  # the table is copied into the launch parameters
+
+    def _rotates(self, s, inv_freq, what):
+        """Refuses frequencies that a splice's keys cannot be rotated by, before anything has changed."""
+        if s.c0 != s.a and s.c and inv_freq.numel() * 2 != self.d:
+            raise ValueError(f"{what}: inv_freq has {inv_freq.numel()} entries, keys need {self.d // 2}")
 
     def truncate(self, n):
         self.table.truncate(n)
@@ -746,8 +752,9 @@ class PagedKVInt4(PagedKV):
     def splice(self, s: Split, inv_freq):
         """A.B.C -> A.C on every layer: B's pages return to the pool, C's keys are rotated by -(c0 - a) positions and
         quantised again where they lie (int4.rotate_keys_int4)."""
-        runs_c, _ = self.table.splice(s)
         gap = int(s.c0) - int(s.a)
+        self._rotates(s, inv_freq, "PagedKVInt4.splice")
+        runs_c, _ = self.table.splice(s)
         if gap and runs_c.shape[0]:
             tiles = torch.from_numpy(PageTable.tiles_of(runs_c)).to(self.device)
             int4.rotate_keys_int4(self.k, tiles, -gap, inv_freq, self.dtype)
