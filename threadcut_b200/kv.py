@@ -421,7 +421,8 @@ def use_paged_cache(enabled=True, max_tokens=32768, page_rows=64, bits=16):
 def new_cache(config, paged=None, max_tokens=None, page_rows=None, bits=None):
     """A DynamicCache of GrowingLayers (the reference's layout, threadcut/kv.py:44-98) or, with
     paged=True, of PagedLayers over one PagedKV sized for max_tokens (plus spare pages for the
-    partly used pages splices leave; a full pool is re-packed by PagedKV.compact). bits=4 (paged only): rows of 4 bits.
+    partly used pages splices leave; a full pool is re-packed by PagedKV.compact). bits=4 (paged only): rows of 4 bits,
+    with the threadcut attention for at most 16 query heads a KV head.
     Arguments left None take the process-wide choice of use_paged_cache (default: contiguous, 32768, 64, 16)."""
     paged = _LAYOUT["paged"] if paged is None else paged
     max_tokens = _LAYOUT["max_tokens"] if max_tokens is None else max_tokens
@@ -432,6 +433,12 @@ def new_cache(config, paged=None, max_tokens=None, page_rows=None, bits=None):
                          f"{'paged' if paged else 'contiguous'} cache")
     cache = DynamicCache(config=config)
     fused = getattr(config, "_attn_implementation", None) == FUSED_ATTENTION
+    if bits == 4 and fused:
+        text = config.get_text_config(decoder=True)
+        heads = text.num_attention_heads
+        group = heads // (getattr(text, "num_key_value_heads", None) or heads)
+        if group > 16:
+            raise ValueError(f"new_cache: 4-bit rows are decoded for at most 16 query heads a KV head, the model has {group}")
     if paged:
         state = _PagedState(len(cache.layers), int(max_tokens), int(page_rows), fused, bits)
         cache.layers = [PagedLayer(state, i) for i in range(len(cache.layers))]
