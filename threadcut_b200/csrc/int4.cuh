@@ -117,14 +117,6 @@ __device__ __forceinline__ uint32_t i4_ones(uint32_t w) {
   }
 }
 
-// Elements of lanes without a head or a row of their own: those of a group that quantise8 takes its usual way (a group of equal
-// elements would send the warp the other).
-template <typename T>
-__device__ __forceinline__ uint4 i4_idle() {
-  constexpr uint32_t k = I4<T>::kOne & 0xffff0000u;  // (0, 1)
-  return make_uint4(k, k, k, k);
-}
-
 // Two products, each rounded: an fma with -0, which is not merged with a sum that follows it, as packed products are. (nz is -0
 // from memory: as a constant it would make them products again.)
 __device__ __forceinline__ float2 product2(float2 a, float2 b, float2 nz) { return ffma2(a, b, nz); }
@@ -335,7 +327,7 @@ __global__ void __launch_bounds__(256) int4_append_kernel(const __grid_constant_
     for (int e = 0; e < 8; ++e) {
       const int i = i0 + e;
       const bool turns = use && i < rot;
-      x[e] = use ? to_f32(src[i]) : (float)(e & 1);  // (see i4_idle)
+      x[e] = use ? to_f32(src[i]) : 0.f;
       y[e] = turns ? to_f32(src[i < rot / 2 ? i + rot / 2 : i - rot / 2]) : 0.f;
       cs[e] = turns ? table_at<T>(p.cos_t, p.table_f32, tok * p.cos_st + i) : 0.f;
       sn[e] = turns ? table_at<T>(p.sin_t, p.table_f32, tok * p.sin_st + i) : 0.f;
@@ -399,8 +391,7 @@ __device__ __forceinline__ void append_tokens(const Int4AppendParams& p, int grp
     uint4 a[U], b[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      a[u] = i4_idle<T>();
-      b[u] = make_uint4(0u, 0u, 0u, 0u);
+      a[u] = b[u] = make_uint4(0u, 0u, 0u, 0u);
       if (h0 + u * RW < heads) {
         a[u] = *reinterpret_cast<const uint4*>(src + u * RW * sh);
         if (turns) b[u] = *reinterpret_cast<const uint4*>(src + u * RW * sh + other);
@@ -544,7 +535,7 @@ __global__ void __launch_bounds__(256, 3) int4_write_kernel(const __grid_constan
     slot = *reinterpret_cast<const int2*>(p.slots + 2 * (int64_t)tok);
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      next[u] = h0 + u * RW < p.hkv ? *reinterpret_cast<const uint4*>(src + tok * st + u * RW * sh) : i4_idle<T>();
+      next[u] = h0 + u * RW < p.hkv ? *reinterpret_cast<const uint4*>(src + tok * st + u * RW * sh) : make_uint4(0u, 0u, 0u, 0u);
   };
   if (tok < p.t) load();
   while (tok < p.t) {
@@ -693,8 +684,7 @@ __global__ void __launch_bounds__(256, 3) int4_rotate_kernel(const __grid_consta
         const int r = r0 + u * RW + lane / L;
         const int64_t pr = first_row + r;
         use[u] = r < rows && pr >= 0 && pr < p.page_rows;
-        wx[u] = wy[u] = 0x76543210u;  // (rows that there are not: see i4_idle)
-        qx[u] = qy[u] = I4<T>::kOne & 0xffffu;
+        wx[u] = wy[u] = qx[u] = qy[u] = 0u;
         if (use[u]) {
           const uint32_t* row = reinterpret_cast<const uint32_t*>(base + r * p.s_row);
           wx[u] = row[c];
