@@ -141,14 +141,49 @@ __device__ __forceinline__ float by_15_16(float x) {
   return fmaf(fmaf(-q, 0.9375f, x), kUnit, q);
 }
 
-// The codes of 8 elements (w0 to w3: pairs of T) under (S, z), each at its nearest level, whatever the two are (not finite: some
-// codes). A level by an approximate reciprocal, off by one at most and only beside a border, then the sign of x - z - S h against
-// the borders h around it: d = x - z rounded, its error exactly (Knuth's two-sum), and d - S h by one fma, which is 0 or larger than
-// that error, as it is a multiple of d's last bit. A bf16 S that x - z would overflow with is taken a fourth of (exact in fp32).
+// 16/S (NaN for an S of 0 or too small), and where among the levels zero lies, -16 z/S - 16.
+__device__ __forceinline__ void i4_line(float s, float z, float& r, float& c) {
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(0.0625f * s));
+  r = fmaf(r, fmaf(-0.0625f * s, r, 1.f), r);
+  c = fmaf(-z, r, -16.f);
+}
+constexpr float kI4Whole = 12582912.f;  // 1.5 * 2^23: adding it leaves a whole number in the low bits
+constexpr float kI4Snap = 192.f;        // 1.5 * 2^7: adding it leaves multiples of 2^-16
+constexpr float kI4Far = 64.f;          // offsets from which on zero is far outside the levels
+// The half next to c, + kI4Snap.
+__device__ __forceinline__ float i4_tie(float c) {
+  return __fsub_rn(__fadd_rn(c + 0.5f, kI4Whole), kI4Whole) + (kI4Snap - 0.5f);
+}
+
+// quantise8 for a warp with groups that its usual way is not for; w0 to w3: this lane's elements (pairs of T).
+// Where S is in order and nothing came out on a border near zero, the usual way again, but from x - z for groups far from zero, and
+// with a clamp; x - z is exact there.
+// Else any group, whatever S and z are (not finite: some codes): a level by an approximate reciprocal, off by one at most and only
+// beside a border, then the sign of x - z - S h against the borders h around it: d = x - z rounded, its error exactly (Knuth's
+// two-sum), and d - S h by one fma, which is 0 or larger than that error, as it is a multiple of d's last bit. A bf16 S that x - z would
+// overflow with is taken a fourth of (exact in fp32).
 // A function of its own, as it is rare and takes registers and instruction cache where it is inlined: with a costlier test for
-// it than there is now, 49,152 keys of 8 heads of 128 were rotated in 42 us so, 43 with this loop inlined, 49 unrolled.
+// it than there is now, 49,152 keys of 8 heads of 128 were rotated in 42 us so, 43 with this loop inlined, 49 unrolled. The same keys
+// far from zero for their spread (8 times) take 60 us, 117 with the comparisons for all such groups.
 template <typename T>
-__device__ __noinline__ uint32_t exact_codes8(uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3, float s, float z) {
+__device__ __noinline__ uint32_t quantise8_rare(uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3, float s, float z) {
+  float r, c;
+  i4_line(s, z, r, c);
+  const bool far = !(fabsf(c) < kI4Far), flat = s == 0.f;
+  const float from = far ? z : 0.f, c0 = far ? -16.f : c, tie = far ? 0.f : i4_tie(c);
+  bool usual = flat || fabsf(c) < INFINITY;
+  uint32_t codes = 0u;
+  {
+    const uint32_t w[4] = {w0, w1, w2, w3};
+#pragma unroll
+    for (int e = 7; e >= 0; --e) {
+      const float x = (e & 1 ? Mma<T>::hi(w[e / 2]) : Mma<T>::lo(w[e / 2])) - from;
+      const float t = __fadd_rn(fminf(fmaxf(fmaf(x, r, c0), 0.f), 15.f), kI4Snap);
+      usual = usual && (flat || t != tie);
+      codes = codes * 16u + __float_as_uint(__fadd_rn(t, kI4Whole - kI4Snap));
+    }
+  }
+  if (__all_sync(0xffffffffu, usual)) return flat ? 0u : codes - 0x4b400000u * 0x11111111u;
   float by = 1.f, up = 1.f;
   if constexpr (I4<T>::kBit == 3) {
     by = s > 1e30f ? 0.25f : 1.f;
@@ -156,10 +191,9 @@ __device__ __noinline__ uint32_t exact_codes8(uint32_t w0, uint32_t w1, uint32_t
     s *= by;
     z *= by;
   }
-  float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s * up));
   r = s > 0.f ? 16.f * r : 0.f;
-  uint32_t codes = 0u;
+  codes = 0u;
 #pragma unroll 1
   for (int e = 0; e < 32; e += 4) {
     const float x = Mma<T>::lo(w0) * by;
@@ -169,7 +203,7 @@ __device__ __noinline__ uint32_t exact_codes8(uint32_t w0, uint32_t w1, uint32_t
     w3 >>= 16;
     const float d = __fsub_rn(x, z), back = __fsub_rn(d, x);
     const float err = __fsub_rn(__fsub_rn(x, __fsub_rn(d, back)), __fadd_rn(z, back));
-    const float c = fminf(fmaxf(rintf(fmaf(d * up, r, -16.f)), 0.f), 15.f);  // NaN gives 0
+    c = fminf(fmaxf(rintf(fmaf(d * up, r, -16.f)), 0.f), 15.f);  // NaN gives 0
     float below = fmaf(-s, (c + 15.5f) * 0.0625f, d), above = fmaf(-s, (c + 16.5f) * 0.0625f, d);
     below = below == 0.f ? err : below;
     above = above == 0.f ? err : above;
@@ -194,10 +228,9 @@ __device__ __noinline__ uint32_t exact_codes8(uint32_t w0, uint32_t w1, uint32_t
 // z and the borders S (33 + 2 j) / 32 + z are multiples of 2^-(p+5) S, so that such an element's last bit must be finer:
 // |x| < 2^(p-20) S, and the border lies as near to zero. That is one border at most, and the offset, which is zero's own place
 // among the levels, is within 2^(p-16) of its number. Groups with such an offset look whether anything came out on that border.
-// Warps where something did, and those with an offset of 64 or more (values many times their spread), with an S too small for the
-// reciprocal, or with a NaN, take exact_codes8 (8,192 tokens of one KV head written in 39 us where half of each warp does so by
-// its idle lanes, 9.4 as it is). Both ways give the nearest level, so that a row's bytes are the same in any
-// company.
+// Warps where something did, and those with an offset of 64 or more (values many times their spread, with coarse last bits
+// therefore), an S too small for the reciprocal, or a NaN, take quantise8_rare. Every way gives the nearest level, so that a row's
+// bytes are the same in any company.
 // 49,152 keys of 8 heads of 128 are rotated in 37 us in bf16 and 39 in fp16; 37 and 37 without that test, 47 and 51 with the
 // elements near such a border compared with it and both ways inlined.
 template <typename T>
@@ -213,25 +246,21 @@ __device__ __forceinline__ uint32_t quantise8(const uint32_t (&w)[4], uint32_t& 
   const float s = Mma<T>::lo(st);
   param = Mma<T>::pack(s, __fsub_rn(lo, s));
   const float z = Mma<T>::hi(param);
-  constexpr float kWhole = 12582912.f;  // 1.5 * 2^23: adding it leaves a whole number in the low bits
-  constexpr float kSnap = 192.f;        // 1.5 * 2^7: adding it leaves multiples of 2^-16
-  float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(0.0625f * s));
-  r = fmaf(r, fmaf(-0.0625f * s, r, 1.f), r);
-  const float c = fmaf(-z, r, -16.f);
+  float r, c;
+  i4_line(s, z, r, c);
   float2 t[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i)
     t[i] = fadd2(ffma2(make_float2(Mma<T>::lo(w[i]), Mma<T>::hi(w[i])), make_float2(r, r), make_float2(c, c)),
-                 make_float2(kSnap, kSnap));
+                 make_float2(kI4Snap, kI4Snap));
   const bool flat = s == 0.f;  // one value throughout, as of lanes without a head or row of their own
-  bool sure = flat || fabsf(c) < 64.f;  // (false for NaN too)
+  bool sure = flat || fabsf(c) < kI4Far;  // (false for NaN too)
   // whether c, to a multiple of 2^(p-18), is within 2^(p-16) of a half: its fraction from 1/2 - 2^(p-16) on, as bits
   constexpr float kFine = bf ? 12288.f : 49152.f;       // 1.5 * 2^13 or 2^15: adding it leaves multiples of 2^-10 or 2^-8
   constexpr float kFrom = bf ? 0.49609375f : 0.46875f;  // 1/2 - 2^-8 or - 2^-5
   constexpr uint32_t kUnit = bf ? 1024 : 256, kWide = bf ? 8 : 16;
   if ((__float_as_uint(c + (kFine - kFrom)) & (kUnit - 1)) <= kWide) {
-    const float tie = __fsub_rn(__fadd_rn(c + 0.5f, kWhole), kWhole) + (kSnap - 0.5f);
+    const float tie = i4_tie(c);
 #pragma unroll
     for (int i = 0; i < 4; ++i) sure = sure && t[i].x != tie && t[i].y != tie;
   }
@@ -239,13 +268,13 @@ __device__ __forceinline__ uint32_t quantise8(const uint32_t (&w)[4], uint32_t& 
     uint32_t codes = 0u;
 #pragma unroll
     for (int i = 3; i >= 0; --i) {
-      const float2 n = fadd2(t[i], make_float2(kWhole - kSnap, kWhole - kSnap));
+      const float2 n = fadd2(t[i], make_float2(kI4Whole - kI4Snap, kI4Whole - kI4Snap));
       codes = (codes * 16u + __float_as_uint(n.y)) * 16u + __float_as_uint(n.x);
     }
-    return flat ? 0u : codes - 0x4b400000u * 0x11111111u;  // the bits of kWhole, as often as they came in
+    return flat ? 0u : codes - 0x4b400000u * 0x11111111u;  // the bits of kI4Whole, as often as they came in
   }
   if (fabsf(z) == INFINITY) param |= 0x7fffu;  // S NaN: a finite S would leave infinities that look like data
-  return exact_codes8<T>(w[0], w[1], w[2], w[3], s, z);
+  return quantise8_rare<T>(w[0], w[1], w[2], w[3], s, z);
 }
 
 // ------------------------------------------------------------------------------------------------ writing
