@@ -614,11 +614,13 @@ int tc_decode_attention_int4_paged(const void* q, const void* k_pool, const void
                                    void* stream);
 
 /* out [m][n] = x [m][k] . w^T for 4-bit weights w [n][k], sums in fp32; group 32, 64 or 128 neighbours of a row share
- * (S, z), not rounded further. codes [ceil(n/16)][ceil(k/64)][512 bytes]: bytes 16 (4r + c).. of a tile are the words of
+ * (S, z), not rounded further. One or two tokens (of a call, or left over by its turns) enter as whole numbers of 20 bits: each
+ * x is off by at most 2^-20 of the largest |x| of its 64 columns, so that a token's result may differ in its last bits with how many
+ * share its call. NaN where the sum of a group's x overflows fp32. codes [ceil(n/16)][ceil(k/64)][512 bytes]: bytes 16 (4r + c).. of a tile are the words of
  * (row r, columns 8c..8c+7), (row r + 8, the same), (row r, columns 32 + 8c..), (row r + 8, the same); code j of a word
  * is column 2j, code 4 + j column 2j + 1. params [ceil(n/16)][ceil(k/group)][8][2][2] of T: (S, z) of rows r, r + 8. Both 0
  * behind n and k, and 16-byte aligned. swiglu: x is [m][2k] (gate | up), the tokens silu(gate) * up. k up to
- * 65,536; more tokens than fit shared memory (32 at most) are taken in turns. Weights are constant, as tc_gemv's are: with
+ * 65,536; more tokens than fit shared memory (32 at most) are taken in turns, each of which reads the weights again. Weights are constant, as tc_gemv's are: with
  * programmatic dependent launch their first tiles are read while the kernel ahead in the stream still runs. */
 int tc_gemv_int4(const void* x, const void* codes, const void* params, void* out, int64_t n, int k, int64_t m, int group,
                  int64_t x_stride, int64_t out_stride, int swiglu, int dtype, void* stream);

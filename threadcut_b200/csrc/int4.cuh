@@ -539,7 +539,7 @@ __global__ void __launch_bounds__(256, i4_append_ctas(U, kNorm)) int4_append_vec
 }
 
 // Keys and values alone, as they are, many of them: the same with the next token's rows loaded before this one's are quantised,
-// as it is bound by the bytes in flight otherwise: 49,152 tokens of 8 heads of 128 in 49 us (5.4 TB/s), 74 without.
+// as it is bound by the bytes in flight otherwise: 49,152 tokens of 8 heads of 128 in 51 us (5.1 TB/s; fp16 55), 74 without.
 constexpr int kI4WriteHeads = 4;  // heads of a lane, times 256/D of a warp
 
 template <typename T, int D>
@@ -677,8 +677,9 @@ struct Int4RotateParams {
 // Keys re-rotated in place by one angle a frequency (the splice of threadcut/kv.py:28-41 over 4-bit rows): a row's
 // values, rotated in fp32 as the 16-bit splice rotates them, rounded to T and quantised again. A warp per
 // (layer, tile, head); a row is D/16 lanes, each with 8 elements of its first half and the 8 that they are paired with. kI4Ahead
-// rows' words are loaded before any is turned. Bound by instructions (18 an element, half of them on the half-rate pipe): 49,152
-// keys of 8 heads of 128 in 36 us, 47 with a lane's partners fetched by shuffles and converted twice.
+// rows' words are loaded before any is turned. Bound by instructions (18 an element, half of them on the half-rate pipe: 72 %
+// of the issue slots used, 59 % of that pipe; its bytes alone would take 10 us): 49,152 keys of 8 heads of 128 in 37 us, 47 with a lane's partners fetched by
+// shuffles and converted twice.
 template <typename T, int D>
 __global__ void __launch_bounds__(256, 3) int4_rotate_kernel(const __grid_constant__ Int4RotateParams p) {
   constexpr int L = D / 16;

@@ -12,10 +12,13 @@
 //                                   its own D/8 neighbouring elements, all of one group
 // P enters in two 16-bit parts; for up to 4 query heads a KV head (NH = 1) these are neighbouring columns of one product.
 //
-// Beside the bytes, instruction issue bounds it: about 800 instructions a tile of d = 128, most of them on the half-rate ALU pipe
-// (masks, shifts, permutes), which is 54 to 57 % busy over a launch, the tensor pipe 20 %. 8 KV heads of 128 with 4 query heads
+// A tile of d = 128 takes about 800 instructions, most of them on the half-rate ALU pipe (masks, shifts, permutes). Over a launch 61
+// to 65 % of the issue slots are used, 54 to 57 % of that pipe and 20 % of the tensor pipe: nothing is full. An instruction waits 1.1
+// cycles for the one ahead of it, 1.0 to 1.1 for that pipe and 1.2 to 1.3 for another warp's turn: the 16 warps that an SM's registers
+// hold do not cover a tile's chain of product, softmax and product with each other. 8 KV heads of 128 with 4 query heads
 // each: 98,304 rows 34 us (3.7 TB/s; start, merge and launch about 10 of it), 64 ragged sequences with 560,000 rows in all
-// 175 us (4.1 TB/s), 1,536 rows 8.2 us.
+// 174 us (4.1 TB/s), 1,536 rows 8.1 us. Below some 12,000 rows of one sequence the 16-bit
+// kernel, whose first tiles may be loaded ahead, is as fast on its own rows.
 #pragma once
 
 #include "decode_attn.cuh"

@@ -38,6 +38,11 @@ cudaError_t launch_int4_append_vec(const Int4AppendParams& p, int sms, cudaStrea
   return launch_ex(fn, grid, dim3(256), 0, st, p);
 }
 
+// Four heads a lane, and for keys and values alone the kernel that loads a token ahead, from 64 warps an SM on (a warp for 256/D heads of a
+// token). With many heads they pay earlier, with few later: 32 + 8 heads of 128, one and four heads a lane, 128 tokens (21 warps an
+// SM) 2.7 and 2.7 us, 256 (42) 3.8 and 2.9, 512 (83) 5.8 and 4.4; 8 + 1 heads 1,024 tokens (42) 5.7 and 5.7, 1,536 (62) 7.8 and 10.1.
+// Keys and values of 8 heads, one head a lane, four, and a token ahead: 1,024 tokens (55) 4.1, 3.5 and 3.1 us, 2,048 (111) 5.7, 4.7 and
+// 4.8, 8,192 17.7, 12.6 and 10.1.
 template <typename T, int D>
 cudaError_t launch_int4_append(const Int4AppendParams& p, bool vec, int sms, cudaStream_t st) {
   constexpr int RW = 256 / D;

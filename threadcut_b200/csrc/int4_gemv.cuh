@@ -11,7 +11,7 @@
 //   sum_k x (S (1 + code/16) + z) = S P + (S + z) X,   P = sum_k x code/16,  X = sum_k x, over the group's columns in a tile.
 // One or two tokens: P as an integer product of the codes, bytes after two masks and a shift (12 instructions for a lane's 32
 // codes), with the digits of x, which are otherwise idle columns: x of each 64 columns, scaled by a power of two and rounded
-// to a whole number below 2^20, is 65536 h + 256 m + l. More tokens: 1 + code/16 and x as they are, 16-bit operands (24 and
+// to a whole number below 2^20 (off by at most 2^-20 of the largest of the 64), is 65536 h + 256 m + l. More tokens: 1 + code/16 and x as they are, 16-bit operands (24 and
 // 8; S P + z X then), 8 tokens a product.
 //
 // A CTA an SM takes neighbouring row tiles, in one or more streams of warps. A stream's warps share out the columns in
@@ -19,7 +19,9 @@
 // added in shared memory in warp order.
 //
 // Groups of 64, bf16: 2,560 x 4,096 with one token 3.7 us and 19,456 x 2,560 7.5 (start and end of a launch), 151,936 x 2,560
-// 34.4 (6.3 TB/s, bound by memory), with 7 tokens 51 (4.2 TB/s, bound by issue: 98 instructions a tile).
+// 35 (6.2 TB/s, bound by memory), with 7 tokens 51 (4.1 TB/s: 98 instructions a tile, 64 % of the issue slots used; an instruction
+// waits 1.3 cycles for the one ahead of it, 1.2 for another warp's turn and 0.8 for the ALU pipe). Tokens beside a small ring, and the
+// turns of those that do not fit, cost more: 8, 16 and 32 tokens 55, 91 and 235.
 #pragma once
 
 #include "int4_attn.cuh"

@@ -372,7 +372,10 @@ def dequantize_weight(w):
 def gemv_int4(x, w, *, swiglu=False):
     """x [..., k] times the transpose of an Int4Weight [n, k] -> [..., n] (tc_gemv_int4), sums in fp32: the
     projections of a decode step. x: bf16 or fp16, the type of w's params. Up to 32 tokens read the weights once (as
-    many as fit shared memory with their k columns: 28 at 2,560, 7 at 12,288); more are taken in turns.
+    many as fit shared memory with their k columns: 28 at 2,560, 7 at 12,288); more are taken in turns, each of which reads
+    the weights again: this is for a few tokens, not for a prompt.
+    One or two tokens, of a call or left over by its turns, enter as whole numbers of 20 bits: each x is off by at most 2^-20 of the
+    largest |x| of its 64 columns. A token's result may so differ in its last bits with how many share its call.
     swiglu: x is [..., 2 k] (gate | up) and the tokens are silu(gate) * up, rounded after each step as
     transformers rounds them, computed on the way."""
     what = "gemv_int4"

@@ -435,7 +435,7 @@ def new_cache(config, paged=None, max_tokens=None, page_rows=None, bits=None):
     fused = getattr(config, "_attn_implementation", None) == FUSED_ATTENTION
     if bits == 4 and fused:
         text = config.get_text_config(decoder=True)
-        heads = text.num_attention_heads
+        heads = getattr(text, "num_attention_heads", None) or 1
         group = heads // (getattr(text, "num_key_value_heads", None) or heads)
         if group > 16:
             raise ValueError(f"new_cache: 4-bit rows are decoded for at most 16 query heads a KV head, the model has {group}")
