@@ -244,7 +244,12 @@ __global__ void __launch_bounds__(32 * kWarps, i4_warps(D, NH) / kWarps)
     if (j + 2 * kWarps < ntiles) ahead = entry(j + 2 * kWarps);
     const uint32_t kst = ring_s + s * G::kStage, vst = kst + kTile * G::kStride;
     if constexpr (kBulk) {
-      if (!mbar_wait(&full[s], phase, TC_DEVERR_PIPE_TIMEOUT)) break;
+      if (!__all_sync(0xffffffffu, mbar_wait(&full[s], phase, TC_DEVERR_PIPE_TIMEOUT))) {
+        // given up by the whole warp, and only once its copies had another chance to end
+        mbar_wait(&full[s], phase, TC_DEVERR_PIPE_TIMEOUT);
+        if (j + kWarps < ntiles) mbar_wait(&full[s ^ 1], phase ^ s, TC_DEVERR_PIPE_TIMEOUT);
+        break;
+      }
       if (valid < kTile) {
         // values of rows that the tile does not have: S = z = 0, so that a weight of 0 never meets a NaN
         if (lane >= valid) {

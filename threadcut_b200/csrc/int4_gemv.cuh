@@ -292,6 +292,7 @@ __global__ void __launch_bounds__(32 * kGvWarps, 1) int4_gemv_kernel(const __gri
   const uint32_t sum_step = kInt ? 32 : 4 * xw;
   const int high = c & 1 ? 0 : 256;  // (kInt) what column 2c counts: an odd lane's columns are both the last digit
   int s = 0, phase = 0, buf = 0;
+  bool alive = true;
   for (int f0 = rt0; f0 < rt1; f0 += p.flush, buf ^= 1) {
     const int nf = rt1 - f0 < p.flush ? rt1 - f0 : p.flush;  // (flush is a multiple of streams)
     float* pb = part + buf * (p.part_bytes / 4);             // [nf][slices][m][16]
@@ -302,7 +303,13 @@ __global__ void __launch_bounds__(32 * kGvWarps, 1) int4_gemv_kernel(const __gri
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[nt][e] = 0.f;
       for (int kt = kt0; kt < kt0 + nk;) {
-        if (!mbar_wait(&full[s], phase, TC_DEVERR_PIPE_TIMEOUT)) break;
+        if (alive && !__all_sync(0xffffffffu, mbar_wait(&full[s], phase, TC_DEVERR_PIPE_TIMEOUT))) {
+          // given up by the whole warp for the rest of the launch, and only once its copies had another chance to end
+          for (int i = 0; i < p.stages; ++i)
+            mbar_wait(&full[s + i < p.stages ? s + i : s + i - p.stages], phase ^ (s + i >= p.stages), TC_DEVERR_PIPE_TIMEOUT);
+          alive = false;
+        }
+        if (!alive) break;
         const uint32_t st = smem_u32(ring) + s * stage_bytes;
         const int end = kt + p.chunk < kt0 + nk ? kt + p.chunk : kt0 + nk;
         uint32_t code = st + 16 * lane, param = st + p.chunk * 512 + 8 * r, xk = kt * (kInt ? 64 : 128), xx = kt * XS * sum_step;
